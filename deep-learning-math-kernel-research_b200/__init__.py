@@ -3,7 +3,8 @@
 This package is the Python door to the C-ABI library ``lib/libeuler_b200.so`` (sources in
 ``csrc/``, interface in ``include/euler_b200.h``).  It mirrors the reference's public surface
 (``include/euler.hpp``): an ``eld_conv_t`` descriptor with the same field names, ``setup()`` and
-``elx_conv(desc, output, input, weights, bias)``.
+``elx_conv(desc, output, input, weights, bias)``.  ``Linear``, ``BlockNorm``, ``Route`` and ``Experts`` are the
+operators of transformer blocks, with the same describe / prepare / enqueue protocol.
 
 There is no CPU implementation here.  Importing works without a GPU (the library loads and its
 symbols can be inspected), but every compute call needs an sm_100 device and fails loudly
@@ -27,11 +28,14 @@ ELB_OK, ELB_UNIMPLEMENTED, ELB_GENERAL_ERROR = 0, 1, 2
 ELD_OK, ELD_UNIMPLEMENTED, ELD_GENERAL_ERROR = 0, 1, 2
 ELX_OK, ELX_UNIMPLEMENTED, ELX_GENERAL_ERROR = 0, 1, 2
 CONV_AUTO, CONV_DIRECT_1X1, CONV_DIRECT, CONV_DIRECT_VMG, CONV_WINOGRAD, DECONV_DIRECT = range(6)
-data_type_undef, f32, f16, u8, s8, s32 = range(6)
+data_type_undef, f32, f16, u8, s8, s32, bf16 = range(7)
 (format_undef, nchw, nhwc, nChw16c, nChw8c, oihw, hwio, OIhw16i16o, OIhw8i8o, goihw, ghwio, gOIhw16i16o,
  gOIhw8i8o) = range(13)
 forward_training, forward_inference, backward_data, backward_weights = range(4)
 FINE, COARSE, CALIBRATED = range(3)
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU = range(5)
+NORM_NONE, NORM_RMS, NORM_LAYER = range(3)
+SCORE_SOFTMAX, SCORE_SIGMOID = range(2)
 EL_NO_CALI = 3.4028234663852886e38
 KERNEL_NAMES = {0: "none", 1: "i8_gemm_umma", 2: "i8_conv_umma", 3: "i8_simt", 4: "wino_f32_umma",
                 5: "wino_i8_umma", 6: "i8_depthwise", 7: "f32_direct_umma", 8: "f32_small_ic", 9: "conv_halo"}
@@ -62,6 +66,31 @@ class ElbConvInfo(C.Structure):
                [(k, C.c_uint64) for k in ("size_input", "size_weights", "size_output", "size_bias", "bytes_input",
                                           "bytes_weights", "bytes_output", "bytes_bias", "workspace_bytes")] + \
                [("launches_per_call", C.c_int32), ("launched_kernel", C.c_int32)]
+
+
+class ElbLinearDesc(C.Structure):
+    _fields_ = [(k, C.c_int32) for k in ("ic", "oc", "dt_input", "dt_output", "dt_bias", "fmt_weights", "activation", "gated",
+                                         "with_bias", "with_residual")] + \
+               [("scale", C.c_float), ("device", C.c_int32)] + \
+               [(k, C.c_int64) for k in ("ld_input", "ld_output", "ld_residual")]
+
+
+class ElbNormDesc(C.Structure):
+    _fields_ = [(k, C.c_int32) for k in ("channels", "dt", "dt_residual", "dt_weights", "post", "pre")] + \
+               [(k, C.c_float) for k in ("post_eps", "pre_eps", "weight_offset", "scale")] + \
+               [(k, C.c_int32) for k in ("with_residual", "gate_rows", "device")] + \
+               [(k, C.c_int64) for k in ("ld_input", "ld_residual", "ld_gate", "ld_sum", "ld_output")]
+
+
+class ElbRouteDesc(C.Structure):
+    _fields_ = [(k, C.c_int32) for k in ("experts", "top_k", "dt_logits", "score", "with_bias", "groups", "top_groups",
+                                         "group_best", "renormalise")] + \
+               [("scale", C.c_float), ("device", C.c_int32), ("ld_logits", C.c_int64)]
+
+
+class ElbExpertsDesc(C.Structure):
+    _fields_ = [(k, C.c_int32) for k in ("experts", "top_k", "ic", "mid", "dt", "activation", "gated", "device")] + \
+               [(k, C.c_int64) for k in ("max_rows", "ld_input", "ld_output")]
 
 
 def _load():
@@ -111,6 +140,22 @@ def _load():
         "elb_conv_multi_destroy": (None, [vp]),
         "elb_wino_f32_conv_noalloc": (i32, [C.POINTER(ElbConvDesc), vp, vp, vp, vp, vp]),
         "elb_wino_f32_noalloc_status": (i32, []),
+        "elb_linear_create": (i32, [C.POINTER(ElbLinearDesc), C.POINTER(vp)]),
+        "elb_linear_prepare": (i32, [vp, vp, vp]),
+        "elb_linear_enqueue": (i32, [vp, vp, vp, vp, C.c_int64, vp]),
+        "elb_norm_create": (i32, [C.POINTER(ElbNormDesc), C.POINTER(vp)]),
+        "elb_norm_prepare": (i32, [vp, vp, vp, vp, vp]),
+        "elb_norm_enqueue": (i32, [vp, vp, vp, vp, vp, vp, C.c_int64, vp]),
+        "elb_route_create": (i32, [C.POINTER(ElbRouteDesc), C.POINTER(vp)]),
+        "elb_route_prepare": (i32, [vp, vp]),
+        "elb_route_enqueue": (i32, [vp, vp, vp, vp, C.c_int64, vp]),
+        "elb_experts_create": (i32, [C.POINTER(ElbExpertsDesc), C.POINTER(vp)]),
+        "elb_experts_prepare": (i32, [vp, vp, vp]),
+        "elb_experts_enqueue": (i32, [vp, vp, vp, vp, vp, C.c_int64, vp]),
+        "elb_op_device_status": (i32, [vp]),
+        "elb_op_launch_count": (u64, [vp]),
+        "elb_op_workspace_bytes": (u64, [vp]),
+        "elb_op_destroy": (None, [vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)          # AttributeError here = stale library
@@ -128,7 +173,11 @@ EXPORTED_SYMBOLS = ["elb_conv_sizes", "elb_conv_create", "elb_conv_info", "elb_c
                     "elb_stack_execute", "elb_stack_layer", "elb_stack_sizes", "elb_stack_launch_count",
                     "elb_stack_layer_output", "elb_stack_set_layer_events", "elb_stack_destroy", "elb_conv_multi_create", "elb_conv_multi_execute", "elb_conv_multi_parts",
                     "elb_conv_multi_destroy", "elb_wino_f32_conv_noalloc", "elb_wino_f32_noalloc_status",
-                    "elb_conv_input_step_supported", "elb_conv_enqueue_strided"]
+                    "elb_conv_input_step_supported", "elb_conv_enqueue_strided",
+                    "elb_linear_create", "elb_linear_prepare", "elb_linear_enqueue", "elb_norm_create", "elb_norm_prepare",
+                    "elb_norm_enqueue", "elb_route_create", "elb_route_prepare", "elb_route_enqueue", "elb_experts_create",
+                    "elb_experts_prepare", "elb_experts_enqueue", "elb_op_device_status", "elb_op_launch_count",
+                    "elb_op_workspace_bytes", "elb_op_destroy"]
 
 
 def last_error() -> str:
@@ -420,3 +469,116 @@ class MultiConv:
             self.close()
         except Exception:
             pass
+
+
+def _dev(x):
+    """Address of a device tensor (torch tensor, raw address or None): what the operators' enqueue calls take."""
+    if x is None or type(x) is int:
+        return x
+    if not x.is_cuda:
+        raise ValueError("the operators' enqueue calls take device tensors")
+    return x.data_ptr()
+
+
+class _Op:
+    """A plan of one of the operators of transformer blocks (``elb_op_t``).  ``prepare`` copies the weights (host or
+    device tensors, read once; later calls do nothing), ``enqueue`` runs on ``stream`` (None: the default stream) and
+    returns an ELB_* code; rows of tensors are ``ld_*`` elements apart (0: dense)."""
+    h = None
+
+    def _create(self, create, desc):
+        h = C.c_void_p()
+        rc = create(C.byref(desc), C.byref(h))
+        if rc != ELB_OK:
+            raise RuntimeError(f"rc={rc}: {last_error()}")
+        self.h = h
+
+    def device_status(self) -> int:
+        return lib.elb_op_device_status(self.h)
+
+    def launch_count(self) -> int:
+        return int(lib.elb_op_launch_count(self.h))
+
+    def workspace_bytes(self) -> int:
+        return int(lib.elb_op_workspace_bytes(self.h))
+
+    def close(self):
+        if self.h is not None:
+            lib.elb_op_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class Linear(_Op):
+    """output = residual + scale * act(input weights^T + bias), or scale * act(gate) * up where ``gated`` (weights and bias
+    then hold the oc gate rows, then the oc up rows).  ``dtype``: bf16 or f16 operands; ``out_dtype``: the same or f32."""
+
+    def __init__(self, ic: int, oc: int, dtype: int = bf16, out_dtype: int | None = None, activation: int = ACT_NONE, gated: bool = False,
+                 with_bias: bool = False, bias_dtype: int = f32, with_residual: bool = False, scale: float = 1.0, weights_format: int = oihw,
+                 ld_input: int = 0, ld_output: int = 0, ld_residual: int = 0, device: int = -1):
+        self._create(lib.elb_linear_create, ElbLinearDesc(ic, oc, dtype, dtype if out_dtype is None else out_dtype, bias_dtype, weights_format,
+                                                          activation, int(gated), int(with_bias), int(with_residual), scale, device,
+                                                          ld_input, ld_output, ld_residual))
+
+    def prepare(self, weights, bias=None) -> int:
+        return lib.elb_linear_prepare(self.h, _ptr(weights), _ptr(bias))
+
+    def enqueue(self, output, input, residual=None, *, rows: int, stream=None) -> int:
+        return lib.elb_linear_enqueue(self.h, _dev(output), _dev(input), _dev(residual), rows, stream)
+
+
+class BlockNorm(_Op):
+    """sum = residual + scale * gate * post(input); output = pre(sum): what lies between two blocks.  ``post`` / ``pre``:
+    NORM_*; ``gate_rows``: consecutive rows that share a row of the gate (0: no gate)."""
+
+    def __init__(self, channels: int, dtype: int = bf16, residual_dtype: int | None = None, weights_dtype: int = f32, post: int = NORM_NONE,
+                 pre: int = NORM_RMS, post_eps: float = 1e-6, pre_eps: float = 1e-6, weight_offset: float = 0.0, scale: float = 1.0,
+                 with_residual: bool = True, gate_rows: int = 0, ld_input: int = 0, ld_residual: int = 0, ld_gate: int = 0, ld_sum: int = 0,
+                 ld_output: int = 0, device: int = -1):
+        self._create(lib.elb_norm_create, ElbNormDesc(channels, dtype, dtype if residual_dtype is None else residual_dtype, weights_dtype, post, pre,
+                                                      post_eps, pre_eps, weight_offset, scale, int(with_residual), gate_rows, device,
+                                                      ld_input, ld_residual, ld_gate, ld_sum, ld_output))
+
+    def prepare(self, post_weight=None, post_bias=None, pre_weight=None, pre_bias=None) -> int:
+        return lib.elb_norm_prepare(self.h, _ptr(post_weight), _ptr(post_bias), _ptr(pre_weight), _ptr(pre_bias))
+
+    def enqueue(self, output, sum, input, residual=None, gate=None, *, rows: int, stream=None) -> int:
+        return lib.elb_norm_enqueue(self.h, _dev(output), _dev(sum), _dev(input), _dev(residual), _dev(gate), rows, stream)
+
+
+class Route(_Op):
+    """The top_k experts of each row of logits, best first, and their weights.  ``with_bias``: a bias for balance counts for
+    the choice alone; ``groups`` / ``top_groups`` / ``group_best``: only experts of the groups with the best choices."""
+
+    def __init__(self, experts: int, top_k: int, dtype: int = f32, score: int = SCORE_SOFTMAX, with_bias: bool = False, groups: int = 1,
+                 top_groups: int = 1, group_best: int = 1, renormalise: bool = True, scale: float = 1.0, ld_logits: int = 0, device: int = -1):
+        self._create(lib.elb_route_create, ElbRouteDesc(experts, top_k, dtype, score, int(with_bias), groups, top_groups, group_best,
+                                                        int(renormalise), scale, device, ld_logits))
+
+    def prepare(self, bias=None) -> int:
+        return lib.elb_route_prepare(self.h, _ptr(bias))
+
+    def enqueue(self, ids, weights, logits, *, rows: int, stream=None) -> int:
+        """ids: int32 [rows, top_k], weights: float32 [rows, top_k] or None, both dense."""
+        return lib.elb_route_enqueue(self.h, _dev(ids), _dev(weights), _dev(logits), rows, stream)
+
+
+class Experts(_Op):
+    """output[t] = sum_j weights[t][j] * w_out[e] f(w_in[e] input[t]), e = ids[t][j]; an id outside 0 .. experts - 1 adds
+    nothing.  w_in: [experts, mid (gated: 2 * mid, gate rows first), ic], w_out: [experts, ic, mid]."""
+
+    def __init__(self, experts: int, top_k: int, ic: int, mid: int, max_rows: int, dtype: int = bf16, activation: int = ACT_SILU,
+                 gated: bool = True, ld_input: int = 0, ld_output: int = 0, device: int = -1):
+        self._create(lib.elb_experts_create, ElbExpertsDesc(experts, top_k, ic, mid, dtype, activation, int(gated), device, max_rows,
+                                                            ld_input, ld_output))
+
+    def prepare(self, w_in, w_out) -> int:
+        return lib.elb_experts_prepare(self.h, _ptr(w_in), _ptr(w_out))
+
+    def enqueue(self, output, input, ids, weights, *, rows: int, stream=None) -> int:
+        return lib.elb_experts_enqueue(self.h, _dev(output), _dev(input), _dev(ids), _dev(weights), rows, stream)

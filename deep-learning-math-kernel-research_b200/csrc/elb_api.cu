@@ -69,6 +69,7 @@ int fail(int code, const char *fmt, ...) {
 
 namespace elb {
 void set_last_error(const char *msg) { g_last_error = msg ? msg : ""; }
+int report_failure(int code, const char *msg) { return fail(code, "%s", msg); }
 }  // namespace elb
 
 namespace {

@@ -51,7 +51,8 @@ enum {
   ELB_CONV_WINOGRAD = 4, ELB_DECONV_DIRECT = 5
 };
 /* Element types (include/euler.hpp:66-73). */
-enum { ELB_DT_UNDEF = 0, ELB_F32 = 1, ELB_F16 = 2, ELB_U8 = 3, ELB_S8 = 4, ELB_S32 = 5 };
+enum { ELB_DT_UNDEF = 0, ELB_F32 = 1, ELB_F16 = 2, ELB_U8 = 3, ELB_S8 = 4, ELB_S32 = 5,
+       ELB_BF16 = 6 /* the transformer operators only; not in the reference */ };
 /* Tensor formats (include/euler.hpp:75-89). */
 enum {
   ELB_FMT_UNDEF = 0, ELB_NCHW, ELB_NHWC, ELB_NCHW16C, ELB_NCHW8C, ELB_OIHW, ELB_HWIO, ELB_OIHW16I16O,
@@ -332,6 +333,121 @@ ELB_API int elb_wino_f32_conv_noalloc(const elb_conv_desc_t *desc, void *output,
  * entry point has not run on this device (or the read failed).  Call it after synchronising the
  * stream the convolution ran on; it copies four bytes to the host and allocates nothing. */
 ELB_API int elb_wino_f32_noalloc_status(void);
+
+/* ---- Operators of transformer blocks --------------------------------------------------------
+ * No counterpart in the reference, whose matrix products are 1x1 convolutions over images.  The
+ * feed-forward half of a transformer block, dense or routed to experts, for inference: four operators
+ * with one protocol, the convolution plans' own: create from a description, prepare once (weights are
+ * copied, converted and laid out; the caller's tensors are not read again, a second prepare does
+ * nothing), enqueue often.  One opaque object serves all four.
+ *
+ * enqueue: tensors are DEVICE memory of the plan's device, output first; work is enqueued on
+ * cuda_stream (NULL = default stream) and not waited for; rows may differ from call to call, and 0
+ * rows is a call that does nothing.  Rows of a tensor are ld elements apart (0 in the description: dense).
+ * Tensors need the alignment of their type only; 16-byte aligned tensors whose rows are multiples of
+ * 16 bytes are read without a copy.  An output may be the residual's tensor (the same address and ld);
+ * no other tensors of a call may overlap an output.  prepare: host or device tensors; it waits for the device.
+ * Calls may be captured in a CUDA graph if the plan is prepared and a call of as many rows has been
+ * made before.  A plan with workspace orders its own calls across streams (not inside a capture, nor between a
+ * captured graph and other calls: those the caller orders). */
+typedef struct elb_op elb_op_t;
+
+enum { ELB_ACT_NONE = 0, ELB_ACT_RELU = 1, ELB_ACT_GELU = 2 /* z Phi(z) */, ELB_ACT_GELU_TANH = 3 /* its tanh form */,
+       ELB_ACT_SILU = 4 /* z / (1 + exp(-z)) */ };
+enum { ELB_NORM_NONE = 0, ELB_NORM_RMS = 1 /* v / sqrt(mean(v^2) + eps) * w + b */,
+       ELB_NORM_LAYER = 2 /* (v - mean) / sqrt(var + eps) * w + b */ };
+enum { ELB_SCORE_SOFTMAX = 0, ELB_SCORE_SIGMOID = 1 };
+
+/* output[t][o] = residual[t][o] + scale * act(z[t][o]),  z[t][o] = bias[o] + sum_i input[t][i] * weights[o][i]
+ * gated: weights and bias hold 2 * oc rows, z of the gate in the first oc, u in the others: scale * act(z) * u.
+ * Products are accumulated in 32 bits, everything up to the output's one rounding is done in 32 bits. */
+typedef struct elb_linear_desc {
+  int32_t ic, oc;                                 /* input and output channels */
+  int32_t dt_input;                               /* ELB_BF16 or ELB_F16; the weights' type too */
+  int32_t dt_output;                              /* dt_input or ELB_F32; the residual's type too */
+  int32_t dt_bias;                                /* ELB_F32 or dt_input */
+  int32_t fmt_weights;                            /* ELB_OIHW: [rows][ic]; ELB_HWIO: [ic][rows] */
+  int32_t activation, gated, with_bias, with_residual;
+  float scale;
+  int32_t device;                                 /* CUDA device ordinal; -1 = current device */
+  int64_t ld_input, ld_output, ld_residual;       /* elements between rows; 0 = dense */
+} elb_linear_desc_t;
+ELB_API int elb_linear_create(const elb_linear_desc_t *desc, elb_op_t **op);
+ELB_API int elb_linear_prepare(elb_op_t *op, const void *weights, const void *bias);
+ELB_API int elb_linear_enqueue(elb_op_t *op, void *output, const void *input, const void *residual, int64_t rows,
+                               void *cuda_stream);
+
+/* What lies between two blocks:
+ *   sum[t] = residual[t] + scale * gate[t / gate_rows] * post(input[t]);   output[t] = pre(sum[t])
+ * post is the norm behind the block that has just run (ELB_NORM_NONE: its output as it is), pre the one in
+ * front of the next block (ELB_NORM_NONE: no output is written).  without residual: sum = scale * gate * post(input).
+ * Statistics and everything between them are held in 32 bits; output is computed from the unrounded sum. */
+typedef struct elb_norm_desc {
+  int32_t channels;                               /* 1 .. 32768 */
+  int32_t dt;                                     /* input, gate, output: ELB_F32, ELB_F16 or ELB_BF16 */
+  int32_t dt_residual;                            /* residual and sum: dt or ELB_F32 */
+  int32_t dt_weights;                             /* the norms' weights and biases: ELB_F32 or dt */
+  int32_t post, pre;                              /* ELB_NORM_* */
+  float post_eps, pre_eps, weight_offset;         /* weight_offset: norms multiply by weight_offset + w */
+  float scale;
+  int32_t with_residual, gate_rows;               /* gate_rows: consecutive rows sharing a row of the gate; 0 = no gate */
+  int32_t device;
+  int64_t ld_input, ld_residual, ld_gate, ld_sum, ld_output;
+} elb_norm_desc_t;
+ELB_API int elb_norm_create(const elb_norm_desc_t *desc, elb_op_t **op);
+/* NULL weights are ones, NULL biases zeros. */
+ELB_API int elb_norm_prepare(elb_op_t *op, const void *post_weight, const void *post_bias, const void *pre_weight,
+                             const void *pre_bias);
+/* output may be NULL where pre is ELB_NORM_NONE, sum where the caller does not need it. */
+ELB_API int elb_norm_enqueue(elb_op_t *op, void *output, void *sum, const void *input, const void *residual,
+                             const void *gate, int64_t rows, void *cuda_stream);
+
+/* Routing: of each row of logits the top_k experts, best first, and their weights.
+ *   score = softmax(logits) or sigmoid(logits); choice = score + bias (bias is for the choice alone)
+ *   groups > 1: an expert is open if its group is among the top_groups best by the sum of its group_best best
+ *   choices; ids = the top_k open experts of the largest choice, ties to the lowest index (groups as well)
+ *   weights = scale * score[ids], divided by their sum first where renormalise is set (a sum of 0 gives weights of 0)
+ * A NaN among the logits counts as -inf; +inf takes softmax's whole weight (shared with others of its row).  Without a bias softmax chooses by
+ * exp(logit - max), which has the order of the scores. */
+typedef struct elb_route_desc {
+  int32_t experts, top_k;                         /* 1 .. 1024; 1 .. 32 */
+  int32_t dt_logits;                              /* ELB_F32, ELB_F16 or ELB_BF16 */
+  int32_t score;                                  /* ELB_SCORE_* */
+  int32_t with_bias, groups, top_groups, group_best;   /* groups divides experts, 1 .. 32; group_best: 1 or 2 */
+  int32_t renormalise;
+  float scale;
+  int32_t device;
+  int64_t ld_logits;
+} elb_route_desc_t;
+ELB_API int elb_route_create(const elb_route_desc_t *desc, elb_op_t **op);
+ELB_API int elb_route_prepare(elb_op_t *op, const float *bias);
+/* ids: int32 [rows][top_k], weights: float [rows][top_k] (NULL: not wanted), dense. */
+ELB_API int elb_route_enqueue(elb_op_t *op, int32_t *ids, float *weights, const void *logits, int64_t rows, void *cuda_stream);
+
+/* The experts' products:  output[t] = sum_j weights[t][j] * W_out[e] * f(W_in[e] * input[t]),  e = ids[t][j]
+ * f is the activation of mid channels; gated: W_in has 2 * mid rows, gate first, as in elb_linear.  The middle
+ * tensor is held in dt, the sum over j in 32 bits.  An id outside 0 .. experts - 1 is a slot that adds nothing. */
+typedef struct elb_experts_desc {
+  int32_t experts, top_k;                         /* 1 .. 1024; 1 .. 32 */
+  int32_t ic, mid;
+  int32_t dt;                                     /* ELB_BF16 or ELB_F16: input, both weights, middle, output */
+  int32_t activation, gated;
+  int32_t device;
+  int64_t max_rows;                               /* the workspace is made for calls of so many rows */
+  int64_t ld_input, ld_output;
+} elb_experts_desc_t;
+ELB_API int elb_experts_create(const elb_experts_desc_t *desc, elb_op_t **op);
+/* w_in: [experts][mid or 2 * mid][ic], w_out: [experts][ic][mid] */
+ELB_API int elb_experts_prepare(elb_op_t *op, const void *w_in, const void *w_out);
+ELB_API int elb_experts_enqueue(elb_op_t *op, void *output, const void *input, const int32_t *ids, const float *weights,
+                                int64_t rows, void *cuda_stream);
+
+/* 0 = every finished call of the plan was well; otherwise the code of the bounded wait that gave up (see
+ * elb_conv_device_status).  Waits for the device; -1: it could not. */
+ELB_API int elb_op_device_status(elb_op_t *op);
+ELB_API uint64_t elb_op_launch_count(const elb_op_t *op);
+ELB_API uint64_t elb_op_workspace_bytes(const elb_op_t *op);   /* device memory the plan holds, weights included */
+ELB_API void elb_op_destroy(elb_op_t *op);
 
 #ifdef __cplusplus
 }
