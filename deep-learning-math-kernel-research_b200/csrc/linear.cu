@@ -1,8 +1,13 @@
 // Matrix products of the transformer operators, dense and grouped by expert, on packed weights (ops.cuh).
 #include "elb_common.cuh"
 #include "ops.cuh"
+#include "umma.cuh"
 
 namespace elb {
+
+// Bytes of the operand rings.  The kernel of few tiles leaves room for a second CTA on its SM: of its own launch, or of the next
+// one, whose weights then arrive while this one ends.
+constexpr int SPLIT_RING = 110 * 1024, TILES_RING = 224 * 1024;
 
 namespace {
 
@@ -44,48 +49,390 @@ __global__ void pack_bias_kernel(float *dst, const void *src, int et, int rows, 
   dst[p] = v;
 }
 
-// The plain form on CUDA cores: a block multiplies 128 packed rows (one per thread) by up to 16 tokens, whose channels lie in
-// shared memory as fp32, tile by tile of 64.
-__global__ void __launch_bounds__(GT_ROWS) gemm_simple_kernel(const GemmParams p) {
-  __shared__ float xt[GEMM_TOKENS][GT_K];
-  const int row_tile = blockIdx.x % p.row_tiles, tt = blockIdx.x / p.row_tiles;
-  int tok0 = tt * GEMM_TOKENS, ntok = min(GEMM_TOKENS, p.rows - tok0);
-  const uint8_t *w = p.w;
-  if (p.tiles) {
-    if (tt >= *p.n_tiles) return;
-    const GroupTile g = p.tiles[tt];
-    tok0 = g.row0;
-    ntok = g.count;
-    w += g.expert * p.w_stride;
-  }
-  w += (size_t)row_tile * p.kt * GT_BYTES;
-  const uint16_t *x = static_cast<const uint16_t *>(p.x) + (long long)tok0 * p.ld_x;
-  const int r = threadIdx.x;
-  float acc[GEMM_TOKENS] = {};
-  auto value = [&](uint16_t b) {
-    return p.in_et == ET_BF16 ? __uint_as_float((uint32_t)b << 16) : __half2float(__ushort_as_half(b));
-  };
-  for (int kt = 0; kt < p.kt; ++kt) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < GEMM_TOKENS * GT_K; i += GT_ROWS) {
-      const int t = i / GT_K, k = i % GT_K;
-      xt[t][k] = t < ntok && kt * GT_K + k < p.ic ? value(x[t * p.ld_x + kt * GT_K + k]) : 0.0f;
+// ---------------------------------------------------------------------------------------------
+// The tensor-core kernels.  Left operand (128 rows, tensor memory lanes): a tile of packed weights, one contiguous bulk copy of
+// 16 KB per 64 channels.  Right operand (BN columns): BN tokens, one tiled copy with the 128-byte swizzle from the caller's
+// tensor (rows and channels outside it arrive as zeros).  Few tokens then cost a narrow MMA and not a padded one, and the
+// weights, which are what a small call is made of, stream through shared memory once.
+// ---------------------------------------------------------------------------------------------
+constexpr int EPI_WARPS = 8, THREADS = (4 + EPI_WARPS) * 32;   // warp 0 producer, 1 MMA, 2 and 3 idle, 4 to 11 epilogue
+
+template <int BN, bool PAIR, int RING>
+struct GemmSmem {
+  static constexpr int X_BYTES = (PAIR ? BN / 2 : BN) * 128;
+  static constexpr int STAGE = GT_BYTES + X_BYTES;
+  static constexpr int STAGES = RING / STAGE;
+  static constexpr int BAR_OFF = STAGES * STAGE;              // full[S], empty[S], tfull[2], tempty[2]
+  static constexpr int MISC_OFF = BAR_OFF + (2 * STAGES + 4) * 8;
+  static constexpr int TOTAL = MISC_OFF + 16 + 1024;          // tmem slot, abort flag; room to align
+};
+
+struct alignas(64) GemmLaunch {
+  CUtensorMap xmap, wmap;      // tokens; packed weights as rows of 128 bytes (pairs only)
+  GemmParams p;
+  int splits;                  // CTAs of a cluster that share a tile's channels
+  int token_tiles, band;       // band: token tiles that neighbouring tiles of the walk share weights over
+};
+
+__device__ __forceinline__ uint8_t *smem_1k(uint8_t *base) { return base + ((1024u - (smem_u32(base) & 1023u)) & 1023u); }
+
+// One tile of BN tokens: accumulator columns of this warp's quarter of the lanes, 16 at a time (the warp of `half` takes every
+// second block); `release` runs when the last of them has been read.
+template <int BN, typename F>
+__device__ __forceinline__ void epilogue_tile(const Epilogue &e, uint32_t taddr, int half, int prow, long long tok0, int ntok, F release) {
+  constexpr int BLOCKS = BN / 16;
+  uint32_t a[16], b[16];
+  float v[16];
+  int k = half;
+  if (k < BLOCKS) tmem_ld16(taddr + k * 16, a);
+#pragma unroll 1
+  for (; k < BLOCKS; k += 4) {
+    tmem_ld_wait16(a);
+    if (k + 2 < BLOCKS) tmem_ld16(taddr + (k + 2) * 16, b);
+    else release();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(a[i]);
+    if (k * 16 < ntok) emit<16>(e, v, prow, tok0 + k * 16, ntok - k * 16);
+    if (k + 2 < BLOCKS) {
+      tmem_ld_wait16(b);
+      if (k + 4 < BLOCKS) tmem_ld16(taddr + (k + 4) * 16, a);
+      else release();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(b[i]);
+      if ((k + 2) * 16 < ntok) emit<16>(e, v, prow, tok0 + (k + 2) * 16, ntok - (k + 2) * 16);
     }
-    __syncthreads();
-    const uint4 *wr = reinterpret_cast<const uint4 *>(w + (size_t)kt * GT_BYTES + r * 128);
-    for (int c = 0; c < 8; ++c) {
-      const uint4 q = wr[c ^ (r & 7)];
-      const uint32_t words[4] = {q.x, q.y, q.z, q.w};
+  }
+  if (half >= BLOCKS) release();
+}
+
+// ---- Few tiles: each belongs to a cluster of CTAs that share its channels.  The partial sums are brought together through
+// distributed shared memory in the order of the ranks, each CTA finishing a part of the tokens.
+template <int BN>
+__global__ void __launch_bounds__(THREADS) gemm_split_kernel(const __grid_constant__ GemmLaunch g) {
+  using L = GemmSmem<BN, false, SPLIT_RING>;
+  constexpr int STAGES = L::STAGES;
+  constexpr uint32_t COLS = BN < 32 ? 32 : BN;
+  static_assert(BN * GT_ROWS * 4 <= L::BAR_OFF, "the partial sums lie in the ring");
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = smem_1k(smem_raw);
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::BAR_OFF), *empty = full + STAGES, *tfull = empty + STAGES;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + L::MISC_OFF);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::MISC_OFF + 4);
+  const GemmParams &p = g.p;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int splits = g.splits, rank = splits > 1 ? (int)cluster_ctarank() : 0;
+  const int tile = blockIdx.x / splits, row_tile = tile % p.row_tiles, tt = tile / p.row_tiles;
+  const int k0 = (int)((long long)p.kt * rank / splits), k1 = (int)((long long)p.kt * (rank + 1) / splits), steps = k1 - k0;
+  const int tok0 = tt * BN, ntok = min(BN, p.rows - tok0);
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&g.xmap);
+    for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    mbar_init(tfull, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    fence_proxy_async_smem();
+  }
+  __syncthreads();
+  if (warp == 1 || warp >= 4) {
+    // Tensor memory is taken when the kernel before this one has ended, and the kernel behind may start when it has been
+    // taken: of two kernels on an SM, one that holds tensor memory never waits for one that still wants some.
+    griddep_wait();
+    if (warp == 1) {
+      tmem_alloc(tmem_slot, COLS);
+      griddep_launch_dependents();
+    }
+    tc_fence_before_sync();
+    named_bar_sync(1, (1 + EPI_WARPS) * 32);
+    tc_fence_after_sync();
+  }
+  const uint32_t tmem = warp == 0 ? 0u : *tmem_slot;
+  int fail_code = 0;
+  if (warp == 0) {
+    const uint32_t el = elect_one();
+    const uint8_t *w = p.w + ((size_t)row_tile * p.kt + k0) * GT_BYTES;
+    // the weights are the plan's own: their first copies need not wait for the kernel before this one
+    const int ahead = min(STAGES, steps);
+    if (el)
+      for (int i = 0; i < ahead; ++i) {
+        mbar_arrive_expect_tx(&full[i], L::STAGE);
+        tma_bulk_g2s(smem + i * L::STAGE, w + (size_t)i * GT_BYTES, GT_BYTES, &full[i]);
+      }
+    griddep_wait();
+    for (int i = 0; i < steps; ++i) {
+      const int s = i % STAGES;
+      if (i >= ahead) {
+        if (!mbar_wait_warp(&empty[s], ((i / STAGES) & 1) ^ 1, abort_flag)) { fail_code = ST_WAIT_TIMEOUT_PRODUCER; break; }
+        if (el) {
+          mbar_arrive_expect_tx(&full[s], L::STAGE);
+          tma_bulk_g2s(smem + s * L::STAGE, w + (size_t)i * GT_BYTES, GT_BYTES, &full[s]);
+        }
+      }
+      if (el) tma_tile_2d(smem + s * L::STAGE + GT_BYTES, &g.xmap, (k0 + i) * GT_K, tok0, &full[s]);
+    }
+  } else if (warp == 1) {
+    const uint32_t el = elect_one();
+    const uint32_t idesc = umma_idesc(1, p.in_et == ET_BF16, p.in_et == ET_BF16, GT_ROWS, BN);
+    bool ok = true;
+    for (int i = 0; i < steps; ++i) {
+      const int s = i % STAGES;
+      if (!mbar_wait_warp(&full[s], (i / STAGES) & 1, abort_flag)) { fail_code = ST_WAIT_TIMEOUT_MMA; ok = false; break; }
+      tc_fence_after_sync();
+      const uint32_t a = smem_u32(smem + s * L::STAGE);
+      const uint64_t ad = umma_desc_sw128(a), bd = umma_desc_sw128(a + GT_BYTES);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float wv = value((uint16_t)(words[j >> 1] >> (16 * (j & 1))));
+      for (int k = 0; k < GT_K / 16; ++k) umma_f16_el(tmem, ad + k * 2, bd + k * 2, idesc, (i | k) != 0, el);
+      umma_commit_el(&empty[s], el);
+    }
+    if (ok) umma_commit_el(tfull, el);
+  }
+  const int quarter = warp & 3, half = (warp - 4) >> 2, prow = row_tile * GT_ROWS + quarter * 32 + lane;
+  const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+  float *part = reinterpret_cast<float *>(smem);              // [token][128 rows]
+  bool ok = true;
+  if (warp >= 4) {
+    ok = mbar_wait_warp(tfull, 0, abort_flag);
+    if (!ok) fail_code = ST_WAIT_TIMEOUT_EPILOGUE;
+    tc_fence_after_sync();
+    if (ok && splits == 1) epilogue_tile<BN>(p.epi, taddr, half, prow, tok0, ntok, [] {});
+    if (ok && splits > 1) {
+#pragma unroll 1
+      for (int k = half; k < BN / 16; k += 2) {
+        uint32_t a[16];
+        tmem_ld16(taddr + k * 16, a);
+        tmem_ld_wait16(a);
 #pragma unroll
-        for (int t = 0; t < GEMM_TOKENS; ++t) acc[t] = fmaf(wv, xt[t][c * 8 + j], acc[t]);
+        for (int i = 0; i < 16; ++i) part[(k * 16 + i) * GT_ROWS + quarter * 32 + lane] = __uint_as_float(a[i]);
       }
     }
   }
-  emit<GEMM_TOKENS>(p.epi, acc, row_tile * GT_ROWS + r, tok0, ntok);
+  if (splits > 1) {
+    __syncwarp();
+    cluster_sync_all();
+    const int share = BN / splits, per = share >= 4 ? share / 2 : share;      // tokens of this CTA, and of one of its warps
+    if (warp >= 4 && half * per < share) {
+      for (int t = rank * share + half * per; t < rank * share + half * per + per && t < ntok; t += 2) {
+        float v[2] = {0.0f, 0.0f};
+        const uint32_t at = smem_u32(part + t * GT_ROWS + quarter * 32 + lane);
+#pragma unroll 1
+        for (int r = 0; r < splits; ++r) {
+          uint32_t from;
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from) : "r"(at), "r"(r));
+          float x, y;
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(from) : "memory");
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(y) : "r"(from + GT_ROWS * 4) : "memory");
+          v[0] += x;
+          v[1] += y;
+        }
+        emit<2>(p.epi, v, prow, tok0 + t, ntok - t);
+      }
+    }
+    __syncwarp();
+    cluster_sync_all();                                       // nobody leaves while its partial sums are read
+  }
+  if (fail_code != 0) report_status(p.status, fail_code);
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  if (warp == 1) tmem_dealloc(tmem, COLS);
 }
+
+// ---- Many tiles: persistent CTAs, or pairs of them (PAIR: one tcgen05.mma.cta_group::2 for 256 packed rows, each CTA
+// holding its 128 and half of the tokens), two accumulators, so that a tile's epilogue runs beside the next one's products.
+template <int BN, bool PAIR, bool GROUPED>
+__global__ void __launch_bounds__(THREADS, 1) gemm_tiles_kernel(const __grid_constant__ GemmLaunch g) {
+  using L = GemmSmem<BN, PAIR, TILES_RING>;
+  constexpr int STAGES = L::STAGES, CTAS = PAIR ? 2 : 1;
+  constexpr uint32_t COLS = 2 * BN;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = smem_1k(smem_raw);
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::BAR_OFF), *empty = full + STAGES, *tfull = empty + STAGES, *tempty = tfull + 2;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + L::MISC_OFF);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::MISC_OFF + 4);
+  const GemmParams &p = g.p;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = PAIR ? (int)cluster_ctarank() : 0;
+  const int row_steps = (p.row_tiles + CTAS - 1) / CTAS;      // tiles along the rows, of one or two row tiles
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&g.xmap);
+    if (PAIR) tma_prefetch_desc(&g.wmap);
+    for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int b = 0; b < 2; ++b) { mbar_init(&tfull[b], 1); mbar_init(&tempty[b], CTAS * EPI_WARPS); }
+    *abort_flag = 0;
+    fence_barrier_init();
+    fence_proxy_async_smem();
+  }
+  griddep_wait();                                             // (before tensor memory is taken, see gemm_split_kernel)
+  if (warp == 1) { if (PAIR) tmem_alloc2(tmem_slot, COLS); else tmem_alloc(tmem_slot, COLS); }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (PAIR) cluster_sync_all();
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  griddep_launch_dependents();
+  const int token_tiles = GROUPED ? *p.n_tiles : g.token_tiles;
+  const int total = token_tiles * row_steps;
+  const int first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
+  struct Tile { int expert, row_tile, tok0, ntok; };
+  auto tile_of = [&](int i) {
+    Tile t;
+    if (GROUPED) {
+      const GroupTile q = p.tiles[i / row_steps];
+      t.expert = q.expert;
+      t.tok0 = q.row0;
+      t.ntok = q.count;
+      t.row_tile = (i % row_steps) * CTAS + rank;
+    } else {
+      // bands of token tiles: inside one the walk goes down the rows, so that the CTAs at work share tokens and weights in L2
+      const int per = g.band * row_steps, b = i / per, in = i - b * per;
+      const int width = min(g.band, token_tiles - b * g.band);
+      t.expert = 0;
+      t.row_tile = in / width * CTAS + rank;
+      t.tok0 = (b * g.band + in % width) * BN;
+      t.ntok = min(BN, p.rows - t.tok0);
+    }
+    return t;
+  };
+  int fail_code = 0;
+  if (warp == 0) {
+    const uint32_t el = elect_one();
+    uint32_t it = 0;
+    bool ok = true;
+    for (int i = first; i < total && ok; i += step) {
+      const Tile t = tile_of(i);
+      const int rt = min(t.row_tile, p.row_tiles - 1);         // (the second of a pair may lie past the last tile)
+      const uint8_t *w = p.w + t.expert * p.w_stride + (size_t)rt * p.kt * GT_BYTES;
+      const int wrow = PAIR ? (int)((t.expert * p.w_stride / GT_BYTES + (size_t)rt * p.kt) * GT_ROWS) : 0;
+      for (int k = 0; k < p.kt; ++k, ++it) {
+        const int s = it % STAGES;
+        if (!mbar_wait_warp(&empty[s], ((it / STAGES) & 1) ^ 1, abort_flag)) { ok = false; fail_code = ST_WAIT_TIMEOUT_PRODUCER; break; }
+        uint8_t *dst = smem + s * L::STAGE;
+        if (el) {
+          if (PAIR) {
+            const uint32_t bar = mapa_u32(&full[s], 0);
+            if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * L::STAGE);
+            tma_tile_2d_pair(dst, &g.wmap, 0, wrow + k * GT_ROWS, bar);
+            tma_tile_2d_pair(dst + GT_BYTES, &g.xmap, k * GT_K, t.tok0 + rank * (BN / 2), bar);
+          } else {
+            mbar_arrive_expect_tx(&full[s], L::STAGE);
+            tma_bulk_g2s(dst, w + (size_t)k * GT_BYTES, GT_BYTES, &full[s]);
+            tma_tile_2d(dst + GT_BYTES, &g.xmap, k * GT_K, t.tok0, &full[s]);
+          }
+        }
+        __syncwarp();
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0) {
+      const uint32_t el = elect_one();
+      const uint32_t idesc = umma_idesc(1, p.in_et == ET_BF16, p.in_et == ET_BF16, GT_ROWS * CTAS, BN);
+      uint32_t it = 0, count = 0;
+      bool ok = true;
+      for (int i = first; i < total && ok; i += step, ++count) {
+        const uint32_t b = count & 1;
+        if (!mbar_wait_warp(&tempty[b], ((count >> 1) & 1) ^ 1, abort_flag)) { fail_code = ST_WAIT_TIMEOUT_MMA; break; }
+        tc_fence_after_sync();
+        const uint32_t d = tmem + b * BN;
+        for (int k = 0; k < p.kt; ++k, ++it) {
+          const int s = it % STAGES;
+          if (!mbar_wait_warp(&full[s], (it / STAGES) & 1, abort_flag)) { ok = false; fail_code = ST_WAIT_TIMEOUT_MMA; break; }
+          tc_fence_after_sync();
+          const uint32_t a = smem_u32(smem + s * L::STAGE);
+          const uint64_t ad = umma_desc_sw128(a), bd = umma_desc_sw128(a + GT_BYTES);
+#pragma unroll
+          for (int j = 0; j < GT_K / 16; ++j) {
+            if (PAIR) umma_f16_2cta_el(d, ad + j * 2, bd + j * 2, idesc, (k | j) != 0, el);
+            else umma_f16_el(d, ad + j * 2, bd + j * 2, idesc, (k | j) != 0, el);
+          }
+          if (PAIR) umma_commit_2cta_el(&empty[s], el);
+          else umma_commit_el(&empty[s], el);
+        }
+        if (ok) { if (PAIR) umma_commit_2cta_el(&tfull[b], el); else umma_commit_el(&tfull[b], el); }
+      }
+    }
+  } else if (warp >= 4) {
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    uint32_t count = 0;
+    for (int i = first; i < total; i += step, ++count) {
+      const Tile t = tile_of(i);
+      const uint32_t b = count & 1;
+      if (!mbar_wait_warp(&tfull[b], (count >> 1) & 1, abort_flag)) { fail_code = ST_WAIT_TIMEOUT_EPILOGUE; break; }
+      tc_fence_after_sync();
+      epilogue_tile<BN>(p.epi, tmem + (static_cast<uint32_t>(quarter * 32) << 16) + b * BN, half, t.row_tile * GT_ROWS + quarter * 32 + lane, t.tok0,
+                        t.ntok, [&] {
+                          tc_fence_before_sync();
+                          __syncwarp();
+                          if (lane == 0) { if (PAIR) mbar_arrive_cluster(mapa_u32(&tempty[b], 0)); else mbar_arrive(&tempty[b]); }
+                        });
+    }
+  }
+  __syncwarp();
+  if (fail_code != 0) report_status(p.status, fail_code);
+  tc_fence_before_sync();
+  __syncthreads();
+  if (PAIR) cluster_sync_all();
+  tc_fence_after_sync();
+  if (warp == 1) { if (PAIR) tmem_dealloc2(tmem, COLS); else tmem_dealloc(tmem, COLS); }
+}
+
+// Rows of any alignment -> rows that a tiled copy can read
+__global__ void align_rows_kernel(uint16_t *dst, long long pitch, const uint16_t *src, long long ld, int rows, int n) {
+  griddep_launch_dependents();
+  griddep_wait();
+  for (long long r = blockIdx.x; r < rows; r += gridDim.x)
+    for (int i = threadIdx.x; i < n; i += blockDim.x) dst[r * pitch + i] = src[r * ld + i];
+}
+
+bool encode_rows(CUtensorMap *m, int et, const void *base, long long inner, long long rows, long long pitch_bytes, int box_inner, int box_rows,
+                 bool swizzle) {
+  PFN_encodeTiled fn = get_encode_tiled();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch_bytes};
+  const cuuint32_t box[2] = {(cuuint32_t)box_inner, (cuuint32_t)box_rows}, one[2] = {1, 1};
+  return fn(m, et == ET_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void *>(base), dims, strides, box, one,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename K>
+cudaError_t launch_gemm_kernel(K kern, const GemmLaunch &g, int grid, int smem, int cluster, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = cluster; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, g);
+}
+
+template <int BN>
+cudaError_t go_split(GemmLaunch &g, cudaStream_t s) {
+  using L = GemmSmem<BN, false, SPLIT_RING>;
+  if (!encode_rows(&g.xmap, g.p.in_et, g.p.x, g.p.ic, g.p.rows, g.p.ld_x * 2, GT_K, BN, true)) return cudaErrorInvalidValue;
+  return launch_gemm_kernel(gemm_split_kernel<BN>, g, g.p.row_tiles * g.token_tiles * g.splits, L::TOTAL, g.splits, s);
+}
+
+template <int BN, bool PAIR, bool GROUPED>
+cudaError_t go_tiles(GemmLaunch &g, cudaStream_t s) {
+  using L = GemmSmem<BN, PAIR, TILES_RING>;
+  const GemmParams &p = g.p;
+  const int ctas = PAIR ? 2 : 1, row_steps = (p.row_tiles + ctas - 1) / ctas;
+  if (!encode_rows(&g.xmap, p.in_et, p.x, p.ic, p.rows, p.ld_x * 2, GT_K, PAIR ? BN / 2 : BN, true)) return cudaErrorInvalidValue;
+  if (PAIR && !encode_rows(&g.wmap, p.in_et, p.w, GT_K, p.w_rows, 128, GT_K, GT_ROWS, false)) return cudaErrorInvalidValue;
+  g.token_tiles = p.tiles ? p.max_tiles : (p.rows + BN - 1) / BN;
+  const long long tiles = (long long)g.token_tiles * row_steps;
+  const int most = PAIR ? p.max_pairs : p.num_sms;
+  const int grid = (int)(tiles < most ? tiles : most) * ctas;
+  return launch_gemm_kernel(gemm_tiles_kernel<BN, PAIR, GROUPED>, g, grid, L::TOTAL, ctas, s);
+}
+
+template <typename K>
+cudaError_t allow(K kern, int smem) { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); }
 
 }  // namespace
 
@@ -103,11 +450,74 @@ cudaError_t launch_pack_bias(float *dst, const void *src, int et, int rows, int 
   return cudaGetLastError();
 }
 
-cudaError_t launch_gemm(const GemmParams &p, int num_sms, cudaStream_t s) {
-  (void)num_sms;
-  const long long tt = p.tiles ? p.max_tiles : (p.rows + GEMM_TOKENS - 1) / GEMM_TOKENS;
-  gemm_simple_kernel<<<(unsigned)(tt * p.row_tiles), GT_ROWS, 0, s>>>(p);
-  return cudaGetLastError();
+cudaError_t launch_align_rows(void *dst, long long pitch, const void *src, long long ld, int rows, int n, cudaStream_t s) {
+  return launch_overlapped(align_rows_kernel, dim3(rows < 148 * 16 ? rows : 148 * 16), dim3(256), 0, s, static_cast<uint16_t *>(dst), pitch,
+                           static_cast<const uint16_t *>(src), ld, rows, n);
+}
+
+// Kernel attributes are a device's: once for each plan.  max_pairs: the pairs of CTAs that the device holds at once (a
+// persistent kernel with more would have them run one after the other).
+cudaError_t init_gemm(int num_sms, int *max_pairs) {
+  cudaError_t e = cudaSuccess;
+  auto want = [&](cudaError_t r) { if (e == cudaSuccess) e = r; };
+  want(allow(gemm_split_kernel<16>, GemmSmem<16, false, SPLIT_RING>::TOTAL));
+  want(allow(gemm_split_kernel<32>, GemmSmem<32, false, SPLIT_RING>::TOTAL));
+  want(allow(gemm_split_kernel<64>, GemmSmem<64, false, SPLIT_RING>::TOTAL));
+  want(allow(gemm_split_kernel<128>, GemmSmem<128, false, SPLIT_RING>::TOTAL));
+  want(allow(gemm_tiles_kernel<128, true, false>, GemmSmem<128, true, TILES_RING>::TOTAL));
+  want(allow(gemm_tiles_kernel<256, true, false>, GemmSmem<256, true, TILES_RING>::TOTAL));
+  want(allow(gemm_tiles_kernel<16, false, true>, GemmSmem<16, false, TILES_RING>::TOTAL));
+  want(allow(gemm_tiles_kernel<32, false, true>, GemmSmem<32, false, TILES_RING>::TOTAL));
+  want(allow(gemm_tiles_kernel<64, false, true>, GemmSmem<64, false, TILES_RING>::TOTAL));
+  want(allow(gemm_tiles_kernel<128, false, true>, GemmSmem<128, false, TILES_RING>::TOTAL));
+  want(allow(gemm_tiles_kernel<256, true, true>, GemmSmem<256, true, TILES_RING>::TOTAL));
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(num_sms / 2 * 2);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = GemmSmem<256, true, TILES_RING>::TOTAL;
+  cudaLaunchAttribute at = {};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = 2; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  e = cudaOccupancyMaxActiveClusters(max_pairs, gemm_tiles_kernel<256, true, false>, &cfg);
+  if (e == cudaSuccess && *max_pairs < 1) e = cudaErrorInvalidConfiguration;
+  return e;
+}
+
+int grouped_tile_tokens(int slots, int experts) {
+  const int mean = (slots + experts - 1) / experts;
+  return mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : mean <= 128 ? 128 : 256;
+}
+
+cudaError_t launch_gemm(const GemmParams &p, cudaStream_t s) {
+  GemmLaunch g;
+  g.p = p;
+  g.splits = 1;
+  g.band = 8;
+  g.token_tiles = 0;
+  if (p.tiles) {
+    switch (p.tile_tokens) {
+      case 16: return go_tiles<16, false, true>(g, s);
+      case 32: return go_tiles<32, false, true>(g, s);
+      case 64: return go_tiles<64, false, true>(g, s);
+      case 128: return go_tiles<128, false, true>(g, s);
+      default: return go_tiles<256, true, true>(g, s);
+    }
+  }
+  const int bn = p.rows <= 16 ? 16 : p.rows <= 32 ? 32 : p.rows <= 64 ? 64 : 128;
+  g.token_tiles = (p.rows + bn - 1) / bn;
+  const long long tiles = (long long)p.row_tiles * g.token_tiles;
+  if (tiles <= p.num_sms || bn < 128) {
+    while (g.splits < 8 && tiles * g.splits * 2 <= p.num_sms && p.kt >= g.splits * 4) g.splits *= 2;
+    if (bn == 16) return go_split<16>(g, s);
+    if (bn == 32) return go_split<32>(g, s);
+    if (bn == 64) return go_split<64>(g, s);
+    return go_split<128>(g, s);
+  }
+  if (tiles <= 4 * p.num_sms) return go_tiles<128, true, false>(g, s);
+  return go_tiles<256, true, false>(g, s);
 }
 
 }  // namespace elb

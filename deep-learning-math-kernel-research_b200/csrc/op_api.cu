@@ -57,7 +57,7 @@ int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
 struct elb_op {
   Kind kind;
-  int device = 0, num_sms = 148;
+  int device = 0, num_sms = 0, max_pairs = 0;
   bool prepared = false;
   uint64_t launches = 0, bytes = 0;
   int *h_status = nullptr, *d_status = nullptr;
@@ -101,6 +101,7 @@ int make(Kind kind, int device, elb_op **out) {
   op->device = device;
   DeviceGuard guard(device);
   if (cudaDeviceGetAttribute(&op->num_sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess ||
+      init_gemm(op->num_sms, &op->max_pairs) != cudaSuccess ||
       cudaHostAlloc(&op->h_status, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable) != cudaSuccess ||
       cudaHostGetDevicePointer(reinterpret_cast<void **>(&op->d_status), op->h_status, 0) != cudaSuccess ||
       cudaEventCreateWithFlags(&op->done, cudaEventDisableTiming) != cudaSuccess) {
@@ -177,6 +178,18 @@ int leave_workspace(elb_op &op, cudaStream_t s, bool capturing) {
   OP_TRY(cudaEventRecord(op.done, s));
   op.last = s;
   op.pending = true;
+  return ELB_OK;
+}
+
+// (cudaFree waits for the calls that still use the old one)
+int grow_workspace(elb_op &op, size_t bytes) {
+  if (bytes <= op.ws_bytes) return ELB_OK;
+  void *q = nullptr;
+  OP_TRY(cudaMalloc(&q, bytes));
+  if (op.ws) cudaFree(op.ws);
+  op.bytes += bytes - op.ws_bytes;
+  op.ws = q;
+  op.ws_bytes = bytes;
   return ELB_OK;
 }
 
@@ -283,7 +296,10 @@ int elb_linear_enqueue(elb_op_t *op, void *output, const void *input, const void
   p.ic = d.ic;
   p.kt = (int)(up(d.ic, GT_K) / GT_K);
   p.row_tiles = (int)(up(d.gated ? 2 * d.oc : d.oc, GT_ROWS) / GT_ROWS);
+  p.w_rows = (long long)p.row_tiles * p.kt * GT_ROWS;
   p.in_et = et_of(d.dt_input);
+  p.num_sms = op->num_sms;
+  p.max_pairs = op->max_pairs;
   p.status = op->d_status;
   p.epi.out = output;
   p.epi.res = d.with_residual ? residual : nullptr;
@@ -296,9 +312,24 @@ int elb_linear_enqueue(elb_op_t *op, void *output, const void *input, const void
   p.epi.out_et = et_of(d.dt_output);
   p.epi.scale = d.scale;
   p.epi.pairs = aligned(output, 4) && d.ld_output % 2 == 0 && (!p.epi.res || (aligned(residual, 4) && d.ld_residual % 2 == 0));
-  OP_TRY(launch_gemm(p, op->num_sms, static_cast<cudaStream_t>(cuda_stream)));
-  ++op->launches;
-  return ELB_OK;
+  const cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
+  if (aligned(input, 16) && d.ld_input % 8 == 0) {
+    OP_TRY(launch_gemm(p, s));
+    ++op->launches;
+    return ELB_OK;
+  }
+  // rows that a tiled copy cannot read go through the plan's workspace
+  const int64_t pitch = up(d.ic, 8);
+  bool capturing = false;
+  rc = enter_workspace(*op, s, capturing);
+  if (rc == ELB_OK) rc = grow_workspace(*op, (size_t)rows * pitch * 2);
+  if (rc != ELB_OK) return rc;
+  OP_TRY(launch_align_rows(op->ws, pitch, input, d.ld_input, (int)rows, d.ic, s));
+  p.x = op->ws;
+  p.ld_x = pitch;
+  OP_TRY(launch_gemm(p, s));
+  op->launches += 2;
+  return leave_workspace(*op, s, capturing);
 }
 
 // ------------------------------------------------------------------------------------------- norm
@@ -449,7 +480,7 @@ int elb_experts_create(const elb_experts_desc_t *desc, elb_op_t **out) {
   op->exp = d;
   DeviceGuard guard(op->device);
   const int64_t slots = d.max_rows * d.top_k, px = up(d.ic, 8), pm = up(d.mid, 8), py = up(d.ic, 4);
-  const int64_t tiles = slots / GEMM_TOKENS + d.experts;
+  const int64_t tiles = slots / MIN_TILE_TOKENS + d.experts;
   size_t at = 0;
   auto part = [&](size_t bytes) { const size_t o = at; at += (bytes + 255) / 256 * 256; return o; };
   const size_t o_xs = part(slots * px * 2), o_mid = part(slots * pm * 2), o_y = part(slots * py * 4), o_pos = part(slots * 4),
@@ -506,13 +537,16 @@ int elb_experts_enqueue(elb_op_t *op, void *output, const void *input, const int
   e.out = output;
   e.ids = ids;
   e.weights = weights;
-  e.tile_tokens = GEMM_TOKENS;
   const int slots = (int)(rows * d.top_k), wide = d.gated ? 2 * d.mid : d.mid;
+  e.tile_tokens = grouped_tile_tokens(slots, d.experts);
   GemmParams p = {};
   p.tiles = e.tiles;
+  p.tile_tokens = e.tile_tokens;
   p.n_tiles = e.n_tiles;
-  p.max_tiles = (int)(slots < d.experts ? slots : slots / GEMM_TOKENS + d.experts);
+  p.max_tiles = slots < d.experts ? slots : slots / e.tile_tokens + d.experts;
   p.in_et = e.et;
+  p.num_sms = op->num_sms;
+  p.max_pairs = op->max_pairs;
   p.status = op->d_status;
   p.epi.pairs = 1;
   p.epi.scale = 1.0f;
@@ -525,6 +559,7 @@ int elb_experts_enqueue(elb_op_t *op, void *output, const void *input, const int
   p.kt = (int)(up(d.ic, GT_K) / GT_K);
   p.row_tiles = (int)(up(wide, GT_ROWS) / GT_ROWS);
   p.w_stride = (size_t)p.row_tiles * p.kt * GT_BYTES;
+  p.w_rows = (long long)d.experts * p.row_tiles * p.kt * GT_ROWS;
   p.epi.out = op->mid;
   p.epi.ld_out = op->pitch_mid;
   p.epi.oc = d.mid;
@@ -539,14 +574,15 @@ int elb_experts_enqueue(elb_op_t *op, void *output, const void *input, const int
   q.kt = (int)(up(d.mid, GT_K) / GT_K);
   q.row_tiles = (int)(up(d.ic, GT_ROWS) / GT_ROWS);
   q.w_stride = (size_t)q.row_tiles * q.kt * GT_BYTES;
+  q.w_rows = (long long)d.experts * q.row_tiles * q.kt * GT_ROWS;
   q.epi.out = const_cast<float *>(e.y);
   q.epi.ld_out = e.pitch_y;
   q.epi.oc = d.ic;
   q.epi.out_et = ET_F32;
   OP_TRY(launch_experts_sort(e, s));
   OP_TRY(launch_experts_gather(e, s));
-  OP_TRY(launch_gemm(p, op->num_sms, s));
-  OP_TRY(launch_gemm(q, op->num_sms, s));
+  OP_TRY(launch_gemm(p, s));
+  OP_TRY(launch_gemm(q, s));
   OP_TRY(launch_experts_combine(e, s));
   op->launches += 5;
   return leave_workspace(*op, s, capturing);

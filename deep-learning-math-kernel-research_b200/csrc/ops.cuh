@@ -177,7 +177,9 @@ struct GemmParams {
   int in_et;                        // ET_BF16 or ET_F16
   const GroupTile *tiles;           // grouped: the token tiles, *n_tiles of them; null: dense
   const int *n_tiles;
-  int max_tiles;                    // grouped: the most that *n_tiles can be
+  int max_tiles, tile_tokens;       // grouped: the most that *n_tiles can be; tokens of a tile (grouped_tile_tokens)
+  long long w_rows;                 // rows of 128 bytes of the whole packed image
+  int num_sms, max_pairs;
   int *status;
   Epilogue epi;
 };
@@ -185,8 +187,12 @@ struct GemmParams {
 // rows: rows of a source matrix per expert (2 * oc where gated), experts matrices behind one another
 cudaError_t launch_pack_weights(void *dst, const void *src, int experts, int rows, int ic, bool gated, bool hwio, cudaStream_t s);
 cudaError_t launch_pack_bias(float *dst, const void *src, int et, int rows, int padded, bool gated, cudaStream_t s);
-cudaError_t launch_gemm(const GemmParams &p, int num_sms, cudaStream_t s);
-constexpr int GEMM_TOKENS = 16;     // tokens of a grouped tile
+cudaError_t launch_gemm(const GemmParams &p, cudaStream_t s);
+cudaError_t init_gemm(int num_sms, int *max_pairs);
+// x and ld_x of GemmParams are multiples of 16 bytes; other rows are copied first
+cudaError_t launch_align_rows(void *dst, long long pitch, const void *src, long long ld, int rows, int n, cudaStream_t s);
+int grouped_tile_tokens(int slots, int experts);
+constexpr int MIN_TILE_TOKENS = 16;
 
 struct ExpertsParams {
   const int *ids;

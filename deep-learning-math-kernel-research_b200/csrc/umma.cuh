@@ -163,6 +163,12 @@ __device__ __forceinline__ void tma_prefetch_l2(const void *gmem_src, uint32_t b
 
 // Tiled tensor copies (descriptor from cuTensorMapEncodeTiled).  Coordinate 0 is the innermost
 // dimension and coordinate0 * element_size must be a multiple of 16 bytes.
+__device__ __forceinline__ void tma_tile_2d(void *smem_dst, const void *tmap, int c0, int c1, uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(smem_u32(smem_dst)), "l"(tmap), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
+      : "memory");
+}
 __device__ __forceinline__ void tma_tile_3d(void *smem_dst, const void *tmap, int c0, int c1, int c2,
                                             uint64_t *bar) {
   asm volatile(
@@ -304,6 +310,26 @@ __device__ __forceinline__ void umma_commit_el(uint64_t *bar, uint32_t el) {
       : "memory");
 }
 
+// kind::f16 (bf16 or f16 operands, fp32 accumulators) for a whole converged warp, see umma_i8_el
+__device__ __forceinline__ void umma_f16_el(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate,
+                                            uint32_t el) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred P, Q;\n\t"
+      "setp.ne.b32 P, %4, 0;\n\t"
+      "setp.ne.b32 Q, %5, 0;\n\t"
+      "@Q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, P;\n\t"
+      "}\n" ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(el)
+      : "memory");
+}
+// Shared-memory descriptor of a K-major operand whose rows are 128 bytes, stored with the 128-byte swizzle (the 16-byte
+// chunk c of row r at chunk c ^ (r & 7)) at a 1024-byte boundary: 8-row groups lie 1024 bytes apart; a K step of 32 bytes
+// is an offset of the start address.
+__device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t saddr) {
+  return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(1) << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) |
+         (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
+}
+
 // ------------------------------------------------------------------------------------ CTA pairs
 // Helpers for kernels launched as clusters of two CTAs that drive ONE tcgen05.mma.cta_group::2 per
 // K step: 256 rows (128 per CTA, each in its own tensor memory), and each CTA supplies half of the
@@ -389,6 +415,17 @@ __device__ __forceinline__ void umma_tf32_2cta_el(uint32_t d_tmem, uint64_t ades
       "setp.ne.b32 P, %4, 0;\n\t"
       "setp.ne.b32 Q, %5, 0;\n\t"
       "@Q tcgen05.mma.cta_group::2.kind::tf32 [%0], %1, %2, %3, P;\n\t"
+      "}\n" ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(el)
+      : "memory");
+}
+__device__ __forceinline__ void umma_f16_2cta_el(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                                 uint32_t accumulate, uint32_t el) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred P, Q;\n\t"
+      "setp.ne.b32 P, %4, 0;\n\t"
+      "setp.ne.b32 Q, %5, 0;\n\t"
+      "@Q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, P;\n\t"
       "}\n" ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(el)
       : "memory");
 }
