@@ -5,9 +5,10 @@
 
 namespace elb {
 
-// Bytes of the operand rings.  The kernel of few tiles leaves room for a second CTA on its SM: of its own launch, or of the next
-// one, whose weights then arrive while this one ends.
-constexpr int SPLIT_RING = 110 * 1024, TILES_RING = 224 * 1024;
+// Bytes of the operand rings.  With few tokens the kernel of few tiles leaves room for a second CTA on its SM: of its own
+// launch, or of the next one, whose weights then arrive while this one ends.
+template <int BN> constexpr int SPLIT_RING = (BN <= 32 ? 110 : 224) * 1024;
+constexpr int TILES_RING = 224 * 1024;
 
 namespace {
 
@@ -71,45 +72,96 @@ struct alignas(64) GemmLaunch {
   CUtensorMap xmap, wmap;      // tokens; packed weights as rows of 128 bytes (pairs only)
   GemmParams p;
   int splits;                  // CTAs of a cluster that share a tile's channels
-  int token_tiles, band;       // band: token tiles that neighbouring tiles of the walk share weights over
+  int token_tiles, tile_tokens;
+  int band;                    // token tiles that neighbouring tiles of the walk share weights over
+  int box;                     // tokens of one tiled copy
 };
 
 __device__ __forceinline__ uint8_t *smem_1k(uint8_t *base) { return base + ((1024u - (smem_u32(base) & 1023u)) & 1023u); }
 
-// One tile of BN tokens: accumulator columns of this warp's quarter of the lanes, 16 at a time (the warp of `half` takes every
-// second block); `release` runs when the last of them has been read.
-template <int BN, typename F>
-__device__ __forceinline__ void epilogue_tile(const Epilogue &e, uint32_t taddr, int half, int prow, long long tok0, int ntok, F release) {
-  constexpr int BLOCKS = BN / 16;
+// One tile: this warp's quarter of the accumulator's lanes, 16 columns (tokens) at a time, the warp of `half` every second block
+// of them; `release` runs when the last has been read.
+template <typename OT, bool GATED, typename F>
+__device__ __forceinline__ void epilogue_blocks(const Epilogue &e, uint32_t taddr, int half, int prow, long long tok0, int ntok, F release) {
+  const int blocks = (ntok + 15) / 16;
+  const int first = prow & ~31;                               // of the warp
+  const bool whole = (GATED ? (first >> 1) + 16 : first + 32) <= e.oc && (sizeof(OT) == 4 || e.pairs);
+  const float bias = e.bias ? e.bias[prow] : 0.0f;
+  const long long t0 = tok0 + first_token<OT, GATED>(prow);
+  const int ch = first_channel<OT, GATED>(prow);
+  OT *out = static_cast<OT *>(e.out) + (t0 + half * 16) * e.ld_out + ch;
+  const OT *res = e.res ? static_cast<const OT *>(e.res) + (t0 + half * 16) * e.ld_res + ch : nullptr;
   uint32_t a[16], b[16];
   float v[16];
+  auto block = [&](int k) {
+    const int t = k * 16;
+    if (whole && t + 16 <= ntok) emit_full<OT, GATED>(e, v, prow, bias, out, res);
+    else emit<16>(e, v, prow, tok0 + t, ntok - t);
+    out += 32 * e.ld_out;
+    if (res) res += 32 * e.ld_res;
+  };
   int k = half;
-  if (k < BLOCKS) tmem_ld16(taddr + k * 16, a);
+  if (k < blocks) tmem_ld16(taddr + k * 16, a);
 #pragma unroll 1
-  for (; k < BLOCKS; k += 4) {
+  for (; k < blocks; k += 4) {
     tmem_ld_wait16(a);
-    if (k + 2 < BLOCKS) tmem_ld16(taddr + (k + 2) * 16, b);
+    if (k + 2 < blocks) tmem_ld16(taddr + (k + 2) * 16, b);
     else release();
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(a[i]);
-    if (k * 16 < ntok) emit<16>(e, v, prow, tok0 + k * 16, ntok - k * 16);
-    if (k + 2 < BLOCKS) {
+    block(k);
+    if (k + 2 < blocks) {
       tmem_ld_wait16(b);
-      if (k + 4 < BLOCKS) tmem_ld16(taddr + (k + 4) * 16, a);
+      if (k + 4 < blocks) tmem_ld16(taddr + (k + 4) * 16, a);
       else release();
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(b[i]);
-      if ((k + 2) * 16 < ntok) emit<16>(e, v, prow, tok0 + (k + 2) * 16, ntok - (k + 2) * 16);
+      block(k + 2);
     }
   }
-  if (half >= BLOCKS) release();
+  if (half >= blocks) release();
+}
+template <typename F>
+__device__ __forceinline__ void epilogue_tile(const Epilogue &e, uint32_t taddr, int half, int prow, long long tok0, int ntok, F release) {
+  if (e.gated) {
+    if (e.out_et == ET_BF16) epilogue_blocks<__nv_bfloat16, true>(e, taddr, half, prow, tok0, ntok, release);
+    else if (e.out_et == ET_F16) epilogue_blocks<__half, true>(e, taddr, half, prow, tok0, ntok, release);
+    else epilogue_blocks<float, true>(e, taddr, half, prow, tok0, ntok, release);
+  } else {
+    if (e.out_et == ET_BF16) epilogue_blocks<__nv_bfloat16, false>(e, taddr, half, prow, tok0, ntok, release);
+    else if (e.out_et == ET_F16) epilogue_blocks<__half, false>(e, taddr, half, prow, tok0, ntok, release);
+    else epilogue_blocks<float, false>(e, taddr, half, prow, tok0, ntok, release);
+  }
+}
+
+// The partial sums of T tokens, one value per lane and token, added up over the CTAs of the cluster in the order of their ranks.
+template <int T>
+__device__ __forceinline__ void join(const Epilogue &e, uint32_t at, int splits, int prow, long long tok0, int ntok) {
+  float v[T];
+#pragma unroll
+  for (int i = 0; i < T; ++i) v[i] = 0.0f;
+#pragma unroll 2
+  for (int r = 0; r < splits; ++r) {
+    uint32_t from;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from) : "r"(at), "r"(r));
+    float4 x[T / 4];
+#pragma unroll
+    for (int i = 0; i < T / 4; ++i)
+      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                   : "=f"(x[i].x), "=f"(x[i].y), "=f"(x[i].z), "=f"(x[i].w) : "r"(from + i * GT_ROWS * 16) : "memory");
+#pragma unroll
+    for (int i = 0; i < T / 4; ++i) {
+      v[4 * i] += x[i].x; v[4 * i + 1] += x[i].y; v[4 * i + 2] += x[i].z; v[4 * i + 3] += x[i].w;
+    }
+  }
+  emit<T>(e, v, prow, tok0, ntok);
 }
 
 // ---- Few tiles: each belongs to a cluster of CTAs that share its channels.  The partial sums are brought together through
 // distributed shared memory in the order of the ranks, each CTA finishing a part of the tokens.
 template <int BN>
 __global__ void __launch_bounds__(THREADS) gemm_split_kernel(const __grid_constant__ GemmLaunch g) {
-  using L = GemmSmem<BN, false, SPLIT_RING>;
+  using L = GemmSmem<BN, false, SPLIT_RING<BN>>;
   constexpr int STAGES = L::STAGES;
   constexpr uint32_t COLS = BN < 32 ? 32 : BN;
   static_assert(BN * GT_ROWS * 4 <= L::BAR_OFF, "the partial sums lie in the ring");
@@ -187,44 +239,35 @@ __global__ void __launch_bounds__(THREADS) gemm_split_kernel(const __grid_consta
   }
   const int quarter = warp & 3, half = (warp - 4) >> 2, prow = row_tile * GT_ROWS + quarter * 32 + lane;
   const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-  float *part = reinterpret_cast<float *>(smem);              // [token][128 rows]
+  float4 *part = reinterpret_cast<float4 *>(smem);            // [token / 4][128 rows][4 tokens]
   bool ok = true;
   if (warp >= 4) {
     ok = mbar_wait_warp(tfull, 0, abort_flag);
     if (!ok) fail_code = ST_WAIT_TIMEOUT_EPILOGUE;
     tc_fence_after_sync();
-    if (ok && splits == 1) epilogue_tile<BN>(p.epi, taddr, half, prow, tok0, ntok, [] {});
+    if (ok && splits == 1) epilogue_tile(p.epi, taddr, half, prow, tok0, ntok, [] {});
     if (ok && splits > 1) {
 #pragma unroll 1
-      for (int k = half; k < BN / 16; k += 2) {
+      for (int k = half; k < (ntok + 15) / 16; k += 2) {
         uint32_t a[16];
         tmem_ld16(taddr + k * 16, a);
         tmem_ld_wait16(a);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) part[(k * 16 + i) * GT_ROWS + quarter * 32 + lane] = __uint_as_float(a[i]);
+        for (int i = 0; i < 4; ++i)
+          part[(k * 4 + i) * GT_ROWS + quarter * 32 + lane] =
+              make_float4(__uint_as_float(a[4 * i]), __uint_as_float(a[4 * i + 1]), __uint_as_float(a[4 * i + 2]), __uint_as_float(a[4 * i + 3]));
       }
     }
   }
   if (splits > 1) {
     __syncwarp();
     cluster_sync_all();
-    const int share = BN / splits, per = share >= 4 ? share / 2 : share;      // tokens of this CTA, and of one of its warps
-    if (warp >= 4 && half * per < share) {
-      for (int t = rank * share + half * per; t < rank * share + half * per + per && t < ntok; t += 2) {
-        float v[2] = {0.0f, 0.0f};
-        const uint32_t at = smem_u32(part + t * GT_ROWS + quarter * 32 + lane);
+    if (warp >= 4 && ok) {
+      // this CTA finishes every splits-th group of tokens, its warps of one half every second of those
+      constexpr int T = BN >= 64 ? 8 : 4;
 #pragma unroll 1
-        for (int r = 0; r < splits; ++r) {
-          uint32_t from;
-          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from) : "r"(at), "r"(r));
-          float x, y;
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(from) : "memory");
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(y) : "r"(from + GT_ROWS * 4) : "memory");
-          v[0] += x;
-          v[1] += y;
-        }
-        emit<2>(p.epi, v, prow, tok0 + t, ntok - t);
-      }
+      for (int t = (rank + half * splits) * T; t < ntok; t += 2 * splits * T)
+        join<T>(p.epi, smem_u32(part + t / 4 * GT_ROWS + quarter * 32 + lane), splits, prow, tok0 + t, ntok - t);
     }
     __syncwarp();
     cluster_sync_all();                                       // nobody leaves while its partial sums are read
@@ -287,11 +330,13 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_tiles_kernel(const __grid_con
       const int width = min(g.band, token_tiles - b * g.band);
       t.expert = 0;
       t.row_tile = in / width * CTAS + rank;
-      t.tok0 = (b * g.band + in % width) * BN;
-      t.ntok = min(BN, p.rows - t.tok0);
+      t.tok0 = (b * g.band + in % width) * g.tile_tokens;
+      t.ntok = min(g.tile_tokens, p.rows - t.tok0);
     }
     return t;
   };
+  // Only as many columns as a tile has tokens are multiplied, in steps of 16 per CTA; CTA 1 of a pair holds the second half.
+  auto columns = [](int ntok) { return (ntok + 16 * CTAS - 1) / (16 * CTAS) * (16 * CTAS); };
   int fail_code = 0;
   if (warp == 0) {
     const uint32_t el = elect_one();
@@ -302,6 +347,8 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_tiles_kernel(const __grid_con
       const int rt = min(t.row_tile, p.row_tiles - 1);         // (the second of a pair may lie past the last tile)
       const uint8_t *w = p.w + t.expert * p.w_stride + (size_t)rt * p.kt * GT_BYTES;
       const int wrow = PAIR ? (int)((t.expert * p.w_stride / GT_BYTES + (size_t)rt * p.kt) * GT_ROWS) : 0;
+      const int mine = columns(t.ntok) / CTAS, boxes = (mine + g.box - 1) / g.box, x0 = t.tok0 + rank * mine;
+      const uint32_t bytes = GT_BYTES + boxes * g.box * 128;
       for (int k = 0; k < p.kt; ++k, ++it) {
         const int s = it % STAGES;
         if (!mbar_wait_warp(&empty[s], ((it / STAGES) & 1) ^ 1, abort_flag)) { ok = false; fail_code = ST_WAIT_TIMEOUT_PRODUCER; break; }
@@ -309,13 +356,13 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_tiles_kernel(const __grid_con
         if (el) {
           if (PAIR) {
             const uint32_t bar = mapa_u32(&full[s], 0);
-            if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * L::STAGE);
+            if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * bytes);
             tma_tile_2d_pair(dst, &g.wmap, 0, wrow + k * GT_ROWS, bar);
-            tma_tile_2d_pair(dst + GT_BYTES, &g.xmap, k * GT_K, t.tok0 + rank * (BN / 2), bar);
+            for (int j = 0; j < boxes; ++j) tma_tile_2d_pair(dst + GT_BYTES + j * g.box * 128, &g.xmap, k * GT_K, x0 + j * g.box, bar);
           } else {
-            mbar_arrive_expect_tx(&full[s], L::STAGE);
+            mbar_arrive_expect_tx(&full[s], bytes);
             tma_bulk_g2s(dst, w + (size_t)k * GT_BYTES, GT_BYTES, &full[s]);
-            tma_tile_2d(dst + GT_BYTES, &g.xmap, k * GT_K, t.tok0, &full[s]);
+            for (int j = 0; j < boxes; ++j) tma_tile_2d(dst + GT_BYTES + j * g.box * 128, &g.xmap, k * GT_K, x0 + j * g.box, &full[s]);
           }
         }
         __syncwarp();
@@ -324,11 +371,11 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_tiles_kernel(const __grid_con
   } else if (warp == 1) {
     if (rank == 0) {
       const uint32_t el = elect_one();
-      const uint32_t idesc = umma_idesc(1, p.in_et == ET_BF16, p.in_et == ET_BF16, GT_ROWS * CTAS, BN);
       uint32_t it = 0, count = 0;
       bool ok = true;
       for (int i = first; i < total && ok; i += step, ++count) {
         const uint32_t b = count & 1;
+        const uint32_t idesc = umma_idesc(1, p.in_et == ET_BF16, p.in_et == ET_BF16, GT_ROWS * CTAS, columns(tile_of(i).ntok));
         if (!mbar_wait_warp(&tempty[b], ((count >> 1) & 1) ^ 1, abort_flag)) { fail_code = ST_WAIT_TIMEOUT_MMA; break; }
         tc_fence_after_sync();
         const uint32_t d = tmem + b * BN;
@@ -357,7 +404,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_tiles_kernel(const __grid_con
       const uint32_t b = count & 1;
       if (!mbar_wait_warp(&tfull[b], (count >> 1) & 1, abort_flag)) { fail_code = ST_WAIT_TIMEOUT_EPILOGUE; break; }
       tc_fence_after_sync();
-      epilogue_tile<BN>(p.epi, tmem + (static_cast<uint32_t>(quarter * 32) << 16) + b * BN, half, t.row_tile * GT_ROWS + quarter * 32 + lane, t.tok0,
+      epilogue_tile(p.epi, tmem + (static_cast<uint32_t>(quarter * 32) << 16) + b * BN, half, t.row_tile * GT_ROWS + quarter * 32 + lane, t.tok0,
                         t.ntok, [&] {
                           tc_fence_before_sync();
                           __syncwarp();
@@ -412,7 +459,7 @@ cudaError_t launch_gemm_kernel(K kern, const GemmLaunch &g, int grid, int smem, 
 
 template <int BN>
 cudaError_t go_split(GemmLaunch &g, cudaStream_t s) {
-  using L = GemmSmem<BN, false, SPLIT_RING>;
+  using L = GemmSmem<BN, false, SPLIT_RING<BN>>;
   if (!encode_rows(&g.xmap, g.p.in_et, g.p.x, g.p.ic, g.p.rows, g.p.ld_x * 2, GT_K, BN, true)) return cudaErrorInvalidValue;
   return launch_gemm_kernel(gemm_split_kernel<BN>, g, g.p.row_tiles * g.token_tiles * g.splits, L::TOTAL, g.splits, s);
 }
@@ -422,9 +469,10 @@ cudaError_t go_tiles(GemmLaunch &g, cudaStream_t s) {
   using L = GemmSmem<BN, PAIR, TILES_RING>;
   const GemmParams &p = g.p;
   const int ctas = PAIR ? 2 : 1, row_steps = (p.row_tiles + ctas - 1) / ctas;
-  if (!encode_rows(&g.xmap, p.in_et, p.x, p.ic, p.rows, p.ld_x * 2, GT_K, PAIR ? BN / 2 : BN, true)) return cudaErrorInvalidValue;
+  // dense: one copy brings a CTA's tokens; grouped: tiles have any number of them, in boxes of up to 32
+  g.box = p.tiles ? (BN / ctas < 32 ? BN / ctas : 32) : g.tile_tokens / ctas;
+  if (!encode_rows(&g.xmap, p.in_et, p.x, p.ic, p.rows, p.ld_x * 2, GT_K, g.box, true)) return cudaErrorInvalidValue;
   if (PAIR && !encode_rows(&g.wmap, p.in_et, p.w, GT_K, p.w_rows, 128, GT_K, GT_ROWS, false)) return cudaErrorInvalidValue;
-  g.token_tiles = p.tiles ? p.max_tiles : (p.rows + BN - 1) / BN;
   const long long tiles = (long long)g.token_tiles * row_steps;
   const int most = PAIR ? p.max_pairs : p.num_sms;
   const int grid = (int)(tiles < most ? tiles : most) * ctas;
@@ -460,11 +508,11 @@ cudaError_t launch_align_rows(void *dst, long long pitch, const void *src, long 
 cudaError_t init_gemm(int num_sms, int *max_pairs) {
   cudaError_t e = cudaSuccess;
   auto want = [&](cudaError_t r) { if (e == cudaSuccess) e = r; };
-  want(allow(gemm_split_kernel<16>, GemmSmem<16, false, SPLIT_RING>::TOTAL));
-  want(allow(gemm_split_kernel<32>, GemmSmem<32, false, SPLIT_RING>::TOTAL));
-  want(allow(gemm_split_kernel<64>, GemmSmem<64, false, SPLIT_RING>::TOTAL));
-  want(allow(gemm_split_kernel<128>, GemmSmem<128, false, SPLIT_RING>::TOTAL));
-  want(allow(gemm_tiles_kernel<128, true, false>, GemmSmem<128, true, TILES_RING>::TOTAL));
+  want(allow(gemm_split_kernel<16>, GemmSmem<16, false, SPLIT_RING<16>>::TOTAL));
+  want(allow(gemm_split_kernel<32>, GemmSmem<32, false, SPLIT_RING<32>>::TOTAL));
+  want(allow(gemm_split_kernel<64>, GemmSmem<64, false, SPLIT_RING<64>>::TOTAL));
+  want(allow(gemm_split_kernel<128>, GemmSmem<128, false, SPLIT_RING<128>>::TOTAL));
+  want(allow(gemm_split_kernel<256>, GemmSmem<256, false, SPLIT_RING<256>>::TOTAL));
   want(allow(gemm_tiles_kernel<256, true, false>, GemmSmem<256, true, TILES_RING>::TOTAL));
   want(allow(gemm_tiles_kernel<16, false, true>, GemmSmem<16, false, TILES_RING>::TOTAL));
   want(allow(gemm_tiles_kernel<32, false, true>, GemmSmem<32, false, TILES_RING>::TOTAL));
@@ -496,8 +544,10 @@ cudaError_t launch_gemm(const GemmParams &p, cudaStream_t s) {
   g.p = p;
   g.splits = 1;
   g.band = 8;
-  g.token_tiles = 0;
+  g.box = 0;
   if (p.tiles) {
+    g.token_tiles = p.max_tiles;
+    g.tile_tokens = p.tile_tokens;
     switch (p.tile_tokens) {
       case 16: return go_tiles<16, false, true>(g, s);
       case 32: return go_tiles<32, false, true>(g, s);
@@ -506,18 +556,43 @@ cudaError_t launch_gemm(const GemmParams &p, cudaStream_t s) {
       default: return go_tiles<256, true, true>(g, s);
     }
   }
-  const int bn = p.rows <= 16 ? 16 : p.rows <= 32 ? 32 : p.rows <= 64 ? 64 : 128;
-  g.token_tiles = (p.rows + bn - 1) / bn;
-  const long long tiles = (long long)p.row_tiles * g.token_tiles;
-  if (tiles <= p.num_sms || bn < 128) {
-    while (g.splits < 8 && tiles * g.splits * 2 <= p.num_sms && p.kt >= g.splits * 4) g.splits *= 2;
-    if (bn == 16) return go_split<16>(g, s);
-    if (bn == 32) return go_split<32>(g, s);
-    if (bn == 64) return go_split<64>(g, s);
-    return go_split<128>(g, s);
+  // Which kernel and tiles: the least of a model of their time in cycles.  A step of 64 channels costs a CTA its bytes at
+  // FILL per cycle (what an SM takes in: 128 KB of steps measured 56 to 64) or its MMAs, whichever is more; a launch its
+  // waves of steps, and sharing a tile's channels the joining of the partial sums.
+  constexpr double FILL = 58.0, JOIN = 1500.0, JOIN_TOKEN = 10.0;
+  double best = 1e30;
+  bool pairs = false;
+  for (int bn = 16; bn <= 256; bn *= 2) {
+    if (bn > 16 && p.rows <= bn / 2) break;
+    const int tt = (p.rows + bn - 1) / bn;
+    const long long tiles = (long long)p.row_tiles * tt;
+    const int per_sm = bn <= 32 ? 2 : 1;
+    for (int splits = 1; splits <= 8; splits *= 2) {
+      if (splits > 1 && (tiles * splits > p.num_sms || p.kt < splits * 2)) break;
+      const double step = fmax((GT_BYTES + bn * 128) / FILL, fmax(bn * 2.0, 370.0));
+      const double waves = (double)((tiles * splits + (long long)p.num_sms * per_sm - 1) / ((long long)p.num_sms * per_sm));
+      const double busy = waves > 1 ? waves * per_sm : (double)((tiles * splits + p.num_sms - 1) / p.num_sms);
+      const double t = busy * ((p.kt + splits - 1) / splits) * step + (splits > 1 ? JOIN + JOIN_TOKEN * bn : 0.0) + waves * 2000.0 + bn * 8.0;
+      if (t < best) { best = t; g.splits = splits; g.tile_tokens = bn; g.token_tiles = tt; }
+    }
   }
-  if (tiles <= 4 * p.num_sms) return go_tiles<128, true, false>(g, s);
-  return go_tiles<256, true, false>(g, s);
+  const int row_pairs = (p.row_tiles + 1) / 2;
+  const int fewest = (p.rows + 255) / 256;
+  for (int tt = fewest; tt <= fewest + 7 && p.rows > 64; ++tt) {          // tiles of equal size, a multiple of 32 tokens
+    const int n = ((p.rows + tt - 1) / tt + 31) / 32 * 32, count = (p.rows + n - 1) / n;
+    const double step = fmax((GT_BYTES + n * 64) / FILL, fmax(n * 2.0, 256.0));
+    const double waves = (double)(((long long)row_pairs * count + p.max_pairs - 1) / p.max_pairs);
+    const double t = waves * p.kt * step + 2500.0 + n * 8.0;
+    if (t < best) { best = t; pairs = true; g.splits = 1; g.tile_tokens = n; g.token_tiles = count; }
+  }
+  if (pairs) return go_tiles<256, true, false>(g, s);
+  switch (g.tile_tokens) {
+    case 16: return go_split<16>(g, s);
+    case 32: return go_split<32>(g, s);
+    case 64: return go_split<64>(g, s);
+    case 128: return go_split<128>(g, s);
+    default: return go_split<256>(g, s);
+  }
 }
 
 }  // namespace elb

@@ -76,6 +76,7 @@ struct elb_op {
   void *ws = nullptr;         // the experts' workspace
   size_t ws_bytes = 0;
   ExpertsParams ep = {};
+  bool count_stale = false;   // a call's launches failed half way: the experts' counts are not zero
   void *mid = nullptr;
   int64_t pitch_mid = 0;
 
@@ -484,20 +485,25 @@ int elb_experts_create(const elb_experts_desc_t *desc, elb_op_t **out) {
   size_t at = 0;
   auto part = [&](size_t bytes) { const size_t o = at; at += (bytes + 255) / 256 * 256; return o; };
   const size_t o_xs = part(slots * px * 2), o_mid = part(slots * pm * 2), o_y = part(slots * py * 4), o_pos = part(slots * 4),
-               o_src = part(slots * 4), o_tiles = part(tiles * sizeof(GroupTile)), o_n = part(8);
+               o_place = part(slots * 4), o_tiles = part(tiles * sizeof(GroupTile)), o_n = part(4), o_count = part(d.experts * 4);
   rc = alloc(*op, &op->ws, at);
   if (rc != ELB_OK) { delete op; return rc; }
   op->ws_bytes = at;
+  if (cudaMemset(static_cast<uint8_t *>(op->ws) + o_count, 0, d.experts * 4) != cudaSuccess || cudaDeviceSynchronize() != cudaSuccess) {
+    cudaGetLastError();
+    delete op;
+    return op_fail(ELB_GENERAL_ERROR, "the workspace could not be cleared");
+  }
   uint8_t *b = static_cast<uint8_t *>(op->ws);
   ExpertsParams &e = op->ep;
   e.xs = b + o_xs;
   op->mid = b + o_mid;
   e.y = reinterpret_cast<float *>(b + o_y);
   e.pos = reinterpret_cast<int *>(b + o_pos);
-  e.src = reinterpret_cast<int *>(b + o_src);
+  e.place = reinterpret_cast<int *>(b + o_place);
+  e.count = reinterpret_cast<int *>(b + o_count);
   e.tiles = reinterpret_cast<GroupTile *>(b + o_tiles);
   e.n_tiles = reinterpret_cast<int *>(b + o_n);
-  e.n_rows = e.n_tiles + 1;
   e.ld_x = d.ld_input; e.ld_out = d.ld_output; e.pitch_x = px; e.pitch_y = py;
   e.top_k = d.top_k; e.experts = d.experts; e.ic = d.ic; e.et = et_of(d.dt);
   op->pitch_mid = pm;
@@ -579,11 +585,14 @@ int elb_experts_enqueue(elb_op_t *op, void *output, const void *input, const int
   q.epi.ld_out = e.pitch_y;
   q.epi.oc = d.ic;
   q.epi.out_et = ET_F32;
-  OP_TRY(launch_experts_sort(e, s));
-  OP_TRY(launch_experts_gather(e, s));
+  if (op->count_stale) OP_TRY(cudaMemsetAsync(e.count, 0, d.experts * sizeof(int), s));
+  op->count_stale = true;
+  OP_TRY(launch_experts_count(e, s));
+  OP_TRY(launch_experts_gather(e, op->num_sms, s));
   OP_TRY(launch_gemm(p, s));
   OP_TRY(launch_gemm(q, s));
   OP_TRY(launch_experts_combine(e, s));
+  op->count_stale = false;
   op->launches += 5;
   return leave_workspace(*op, s, capturing);
 }

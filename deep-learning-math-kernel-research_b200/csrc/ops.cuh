@@ -158,6 +158,88 @@ __device__ __forceinline__ void emit(const Epilogue &e, float (&v)[NT], int prow
   else emit_as<float, NT>(e, v, prow, tok0, ntok);
 }
 
+// The same for 16 real tokens and a warp whose channels all exist, 16-bit results and residuals at even channels in 4-byte
+// words: `out` and `res` are this lane's first element, from first_element().  Without the tests of the general form a
+// token costs a warp about 5 instructions instead of 38, which is what a long call's epilogue is bound by.
+template <typename OT, bool GATED>
+__device__ __forceinline__ long long first_token(int prow) {     // of the 16, the first that this lane stores
+  if (!GATED) return sizeof(OT) == 2 ? prow & 1 : 0;
+  return sizeof(OT) == 2 ? (prow & 2) + (prow & 1) : prow & 1;
+}
+template <typename OT, bool GATED>
+__device__ __forceinline__ int first_channel(int prow) {
+  if (!GATED) return sizeof(OT) == 2 ? prow & ~1 : prow;
+  return sizeof(OT) == 2 ? (prow >> 1) & ~1 : prow >> 1;
+}
+template <typename OT, bool GATED>
+__device__ __forceinline__ void emit_full(const Epilogue &e, float (&v)[16], int prow, float bias, OT *out, const OT *res) {
+  const int odd = prow & 1;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) v[j] += bias;
+  constexpr int EACH = sizeof(OT) == 2 ? (GATED ? 4 : 2) : (GATED ? 2 : 1);     // tokens from one of this lane's stores to the next
+  constexpr int N = 16 / EACH;
+  const long long so = e.ld_out * EACH, sr = e.ld_res * EACH;
+  if constexpr (GATED) {
+    float y[8], u[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float got = __shfl_xor_sync(0xFFFFFFFFu, odd ? v[2 * j] : v[2 * j + 1], 1);
+      y[j] = odd ? got : v[2 * j];
+      u[j] = odd ? v[2 * j + 1] : got;
+    }
+    activate(y, e.act);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = y[j] * u[j] * e.scale;
+    if constexpr (sizeof(OT) == 4) {
+      float r[8] = {};
+      if (res) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r[j] = res[j * sr];
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) out[j * so] = y[j] + r[j];
+    } else {
+      // a second trade, between lanes of neighbouring channels: two channels of every fourth token
+      const int high = prow & 2;
+      uint32_t r[4] = {};
+      if (res) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[j] = *reinterpret_cast<const uint32_t *>(res + j * sr);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float got = __shfl_xor_sync(0xFFFFFFFFu, high ? y[2 * j] : y[2 * j + 1], 2);
+        const float2 add = unpack2<OT>(r[j]);
+        *reinterpret_cast<uint32_t *>(out + j * so) = pack2<OT>((high ? got : y[2 * j]) + add.x, (high ? y[2 * j + 1] : got) + add.y);
+      }
+    }
+  } else {
+    activate(v, e.act);
+    if constexpr (sizeof(OT) == 4) {
+      float r[16] = {};
+      if (res) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) r[j] = res[j * sr];
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) out[j * so] = fmaf(v[j], e.scale, r[j]);
+    } else {
+      uint32_t r[N] = {};
+      if (res) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) r[j] = *reinterpret_cast<const uint32_t *>(res + j * sr);
+      }
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float got = __shfl_xor_sync(0xFFFFFFFFu, odd ? v[2 * j] : v[2 * j + 1], 1);
+        const float2 add = unpack2<OT>(r[j]);
+        *reinterpret_cast<uint32_t *>(out + j * so) =
+            pack2<OT>(fmaf(odd ? got : v[2 * j], e.scale, add.x), fmaf(odd ? v[2 * j + 1] : got, e.scale, add.y));
+      }
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------------------------
 // Matrix products on packed weights.  The packed image is the shared-memory operand image itself: tiles of 128 rows x
 // 64 channels, [row tile][channel tile][128 rows][128 bytes], the 16-byte chunks of a row permuted as the 128-byte
@@ -201,14 +283,15 @@ struct ExpertsParams {
   void *xs;                         // sorted rows [slots][pitch_x]
   const float *y;                   // products of the sorted rows [slots][pitch_y]
   void *out;
-  int *pos, *src;                   // slot -> sorted row (-1: none); sorted row -> token
+  int *count;                       // slots of each expert; zero between calls
+  int *pos, *place;                 // of each slot: among those of its expert; its sorted row
   GroupTile *tiles;
-  int *n_tiles, *n_rows;
+  int *n_tiles;
   long long ld_x, ld_out, pitch_x, pitch_y;
-  int rows, top_k, experts, ic, et, tile_tokens;
+  int rows, top_k, experts, ic, et, tile_tokens;    // tile_tokens: the most that a token tile holds
 };
-cudaError_t launch_experts_sort(const ExpertsParams &p, cudaStream_t s);
-cudaError_t launch_experts_gather(const ExpertsParams &p, cudaStream_t s);
+cudaError_t launch_experts_count(const ExpertsParams &p, cudaStream_t s);
+cudaError_t launch_experts_gather(const ExpertsParams &p, int num_sms, cudaStream_t s);
 cudaError_t launch_experts_combine(const ExpertsParams &p, cudaStream_t s);
 
 struct NormParams {
