@@ -1,5 +1,6 @@
 // Matrix products of the transformer operators, dense and grouped by expert, on packed weights (ops.cuh).
 #include "elb_common.cuh"
+#include "gemm_epilogue.cuh"
 #include "ops.cuh"
 #include "umma.cuh"
 
@@ -8,7 +9,7 @@ namespace elb {
 // Bytes of the operand rings.  With few tokens the kernel of few tiles leaves room for a second CTA on its SM: of its own
 // launch, or of the next one, whose weights then arrive while this one ends.
 template <int BN> constexpr int SPLIT_RING = (BN <= 32 ? 110 : 224) * 1024;
-constexpr int TILES_RING = 224 * 1024;
+constexpr int TILES_RING = 192 * 1024;
 
 namespace {
 
@@ -24,14 +25,14 @@ __global__ void pack_weights_kernel(uint4 *dst, const uint16_t *src, int rows, i
     r >>= 7;
     const int k_tile = (int)(r % kt), row_tile = (int)(r / kt);
     const int p = row_tile * GT_ROWS + in_tile;                          // packed row
-    const int row = gated ? (p & 1) * (rows >> 1) + (p >> 1) : p;        // row of the source
+    const int row = packed_source(p, rows, gated);                       // row of the source
     const int k0 = k_tile * GT_K + ((slot ^ (in_tile & 7)) << 3);
     uint16_t v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int k = k0 + j;
       v[j] = 0;
-      if (p < rows && k < ic)
+      if (row < rows && k < ic)
         v[j] = hwio ? src[(e * ic + k) * rows + row] : src[(e * rows + row) * (long long)ic + k];
     }
     dst[i] = *reinterpret_cast<uint4 *>(v);
@@ -42,8 +43,8 @@ __global__ void pack_bias_kernel(float *dst, const void *src, int et, int rows, 
   const int p = blockIdx.x * blockDim.x + threadIdx.x;
   if (p >= padded) return;
   float v = 0.0f;
-  if (p < rows) {
-    const int row = gated ? (p & 1) * (rows >> 1) + (p >> 1) : p;
+  const int row = packed_source(p, rows, gated);
+  if (row < rows) {
     v = et == ET_F32 ? static_cast<const float *>(src)[row]
       : et == ET_BF16 ? to_f32(static_cast<const __nv_bfloat16 *>(src)[row]) : to_f32(static_cast<const __half *>(src)[row]);
   }
@@ -56,14 +57,16 @@ __global__ void pack_bias_kernel(float *dst, const void *src, int et, int rows, 
 // tensor (rows and channels outside it arrive as zeros).  Few tokens then cost a narrow MMA and not a padded one, and the
 // weights, which are what a small call is made of, stream through shared memory once.
 // ---------------------------------------------------------------------------------------------
-constexpr int EPI_WARPS = 8, THREADS = (4 + EPI_WARPS) * 32;   // warp 0 producer, 1 MMA, 2 and 3 idle, 4 to 11 epilogue
+// Warp 0 produces, 1 issues the MMAs, the others are the epilogue's: more of them where a CTA has its SM to itself
+constexpr int SPLIT_WARPS = 8, TILES_WARPS = 12;
 
-template <int BN, bool PAIR, int RING>
+template <int BN, bool PAIR, int RING, int EPI_WARPS>
 struct GemmSmem {
   static constexpr int X_BYTES = (PAIR ? BN / 2 : BN) * 128;
   static constexpr int STAGE = GT_BYTES + X_BYTES;
   static constexpr int STAGES = RING / STAGE;
-  static constexpr int BAR_OFF = STAGES * STAGE;              // full[S], empty[S], tfull[2], tempty[2]
+  static constexpr int EPI_OFF = STAGES * STAGE;                     // staging of the epilogue, where it runs beside the ring
+  static constexpr int BAR_OFF = EPI_OFF + EPI_WARPS * EPI_STAGE;    // full[S], empty[S], tfull[2], tempty[2]
   static constexpr int MISC_OFF = BAR_OFF + (2 * STAGES + 4) * 8;
   static constexpr int TOTAL = MISC_OFF + 16 + 1024;          // tmem slot, abort flag; room to align
 };
@@ -79,92 +82,70 @@ struct alignas(64) GemmLaunch {
 
 __device__ __forceinline__ uint8_t *smem_1k(uint8_t *base) { return base + ((1024u - (smem_u32(base) & 1023u)) & 1023u); }
 
-// One tile: this warp's quarter of the accumulator's lanes, 16 columns (tokens) at a time, the warp of `half` every second block
-// of them; `release` runs when the last has been read.
-template <typename OT, bool GATED, typename F>
-__device__ __forceinline__ void epilogue_blocks(const Epilogue &e, uint32_t taddr, int half, int prow, long long tok0, int ntok, F release) {
-  const int blocks = (ntok + 15) / 16;
-  const int first = prow & ~31;                               // of the warp
-  const bool whole = (GATED ? (first >> 1) + 16 : first + 32) <= e.oc && (sizeof(OT) == 4 || e.pairs);
-  const float bias = e.bias ? e.bias[prow] : 0.0f;
-  const long long t0 = tok0 + first_token<OT, GATED>(prow);
-  const int ch = first_channel<OT, GATED>(prow);
-  OT *out = static_cast<OT *>(e.out) + (t0 + half * 16) * e.ld_out + ch;
-  const OT *res = e.res ? static_cast<const OT *>(e.res) + (t0 + half * 16) * e.ld_res + ch : nullptr;
-  uint32_t a[16], b[16];
-  float v[16];
-  auto block = [&](int k) {
-    const int t = k * 16;
-    if (whole && t + 16 <= ntok) emit_full<OT, GATED>(e, v, prow, bias, out, res);
-    else emit<16>(e, v, prow, tok0 + t, ntok - t);
-    out += 32 * e.ld_out;
-    if (res) res += 32 * e.ld_res;
-  };
-  int k = half;
-  if (k < blocks) tmem_ld16(taddr + k * 16, a);
-#pragma unroll 1
-  for (; k < blocks; k += 4) {
-    tmem_ld_wait16(a);
-    if (k + 2 < blocks) tmem_ld16(taddr + (k + 2) * 16, b);
-    else release();
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(a[i]);
-    block(k);
-    if (k + 2 < blocks) {
-      tmem_ld_wait16(b);
-      if (k + 4 < blocks) tmem_ld16(taddr + (k + 4) * 16, a);
-      else release();
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(b[i]);
-      block(k + 2);
-    }
-  }
-  if (half >= blocks) release();
-}
+struct EpilogueTile {
+  const Epilogue &e;
+  uint8_t *stage;
+  uint32_t taddr;
+  int part, parts, lane, prow0;
+  long long tok0;
+  int ntok;
+};
 template <typename F>
-__device__ __forceinline__ void epilogue_tile(const Epilogue &e, uint32_t taddr, int half, int prow, long long tok0, int ntok, F release) {
-  if (e.gated) {
-    if (e.out_et == ET_BF16) epilogue_blocks<__nv_bfloat16, true>(e, taddr, half, prow, tok0, ntok, release);
-    else if (e.out_et == ET_F16) epilogue_blocks<__half, true>(e, taddr, half, prow, tok0, ntok, release);
-    else epilogue_blocks<float, true>(e, taddr, half, prow, tok0, ntok, release);
-  } else {
-    if (e.out_et == ET_BF16) epilogue_blocks<__nv_bfloat16, false>(e, taddr, half, prow, tok0, ntok, release);
-    else if (e.out_et == ET_F16) epilogue_blocks<__half, false>(e, taddr, half, prow, tok0, ntok, release);
-    else epilogue_blocks<float, false>(e, taddr, half, prow, tok0, ntok, release);
-  }
-}
+struct EpilogueCall : EpilogueTile {
+  F release;
+  template <typename OT, bool GATED>
+  __device__ __forceinline__ void operator()() { epilogue_tile_as<OT, GATED>(e, stage, taddr, part, parts, lane, prow0, tok0, ntok, release); }
+};
+template <typename F>
+__device__ __forceinline__ void epilogue_tile(const EpilogueTile &t, F release) { by_kind(t.e, EpilogueCall<F>{t, release}); }
 
-// The partial sums of T tokens, one value per lane and token, added up over the CTAs of the cluster in the order of their ranks.
-template <int T>
-__device__ __forceinline__ void join(const Epilogue &e, uint32_t at, int splits, int prow, long long tok0, int ntok) {
-  float v[T];
+// The partial sums of a tile, brought together over the CTAs of a cluster in the order of their ranks: blocks of 16 tokens go round the
+// CTAs, those of one CTA round its two halves of warps.  A thread's accumulators lie in the same place everywhere.
+struct JoinCall {
+  const Epilogue &e;
+  uint8_t *stage;
+  uint32_t part;          // of this thread's first accumulators in its own CTA's shared memory
+  int half, lane, prow0, rank, splits;
+  long long tok0;
+  int ntok;
+  template <typename OT, bool GATED>
+  __device__ __forceinline__ void operator()() {
+    EpilogueWarp<OT, GATED> w(e, stage, lane, prow0);
+#pragma unroll 1
+    for (int k = rank + half * splits; k * 16 < ntok; k += 2 * splits) {
+      w.fetch(tok0 + k * 16, ntok - k * 16);
+      float v[16];
 #pragma unroll
-  for (int i = 0; i < T; ++i) v[i] = 0.0f;
+      for (int i = 0; i < 16; ++i) v[i] = 0.0f;
 #pragma unroll 2
-  for (int r = 0; r < splits; ++r) {
-    uint32_t from;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from) : "r"(at), "r"(r));
-    float4 x[T / 4];
+      for (int r = 0; r < splits; ++r) {
+        uint32_t from;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from) : "r"(part + k * 4 * (GT_ROWS * 16)), "r"(r));
+        float4 x[4];
 #pragma unroll
-    for (int i = 0; i < T / 4; ++i)
-      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                   : "=f"(x[i].x), "=f"(x[i].y), "=f"(x[i].z), "=f"(x[i].w) : "r"(from + i * GT_ROWS * 16) : "memory");
+        for (int i = 0; i < 4; ++i)
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(x[i].x), "=f"(x[i].y), "=f"(x[i].z), "=f"(x[i].w) : "r"(from + i * (GT_ROWS * 16)) : "memory");
 #pragma unroll
-    for (int i = 0; i < T / 4; ++i) {
-      v[4 * i] += x[i].x; v[4 * i + 1] += x[i].y; v[4 * i + 2] += x[i].z; v[4 * i + 3] += x[i].w;
+        for (int i = 0; i < 4; ++i) { v[4 * i] += x[i].x; v[4 * i + 1] += x[i].y; v[4 * i + 2] += x[i].z; v[4 * i + 3] += x[i].w; }
+      }
+      uint32_t a[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) a[i] = __float_as_uint(v[i]);
+      w.block(a, tok0 + k * 16, ntok - k * 16, 0, 0, [] {});
     }
   }
-  emit<T>(e, v, prow, tok0, ntok);
-}
+};
 
 // ---- Few tiles: each belongs to a cluster of CTAs that share its channels.  The partial sums are brought together through
 // distributed shared memory in the order of the ranks, each CTA finishing a part of the tokens.
 template <int BN>
-__global__ void __launch_bounds__(THREADS) gemm_split_kernel(const __grid_constant__ GemmLaunch g) {
-  using L = GemmSmem<BN, false, SPLIT_RING<BN>>;
+__global__ void __launch_bounds__(64 + SPLIT_WARPS * 32) gemm_split_kernel(const __grid_constant__ GemmLaunch g) {
+  using L = GemmSmem<BN, false, SPLIT_RING<BN>, 0>;
   constexpr int STAGES = L::STAGES;
   constexpr uint32_t COLS = BN < 32 ? 32 : BN;
-  static_assert(BN * GT_ROWS * 4 <= L::BAR_OFF, "the partial sums lie in the ring");
+  constexpr int PART = BN * GT_ROWS * 4;                      // the epilogue runs when the ring has done: partial sums and staging lie in it
+  static_assert(PART + SPLIT_WARPS * EPI_STAGE <= L::STAGES * L::STAGE, "");
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = smem_1k(smem_raw);
   uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::BAR_OFF), *empty = full + STAGES, *tfull = empty + STAGES;
@@ -185,7 +166,7 @@ __global__ void __launch_bounds__(THREADS) gemm_split_kernel(const __grid_consta
     fence_proxy_async_smem();
   }
   __syncthreads();
-  if (warp == 1 || warp >= 4) {
+  if (warp >= 1) {
     // Tensor memory is taken when the kernel before this one has ended, and the kernel behind may start when it has been
     // taken: of two kernels on an SM, one that holds tensor memory never waits for one that still wants some.
     griddep_wait();
@@ -194,7 +175,7 @@ __global__ void __launch_bounds__(THREADS) gemm_split_kernel(const __grid_consta
       griddep_launch_dependents();
     }
     tc_fence_before_sync();
-    named_bar_sync(1, (1 + EPI_WARPS) * 32);
+    named_bar_sync(1, (1 + SPLIT_WARPS) * 32);
     tc_fence_after_sync();
   }
   const uint32_t tmem = warp == 0 ? 0u : *tmem_slot;
@@ -237,24 +218,25 @@ __global__ void __launch_bounds__(THREADS) gemm_split_kernel(const __grid_consta
     }
     if (ok) umma_commit_el(tfull, el);
   }
-  const int quarter = warp & 3, half = (warp - 4) >> 2, prow = row_tile * GT_ROWS + quarter * 32 + lane;
+  const int quarter = warp & 3, half = (warp - 2) >> 2, prow0 = row_tile * GT_ROWS + quarter * 32;
+  uint8_t *stage = smem + PART + (warp - 2) * EPI_STAGE;
   const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-  float4 *part = reinterpret_cast<float4 *>(smem);            // [token / 4][128 rows][4 tokens]
+  float4 *part = reinterpret_cast<float4 *>(smem) + quarter * 32 + lane;     // [block of 16 tokens][4][128 threads]
   bool ok = true;
-  if (warp >= 4) {
+  if (warp >= 2) {
     ok = mbar_wait_warp(tfull, 0, abort_flag);
     if (!ok) fail_code = ST_WAIT_TIMEOUT_EPILOGUE;
     tc_fence_after_sync();
-    if (ok && splits == 1) epilogue_tile(p.epi, taddr, half, prow, tok0, ntok, [] {});
+    if (ok && splits == 1) epilogue_tile({p.epi, stage, taddr, half, SPLIT_WARPS / 4, lane, prow0, tok0, ntok}, [] {});
     if (ok && splits > 1) {
 #pragma unroll 1
       for (int k = half; k < (ntok + 15) / 16; k += 2) {
         uint32_t a[16];
-        tmem_ld16(taddr + k * 16, a);
+        tmem_ld_block(taddr + k * 16, a);
         tmem_ld_wait16(a);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          part[(k * 4 + i) * GT_ROWS + quarter * 32 + lane] =
+          part[(k * 4 + i) * GT_ROWS] =
               make_float4(__uint_as_float(a[4 * i]), __uint_as_float(a[4 * i + 1]), __uint_as_float(a[4 * i + 2]), __uint_as_float(a[4 * i + 3]));
       }
     }
@@ -262,13 +244,7 @@ __global__ void __launch_bounds__(THREADS) gemm_split_kernel(const __grid_consta
   if (splits > 1) {
     __syncwarp();
     cluster_sync_all();
-    if (warp >= 4 && ok) {
-      // this CTA finishes every splits-th group of tokens, its warps of one half every second of those
-      constexpr int T = BN >= 64 ? 8 : 4;
-#pragma unroll 1
-      for (int t = (rank + half * splits) * T; t < ntok; t += 2 * splits * T)
-        join<T>(p.epi, smem_u32(part + t / 4 * GT_ROWS + quarter * 32 + lane), splits, prow, tok0 + t, ntok - t);
-    }
+    if (warp >= 2 && ok) by_kind(p.epi, JoinCall{p.epi, stage, smem_u32(part), half, lane, prow0, rank, splits, tok0, ntok});
     __syncwarp();
     cluster_sync_all();                                       // nobody leaves while its partial sums are read
   }
@@ -282,10 +258,10 @@ __global__ void __launch_bounds__(THREADS) gemm_split_kernel(const __grid_consta
 // ---- Many tiles: persistent CTAs, or pairs of them (PAIR: one tcgen05.mma.cta_group::2 for 256 packed rows, each CTA
 // holding its 128 and half of the tokens), two accumulators, so that a tile's epilogue runs beside the next one's products.
 template <int BN, bool PAIR, bool GROUPED>
-__global__ void __launch_bounds__(THREADS, 1) gemm_tiles_kernel(const __grid_constant__ GemmLaunch g) {
-  using L = GemmSmem<BN, PAIR, TILES_RING>;
+__global__ void __launch_bounds__(64 + TILES_WARPS * 32, 1) gemm_tiles_kernel(const __grid_constant__ GemmLaunch g) {
+  using L = GemmSmem<BN, PAIR, TILES_RING, TILES_WARPS>;
   constexpr int STAGES = L::STAGES, CTAS = PAIR ? 2 : 1;
-  constexpr uint32_t COLS = 2 * BN;
+  constexpr uint32_t ACC = BN < 32 ? 32 : BN, COLS = 2 * ACC;       // columns of an accumulator
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = smem_1k(smem_raw);
   uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::BAR_OFF), *empty = full + STAGES, *tfull = empty + STAGES, *tempty = tfull + 2;
@@ -299,7 +275,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_tiles_kernel(const __grid_con
     tma_prefetch_desc(&g.xmap);
     if (PAIR) tma_prefetch_desc(&g.wmap);
     for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-    for (int b = 0; b < 2; ++b) { mbar_init(&tfull[b], 1); mbar_init(&tempty[b], CTAS * EPI_WARPS); }
+    for (int b = 0; b < 2; ++b) { mbar_init(&tfull[b], 1); mbar_init(&tempty[b], CTAS * TILES_WARPS); }
     *abort_flag = 0;
     fence_barrier_init();
     fence_proxy_async_smem();
@@ -378,7 +354,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_tiles_kernel(const __grid_con
         const uint32_t idesc = umma_idesc(1, p.in_et == ET_BF16, p.in_et == ET_BF16, GT_ROWS * CTAS, columns(tile_of(i).ntok));
         if (!mbar_wait_warp(&tempty[b], ((count >> 1) & 1) ^ 1, abort_flag)) { fail_code = ST_WAIT_TIMEOUT_MMA; break; }
         tc_fence_after_sync();
-        const uint32_t d = tmem + b * BN;
+        const uint32_t d = tmem + b * ACC;
         for (int k = 0; k < p.kt; ++k, ++it) {
           const int s = it % STAGES;
           if (!mbar_wait_warp(&full[s], (it / STAGES) & 1, abort_flag)) { ok = false; fail_code = ST_WAIT_TIMEOUT_MMA; break; }
@@ -396,20 +372,22 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_tiles_kernel(const __grid_con
         if (ok) { if (PAIR) umma_commit_2cta_el(&tfull[b], el); else umma_commit_el(&tfull[b], el); }
       }
     }
-  } else if (warp >= 4) {
-    const int quarter = warp & 3, half = (warp - 4) >> 2;
+  } else if (warp >= 2) {
+    const int quarter = warp & 3, part = (warp - 2) >> 2;
     uint32_t count = 0;
     for (int i = first; i < total; i += step, ++count) {
       const Tile t = tile_of(i);
       const uint32_t b = count & 1;
       if (!mbar_wait_warp(&tfull[b], (count >> 1) & 1, abort_flag)) { fail_code = ST_WAIT_TIMEOUT_EPILOGUE; break; }
       tc_fence_after_sync();
-      epilogue_tile(p.epi, tmem + (static_cast<uint32_t>(quarter * 32) << 16) + b * BN, half, t.row_tile * GT_ROWS + quarter * 32 + lane, t.tok0,
-                        t.ntok, [&] {
-                          tc_fence_before_sync();
-                          __syncwarp();
-                          if (lane == 0) { if (PAIR) mbar_arrive_cluster(mapa_u32(&tempty[b], 0)); else mbar_arrive(&tempty[b]); }
-                        });
+      const int prow0 = t.row_tile * GT_ROWS + quarter * 32;
+      epilogue_tile({p.epi, smem + L::EPI_OFF + (warp - 2) * EPI_STAGE, tmem + (static_cast<uint32_t>(quarter * 32) << 16) + b * ACC, part, TILES_WARPS / 4, lane,
+                     prow0, t.tok0, t.ntok},
+                    [&] {
+                      tc_fence_before_sync();
+                      __syncwarp();
+                      if (lane == 0) { if (PAIR) mbar_arrive_cluster(mapa_u32(&tempty[b], 0)); else mbar_arrive(&tempty[b]); }
+                    });
     }
   }
   __syncwarp();
@@ -441,10 +419,10 @@ bool encode_rows(CUtensorMap *m, int et, const void *base, long long inner, long
 }
 
 template <typename K>
-cudaError_t launch_gemm_kernel(K kern, const GemmLaunch &g, int grid, int smem, int cluster, cudaStream_t s) {
+cudaError_t launch_gemm_kernel(K kern, const GemmLaunch &g, int grid, int warps, int smem, int cluster, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(THREADS);
+  cfg.blockDim = dim3(64 + warps * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute at[2];
@@ -459,14 +437,14 @@ cudaError_t launch_gemm_kernel(K kern, const GemmLaunch &g, int grid, int smem, 
 
 template <int BN>
 cudaError_t go_split(GemmLaunch &g, cudaStream_t s) {
-  using L = GemmSmem<BN, false, SPLIT_RING<BN>>;
+  using L = GemmSmem<BN, false, SPLIT_RING<BN>, 0>;
   if (!encode_rows(&g.xmap, g.p.in_et, g.p.x, g.p.ic, g.p.rows, g.p.ld_x * 2, GT_K, BN, true)) return cudaErrorInvalidValue;
-  return launch_gemm_kernel(gemm_split_kernel<BN>, g, g.p.row_tiles * g.token_tiles * g.splits, L::TOTAL, g.splits, s);
+  return launch_gemm_kernel(gemm_split_kernel<BN>, g, g.p.row_tiles * g.token_tiles * g.splits, SPLIT_WARPS, L::TOTAL, g.splits, s);
 }
 
 template <int BN, bool PAIR, bool GROUPED>
 cudaError_t go_tiles(GemmLaunch &g, cudaStream_t s) {
-  using L = GemmSmem<BN, PAIR, TILES_RING>;
+  using L = GemmSmem<BN, PAIR, TILES_RING, TILES_WARPS>;
   const GemmParams &p = g.p;
   const int ctas = PAIR ? 2 : 1, row_steps = (p.row_tiles + ctas - 1) / ctas;
   // dense: one copy brings a CTA's tokens; grouped: tiles have any number of them, in boxes of up to 32
@@ -476,7 +454,7 @@ cudaError_t go_tiles(GemmLaunch &g, cudaStream_t s) {
   const long long tiles = (long long)g.token_tiles * row_steps;
   const int most = PAIR ? p.max_pairs : p.num_sms;
   const int grid = (int)(tiles < most ? tiles : most) * ctas;
-  return launch_gemm_kernel(gemm_tiles_kernel<BN, PAIR, GROUPED>, g, grid, L::TOTAL, ctas, s);
+  return launch_gemm_kernel(gemm_tiles_kernel<BN, PAIR, GROUPED>, g, grid, TILES_WARPS, L::TOTAL, ctas, s);
 }
 
 template <typename K>
@@ -485,7 +463,7 @@ cudaError_t allow(K kern, int smem) { return cudaFuncSetAttribute(kern, cudaFunc
 }  // namespace
 
 cudaError_t launch_pack_weights(void *dst, const void *src, int experts, int rows, int ic, bool gated, bool hwio, cudaStream_t s) {
-  const int kt = (ic + GT_K - 1) / GT_K, row_tiles = (rows + GT_ROWS - 1) / GT_ROWS;
+  const int kt = (ic + GT_K - 1) / GT_K, row_tiles = (packed_rows(gated ? rows / 2 : rows, gated) + GT_ROWS - 1) / GT_ROWS;
   const long long per = (long long)row_tiles * kt * GT_ROWS * 8, chunks = per * experts;
   const int blocks = (int)(chunks / 256 + 1 < 148 * 64 ? chunks / 256 + 1 : 148 * 64);
   pack_weights_kernel<<<blocks, 256, 0, s>>>(static_cast<uint4 *>(dst), static_cast<const uint16_t *>(src), rows, ic, kt, row_tiles,
@@ -508,22 +486,22 @@ cudaError_t launch_align_rows(void *dst, long long pitch, const void *src, long 
 cudaError_t init_gemm(int num_sms, int *max_pairs) {
   cudaError_t e = cudaSuccess;
   auto want = [&](cudaError_t r) { if (e == cudaSuccess) e = r; };
-  want(allow(gemm_split_kernel<16>, GemmSmem<16, false, SPLIT_RING<16>>::TOTAL));
-  want(allow(gemm_split_kernel<32>, GemmSmem<32, false, SPLIT_RING<32>>::TOTAL));
-  want(allow(gemm_split_kernel<64>, GemmSmem<64, false, SPLIT_RING<64>>::TOTAL));
-  want(allow(gemm_split_kernel<128>, GemmSmem<128, false, SPLIT_RING<128>>::TOTAL));
-  want(allow(gemm_split_kernel<256>, GemmSmem<256, false, SPLIT_RING<256>>::TOTAL));
-  want(allow(gemm_tiles_kernel<256, true, false>, GemmSmem<256, true, TILES_RING>::TOTAL));
-  want(allow(gemm_tiles_kernel<16, false, true>, GemmSmem<16, false, TILES_RING>::TOTAL));
-  want(allow(gemm_tiles_kernel<32, false, true>, GemmSmem<32, false, TILES_RING>::TOTAL));
-  want(allow(gemm_tiles_kernel<64, false, true>, GemmSmem<64, false, TILES_RING>::TOTAL));
-  want(allow(gemm_tiles_kernel<128, false, true>, GemmSmem<128, false, TILES_RING>::TOTAL));
-  want(allow(gemm_tiles_kernel<256, true, true>, GemmSmem<256, true, TILES_RING>::TOTAL));
+  want(allow(gemm_split_kernel<16>, GemmSmem<16, false, SPLIT_RING<16>, 0>::TOTAL));
+  want(allow(gemm_split_kernel<32>, GemmSmem<32, false, SPLIT_RING<32>, 0>::TOTAL));
+  want(allow(gemm_split_kernel<64>, GemmSmem<64, false, SPLIT_RING<64>, 0>::TOTAL));
+  want(allow(gemm_split_kernel<128>, GemmSmem<128, false, SPLIT_RING<128>, 0>::TOTAL));
+  want(allow(gemm_split_kernel<256>, GemmSmem<256, false, SPLIT_RING<256>, 0>::TOTAL));
+  want(allow(gemm_tiles_kernel<256, true, false>, GemmSmem<256, true, TILES_RING, TILES_WARPS>::TOTAL));
+  want(allow(gemm_tiles_kernel<16, false, true>, GemmSmem<16, false, TILES_RING, TILES_WARPS>::TOTAL));
+  want(allow(gemm_tiles_kernel<32, false, true>, GemmSmem<32, false, TILES_RING, TILES_WARPS>::TOTAL));
+  want(allow(gemm_tiles_kernel<64, false, true>, GemmSmem<64, false, TILES_RING, TILES_WARPS>::TOTAL));
+  want(allow(gemm_tiles_kernel<128, false, true>, GemmSmem<128, false, TILES_RING, TILES_WARPS>::TOTAL));
+  want(allow(gemm_tiles_kernel<256, true, true>, GemmSmem<256, true, TILES_RING, TILES_WARPS>::TOTAL));
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(num_sms / 2 * 2);
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = GemmSmem<256, true, TILES_RING>::TOTAL;
+  cfg.blockDim = dim3(64 + TILES_WARPS * 32);
+  cfg.dynamicSmemBytes = GemmSmem<256, true, TILES_RING, TILES_WARPS>::TOTAL;
   cudaLaunchAttribute at = {};
   at.id = cudaLaunchAttributeClusterDimension;
   at.val.clusterDim.x = 2; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;

@@ -199,7 +199,7 @@ int pack(elb_op &op, void **dst, const void *src, int experts, int64_t rows, int
   Staged st;
   int rc = st.take(src, (size_t)experts * rows * ic * 2);
   if (rc != ELB_OK) return rc;
-  const size_t bytes = (size_t)experts * (up(rows, GT_ROWS) / GT_ROWS) * (up(ic, GT_K) / GT_K) * GT_BYTES;
+  const size_t bytes = (size_t)experts * (up(packed_rows(gated ? rows / 2 : rows, gated), GT_ROWS) / GT_ROWS) * (up(ic, GT_K) / GT_K) * GT_BYTES;
   rc = alloc(op, dst, bytes);
   if (rc != ELB_OK) return rc;
   OP_TRY(launch_pack_weights(*dst, st.p, experts, (int)rows, ic, gated, hwio, nullptr));
@@ -276,7 +276,7 @@ int elb_linear_prepare(elb_op_t *op, const void *weights, const void *bias) {
   const int rows = d.gated ? 2 * d.oc : d.oc;
   OP_TRY(cudaDeviceSynchronize());                // whatever stream the caller's tensors come from
   rc = pack(*op, &op->w[0], weights, 1, rows, d.ic, d.gated, d.fmt_weights == ELB_HWIO);
-  if (rc == ELB_OK && d.with_bias) rc = vector_f32(*op, &op->f[0], bias, et_of(d.dt_bias), rows, (int)up(rows, 2 * GT_ROWS), d.gated);
+  if (rc == ELB_OK && d.with_bias) rc = vector_f32(*op, &op->f[0], bias, et_of(d.dt_bias), rows, (int)up(packed_rows(d.oc, d.gated), 2 * GT_ROWS), d.gated);
   return drop(*op, rc);
 }
 
@@ -296,7 +296,7 @@ int elb_linear_enqueue(elb_op_t *op, void *output, const void *input, const void
   p.rows = (int)rows;
   p.ic = d.ic;
   p.kt = (int)(up(d.ic, GT_K) / GT_K);
-  p.row_tiles = (int)(up(d.gated ? 2 * d.oc : d.oc, GT_ROWS) / GT_ROWS);
+  p.row_tiles = (int)(up(packed_rows(d.oc, d.gated), GT_ROWS) / GT_ROWS);
   p.w_rows = (long long)p.row_tiles * p.kt * GT_ROWS;
   p.in_et = et_of(d.dt_input);
   p.num_sms = op->num_sms;
@@ -312,7 +312,8 @@ int elb_linear_enqueue(elb_op_t *op, void *output, const void *input, const void
   p.epi.gated = d.gated;
   p.epi.out_et = et_of(d.dt_output);
   p.epi.scale = d.scale;
-  p.epi.pairs = aligned(output, 4) && d.ld_output % 2 == 0 && (!p.epi.res || (aligned(residual, 4) && d.ld_residual % 2 == 0));
+  const int64_t per = 16 / ob;       // elements of 16 bytes
+  p.epi.words = aligned(output, 16) && d.ld_output % per == 0 && (!p.epi.res || (aligned(residual, 16) && d.ld_residual % per == 0));
   const cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
   if (aligned(input, 16) && d.ld_input % 8 == 0) {
     OP_TRY(launch_gemm(p, s));
@@ -543,7 +544,7 @@ int elb_experts_enqueue(elb_op_t *op, void *output, const void *input, const int
   e.out = output;
   e.ids = ids;
   e.weights = weights;
-  const int slots = (int)(rows * d.top_k), wide = d.gated ? 2 * d.mid : d.mid;
+  const int slots = (int)(rows * d.top_k), wide = packed_rows(d.mid, d.gated);
   e.tile_tokens = grouped_tile_tokens(slots, d.experts);
   GemmParams p = {};
   p.tiles = e.tiles;
@@ -554,7 +555,7 @@ int elb_experts_enqueue(elb_op_t *op, void *output, const void *input, const int
   p.num_sms = op->num_sms;
   p.max_pairs = op->max_pairs;
   p.status = op->d_status;
-  p.epi.pairs = 1;
+  p.epi.words = 1;
   p.epi.scale = 1.0f;
   GemmParams q = p;
   p.w = static_cast<const uint8_t *>(op->w[0]);
@@ -568,7 +569,7 @@ int elb_experts_enqueue(elb_op_t *op, void *output, const void *input, const int
   p.w_rows = (long long)d.experts * p.row_tiles * p.kt * GT_ROWS;
   p.epi.out = op->mid;
   p.epi.ld_out = op->pitch_mid;
-  p.epi.oc = d.mid;
+  p.epi.oc = (int)op->pitch_mid;          // (channels past the end are products with rows of zeros)
   p.epi.act = d.activation;
   p.epi.gated = d.gated;
   p.epi.out_et = e.et;
@@ -583,7 +584,7 @@ int elb_experts_enqueue(elb_op_t *op, void *output, const void *input, const int
   q.w_rows = (long long)d.experts * q.row_tiles * q.kt * GT_ROWS;
   q.epi.out = const_cast<float *>(e.y);
   q.epi.ld_out = e.pitch_y;
-  q.epi.oc = d.ic;
+  q.epi.oc = (int)e.pitch_y;
   q.epi.out_et = ET_F32;
   if (op->count_stale) OP_TRY(cudaMemsetAsync(e.count, 0, d.experts * sizeof(int), s));
   op->count_stale = true;

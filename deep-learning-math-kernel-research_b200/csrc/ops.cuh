@@ -40,211 +40,31 @@ template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
   return __half22float2(*reinterpret_cast<const __half2 *>(&w));
 }
 
-// ---------------------------------------------------------------------------------------------
-// Epilogue of the matrix products.  The products are computed with the weights as the left operand, so
-// that a lane of a warp holds one weight row for several tokens: 32 lanes are 32 consecutive packed rows,
-// which are channels, or gate and up rows in turn (row 2q the gate of channel q, row 2q + 1 its up).
-// ---------------------------------------------------------------------------------------------
+// What becomes of the products (gemm_epilogue.cuh).  Packed rows are output channels in order, or, gated, groups of 16: the
+// gates of eight channels, then their ups.
 struct Epilogue {
   void *out;
   const void *res;          // null: no residual
-  const float *bias;        // in packed row order, padded with zeros to whole tiles; null: none
+  const float *bias;        // in packed row order, padded with zeros to whole pairs of tiles; null: none
   long long ld_out, ld_res;
   int oc;                   // output channels (packed rows are 2 * oc where gated)
   int act, gated, out_et;
-  int pairs;                // 16-bit results: out and res allow 4-byte accesses at even channels
+  int words;                // rows of out and res start at 16-byte boundaries
   float scale;
 };
-
-template <int N>
-__device__ __forceinline__ void activate(float (&v)[N], int act) {
-  switch (act) {
-    case 1:
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];       // (a NaN stays one)
-      break;
-    case 2:
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = 0.5f * v[i] * (1.0f + erff(v[i] * 0.70710678118654752f));
-      break;
-    case 3:   // 0.5 z (1 + tanh u) = z / (1 + exp(-2 u))
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float u2 = 1.5957691216057308f * (v[i] + 0.044715f * v[i] * v[i] * v[i]);
-        v[i] = __fdividef(v[i], 1.0f + __expf(-u2));
-      }
-      break;
-    case 4:
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = __fdividef(v[i], 1.0f + __expf(-v[i]));
-      break;
-    default: break;
-  }
-}
-
-// v[j]: packed row `prow` (this lane's) of token tok0 + j, of which ntok are real.  A converged warp, prow - lane a
-// multiple of 32.
-template <typename OT, int NT>
-__device__ __forceinline__ void emit_as(const Epilogue &e, float (&v)[NT], int prow, long long tok0, int ntok) {
-  const int odd = prow & 1;
-  OT *out = static_cast<OT *>(e.out);
-  const OT *res = static_cast<const OT *>(e.res);
-  if (e.bias) {
-    const float b = e.bias[prow];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) v[j] += b;
-  }
-  if (e.gated) {
-    // The even lane holds the gate and the odd one the up row of a channel: they trade half of their tokens, after
-    // which the even lane has both for the even tokens and the odd lane for the odd ones.
-    float g[NT / 2], u[NT / 2];
-#pragma unroll
-    for (int j = 0; j < NT / 2; ++j) {
-      const float got = __shfl_xor_sync(0xFFFFFFFFu, odd ? v[2 * j] : v[2 * j + 1], 1);
-      g[j] = odd ? got : v[2 * j];
-      u[j] = odd ? v[2 * j + 1] : got;
-    }
-    activate(g, e.act);
-    const int ch = prow >> 1;
-#pragma unroll
-    for (int j = 0; j < NT / 2; ++j) {
-      const int t = 2 * j + odd;
-      if (t < ntok && ch < e.oc) {
-        float y = g[j] * u[j] * e.scale;
-        if (res) y += to_f32(res[(tok0 + t) * e.ld_res + ch]);
-        out[(tok0 + t) * e.ld_out + ch] = from_f32<OT>(y);
-      }
-    }
-    return;
-  }
-  activate(v, e.act);
-  if constexpr (sizeof(OT) == 2) {
-    if (e.pairs) {
-      // neighbouring lanes trade half of their tokens, so that each holds two channels of every second token
-      const int ch = prow & ~1;
-#pragma unroll
-      for (int j = 0; j < NT / 2; ++j) {
-        const float got = __shfl_xor_sync(0xFFFFFFFFu, odd ? v[2 * j] : v[2 * j + 1], 1);
-        float lo = (odd ? got : v[2 * j]) * e.scale, hi = (odd ? v[2 * j + 1] : got) * e.scale;
-        const int t = 2 * j + odd;
-        if (t < ntok && ch + 1 < e.oc) {
-          if (res) {
-            const float2 r = unpack2<OT>(*reinterpret_cast<const uint32_t *>(res + (tok0 + t) * e.ld_res + ch));
-            lo += r.x;
-            hi += r.y;
-          }
-          *reinterpret_cast<uint32_t *>(out + (tok0 + t) * e.ld_out + ch) = pack2<OT>(lo, hi);
-        } else if (t < ntok && ch < e.oc) {
-          if (res) lo += to_f32(res[(tok0 + t) * e.ld_res + ch]);
-          out[(tok0 + t) * e.ld_out + ch] = from_f32<OT>(lo);
-        }
-      }
-      return;
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    if (j < ntok && prow < e.oc) {
-      float y = v[j] * e.scale;
-      if (res) y += to_f32(res[(tok0 + j) * e.ld_res + prow]);
-      out[(tok0 + j) * e.ld_out + prow] = from_f32<OT>(y);
-    }
-  }
-}
-template <int NT>
-__device__ __forceinline__ void emit(const Epilogue &e, float (&v)[NT], int prow, long long tok0, int ntok) {
-  if (e.out_et == ET_BF16) emit_as<__nv_bfloat16, NT>(e, v, prow, tok0, ntok);
-  else if (e.out_et == ET_F16) emit_as<__half, NT>(e, v, prow, tok0, ntok);
-  else emit_as<float, NT>(e, v, prow, tok0, ntok);
-}
-
-// The same for 16 real tokens and a warp whose channels all exist, 16-bit results and residuals at even channels in 4-byte
-// words: `out` and `res` are this lane's first element, from first_element().  Without the tests of the general form a
-// token costs a warp about 5 instructions instead of 38, which is what a long call's epilogue is bound by.
-template <typename OT, bool GATED>
-__device__ __forceinline__ long long first_token(int prow) {     // of the 16, the first that this lane stores
-  if (!GATED) return sizeof(OT) == 2 ? prow & 1 : 0;
-  return sizeof(OT) == 2 ? (prow & 2) + (prow & 1) : prow & 1;
-}
-template <typename OT, bool GATED>
-__device__ __forceinline__ int first_channel(int prow) {
-  if (!GATED) return sizeof(OT) == 2 ? prow & ~1 : prow;
-  return sizeof(OT) == 2 ? (prow >> 1) & ~1 : prow >> 1;
-}
-template <typename OT, bool GATED>
-__device__ __forceinline__ void emit_full(const Epilogue &e, float (&v)[16], int prow, float bias, OT *out, const OT *res) {
-  const int odd = prow & 1;
-#pragma unroll
-  for (int j = 0; j < 16; ++j) v[j] += bias;
-  constexpr int EACH = sizeof(OT) == 2 ? (GATED ? 4 : 2) : (GATED ? 2 : 1);     // tokens from one of this lane's stores to the next
-  constexpr int N = 16 / EACH;
-  const long long so = e.ld_out * EACH, sr = e.ld_res * EACH;
-  if constexpr (GATED) {
-    float y[8], u[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float got = __shfl_xor_sync(0xFFFFFFFFu, odd ? v[2 * j] : v[2 * j + 1], 1);
-      y[j] = odd ? got : v[2 * j];
-      u[j] = odd ? v[2 * j + 1] : got;
-    }
-    activate(y, e.act);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = y[j] * u[j] * e.scale;
-    if constexpr (sizeof(OT) == 4) {
-      float r[8] = {};
-      if (res) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) r[j] = res[j * sr];
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) out[j * so] = y[j] + r[j];
-    } else {
-      // a second trade, between lanes of neighbouring channels: two channels of every fourth token
-      const int high = prow & 2;
-      uint32_t r[4] = {};
-      if (res) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) r[j] = *reinterpret_cast<const uint32_t *>(res + j * sr);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float got = __shfl_xor_sync(0xFFFFFFFFu, high ? y[2 * j] : y[2 * j + 1], 2);
-        const float2 add = unpack2<OT>(r[j]);
-        *reinterpret_cast<uint32_t *>(out + j * so) = pack2<OT>((high ? got : y[2 * j]) + add.x, (high ? y[2 * j + 1] : got) + add.y);
-      }
-    }
-  } else {
-    activate(v, e.act);
-    if constexpr (sizeof(OT) == 4) {
-      float r[16] = {};
-      if (res) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) r[j] = res[j * sr];
-      }
-#pragma unroll
-      for (int j = 0; j < 16; ++j) out[j * so] = fmaf(v[j], e.scale, r[j]);
-    } else {
-      uint32_t r[N] = {};
-      if (res) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) r[j] = *reinterpret_cast<const uint32_t *>(res + j * sr);
-      }
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const float got = __shfl_xor_sync(0xFFFFFFFFu, odd ? v[2 * j] : v[2 * j + 1], 1);
-        const float2 add = unpack2<OT>(r[j]);
-        *reinterpret_cast<uint32_t *>(out + j * so) =
-            pack2<OT>(fmaf(odd ? got : v[2 * j], e.scale, add.x), fmaf(odd ? v[2 * j + 1] : got, e.scale, add.y));
-      }
-    }
-  }
+// the source's row of packed row p, of `rows` (2 * oc where gated); rows or more: none, a row of zeros
+__host__ __device__ inline int packed_source(int p, int rows, bool gated) {
+  if (!gated) return p;
+  const int ch = (p >> 4) * 8 + (p & 7), oc = rows >> 1;
+  return ch < oc ? ch + ((p >> 3) & 1) * oc : rows;
 }
 
 // ---------------------------------------------------------------------------------------------
 // Matrix products on packed weights.  The packed image is the shared-memory operand image itself: tiles of 128 rows x
 // 64 channels, [row tile][channel tile][128 rows][128 bytes], the 16-byte chunks of a row permuted as the 128-byte
-// swizzle has them; rows and channels past the end are zero.
+// swizzle has them; rows and channels past the end are zero.  (packed_rows: 16 for every 8 channels where gated.)
 // ---------------------------------------------------------------------------------------------
+inline int packed_rows(int oc, bool gated) { return gated ? (oc + 7) / 8 * 16 : oc; }
 constexpr int GT_ROWS = 128, GT_K = 64, GT_BYTES = GT_ROWS * GT_K * 2;
 
 // Rows of one expert: input rows [row0, row0 + count) of the sorted rows.
