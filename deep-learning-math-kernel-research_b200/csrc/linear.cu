@@ -1,4 +1,6 @@
 // Matrix products of the transformer operators, dense and grouped by expert, on packed weights (ops.cuh).
+#include <cmath>
+
 #include "elb_common.cuh"
 #include "gemm_epilogue.cuh"
 #include "ops.cuh"
@@ -6,9 +8,11 @@
 
 namespace elb {
 
-// Bytes of the operand rings.  With few tokens the kernel of few tiles leaves room for a second CTA on its SM: of its own
-// launch, or of the next one, whose weights then arrive while this one ends.
-template <int BN> constexpr int SPLIT_RING = (BN <= 32 ? 110 : 224) * 1024;
+// Bytes of the operand rings.  The kernel of few tiles with few tokens and shared channels leaves room for a second CTA on its
+// SM (the next launch's weights arrive while this one ends, and clusters of eight find a place: 16 x 2048 -> 2048 8.6 us, 12.8 with
+// the large ring); a CTA that streams a whole row tile wants all of the SM's memory for loads in flight (24 x 4096 -> 16384
+// 23.4 us, 29.0 with the small ring).
+constexpr int SMALL_RING = 110 * 1024, LARGE_RING = 224 * 1024;
 constexpr int TILES_RING = 192 * 1024;
 
 namespace {
@@ -57,7 +61,8 @@ __global__ void pack_bias_kernel(float *dst, const void *src, int et, int rows, 
 // tensor (rows and channels outside it arrive as zeros).  Few tokens then cost a narrow MMA and not a padded one, and the
 // weights, which are what a small call is made of, stream through shared memory once.
 // ---------------------------------------------------------------------------------------------
-// Warp 0 produces, 1 issues the MMAs, the others are the epilogue's: more of them where a CTA has its SM to itself
+// Few tiles: warp 0 produces, 1 issues the MMAs, 2 to 9 are the epilogue's.  Many tiles: 0 and 2 produce, 1 issues, 3 idles, 4 to
+// 15 are the epilogue's.
 constexpr int SPLIT_WARPS = 8, TILES_WARPS = 12;
 
 template <int BN, bool PAIR, int RING, int EPI_WARPS>
@@ -139,9 +144,9 @@ struct JoinCall {
 
 // ---- Few tiles: each belongs to a cluster of CTAs that share its channels.  The partial sums are brought together through
 // distributed shared memory in the order of the ranks, each CTA finishing a part of the tokens.
-template <int BN>
+template <int BN, int RING>
 __global__ void __launch_bounds__(64 + SPLIT_WARPS * 32) gemm_split_kernel(const __grid_constant__ GemmLaunch g) {
-  using L = GemmSmem<BN, false, SPLIT_RING<BN>, 0>;
+  using L = GemmSmem<BN, false, RING, 0>;
   constexpr int STAGES = L::STAGES;
   constexpr uint32_t COLS = BN < 32 ? 32 : BN;
   constexpr int PART = BN * GT_ROWS * 4;                      // the epilogue runs when the ring has done: partial sums and staging lie in it
@@ -183,24 +188,24 @@ __global__ void __launch_bounds__(64 + SPLIT_WARPS * 32) gemm_split_kernel(const
   if (warp == 0) {
     const uint32_t el = elect_one();
     const uint8_t *w = p.w + ((size_t)row_tile * p.kt + k0) * GT_BYTES;
-    // the weights are the plan's own: their first copies need not wait for the kernel before this one
+    // The weights are the plan's own: their first copies need not wait for the kernel before this one.  Issuing a copy takes a
+    // thread some 250 cycles, lanes side by side take them together: the first stages are a lane's each.
     const int ahead = min(STAGES, steps);
-    if (el)
-      for (int i = 0; i < ahead; ++i) {
-        mbar_arrive_expect_tx(&full[i], L::STAGE);
-        tma_bulk_g2s(smem + i * L::STAGE, w + (size_t)i * GT_BYTES, GT_BYTES, &full[i]);
-      }
+    if (lane < ahead) {
+      mbar_arrive_expect_tx(&full[lane], L::STAGE);
+      tma_bulk_g2s(smem + lane * L::STAGE, w + (size_t)lane * GT_BYTES, GT_BYTES, &full[lane]);
+    }
     griddep_wait();
-    for (int i = 0; i < steps; ++i) {
+    if (lane < ahead) tma_tile_2d(smem + lane * L::STAGE + GT_BYTES, &g.xmap, (k0 + lane) * GT_K, tok0, &full[lane]);
+    __syncwarp();
+    for (int i = ahead; i < steps; ++i) {
       const int s = i % STAGES;
-      if (i >= ahead) {
-        if (!mbar_wait_warp(&empty[s], ((i / STAGES) & 1) ^ 1, abort_flag)) { fail_code = ST_WAIT_TIMEOUT_PRODUCER; break; }
-        if (el) {
-          mbar_arrive_expect_tx(&full[s], L::STAGE);
-          tma_bulk_g2s(smem + s * L::STAGE, w + (size_t)i * GT_BYTES, GT_BYTES, &full[s]);
-        }
+      if (!mbar_wait_warp(&empty[s], ((i / STAGES) & 1) ^ 1, abort_flag)) { fail_code = ST_WAIT_TIMEOUT_PRODUCER; break; }
+      if (el) {
+        mbar_arrive_expect_tx(&full[s], L::STAGE);
+        tma_bulk_g2s(smem + s * L::STAGE, w + (size_t)i * GT_BYTES, GT_BYTES, &full[s]);
+        tma_tile_2d(smem + s * L::STAGE + GT_BYTES, &g.xmap, (k0 + i) * GT_K, tok0, &full[s]);
       }
-      if (el) tma_tile_2d(smem + s * L::STAGE + GT_BYTES, &g.xmap, (k0 + i) * GT_K, tok0, &full[s]);
     }
   } else if (warp == 1) {
     const uint32_t el = elect_one();
@@ -258,7 +263,7 @@ __global__ void __launch_bounds__(64 + SPLIT_WARPS * 32) gemm_split_kernel(const
 // ---- Many tiles: persistent CTAs, or pairs of them (PAIR: one tcgen05.mma.cta_group::2 for 256 packed rows, each CTA
 // holding its 128 and half of the tokens), two accumulators, so that a tile's epilogue runs beside the next one's products.
 template <int BN, bool PAIR, bool GROUPED>
-__global__ void __launch_bounds__(64 + TILES_WARPS * 32, 1) gemm_tiles_kernel(const __grid_constant__ GemmLaunch g) {
+__global__ void __launch_bounds__(128 + TILES_WARPS * 32, 1) gemm_tiles_kernel(const __grid_constant__ GemmLaunch g) {
   using L = GemmSmem<BN, PAIR, TILES_RING, TILES_WARPS>;
   constexpr int STAGES = L::STAGES, CTAS = PAIR ? 2 : 1;
   constexpr uint32_t ACC = BN < 32 ? 32 : BN, COLS = 2 * ACC;       // columns of an accumulator
@@ -314,9 +319,13 @@ __global__ void __launch_bounds__(64 + TILES_WARPS * 32, 1) gemm_tiles_kernel(co
   // Only as many columns as a tile has tokens are multiplied, in steps of 16 per CTA; CTA 1 of a pair holds the second half.
   auto columns = [](int ntok) { return (ntok + 16 * CTAS - 1) / (16 * CTAS) * (16 * CTAS); };
   int fail_code = 0;
-  if (warp == 0) {
+  if (warp == 0 || warp == 2) {
+    // Two producers, of the weights and of the tokens: issuing a stage's copies from one thread took 500 cycles, as long as the
+    // stage's MMAs.
+    const bool weights = warp == 0;
     const uint32_t el = elect_one();
-    uint32_t it = 0;
+    int s = 0;
+    uint32_t phase = 1;
     bool ok = true;
     for (int i = first; i < total && ok; i += step) {
       const Tile t = tile_of(i);
@@ -324,30 +333,30 @@ __global__ void __launch_bounds__(64 + TILES_WARPS * 32, 1) gemm_tiles_kernel(co
       const uint8_t *w = p.w + t.expert * p.w_stride + (size_t)rt * p.kt * GT_BYTES;
       const int wrow = PAIR ? (int)((t.expert * p.w_stride / GT_BYTES + (size_t)rt * p.kt) * GT_ROWS) : 0;
       const int mine = columns(t.ntok) / CTAS, boxes = (mine + g.box - 1) / g.box, x0 = t.tok0 + rank * mine;
-      const uint32_t bytes = GT_BYTES + boxes * g.box * 128;
-      for (int k = 0; k < p.kt; ++k, ++it) {
-        const int s = it % STAGES;
-        if (!mbar_wait_warp(&empty[s], ((it / STAGES) & 1) ^ 1, abort_flag)) { ok = false; fail_code = ST_WAIT_TIMEOUT_PRODUCER; break; }
+      const uint32_t bytes = CTAS * (GT_BYTES + boxes * g.box * 128);
+      for (int k = 0; k < p.kt; ++k) {
+        if (!mbar_wait_warp(&empty[s], phase, abort_flag)) { ok = false; fail_code = ST_WAIT_TIMEOUT_PRODUCER; break; }
         uint8_t *dst = smem + s * L::STAGE;
-        if (el) {
-          if (PAIR) {
-            const uint32_t bar = mapa_u32(&full[s], 0);
-            if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * bytes);
-            tma_tile_2d_pair(dst, &g.wmap, 0, wrow + k * GT_ROWS, bar);
-            for (int j = 0; j < boxes; ++j) tma_tile_2d_pair(dst + GT_BYTES + j * g.box * 128, &g.xmap, k * GT_K, x0 + j * g.box, bar);
-          } else {
-            mbar_arrive_expect_tx(&full[s], bytes);
-            tma_bulk_g2s(dst, w + (size_t)k * GT_BYTES, GT_BYTES, &full[s]);
-            for (int j = 0; j < boxes; ++j) tma_tile_2d(dst + GT_BYTES + j * g.box * 128, &g.xmap, k * GT_K, x0 + j * g.box, &full[s]);
+        if (weights) {
+          if (el) {
+            if (rank == 0) mbar_arrive_expect_tx(&full[s], bytes);
+            if (PAIR) tma_tile_2d_pair(dst, &g.wmap, 0, wrow + k * GT_ROWS, mapa_u32(&full[s], 0));
+            else tma_bulk_g2s(dst, w + (size_t)k * GT_BYTES, GT_BYTES, &full[s]);
           }
+        } else if (lane < boxes) {                             // (a lane per box)
+          uint8_t *to = dst + GT_BYTES + lane * g.box * 128;
+          if (PAIR) tma_tile_2d_pair(to, &g.xmap, k * GT_K, x0 + lane * g.box, mapa_u32(&full[s], 0));
+          else tma_tile_2d(to, &g.xmap, k * GT_K, x0 + lane * g.box, &full[s]);
         }
         __syncwarp();
+        if (++s == STAGES) { s = 0; phase ^= 1; }
       }
     }
   } else if (warp == 1) {
     if (rank == 0) {
       const uint32_t el = elect_one();
-      uint32_t it = 0, count = 0;
+      uint32_t count = 0, phase = 0;
+      int s = 0;
       bool ok = true;
       for (int i = first; i < total && ok; i += step, ++count) {
         const uint32_t b = count & 1;
@@ -355,9 +364,8 @@ __global__ void __launch_bounds__(64 + TILES_WARPS * 32, 1) gemm_tiles_kernel(co
         if (!mbar_wait_warp(&tempty[b], ((count >> 1) & 1) ^ 1, abort_flag)) { fail_code = ST_WAIT_TIMEOUT_MMA; break; }
         tc_fence_after_sync();
         const uint32_t d = tmem + b * ACC;
-        for (int k = 0; k < p.kt; ++k, ++it) {
-          const int s = it % STAGES;
-          if (!mbar_wait_warp(&full[s], (it / STAGES) & 1, abort_flag)) { ok = false; fail_code = ST_WAIT_TIMEOUT_MMA; break; }
+        for (int k = 0; k < p.kt; ++k) {
+          if (!mbar_wait_warp(&full[s], phase, abort_flag)) { ok = false; fail_code = ST_WAIT_TIMEOUT_MMA; break; }
           tc_fence_after_sync();
           const uint32_t a = smem_u32(smem + s * L::STAGE);
           const uint64_t ad = umma_desc_sw128(a), bd = umma_desc_sw128(a + GT_BYTES);
@@ -368,12 +376,13 @@ __global__ void __launch_bounds__(64 + TILES_WARPS * 32, 1) gemm_tiles_kernel(co
           }
           if (PAIR) umma_commit_2cta_el(&empty[s], el);
           else umma_commit_el(&empty[s], el);
+          if (++s == STAGES) { s = 0; phase ^= 1; }
         }
         if (ok) { if (PAIR) umma_commit_2cta_el(&tfull[b], el); else umma_commit_el(&tfull[b], el); }
       }
     }
-  } else if (warp >= 2) {
-    const int quarter = warp & 3, part = (warp - 2) >> 2;
+  } else if (warp >= 4) {
+    const int quarter = warp & 3, part = (warp - 4) >> 2;
     uint32_t count = 0;
     for (int i = first; i < total; i += step, ++count) {
       const Tile t = tile_of(i);
@@ -381,7 +390,7 @@ __global__ void __launch_bounds__(64 + TILES_WARPS * 32, 1) gemm_tiles_kernel(co
       if (!mbar_wait_warp(&tfull[b], (count >> 1) & 1, abort_flag)) { fail_code = ST_WAIT_TIMEOUT_EPILOGUE; break; }
       tc_fence_after_sync();
       const int prow0 = t.row_tile * GT_ROWS + quarter * 32;
-      epilogue_tile({p.epi, smem + L::EPI_OFF + (warp - 2) * EPI_STAGE, tmem + (static_cast<uint32_t>(quarter * 32) << 16) + b * ACC, part, TILES_WARPS / 4, lane,
+      epilogue_tile({p.epi, smem + L::EPI_OFF + (warp - 4) * EPI_STAGE, tmem + (static_cast<uint32_t>(quarter * 32) << 16) + b * ACC, part, TILES_WARPS / 4, lane,
                      prow0, t.tok0, t.ntok},
                     [&] {
                       tc_fence_before_sync();
@@ -419,10 +428,10 @@ bool encode_rows(CUtensorMap *m, int et, const void *base, long long inner, long
 }
 
 template <typename K>
-cudaError_t launch_gemm_kernel(K kern, const GemmLaunch &g, int grid, int warps, int smem, int cluster, cudaStream_t s) {
+cudaError_t launch_gemm_kernel(K kern, const GemmLaunch &g, int grid, int threads, int smem, int cluster, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(64 + warps * 32);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute at[2];
@@ -435,11 +444,11 @@ cudaError_t launch_gemm_kernel(K kern, const GemmLaunch &g, int grid, int warps,
   return cudaLaunchKernelEx(&cfg, kern, g);
 }
 
-template <int BN>
+template <int BN, int RING>
 cudaError_t go_split(GemmLaunch &g, cudaStream_t s) {
-  using L = GemmSmem<BN, false, SPLIT_RING<BN>, 0>;
+  using L = GemmSmem<BN, false, RING, 0>;
   if (!encode_rows(&g.xmap, g.p.in_et, g.p.x, g.p.ic, g.p.rows, g.p.ld_x * 2, GT_K, BN, true)) return cudaErrorInvalidValue;
-  return launch_gemm_kernel(gemm_split_kernel<BN>, g, g.p.row_tiles * g.token_tiles * g.splits, SPLIT_WARPS, L::TOTAL, g.splits, s);
+  return launch_gemm_kernel(gemm_split_kernel<BN, RING>, g, g.p.row_tiles * g.token_tiles * g.splits, 64 + SPLIT_WARPS * 32, L::TOTAL, g.splits, s);
 }
 
 template <int BN, bool PAIR, bool GROUPED>
@@ -454,7 +463,7 @@ cudaError_t go_tiles(GemmLaunch &g, cudaStream_t s) {
   const long long tiles = (long long)g.token_tiles * row_steps;
   const int most = PAIR ? p.max_pairs : p.num_sms;
   const int grid = (int)(tiles < most ? tiles : most) * ctas;
-  return launch_gemm_kernel(gemm_tiles_kernel<BN, PAIR, GROUPED>, g, grid, TILES_WARPS, L::TOTAL, ctas, s);
+  return launch_gemm_kernel(gemm_tiles_kernel<BN, PAIR, GROUPED>, g, grid, 128 + TILES_WARPS * 32, L::TOTAL, ctas, s);
 }
 
 template <typename K>
@@ -486,11 +495,13 @@ cudaError_t launch_align_rows(void *dst, long long pitch, const void *src, long 
 cudaError_t init_gemm(int num_sms, int *max_pairs) {
   cudaError_t e = cudaSuccess;
   auto want = [&](cudaError_t r) { if (e == cudaSuccess) e = r; };
-  want(allow(gemm_split_kernel<16>, GemmSmem<16, false, SPLIT_RING<16>, 0>::TOTAL));
-  want(allow(gemm_split_kernel<32>, GemmSmem<32, false, SPLIT_RING<32>, 0>::TOTAL));
-  want(allow(gemm_split_kernel<64>, GemmSmem<64, false, SPLIT_RING<64>, 0>::TOTAL));
-  want(allow(gemm_split_kernel<128>, GemmSmem<128, false, SPLIT_RING<128>, 0>::TOTAL));
-  want(allow(gemm_split_kernel<256>, GemmSmem<256, false, SPLIT_RING<256>, 0>::TOTAL));
+  want(allow(gemm_split_kernel<16, SMALL_RING>, GemmSmem<16, false, SMALL_RING, 0>::TOTAL));
+  want(allow(gemm_split_kernel<32, SMALL_RING>, GemmSmem<32, false, SMALL_RING, 0>::TOTAL));
+  want(allow(gemm_split_kernel<16, LARGE_RING>, GemmSmem<16, false, LARGE_RING, 0>::TOTAL));
+  want(allow(gemm_split_kernel<32, LARGE_RING>, GemmSmem<32, false, LARGE_RING, 0>::TOTAL));
+  want(allow(gemm_split_kernel<64, LARGE_RING>, GemmSmem<64, false, LARGE_RING, 0>::TOTAL));
+  want(allow(gemm_split_kernel<128, LARGE_RING>, GemmSmem<128, false, LARGE_RING, 0>::TOTAL));
+  want(allow(gemm_split_kernel<256, LARGE_RING>, GemmSmem<256, false, LARGE_RING, 0>::TOTAL));
   want(allow(gemm_tiles_kernel<256, true, false>, GemmSmem<256, true, TILES_RING, TILES_WARPS>::TOTAL));
   want(allow(gemm_tiles_kernel<16, false, true>, GemmSmem<16, false, TILES_RING, TILES_WARPS>::TOTAL));
   want(allow(gemm_tiles_kernel<32, false, true>, GemmSmem<32, false, TILES_RING, TILES_WARPS>::TOTAL));
@@ -500,7 +511,7 @@ cudaError_t init_gemm(int num_sms, int *max_pairs) {
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(num_sms / 2 * 2);
-  cfg.blockDim = dim3(64 + TILES_WARPS * 32);
+  cfg.blockDim = dim3(128 + TILES_WARPS * 32);
   cfg.dynamicSmemBytes = GemmSmem<256, true, TILES_RING, TILES_WARPS>::TOTAL;
   cudaLaunchAttribute at = {};
   at.id = cudaLaunchAttributeClusterDimension;
@@ -535,22 +546,22 @@ cudaError_t launch_gemm(const GemmParams &p, cudaStream_t s) {
     }
   }
   // Which kernel and tiles: the least of a model of their time in cycles.  A step of 64 channels costs a CTA its bytes at
-  // FILL per cycle (what an SM takes in: 128 KB of steps measured 56 to 64) or its MMAs, whichever is more; a launch its
-  // waves of steps, and sharing a tile's channels the joining of the partial sums.
-  constexpr double FILL = 58.0, JOIN = 1500.0, JOIN_TOKEN = 10.0;
+  // FILL per cycle (what an SM takes in, measured 50 to 64) or its MMAs, whichever is more; a launch the most steps that an SM
+  // has, but no less than its weights at DRAM per cycle, and sharing a tile's channels the joining of the partial sums (two
+  // cluster barriers and the distributed reads, measured 2.3 us).
+  constexpr double FILL = 55.0, DRAM = 3400.0, JOIN = 4200.0, JOIN_TOKEN = 10.0;
+  const double weights = (double)p.row_tiles * p.kt * GT_BYTES / DRAM;
   double best = 1e30;
   bool pairs = false;
   for (int bn = 16; bn <= 256; bn *= 2) {
     if (bn > 16 && p.rows <= bn / 2) break;
     const int tt = (p.rows + bn - 1) / bn;
     const long long tiles = (long long)p.row_tiles * tt;
-    const int per_sm = bn <= 32 ? 2 : 1;
-    for (int splits = 1; splits <= 8; splits *= 2) {
+    const double step = fmax((GT_BYTES + bn * 128) / FILL, fmax(bn * 2.0, 370.0));
+    for (int splits = 1; splits <= (bn <= 32 ? 8 : 4); splits *= 2) {
       if (splits > 1 && (tiles * splits > p.num_sms || p.kt < splits * 2)) break;
-      const double step = fmax((GT_BYTES + bn * 128) / FILL, fmax(bn * 2.0, 370.0));
-      const double waves = (double)((tiles * splits + (long long)p.num_sms * per_sm - 1) / ((long long)p.num_sms * per_sm));
-      const double busy = waves > 1 ? waves * per_sm : (double)((tiles * splits + p.num_sms - 1) / p.num_sms);
-      const double t = busy * ((p.kt + splits - 1) / splits) * step + (splits > 1 ? JOIN + JOIN_TOKEN * bn : 0.0) + waves * 2000.0 + bn * 8.0;
+      const double busy = (double)((tiles * splits + p.num_sms - 1) / p.num_sms);
+      const double t = fmax(busy * ((p.kt + splits - 1) / splits) * step, weights) + (splits > 1 ? JOIN + JOIN_TOKEN * bn : 0.0) + busy * 2000.0 + bn * 16.0;
       if (t < best) { best = t; g.splits = splits; g.tile_tokens = bn; g.token_tiles = tt; }
     }
   }
@@ -560,17 +571,37 @@ cudaError_t launch_gemm(const GemmParams &p, cudaStream_t s) {
     const int n = ((p.rows + tt - 1) / tt + 31) / 32 * 32, count = (p.rows + n - 1) / n;
     const double step = fmax((GT_BYTES + n * 64) / FILL, fmax(n * 2.0, 256.0));
     const double waves = (double)(((long long)row_pairs * count + p.max_pairs - 1) / p.max_pairs);
-    const double t = waves * p.kt * step + 2500.0 + n * 8.0;
+    const double t = fmax(waves * fmax(p.kt * step, n * 18.0), weights) + 3500.0 + n * 18.0;
     if (t < best) { best = t; pairs = true; g.splits = 1; g.tile_tokens = n; g.token_tiles = count; }
   }
   if (pairs) return go_tiles<256, true, false>(g, s);
   switch (g.tile_tokens) {
-    case 16: return go_split<16>(g, s);
-    case 32: return go_split<32>(g, s);
-    case 64: return go_split<64>(g, s);
-    case 128: return go_split<128>(g, s);
-    default: return go_split<256>(g, s);
+    case 16: return g.splits > 1 ? go_split<16, SMALL_RING>(g, s) : go_split<16, LARGE_RING>(g, s);
+    case 32: return g.splits > 1 ? go_split<32, SMALL_RING>(g, s) : go_split<32, LARGE_RING>(g, s);
+    case 64: return go_split<64, LARGE_RING>(g, s);
+    case 128: return go_split<128, LARGE_RING>(g, s);
+    default: return go_split<256, LARGE_RING>(g, s);
   }
+}
+
+// On CUDA cores the weights are read once for every two rows, from L2 at 5.3 TB/s behind a start of 1.5 us; on tensor cores once
+// behind 3.6 us (up to 4 channel tiles) to 6.4 us (16).  Measured in us, here / there: 2 x 4096 -> 4096 9.2 / 11.2, 4 x
+// 4096 -> 4096 15.4 / 11.3, 4 x 2048 -> 2048 5.4 / 8.4, 16 x 1024 -> 1024 5.2 / 6.5, 32 x 512 -> 512 2.9 / 5.3, 8 x 256 -> 8192 5.8 /
+// 3.6, one row of 4096 -> 16384 23.5 / 23.5.
+bool gemm_wants_gemv(long long rows, int row_tiles, int kt) {
+  if (rows <= 1) return true;
+  if (rows > 64) return false;
+  const long long bytes = (long long)row_tiles * kt * GT_BYTES * ((rows + 1) / 2);
+  return bytes <= (2ll << 20) * (kt < 20 ? kt : 20);
+}
+
+// The same choice for experts.  On CUDA cores each slot reads its expert's weights, at 4.9 TB/s behind 4 us; on tensor cores
+// each expert that is hit is read once, at 7.5 TB/s behind 27 us.  Measured in us, here / there, 64 experts of 12.6 MB, 8 per
+// token: 1 token 24.8 / 38.4, 2 tokens 41.5 / 54.9, 4 tokens 74.0 / 72.4, 8 tokens 138 / 92; 16 experts of 0.8 MB, 2 per
+// token, 16 tokens 7.5 / 20.0; 4 experts of 3.1 MB, 4 per token, 16 tokens 30.9 / 24.3.
+bool experts_want_gemv(int slots, int experts, double expert_bytes) {
+  const double hit = experts * (1.0 - pow(1.0 - 1.0 / experts, slots)), mb = expert_bytes * 1e-6;
+  return slots <= 256 && 4.0 + slots * mb / 4.9 <= 27.0 + hit * mb / 7.5;
 }
 
 }  // namespace elb

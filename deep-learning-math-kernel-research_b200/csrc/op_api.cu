@@ -315,6 +315,11 @@ int elb_linear_enqueue(elb_op_t *op, void *output, const void *input, const void
   const int64_t per = 16 / ob;       // elements of 16 bytes
   p.epi.words = aligned(output, 16) && d.ld_output % per == 0 && (!p.epi.res || (aligned(residual, 16) && d.ld_residual % per == 0));
   const cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
+  if (gemm_wants_gemv(rows, p.row_tiles, p.kt)) {
+    OP_TRY(launch_gemv(p, s));
+    ++op->launches;
+    return ELB_OK;
+  }
   if (aligned(input, 16) && d.ld_input % 8 == 0) {
     OP_TRY(launch_gemm(p, s));
     ++op->launches;
@@ -586,6 +591,17 @@ int elb_experts_enqueue(elb_op_t *op, void *output, const void *input, const int
   q.epi.ld_out = e.pitch_y;
   q.epi.oc = (int)e.pitch_y;
   q.epi.out_et = ET_F32;
+  if (experts_want_gemv(slots, d.experts, (double)p.w_stride + (double)q.w_stride)) {
+    p.x = input;
+    p.ld_x = d.ld_input;
+    q.epi.out = output;
+    q.epi.ld_out = d.ld_output;
+    q.epi.oc = d.ic;
+    q.epi.out_et = e.et;
+    OP_TRY(launch_gemv_experts(p, q, ids, weights, (int)rows, d.top_k, d.experts, s));
+    op->launches += 2;
+    return leave_workspace(*op, s, capturing);
+  }
   if (op->count_stale) OP_TRY(cudaMemsetAsync(e.count, 0, d.experts * sizeof(int), s));
   op->count_stale = true;
   OP_TRY(launch_experts_count(e, s));

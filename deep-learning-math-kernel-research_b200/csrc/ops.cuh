@@ -93,6 +93,13 @@ cudaError_t launch_gemm(const GemmParams &p, cudaStream_t s);
 cudaError_t init_gemm(int num_sms, int *max_pairs);
 // x and ld_x of GemmParams are multiples of 16 bytes; other rows are copied first
 cudaError_t launch_align_rows(void *dst, long long pitch, const void *src, long long ld, int rows, int n, cudaStream_t s);
+// A handful of rows, any alignment of x
+bool gemm_wants_gemv(long long rows, int row_tiles, int kt);
+bool experts_want_gemv(int slots, int experts, double expert_bytes);
+cudaError_t launch_gemv(const GemmParams &p, cudaStream_t s);
+// Both products and the sum over a token's experts, slot by slot: in.x the tokens, in.epi.out and out.x the middle rows of the slots
+cudaError_t launch_gemv_experts(const GemmParams &in, const GemmParams &out, const int *ids, const float *share, int rows, int top_k, int experts,
+                                cudaStream_t s);
 int grouped_tile_tokens(int slots, int experts);
 constexpr int MIN_TILE_TOKENS = 16;
 
