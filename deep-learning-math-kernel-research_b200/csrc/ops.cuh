@@ -141,6 +141,7 @@ struct RouteParams {
   float *weights;
   long long ld, rows;
   int experts, top_k, et, sigmoid, groups, top_groups, group_best, renormalise;
+  int lanes_per_group, words;       // set by the launch: whole lanes of a group (0: groups and lanes do not fit), 16-byte rows
   float scale;
 };
 cudaError_t launch_route(const RouteParams &p, cudaStream_t s);
