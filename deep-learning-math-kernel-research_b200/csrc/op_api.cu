@@ -218,13 +218,15 @@ int vector_f32(elb_op &op, float **dst, const void *src, int et, int n, int padd
   return ELB_OK;
 }
 
+int64_t norm_pitch(int n) { return up(n + 16, 8); }
+
 // A norm's weights as fp32, offset included; null: ones (offset and all), or no vector for a bias
 int norm_vector(elb_op &op, float **dst, const void *src, int et, int n, float offset) {
   Staged st;
   int rc = src ? st.take(src, n * et_bytes(et)) : ELB_OK;
-  if (rc == ELB_OK) rc = alloc(op, dst, (size_t)n * 4);
+  if (rc == ELB_OK) rc = alloc(op, dst, (size_t)norm_pitch(n) * 8 * 4);
   if (rc != ELB_OK) return rc;
-  OP_TRY(launch_norm_vector(*dst, st.p, et, n, offset, nullptr));
+  OP_TRY(launch_norm_vector(*dst, st.p, et, n, norm_pitch(n), offset, nullptr));
   OP_TRY(cudaDeviceSynchronize());
   return ELB_OK;
 }
@@ -401,6 +403,8 @@ int elb_norm_enqueue(elb_op_t *op, void *output, void *sum, const void *input, c
   p.post_w = op->f[0]; p.post_b = op->f[1]; p.pre_w = op->f[2]; p.pre_b = op->f[3];
   p.ld_x = d.ld_input; p.ld_res = d.ld_residual; p.ld_gate = d.ld_gate; p.ld_sum = d.ld_sum; p.ld_y = d.ld_output;
   p.rows = rows;
+  p.w_pitch = norm_pitch(d.channels);
+  p.num_sms = op->num_sms;
   p.channels = d.channels;
   p.gate_rows = d.gate_rows;
   p.post = d.post; p.pre = d.pre;

@@ -126,12 +126,12 @@ struct NormParams {
   void *sum, *y;
   const float *post_w, *post_b, *pre_w, *pre_b;     // never null where their norm is not NONE
   long long ld_x, ld_res, ld_gate, ld_sum, ld_y;
-  long long rows;
-  int channels, gate_rows, post, pre, et, et_res;
+  long long rows, w_pitch;                          // elements from one of the eight copies of a weight vector to the next
+  int channels, gate_rows, post, pre, et, et_res, num_sms;
   float post_eps, pre_eps, scale;
 };
-// dst = offset + src, or ones where src is null
-cudaError_t launch_norm_vector(float *dst, const void *src, int et, int n, float offset, cudaStream_t s);
+// eight copies of offset + src (of ones where src is null), copy a from index a on, zeros around
+cudaError_t launch_norm_vector(float *dst, const void *src, int et, int n, long long pitch, float offset, cudaStream_t s);
 cudaError_t launch_block_norm(const NormParams &p, cudaStream_t s);
 
 struct RouteParams {

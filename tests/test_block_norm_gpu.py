@@ -111,6 +111,26 @@ def test_strides_and_alignment(U, n, pad, shift):
     _run(U, 9, n, "bf16", "f32", post="layer", pre="rms", gate_rows=5, pad=pad, shift=shift)
 
 
+@pytest.mark.parametrize("rows,n", [(3001, 2048), (2500, 4096), (1300, 4104), (1200, 8192), (1500, 1544)])
+@pytest.mark.parametrize("types", [("bf16", "same"), ("f16", "f32"), ("f32", "same")], ids="-".join)
+def test_long_calls(U, rows, n, types):
+    """Rows that stream through shared memory, more of them than blocks at a time."""
+    _run(U, rows, n, *types, post="rms", pre="layer", gate_rows=7, scale=0.5)
+    _run(U, rows, n, *types, post="none", pre="rms")
+    _run(U, rows, n, *types, post="layer", pre="none", with_residual=False, pad=16)
+
+
+@pytest.mark.parametrize("n", [9, 37, 250, 511, 1001, 1155, 1537, 2049, 4099, 9001, 16387])
+@pytest.mark.parametrize("types", [("bf16", "same"), ("f16", "f32"), ("f32", "same")], ids="-".join)
+@pytest.mark.parametrize("rows", [3, 9, 700])
+def test_rows_that_start_anywhere(U, n, types, rows):
+    """Dense rows of odd lengths: every place of a 16-byte boundary occurs."""
+    if rows * n > 4_000_000:
+        rows = 17
+    _run(U, rows, n, *types, post="layer", pre="rms", gate_rows=2)
+    _run(U, rows, n, *types, pre="layer", shift=5, in_place=True)
+
+
 def test_weights_types_offset_and_no_sum(U):
     _run(U, 5, 200, wt="bf16", post="rms", pre="layer", offset=1.0)
     _run(U, 5, 2000, "f16", wt="f16", post="rms", pre="rms", offset=1.0, want_sum=False)
