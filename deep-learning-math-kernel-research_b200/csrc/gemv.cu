@@ -5,6 +5,8 @@
 // flight before it needs the first, and the loads of a dense call are issued before the kernel in front of it has ended.  No
 // tensor memory, clusters or barriers in memory: 1 x 4096 -> 4096 takes the tensor-core kernel 10.7 us a call in a stream of
 // calls, most of it set-up and hand-overs.
+#include <type_traits>
+
 #include "elb_common.cuh"
 #include "gemm_epilogue.cuh"
 #include "ops.cuh"
@@ -19,7 +21,7 @@ constexpr int LOADS = 8;          // of a thread at a time: packed rows of a blo
 struct GemvParams {
   const uint8_t *w;
   size_t w_stride;
-  const uint16_t *x;
+  const void *x;                // operands' type; fp32 in the experts' second product
   long long ld_x;
   int rows, ic, kt, words;      // words: rows of x are 16-byte aligned
   const int *ids;               // experts: of each slot; null: dense
@@ -62,13 +64,22 @@ __device__ __forceinline__ int row_of(int block, int i) {
 }
 
 // eight values of a row of x from channel k; past the end zeros
-template <typename E>
-__device__ __forceinline__ void load_x(uint64_t (&f)[4], const uint16_t *x, int k, int ic, bool words) {
+template <typename X>
+__device__ __forceinline__ void load_x(uint64_t (&f)[4], const X *x, int k, int ic, bool words) {
   if (words && k + 8 <= ic) {
-    unpack8<E>(*reinterpret_cast<const uint4 *>(x + k), f);
+    if constexpr (sizeof(X) == 2) {
+      unpack8<X>(*reinterpret_cast<const uint4 *>(x + k), f);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float4 q = reinterpret_cast<const float4 *>(x + k)[i];
+        f[2 * i] = both(q.x, q.y);
+        f[2 * i + 1] = both(q.z, q.w);
+      }
+    }
     return;
   }
-  auto one = [&](int i) { return k + i < ic ? to_f32(reinterpret_cast<const E *>(x)[k + i]) : 0.0f; };
+  auto one = [&](int i) { return k + i < ic ? to_f32(x[k + i]) : 0.0f; };
 #pragma unroll
   for (int i = 0; i < 4; ++i) f[i] = both(one(2 * i), one(2 * i + 1));
 }
@@ -88,6 +99,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, T == 1 ? 3 : 2) gemv_kernel(co
     const int r = row_of<GATED, ROWS>(blockIdx.x, i) & 127;
     return r * 128 + ((chunk ^ (r & 7)) << 4);
   };
+  using X = std::conditional_t<MODE == 2, float, E>;
   uint64_t acc[T][ROWS] = {};
   griddep_launch_dependents();
   if (MODE != 0) griddep_wait();                                // (the experts come from the router)
@@ -126,7 +138,7 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, T == 1 ? 3 : 2) gemv_kernel(co
 #pragma unroll
       for (int t = 0; t < T; ++t) {
         const int r = MODE == 0 ? min((int)blockIdx.y * T + t, p.rows - 1) : MODE == 1 ? blockIdx.y / p.top_k : first + slot[u];
-        load_x<E>(x[t], p.x + r * p.ld_x, kt[u] * GT_K + chunk * 8, p.ic, p.words);
+        load_x<X>(x[t], static_cast<const X *>(p.x) + r * p.ld_x, kt[u] * GT_K + chunk * 8, p.ic, p.words);
       }
 #pragma unroll
       for (int i = 0; i < ROWS; ++i) {
@@ -212,7 +224,7 @@ GemvParams from(const GemmParams &g) {
   GemvParams p = {};
   p.w = g.w;
   p.w_stride = g.w_stride;
-  p.x = static_cast<const uint16_t *>(g.x);
+  p.x = g.x;
   p.ld_x = g.ld_x;
   p.rows = g.rows;
   p.ic = g.ic;
@@ -224,7 +236,7 @@ GemvParams from(const GemmParams &g) {
 
 template <typename E>
 cudaError_t experts_as(const GemvParams &p, const GemvParams &q, int rows, cudaStream_t s) {
-  const cudaError_t e = p.epi.gated ? go<E, E, 1, true, 1>(p, rows * p.top_k, s) : go<E, E, 1, false, 1>(p, rows * p.top_k, s);
+  const cudaError_t e = p.epi.gated ? go<E, float, 1, true, 1>(p, rows * p.top_k, s) : go<E, float, 1, false, 1>(p, rows * p.top_k, s);
   return e != cudaSuccess ? e : go<E, E, 1, false, 2>(q, rows, s);
 }
 

@@ -601,7 +601,7 @@ bool gemm_wants_gemv(long long rows, int row_tiles, int kt) {
 // token, 16 tokens 7.5 / 20.0; 4 experts of 3.1 MB, 4 per token, 16 tokens 30.9 / 24.3.
 bool experts_want_gemv(int slots, int experts, double expert_bytes) {
   const double hit = experts * (1.0 - pow(1.0 - 1.0 / experts, slots)), mb = expert_bytes * 1e-6;
-  return slots <= 256 && 4.0 + slots * mb / 4.9 <= 27.0 + hit * mb / 7.5;
+  return slots <= GEMV_SLOTS && 4.0 + slots * mb / 4.9 <= 27.0 + hit * mb / 7.5;
 }
 
 }  // namespace elb

@@ -3,6 +3,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <mutex>
 #include <new>
 
 #include "../../include/euler_b200.h"
@@ -55,6 +56,61 @@ int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
 }  // namespace
 
+namespace {
+
+// What every plan of a device needs and is slow to ask for: 10 ms and more of a plan's making went into device properties, kernel
+// attributes and a pinned page of its own.
+struct DeviceInfo { bool known = false; int num_sms = 0, max_pairs = 0; };
+constexpr int MAX_DEVICES = 64;
+std::mutex g_mutex;
+DeviceInfo g_devices[MAX_DEVICES];
+
+int device_info(int device, DeviceInfo &out) {
+  if (device >= MAX_DEVICES) return op_fail(ELB_UNIMPLEMENTED, "device %d", device);
+  std::lock_guard<std::mutex> lock(g_mutex);
+  DeviceInfo &d = g_devices[device];
+  if (!d.known) {
+    const int rc = elb_device_supported(device);
+    if (rc != ELB_OK) return rc;
+    OP_TRY(cudaDeviceGetAttribute(&d.num_sms, cudaDevAttrMultiProcessorCount, device));
+    OP_TRY(init_gemm(d.num_sms, &d.max_pairs));
+    d.known = true;
+  }
+  out = d;
+  return ELB_OK;
+}
+
+// Status words of the plans, in pages of mapped host memory that stay for the next plans.
+constexpr int PAGE_WORDS = 1024, MAX_PAGES = 256;
+int *g_pages[MAX_PAGES];
+bool g_used[MAX_PAGES][PAGE_WORDS];
+
+int *take_status() {
+  std::lock_guard<std::mutex> lock(g_mutex);
+  for (int i = 0; i < MAX_PAGES; ++i) {
+    if (!g_pages[i]) {
+      void *q = nullptr;
+      if (cudaHostAlloc(&q, PAGE_WORDS * sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable) != cudaSuccess) return nullptr;
+      g_pages[i] = static_cast<int *>(q);
+    }
+    for (int k = 0; k < PAGE_WORDS; ++k)
+      if (!g_used[i][k]) {
+        g_used[i][k] = true;
+        g_pages[i][k] = 0;
+        return &g_pages[i][k];
+      }
+  }
+  return nullptr;
+}
+void put_status(int *p) {
+  if (!p) return;
+  std::lock_guard<std::mutex> lock(g_mutex);
+  for (int i = 0; i < MAX_PAGES && g_pages[i]; ++i)
+    if (p >= g_pages[i] && p < g_pages[i] + PAGE_WORDS) g_used[i][p - g_pages[i]] = false;
+}
+
+}  // namespace
+
 struct elb_op {
   Kind kind;
   int device = 0, num_sms = 0, max_pairs = 0;
@@ -87,30 +143,33 @@ struct elb_op {
     for (float *q : f) if (q) cudaFree(q);
     if (ws) cudaFree(ws);
     if (done) cudaEventDestroy(done);
-    if (h_status) cudaFreeHost(h_status);
+    put_status(h_status);       // (behind the cudaFree above, which has waited for the plan's kernels)
   }
 };
 
 namespace {
 
 int make(Kind kind, int device, elb_op **out) {
-  int rc = elb_device_supported(device);
-  if (rc != ELB_OK) return rc;
+  int count = 0;
+  if (cudaGetDeviceCount(&count) != cudaSuccess || count == 0) return elb_device_supported(device);     // (says what is missing)
   if (device < 0) OP_TRY(cudaGetDevice(&device));
+  if (device >= count) return elb_device_supported(device);
+  DeviceGuard guard(device);
+  DeviceInfo info;
+  const int rc = device_info(device, info);
+  if (rc != ELB_OK) return rc;
   elb_op *op = new (std::nothrow) elb_op(kind);
   if (!op) return op_fail(ELB_GENERAL_ERROR, "out of host memory");
   op->device = device;
-  DeviceGuard guard(device);
-  if (cudaDeviceGetAttribute(&op->num_sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess ||
-      init_gemm(op->num_sms, &op->max_pairs) != cudaSuccess ||
-      cudaHostAlloc(&op->h_status, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable) != cudaSuccess ||
-      cudaHostGetDevicePointer(reinterpret_cast<void **>(&op->d_status), op->h_status, 0) != cudaSuccess ||
+  op->num_sms = info.num_sms;
+  op->max_pairs = info.max_pairs;
+  op->h_status = take_status();
+  if (!op->h_status || cudaHostGetDevicePointer(reinterpret_cast<void **>(&op->d_status), op->h_status, 0) != cudaSuccess ||
       cudaEventCreateWithFlags(&op->done, cudaEventDisableTiming) != cudaSuccess) {
     cudaGetLastError();
     delete op;
     return op_fail(ELB_GENERAL_ERROR, "device allocation failed");
   }
-  *op->h_status = 0;
   *out = op;
   return ELB_OK;
 }
@@ -491,10 +550,11 @@ int elb_experts_create(const elb_experts_desc_t *desc, elb_op_t **out) {
   op->exp = d;
   DeviceGuard guard(op->device);
   const int64_t slots = d.max_rows * d.top_k, px = up(d.ic, 8), pm = up(d.mid, 8), py = up(d.ic, 4);
-  const int64_t tiles = slots / MIN_TILE_TOKENS + d.experts;
+  const int64_t tiles = slots / MIN_TILE_TOKENS + d.experts, few = slots < GEMV_SLOTS ? slots : GEMV_SLOTS;    // (those have fp32 middle rows)
   size_t at = 0;
   auto part = [&](size_t bytes) { const size_t o = at; at += (bytes + 255) / 256 * 256; return o; };
-  const size_t o_xs = part(slots * px * 2), o_mid = part(slots * pm * 2), o_y = part(slots * py * 4), o_pos = part(slots * 4),
+  const size_t o_xs = part(slots * px * 2),
+               o_mid = part(slots * pm * 2 > few * pm * 4 ? slots * pm * 2 : few * pm * 4), o_y = part(slots * py * 4), o_pos = part(slots * 4),
                o_place = part(slots * 4), o_tiles = part(tiles * sizeof(GroupTile)), o_n = part(4), o_count = part(d.experts * 4);
   rc = alloc(*op, &op->ws, at);
   if (rc != ELB_OK) { delete op; return rc; }
@@ -598,6 +658,7 @@ int elb_experts_enqueue(elb_op_t *op, void *output, const void *input, const int
   if (experts_want_gemv(slots, d.experts, (double)p.w_stride + (double)q.w_stride)) {
     p.x = input;
     p.ld_x = d.ld_input;
+    p.epi.out_et = ET_F32;
     q.epi.out = output;
     q.epi.ld_out = d.ld_output;
     q.epi.oc = d.ic;

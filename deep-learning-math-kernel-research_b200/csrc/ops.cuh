@@ -97,7 +97,9 @@ cudaError_t launch_align_rows(void *dst, long long pitch, const void *src, long 
 bool gemm_wants_gemv(long long rows, int row_tiles, int kt);
 bool experts_want_gemv(int slots, int experts, double expert_bytes);
 cudaError_t launch_gemv(const GemmParams &p, cudaStream_t s);
-// Both products and the sum over a token's experts, slot by slot: in.x the tokens, in.epi.out and out.x the middle rows of the slots
+// Both products and the sum over a token's experts, slot by slot, GEMV_SLOTS at most: in.x the tokens, in.epi.out and out.x the middle
+// rows of the slots, in fp32 (few slots cost little more so, and the middle needs no rounding)
+constexpr int GEMV_SLOTS = 256;
 cudaError_t launch_gemv_experts(const GemmParams &in, const GemmParams &out, const int *ids, const float *share, int rows, int top_k, int experts,
                                 cudaStream_t s);
 int grouped_tile_tokens(int slots, int experts);
