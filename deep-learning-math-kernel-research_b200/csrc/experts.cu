@@ -42,20 +42,33 @@ __global__ void __launch_bounds__(COUNT_THREADS) experts_count_kernel(const Expe
 
 // Rows of the experts lie behind one another.  Every block adds up the counts for itself, brings its slots' rows to their
 // places and notes these; the first writes the list of token tiles.
-constexpr int GATHER_THREADS = 256;
-template <bool WORDS>                                  // rows in 16-byte words
+// COUNT: few slots, which every block counts for itself, places and all, in the slots' order; there is no kernel before it.
+constexpr int GATHER_THREADS = 256, COUNT_HERE = 2048;
+template <bool WORDS, bool COUNT>                      // WORDS: rows in 16-byte words
 __global__ void __launch_bounds__(GATHER_THREADS) experts_gather_kernel(const ExpertsParams p, int per_block) {
   __shared__ int row0[MAX_EXPERTS];
   __shared__ int2 part[GATHER_THREADS / 32];
+  __shared__ short ids[COUNT ? COUNT_HERE : 1];
   griddep_launch_dependents();
   griddep_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int slots = p.rows * p.top_k;
+  if (COUNT) {
+    for (int e = tid; e < p.experts; e += GATHER_THREADS) row0[e] = 0;
+    __syncthreads();
+    for (int i = tid; i < slots; i += GATHER_THREADS) {
+      const int e = p.ids[i];
+      ids[i] = (short)(e >= 0 && e < p.experts ? e : -1);
+      if (e >= 0 && e < p.experts) atomicAdd(&row0[e], 1);
+    }
+    __syncthreads();
+  }
   constexpr int EACH = MAX_EXPERTS / GATHER_THREADS;   // experts of a thread, neighbours
   int c[EACH], rows = 0, tiles = 0;
 #pragma unroll
   for (int j = 0; j < EACH; ++j) {
     const int e = tid * EACH + j;
-    c[j] = e < p.experts ? p.count[e] : 0;
+    c[j] = e >= p.experts ? 0 : COUNT ? row0[e] : p.count[e];
     rows += c[j];
     tiles += (c[j] + p.tile_tokens - 1) / p.tile_tokens;
   }
@@ -84,11 +97,18 @@ __global__ void __launch_bounds__(GATHER_THREADS) experts_gather_kernel(const Ex
   if (blockIdx.x == 0 && tid == GATHER_THREADS - 1) *p.n_tiles = t;
   __syncthreads();
   // a warp per slot
-  const int slots = p.rows * p.top_k, end = min(slots, (int)(blockIdx.x + 1) * per_block);
+  const int end = min(slots, (int)(blockIdx.x + 1) * per_block);
   for (int i = blockIdx.x * per_block + warp; i < end; i += GATHER_THREADS / 32) {
-    const int e = p.ids[i];
+    const int e = COUNT ? ids[i] : p.ids[i];
     if (e < 0 || e >= p.experts) continue;
-    const long long to = row0[e] + p.pos[i], from = i / p.top_k;
+    int place = 0;
+    if (COUNT) {
+      for (int k = lane; k < i; k += 32) place += ids[k] == e;
+      place = __reduce_add_sync(0xFFFFFFFFu, place);
+    } else {
+      place = p.pos[i];
+    }
+    const long long to = row0[e] + place, from = i / p.top_k;
     __syncwarp();
     if (lane == 0) p.place[i] = (int)to;
     if (WORDS) {
@@ -123,7 +143,7 @@ __global__ void __launch_bounds__(COMBINE_THREADS) experts_combine_kernel(const 
     at[threadIdx.x] = e >= 0 && e < p.experts ? p.place[i] : -1;
     by[threadIdx.x] = p.weights[i];
   }
-  if (blockIdx.x == 0)                                 // for the next call
+  if (blockIdx.x == 0 && p.clear)                      // for the next call
     for (int i = threadIdx.x; i < p.experts; i += COMBINE_THREADS) p.count[i] = 0;
   __syncthreads();
   T *out = static_cast<T *>(p.out) + t * p.ld_out;
@@ -151,6 +171,7 @@ __global__ void __launch_bounds__(COMBINE_THREADS) experts_combine_kernel(const 
 
 }  // namespace
 
+bool experts_count_here(int slots) { return slots <= COUNT_HERE; }
 cudaError_t launch_experts_count(const ExpertsParams &p, cudaStream_t s) {
   const int slots = p.rows * p.top_k;
   return launch_overlapped(experts_count_kernel, dim3((slots + COUNT_SLOTS - 1) / COUNT_SLOTS), dim3(COUNT_THREADS), 0, s, p);
@@ -160,7 +181,10 @@ cudaError_t launch_experts_gather(const ExpertsParams &p, int num_sms, cudaStrea
   const int warps = GATHER_THREADS / 32, blocks = (slots + warps - 1) / warps < most ? (slots + warps - 1) / warps : most;
   const int per = (slots + blocks - 1) / blocks;
   const bool words = (reinterpret_cast<uintptr_t>(p.x) & 15) == 0 && p.ld_x % 8 == 0 && p.ic % 8 == 0;
-  return launch_overlapped(words ? experts_gather_kernel<true> : experts_gather_kernel<false>, dim3((slots + per - 1) / per), dim3(GATHER_THREADS), 0, s, p, per);
+  const bool here = experts_count_here(slots);
+  auto k = words ? (here ? experts_gather_kernel<true, true> : experts_gather_kernel<true, false>)
+                 : (here ? experts_gather_kernel<false, true> : experts_gather_kernel<false, false>);
+  return launch_overlapped(k, dim3((slots + per - 1) / per), dim3(GATHER_THREADS), 0, s, p, per);
 }
 cudaError_t launch_experts_combine(const ExpertsParams &p, cudaStream_t s) {
   const bool words = (reinterpret_cast<uintptr_t>(p.out) & 7) == 0 && p.ld_out % 4 == 0 && p.ic % 4 == 0;

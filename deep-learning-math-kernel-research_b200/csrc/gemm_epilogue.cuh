@@ -136,14 +136,24 @@ struct EpilogueWarp {
     for (int n = 0; n < N; ++n)
       if (n * STEP + sub_t < ntok) ahead[n] = *reinterpret_cast<const uint4 *>(res + n * STEP * e.ld_res);
   }
-  // One by one, where the rows are not aligned or channels are missing: f(element in shared memory, token, channel)
-  template <typename F>
-  __device__ __forceinline__ void each(int ntok, F f) {
-#pragma unroll 1
-    for (int i = lane; i < min(ntok, 16) * CH; i += 32) {
-      const int t = i / CH, c = i % CH;
-      if (ch0 + c < e.oc) f(reinterpret_cast<OT *>(at(t, c >> 3))[c & 7], t, ch0 + c);
-    }
+  // One by one, where the rows are not aligned or channels are missing: neighbouring lanes, neighbouring channels
+  static constexpr int TP = 32 / CH, PASSES = 16 / TP;
+  __device__ __forceinline__ OT &single(int n) const { return reinterpret_cast<OT *>(at(n * TP + lane / CH, lane % CH >> 3))[lane & 7]; }
+  __device__ __forceinline__ void singles_in(long long tok0, int ntok) {
+    const OT *res = static_cast<const OT *>(e.res) + (tok0 + lane / CH) * e.ld_res + ch0 + lane % CH;
+    const bool has = ch0 + lane % CH < e.oc;
+    OT r[PASSES];
+#pragma unroll
+    for (int n = 0; n < PASSES; ++n) r[n] = has && n * TP + lane / CH < ntok ? res[n * TP * e.ld_res] : from_f32<OT>(0.0f);
+#pragma unroll
+    for (int n = 0; n < PASSES; ++n) single(n) = r[n];
+  }
+  __device__ __forceinline__ void singles_out(long long tok0, int ntok) {
+    OT *out = static_cast<OT *>(e.out) + (tok0 + lane / CH) * e.ld_out + ch0 + lane % CH;
+    const bool has = ch0 + lane % CH < e.oc;
+#pragma unroll
+    for (int n = 0; n < PASSES; ++n)
+      if (has && n * TP + lane / CH < ntok) out[n * TP * e.ld_out] = single(n);
   }
   // acc: the block's accumulators as tmem_ld_block has them, ntok real tokens from tok0.  read() runs when they have been taken, and
   // may load the next block's into the same registers; that one's residual (`next` tokens from next0) is fetched here too.
@@ -202,7 +212,7 @@ struct EpilogueWarp {
           for (int n = 0; n < N; ++n) *reinterpret_cast<uint4 *>(at(n * STEP + sub_t, sub_c)) = ahead[n];
           fetch(next0, next);
         } else {
-          each(ntok, [&](OT &v, int t, int c) { v = static_cast<const OT *>(e.res)[(tok0 + t) * e.ld_res + c]; });
+          singles_in(tok0, ntok);
         }
         __syncwarp();
 #pragma unroll
@@ -234,7 +244,7 @@ struct EpilogueWarp {
         for (int n = 0; n < N; ++n)
           if (n * STEP + sub_t < ntok) *reinterpret_cast<uint4 *>(out + n * STEP * e.ld_out) = q[n];
       } else {
-        each(ntok, [&](OT &v, int t, int c) { static_cast<OT *>(e.out)[(tok0 + t) * e.ld_out + c] = v; });
+        singles_out(tok0, ntok);
       }
       __syncwarp();
     }

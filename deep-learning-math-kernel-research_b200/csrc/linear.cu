@@ -286,6 +286,8 @@ __global__ void __launch_bounds__(128 + TILES_WARPS * 32, 1) gemm_tiles_kernel(c
     fence_proxy_async_smem();
   }
   griddep_wait();                                             // (before tensor memory is taken, see gemm_split_kernel)
+  const int token_tiles = GROUPED ? *p.n_tiles : g.token_tiles;
+  if (GROUPED && threadIdx.x == 0) asm volatile("prefetch.global.L1 [%0];" ::"l"(p.tiles + blockIdx.x / CTAS / row_steps));
   if (warp == 1) { if (PAIR) tmem_alloc2(tmem_slot, COLS); else tmem_alloc(tmem_slot, COLS); }
   tc_fence_before_sync();
   __syncthreads();
@@ -293,7 +295,6 @@ __global__ void __launch_bounds__(128 + TILES_WARPS * 32, 1) gemm_tiles_kernel(c
   tc_fence_after_sync();
   const uint32_t tmem = *tmem_slot;
   griddep_launch_dependents();
-  const int token_tiles = GROUPED ? *p.n_tiles : g.token_tiles;
   const int total = token_tiles * row_steps;
   const int first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
   struct Tile { int expert, row_tile, tok0, ntok; };

@@ -667,15 +667,19 @@ int elb_experts_enqueue(elb_op_t *op, void *output, const void *input, const int
     op->launches += 2;
     return leave_workspace(*op, s, capturing);
   }
-  if (op->count_stale) OP_TRY(cudaMemsetAsync(e.count, 0, d.experts * sizeof(int), s));
-  op->count_stale = true;
-  OP_TRY(launch_experts_count(e, s));
+  const bool count = !experts_count_here(slots);
+  e.clear = count;
+  if (count) {
+    if (op->count_stale) OP_TRY(cudaMemsetAsync(e.count, 0, d.experts * sizeof(int), s));
+    op->count_stale = true;
+    OP_TRY(launch_experts_count(e, s));
+  }
   OP_TRY(launch_experts_gather(e, op->num_sms, s));
   OP_TRY(launch_gemm(p, s));
   OP_TRY(launch_gemm(q, s));
   OP_TRY(launch_experts_combine(e, s));
-  op->count_stale = false;
-  op->launches += 5;
+  if (count) op->count_stale = false;
+  op->launches += count ? 5 : 4;
   return leave_workspace(*op, s, capturing);
 }
 

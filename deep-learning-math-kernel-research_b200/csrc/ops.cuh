@@ -117,8 +117,10 @@ struct ExpertsParams {
   GroupTile *tiles;
   int *n_tiles;
   long long ld_x, ld_out, pitch_x, pitch_y;
+  int clear;                        // the combine kernel leaves zero counts
   int rows, top_k, experts, ic, et, tile_tokens;    // tile_tokens: the most that a token tile holds
 };
+bool experts_count_here(int slots);      // the gather kernel counts few slots itself
 cudaError_t launch_experts_count(const ExpertsParams &p, cudaStream_t s);
 cudaError_t launch_experts_gather(const ExpertsParams &p, int num_sms, cudaStream_t s);
 cudaError_t launch_experts_combine(const ExpertsParams &p, cudaStream_t s);
