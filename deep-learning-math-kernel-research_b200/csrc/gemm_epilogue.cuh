@@ -155,10 +155,9 @@ struct EpilogueWarp {
     for (int n = 0; n < PASSES; ++n)
       if (has && n * TP + lane / CH < ntok) out[n * TP * e.ld_out] = single(n);
   }
-  // acc: the block's accumulators as tmem_ld_block has them, ntok real tokens from tok0.  read() runs when they have been taken, and
-  // may load the next block's into the same registers; that one's residual (`next` tokens from next0) is fetched here too.
-  template <typename R>
-  __device__ __forceinline__ void block(uint32_t (&acc)[16], long long tok0, int ntok, long long next0, int next, R read) {
+  // acc: the block's accumulators as tmem_ld_block has them, ntok real tokens from tok0; the residual of the block behind (`next`
+  // tokens from next0) is fetched here.
+  __device__ __forceinline__ void block(const uint32_t (&acc)[16], long long tok0, int ntok, long long next0, int next) {
     // y[4 i + 2 g + j]: channel 8 i + T / 4 of the warp's, token 8 g + 2 (T % 4) + j
     float y[VALUES], u[GATED ? VALUES : 1];
 #pragma unroll
@@ -178,7 +177,6 @@ struct EpilogueWarp {
         else y[v] += bias[v / 4];
       }
     }
-    read();
     activate(y, e.act);
     if constexpr (GATED) {
 #pragma unroll
@@ -240,9 +238,14 @@ struct EpilogueWarp {
         uint4 q[N];
 #pragma unroll
         for (int n = 0; n < N; ++n) q[n] = *reinterpret_cast<const uint4 *>(at(n * STEP + sub_t, sub_c));
+        if (ntok >= 16) {
 #pragma unroll
-        for (int n = 0; n < N; ++n)
-          if (n * STEP + sub_t < ntok) *reinterpret_cast<uint4 *>(out + n * STEP * e.ld_out) = q[n];
+          for (int n = 0; n < N; ++n) *reinterpret_cast<uint4 *>(out + n * STEP * e.ld_out) = q[n];
+        } else {
+#pragma unroll
+          for (int n = 0; n < N; ++n)
+            if (n * STEP + sub_t < ntok) *reinterpret_cast<uint4 *>(out + n * STEP * e.ld_out) = q[n];
+        }
       } else {
         singles_out(tok0, ntok);
       }
@@ -257,19 +260,15 @@ template <typename OT, bool GATED, typename F>
 __device__ __forceinline__ void epilogue_tile_as(const Epilogue &e, uint8_t *stage, uint32_t taddr, int part, int parts, int lane, int prow0,
                                                  long long tok0, int ntok, F release) {
   EpilogueWarp<OT, GATED> w(e, stage, lane, prow0);
-  uint32_t a[16];
-  if (part * 16 < ntok) {
-    tmem_ld_block(taddr + part * 16, a);
-    w.fetch(tok0 + part * 16, ntok - part * 16);
-  }
+  const int step = parts * 16;
+  if (part * 16 < ntok) w.fetch(tok0 + part * 16, ntok - part * 16);
 #pragma unroll 1
-  for (int t = part * 16; t < ntok; t += parts * 16) {
-    const int after = t + parts * 16;
+  for (int t = part * 16; t < ntok; t += step) {
+    uint32_t a[16];             // (asking for the next block's meanwhile costs more in moved registers than it hides)
+    tmem_ld_block(taddr + t, a);
     tmem_ld_wait16(a);
-    w.block(a, tok0 + t, ntok - t, tok0 + after, ntok - after, [&] {
-      if (after < ntok) tmem_ld_block(taddr + after, a);
-      else release();
-    });
+    if (t + step >= ntok) release();
+    w.block(a, tok0 + t, ntok - t, tok0 + t + step, ntok - t - step);
   }
   if (part * 16 >= ntok) release();
 }
