@@ -9,9 +9,8 @@
 namespace elb {
 
 // Bytes of the operand rings.  The kernel of few tiles with few tokens and shared channels leaves room for a second CTA on its
-// SM (the next launch's weights arrive while this one ends, and clusters of eight find a place: 16 x 2048 -> 2048 8.6 us, 12.8 with
-// the large ring); a CTA that streams a whole row tile wants all of the SM's memory for loads in flight (24 x 4096 -> 16384
-// 23.4 us, 29.0 with the small ring).
+// SM (the next launch's weights arrive while this one ends, and a cluster finds its SMs); a CTA that streams a whole row tile
+// wants all of the SM's memory for loads in flight (24 x 4096 -> 16384 23.4 us, 29.0 with the small ring).
 constexpr int SMALL_RING = 110 * 1024, LARGE_RING = 224 * 1024;
 constexpr int TILES_RING = 192 * 1024;
 
@@ -554,11 +553,12 @@ cudaError_t launch_gemm(const GemmParams &p, cudaStream_t s) {
       default: return go_tiles<256, true, true>(g, s);
     }
   }
-  // Which kernel and tiles: the least of a model of their time in cycles.  A step of 64 channels costs a CTA its bytes at
-  // FILL per cycle (what an SM takes in, measured 50 to 64) or its MMAs, whichever is more; a launch the most steps that an SM
-  // has, but no less than its weights at DRAM per cycle, and sharing a tile's channels the joining of the partial sums (two
-  // cluster barriers and the distributed reads, measured 2.3 us).
-  constexpr double FILL = 55.0, DRAM = 3400.0, JOIN = 4200.0, JOIN_TOKEN = 10.0;
+  // Which kernel and tiles: the least of a model of their time in cycles, fitted to 25 shapes with every
+  // choice measured (its choice costs up to 12 % over the best of them, mostly under 4).  A step of
+  // 64 channels costs a CTA about the shared memory's traffic (operands in and out, at 134 bytes per cycle, 97 in a pair) or the
+  // hand-overs of its roles; a launch the steps of its busiest SM, but no less than the weights at DRAM per cycle; sharing a tile's
+  // channels costs the joining of the partial sums (two cluster barriers and the distributed reads).
+  constexpr double DRAM = 3400.0, JOIN = 2500.0, JOIN_TOKEN = 30.0;
   const double weights = (double)p.row_tiles * p.kt * GT_BYTES / DRAM;
   double best = 1e30;
   bool pairs = false;
@@ -566,21 +566,21 @@ cudaError_t launch_gemm(const GemmParams &p, cudaStream_t s) {
     if (bn > 16 && p.rows <= bn / 2) break;
     const int tt = (p.rows + bn - 1) / bn;
     const long long tiles = (long long)p.row_tiles * tt;
-    const double step = fmax((GT_BYTES + bn * 128) / FILL, fmax(bn * 2.0, 370.0));
-    for (int splits = 1; splits <= (bn <= 32 ? 8 : 4); splits *= 2) {
+    const double step = fmax((GT_BYTES + bn * 128) * 2 / 134.0, 385.0);
+    for (int splits = 1; splits <= 4; splits *= 2) {
       if (splits > 1 && (tiles * splits > p.num_sms || p.kt < splits * 2)) break;
       const double busy = (double)((tiles * splits + p.num_sms - 1) / p.num_sms);
-      const double t = fmax(busy * ((p.kt + splits - 1) / splits) * step, weights) + (splits > 1 ? JOIN + JOIN_TOKEN * bn : 0.0) + busy * 2000.0 + bn * 16.0;
+      const double t = fmax(busy * ((p.kt + splits - 1) / splits) * step, weights) + (splits > 1 ? JOIN + JOIN_TOKEN * bn : 0.0) +
+                       (busy - 1) * (3500.0 + bn * 10.0) + 6500.0 + bn * 10.0;
       if (t < best) { best = t; g.splits = splits; g.tile_tokens = bn; g.token_tiles = tt; }
     }
   }
   const int row_pairs = (p.row_tiles + 1) / 2;
-  const int fewest = (p.rows + 255) / 256;
-  for (int tt = fewest; tt <= fewest + 7 && p.rows > 64; ++tt) {          // tiles of equal size, a multiple of 32 tokens
-    const int n = ((p.rows + tt - 1) / tt + 31) / 32 * 32, count = (p.rows + n - 1) / n;
-    const double step = fmax((GT_BYTES + n * 64) / FILL, fmax(n * 2.0, 256.0));
+  for (int most = 256; most >= 96 && p.rows > 64; most -= 32) {            // tiles of equal size, a multiple of 32 tokens
+    const int tt = (p.rows + most - 1) / most, n = ((p.rows + tt - 1) / tt + 31) / 32 * 32, count = (p.rows + n - 1) / n;
+    const double step = fmax((GT_BYTES + n * 64) * 2 / 97.0, 400.0);
     const double waves = (double)(((long long)row_pairs * count + p.max_pairs - 1) / p.max_pairs);
-    const double t = fmax(waves * fmax(p.kt * step, n * 18.0), weights) + 3500.0 + n * 18.0;
+    const double t = fmax(waves * (fmax(p.kt * step, n * 20.0) + 2500.0), weights) + 5000.0 + n * 16.0;
     if (t < best) { best = t; pairs = true; g.splits = 1; g.tile_tokens = n; g.token_tiles = count; }
   }
   if (pairs) return go_tiles<256, true, false>(g, s);
