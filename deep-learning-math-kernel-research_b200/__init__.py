@@ -480,6 +480,26 @@ def _dev(x):
     return x.data_ptr()
 
 
+def _dense(x, shape, dtypes, what):
+    """Address of a weight tensor for an operator's prepare, which reads all of ``shape``: a dense torch tensor or numpy array of that many
+    elements of one of ``dtypes`` (ELB types), a raw address, or None."""
+    if x is None or isinstance(x, int):
+        return x
+    n = 1
+    for d in shape:
+        n *= d
+    contiguous = x.is_contiguous() if hasattr(x, "is_contiguous") else x.flags["C_CONTIGUOUS"]
+    count = x.numel() if hasattr(x, "numel") else x.size
+    name = str(x.dtype).replace("torch.", "")
+    if not contiguous or count != n or name not in [_DTYPE_NAMES[t] for t in dtypes]:
+        raise ValueError(f"{what}: a dense tensor of {n} elements {shape} in {[_DTYPE_NAMES[t] for t in dtypes]} is wanted, got {tuple(x.shape)} "
+                         f"in {name}{'' if contiguous else ', not dense'}")
+    return _ptr(x)
+
+
+_DTYPE_NAMES = {f32: "float32", f16: "float16", bf16: "bfloat16"}
+
+
 class _Op:
     """A plan of one of the operators of transformer blocks (``elb_op_t``).  ``prepare`` copies the weights (host or
     device tensors, read once; later calls do nothing), ``enqueue`` runs on ``stream`` (None: the default stream) and
@@ -524,9 +544,12 @@ class Linear(_Op):
         self._create(lib.elb_linear_create, ElbLinearDesc(ic, oc, dtype, dtype if out_dtype is None else out_dtype, bias_dtype, weights_format,
                                                           activation, int(gated), int(with_bias), int(with_residual), scale, device,
                                                           ld_input, ld_output, ld_residual))
+        wide = 2 * oc if gated else oc
+        self._weights = ((wide, ic) if weights_format == oihw else (ic, wide), (dtype,))
+        self._bias = ((wide,), (bias_dtype,))
 
     def prepare(self, weights, bias=None) -> int:
-        return lib.elb_linear_prepare(self.h, _ptr(weights), _ptr(bias))
+        return lib.elb_linear_prepare(self.h, _dense(weights, *self._weights, "weights"), _dense(bias, *self._bias, "bias"))
 
     def enqueue(self, output, input, residual=None, *, rows: int, stream=None) -> int:
         return lib.elb_linear_enqueue(self.h, _dev(output), _dev(input), _dev(residual), rows, stream)
@@ -543,9 +566,10 @@ class BlockNorm(_Op):
         self._create(lib.elb_norm_create, ElbNormDesc(channels, dtype, dtype if residual_dtype is None else residual_dtype, weights_dtype, post, pre,
                                                       post_eps, pre_eps, weight_offset, scale, int(with_residual), gate_rows, device,
                                                       ld_input, ld_residual, ld_gate, ld_sum, ld_output))
+        self._vector = ((channels,), (weights_dtype,), "weights")
 
     def prepare(self, post_weight=None, post_bias=None, pre_weight=None, pre_bias=None) -> int:
-        return lib.elb_norm_prepare(self.h, _ptr(post_weight), _ptr(post_bias), _ptr(pre_weight), _ptr(pre_bias))
+        return lib.elb_norm_prepare(self.h, *(_dense(v, *self._vector) for v in (post_weight, post_bias, pre_weight, pre_bias)))
 
     def enqueue(self, output, sum, input, residual=None, gate=None, *, rows: int, stream=None) -> int:
         return lib.elb_norm_enqueue(self.h, _dev(output), _dev(sum), _dev(input), _dev(residual), _dev(gate), rows, stream)
@@ -559,9 +583,10 @@ class Route(_Op):
                  top_groups: int = 1, group_best: int = 1, renormalise: bool = True, scale: float = 1.0, ld_logits: int = 0, device: int = -1):
         self._create(lib.elb_route_create, ElbRouteDesc(experts, top_k, dtype, score, int(with_bias), groups, top_groups, group_best,
                                                         int(renormalise), scale, device, ld_logits))
+        self._bias = ((experts,), (f32,), "bias")
 
     def prepare(self, bias=None) -> int:
-        return lib.elb_route_prepare(self.h, _ptr(bias))
+        return lib.elb_route_prepare(self.h, _dense(bias, *self._bias))
 
     def enqueue(self, ids, weights, logits, *, rows: int, stream=None) -> int:
         """ids: int32 [rows, top_k], weights: float32 [rows, top_k] or None, both dense."""
@@ -576,9 +601,11 @@ class Experts(_Op):
                  gated: bool = True, ld_input: int = 0, ld_output: int = 0, device: int = -1):
         self._create(lib.elb_experts_create, ElbExpertsDesc(experts, top_k, ic, mid, dtype, activation, int(gated), device, max_rows,
                                                             ld_input, ld_output))
+        self._in = ((experts, 2 * mid if gated else mid, ic), (dtype,), "w_in")
+        self._out = ((experts, ic, mid), (dtype,), "w_out")
 
     def prepare(self, w_in, w_out) -> int:
-        return lib.elb_experts_prepare(self.h, _ptr(w_in), _ptr(w_out))
+        return lib.elb_experts_prepare(self.h, _dense(w_in, *self._in), _dense(w_out, *self._out))
 
     def enqueue(self, output, input, ids, weights, *, rows: int, stream=None) -> int:
         return lib.elb_experts_enqueue(self.h, _dev(output), _dev(input), _dev(ids), _dev(weights), rows, stream)

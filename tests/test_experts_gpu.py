@@ -158,3 +158,38 @@ def test_streams_graphs_and_repeats(U):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, outs[n])
+
+
+@pytest.mark.parametrize("rows,channels,dtype", [(1, 256, "bf16"), (3, 512, "f16"), (40, 264, "bf16"), (300, 1024, "bf16"), (700, 520, "f16")])
+def test_the_four_together(U, rows, channels, dtype):
+    """The example's two feed-forward halves against the same chain in 64 bits.  Each of its seven 16-bit tensors rounds once (a relative
+    half unit in the last place at most, in the norm of a vector a third root of that at most), what a rounding becomes on its way
+    through a product is about as large as it was, and through the gate at most twice: 16 roundings are allowed."""
+    import importlib.util
+    from pathlib import Path
+    spec = importlib.util.spec_from_file_location("feed_forward", Path(__file__).resolve().parent.parent / "examples" / "feed_forward.py")
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    E = U.E
+    dt = getattr(E, dtype)
+    ff = mod.FeedForward(channels, 4 * channels, 32, 4, channels // 2, rows, dt)
+    x = U.randn(rows, channels, dtype=U.TORCH[dt], seed=1)
+    s0 = U.randn(rows, channels, dtype=torch.float32, seed=2, scale=2.0)
+    s = s0.clone()
+    torch.cuda.synchronize()
+    out = ff(x, s).clone()
+    torch.cuda.synchronize()
+    assert all(p.device_status() == 0 for p in ff.plans())
+    want, want_s = ff.in_64_bits(x, s0, ff.ids[:rows])
+    for got, w in ((out, want), (s, want_s)):
+        assert float((got.double() - w).norm() / w.norm()) <= 16 * U.UNIT[dt]
+    # captured, the pass gives the same bits
+    s2, y2 = s0.clone(), torch.empty_like(out)
+    g, q = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(g, stream=q):
+        ff(x, s2, stream=q.cuda_stream)
+    s2.copy_(s0)
+    g.replay()
+    torch.cuda.synchronize()
+    y2.copy_(ff.out[:rows])
+    assert torch.equal(y2, out) and torch.equal(s2, s)

@@ -59,6 +59,20 @@ def test_sizes(U, size, dt):
     _run(U, *size, dt=getattr(U.E, dt))
 
 
+# every tile width, with and without shared channels, pairs of CTAs with full, ragged and several tiles, and CUDA cores
+FORMS = [(5, 4096, 4096, False), (24, 4096, 8192, True), (33, 2048, 4096, False), (64, 4096, 2048, True), (128, 4096, 4096, False), (200, 3000, 2048, True),
+         (256, 4096, 4096, False), (512, 2048, 4096, False), (1024, 4096, 2100, True), (1500, 640, 5120, False), (4000, 256, 1280, False), (3000, 1024, 511, True),
+         (240, 2048, 18944, False), (20, 4096, 9000, False), (160, 1024, 10000, True), (96, 8192, 1024, False), (1000, 7168, 250, False), (2, 4096, 4096, True),
+         (7, 1000, 600, True), (1, 16384, 300, False)]
+
+
+@pytest.mark.parametrize("form", FORMS, ids=lambda f: "x".join(map(str, f)))
+def test_every_form(U, form):
+    rows, ic, oc, gated = form
+    _run(U, rows, ic, oc, act="silu" if gated else "gelu_tanh", gated=gated, bias=U.E.f32, residual=True, scale=0.5)
+    _run(U, rows, ic, oc, dt=U.E.f16, gated=gated, seed=5)
+
+
 @pytest.mark.parametrize("size", [(1, 64, 1), (3, 200, 129), (16, 1003, 64), (40, 256, 192), (130, 320, 333), (300, 512, 1024), (1100, 1000, 515)],
                          ids=lambda s: "x".join(map(str, s)))
 @pytest.mark.parametrize("act", ["none", "relu", "gelu", "gelu_tanh", "silu"])
@@ -204,8 +218,13 @@ def test_refusals_of_calls(U):
     lin = E.Linear(64, 64, with_residual=True, with_bias=True)
     x = torch.zeros(4, 64, dtype=torch.bfloat16, device="cuda")
     assert lin.enqueue(x, x, x, rows=4) == E.ELB_GENERAL_ERROR and "not prepared" in E.last_error()
-    assert lin.prepare(x) == E.ELB_GENERAL_ERROR and lin.prepare(None) == E.ELB_GENERAL_ERROR
     w, b = torch.zeros(64, 64, dtype=torch.bfloat16, device="cuda"), torch.zeros(64, device="cuda")
+    assert lin.prepare(w) == E.ELB_GENERAL_ERROR and lin.prepare(None) == E.ELB_GENERAL_ERROR
+    for bad in (x, w.float(), w.t(), w[:, :32], w.cpu().float().numpy()):
+        with pytest.raises(ValueError):
+            lin.prepare(bad, b)
+    with pytest.raises(ValueError):
+        lin.prepare(w, b.half())
     assert lin.prepare(w, b) == 0
     assert lin.enqueue(x, x, None, rows=4) == E.ELB_GENERAL_ERROR
     assert lin.enqueue(None, x, x, rows=4) == E.ELB_GENERAL_ERROR
