@@ -6,8 +6,8 @@
 // of a channel lie 8 lanes apart and so meet in one thread; two tokens of a channel become one word of 16-bit values, and
 // stmatrix.trans turns 8 channels by 8 tokens of those round, so that shared memory holds each token's channels in
 // order and global memory is written (and the residual read) 16 bytes per thread.  Measured for a tile of 128 channels
-// by 256 tokens, bf16, one CTA on every SM: 2300 cycles; with one lane of tensor memory per thread, neighbouring lanes trading
-// values and 4-byte stores 6700, of which the reads of tensor memory are 730.
+// by 256 tokens, bf16, 12 warps, one CTA on every SM: 2700 cycles (gated silu 3500, silu 5800, gelu 7700, fp32 results 4900), bound by the
+// warps' instructions; with one lane of tensor memory per thread, neighbouring lanes trading values and 4-byte stores 6700.
 #pragma once
 #include "ops.cuh"
 #include "umma.cuh"
@@ -114,7 +114,7 @@ struct EpilogueWarp {
   uint32_t matrix;                  // this thread's row of the first four matrices in shared memory, the others 512 bytes behind
   float bias[4];
   bool whole;                       // all of the warp's channels exist and rows are aligned
-  uint4 ahead[N];                   // the next block's residual
+  uint4 ahead[N];                   // the next block's residual: 16-byte chunks, or, where not whole, one value per pass
 
   __device__ __forceinline__ EpilogueWarp(const Epilogue &e_, uint8_t *stage_, int lane_, int prow0) : e(e_), stage(stage_), lane(lane_) {
     ch0 = GATED ? prow0 >> 1 : prow0;
@@ -130,23 +130,33 @@ struct EpilogueWarp {
   // the first of the two values of matrix q of the m-th four (of 8 channels by 8 tokens: all channels of 8 tokens, or, gated, of 16)
   static __device__ __forceinline__ constexpr int index(int m, int q) { return GATED ? 4 * (q & 1) + 2 * (q >> 1) : 4 * q + 2 * m; }
   __device__ __forceinline__ void fetch(long long tok0, int ntok) {
-    if (!e.res || !whole) return;
-    const OT *res = static_cast<const OT *>(e.res) + (tok0 + sub_t) * e.ld_res + ch0 + sub_c * 8;
+    if (!HALF || !e.res || ntok <= 0) return;
+    if (whole) {
+      const OT *res = static_cast<const OT *>(e.res) + (tok0 + sub_t) * e.ld_res + ch0 + sub_c * 8;
 #pragma unroll
-    for (int n = 0; n < N; ++n)
-      if (n * STEP + sub_t < ntok) ahead[n] = *reinterpret_cast<const uint4 *>(res + n * STEP * e.ld_res);
+      for (int n = 0; n < N; ++n)
+        if (n * STEP + sub_t < ntok) ahead[n] = *reinterpret_cast<const uint4 *>(res + n * STEP * e.ld_res);
+    } else {
+      const uint16_t *res = static_cast<const uint16_t *>(e.res) + (tok0 + lane / CH) * e.ld_res + ch0 + lane % CH;
+      const bool has = ch0 + lane % CH < e.oc;
+      uint32_t one[PASSES];
+#pragma unroll
+      for (int n = 0; n < PASSES; ++n) one[n] = has && n * TP + lane / CH < ntok ? res[n * TP * e.ld_res] : 0u;
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        ahead[n] = make_uint4(one[8 * n] | one[8 * n + 1] << 16, one[8 * n + 2] | one[8 * n + 3] << 16, one[8 * n + 4] | one[8 * n + 5] << 16,
+                              one[8 * n + 6] | one[8 * n + 7] << 16);
+    }
   }
   // One by one, where the rows are not aligned or channels are missing: neighbouring lanes, neighbouring channels
   static constexpr int TP = 32 / CH, PASSES = 16 / TP;
   __device__ __forceinline__ OT &single(int n) const { return reinterpret_cast<OT *>(at(n * TP + lane / CH, lane % CH >> 3))[lane & 7]; }
-  __device__ __forceinline__ void singles_in(long long tok0, int ntok) {
-    const OT *res = static_cast<const OT *>(e.res) + (tok0 + lane / CH) * e.ld_res + ch0 + lane % CH;
-    const bool has = ch0 + lane % CH < e.oc;
-    OT r[PASSES];
+  __device__ __forceinline__ void singles_in() {
 #pragma unroll
-    for (int n = 0; n < PASSES; ++n) r[n] = has && n * TP + lane / CH < ntok ? res[n * TP * e.ld_res] : from_f32<OT>(0.0f);
-#pragma unroll
-    for (int n = 0; n < PASSES; ++n) single(n) = r[n];
+    for (int n = 0; n < PASSES; ++n) {
+      const uint32_t w[4] = {ahead[n / 8].x, ahead[n / 8].y, ahead[n / 8].z, ahead[n / 8].w};
+      reinterpret_cast<uint16_t &>(single(n)) = (uint16_t)(w[n / 2 % 4] >> (16 * (n & 1)));
+    }
   }
   __device__ __forceinline__ void singles_out(long long tok0, int ntok) {
     OT *out = static_cast<OT *>(e.out) + (tok0 + lane / CH) * e.ld_out + ch0 + lane % CH;
@@ -208,10 +218,10 @@ struct EpilogueWarp {
         if (whole) {
 #pragma unroll
           for (int n = 0; n < N; ++n) *reinterpret_cast<uint4 *>(at(n * STEP + sub_t, sub_c)) = ahead[n];
-          fetch(next0, next);
         } else {
-          singles_in(tok0, ntok);
+          singles_in();
         }
+        fetch(next0, next);
         __syncwarp();
 #pragma unroll
         for (int m = 0; m < G / 2; ++m) {
@@ -254,14 +264,16 @@ struct EpilogueWarp {
   }
 };
 
-// All tokens of a tile, in blocks of 16 that go round the `parts` warps of a quarter of the lanes; `release` runs when the last of
-// this warp's accumulators has been read.  A block's last columns may lie past the tile's: the accumulator has them.
-template <typename OT, bool GATED, typename F>
-__device__ __forceinline__ void epilogue_tile_as(const Epilogue &e, uint8_t *stage, uint32_t taddr, int part, int parts, int lane, int prow0,
-                                                 long long tok0, int ntok, F release) {
+// All tokens of a tile, in blocks of 16 that go round the `parts` warps of a quarter of the lanes.  wait() returns when the
+// accumulator is complete (false: never); the bias and the first residual are on their way before.  release() runs when the last
+// of this warp's accumulators has been read.  A block's last columns may lie past the tile's: the accumulator has them.
+template <typename OT, bool GATED, typename W, typename F>
+__device__ __forceinline__ bool epilogue_tile_as(const Epilogue &e, uint8_t *stage, uint32_t taddr, int part, int parts, int lane, int prow0,
+                                                 long long tok0, int ntok, W wait, F release) {
   EpilogueWarp<OT, GATED> w(e, stage, lane, prow0);
   const int step = parts * 16;
-  if (part * 16 < ntok) w.fetch(tok0 + part * 16, ntok - part * 16);
+  w.fetch(tok0 + part * 16, ntok - part * 16);
+  if (!wait()) return false;
 #pragma unroll 1
   for (int t = part * 16; t < ntok; t += step) {
     uint32_t a[16];             // (asking for the next block's meanwhile costs more in moved registers than it hides)
@@ -271,19 +283,19 @@ __device__ __forceinline__ void epilogue_tile_as(const Epilogue &e, uint8_t *sta
     w.block(a, tok0 + t, ntok - t, tok0 + t + step, ntok - t - step);
   }
   if (part * 16 >= ntok) release();
+  return true;
 }
 // f: a call with the result's type and the gate as template arguments
 template <typename F>
-__device__ __forceinline__ void by_kind(const Epilogue &e, F f) {
+__device__ __forceinline__ bool by_kind(const Epilogue &e, F f) {
   if (e.gated) {
-    if (e.out_et == ET_BF16) f.template operator()<__nv_bfloat16, true>();
-    else if (e.out_et == ET_F16) f.template operator()<__half, true>();
-    else f.template operator()<float, true>();
-  } else {
-    if (e.out_et == ET_BF16) f.template operator()<__nv_bfloat16, false>();
-    else if (e.out_et == ET_F16) f.template operator()<__half, false>();
-    else f.template operator()<float, false>();
+    if (e.out_et == ET_BF16) return f.template operator()<__nv_bfloat16, true>();
+    if (e.out_et == ET_F16) return f.template operator()<__half, true>();
+    return f.template operator()<float, true>();
   }
+  if (e.out_et == ET_BF16) return f.template operator()<__nv_bfloat16, false>();
+  if (e.out_et == ET_F16) return f.template operator()<__half, false>();
+  return f.template operator()<float, false>();
 }
 
 }  // namespace elb

@@ -82,6 +82,7 @@ struct alignas(64) GemmLaunch {
   int token_tiles, tile_tokens;
   int band;                    // token tiles that neighbouring tiles of the walk share weights over
   int box;                     // tokens of one tiled copy
+  int early;                   // the tiles are known before the kernel in front of this one has ended
 };
 
 __device__ __forceinline__ uint8_t *smem_1k(uint8_t *base) { return base + ((1024u - (smem_u32(base) & 1023u)) & 1023u); }
@@ -102,14 +103,17 @@ struct EpilogueTile {
   long long tok0;
   int ntok;
 };
-template <typename F>
+template <typename W, typename F>
 struct EpilogueCall : EpilogueTile {
+  W wait;
   F release;
   template <typename OT, bool GATED>
-  __device__ __forceinline__ void operator()() { epilogue_tile_as<OT, GATED>(e, stage, taddr, part, parts, lane, prow0, tok0, ntok, release); }
+  __device__ __forceinline__ bool operator()() {
+    return epilogue_tile_as<OT, GATED>(e, stage, taddr, part, parts, lane, prow0, tok0, ntok, wait, release);
+  }
 };
-template <typename F>
-__device__ __forceinline__ void epilogue_tile(const EpilogueTile &t, F release) { by_kind(t.e, EpilogueCall<F>{t, release}); }
+template <typename W, typename F>
+__device__ __forceinline__ bool epilogue_tile(const EpilogueTile &t, W wait, F release) { return by_kind(t.e, EpilogueCall<W, F>{t, wait, release}); }
 
 // The partial sums of a tile, brought together over the CTAs of a cluster in the order of their ranks: blocks of 16 tokens go round the
 // CTAs, those of one CTA round its two halves of warps.  A thread's accumulators lie in the same place everywhere.
@@ -121,7 +125,7 @@ struct JoinCall {
   long long tok0;
   int ntok;
   template <typename OT, bool GATED>
-  __device__ __forceinline__ void operator()() {
+  __device__ __forceinline__ bool operator()() {
     EpilogueWarp<OT, GATED> w(e, stage, lane, prow0);
 #pragma unroll 1
     for (int k = rank + half * splits; k * 16 < ntok; k += 2 * splits) {
@@ -146,6 +150,7 @@ struct JoinCall {
       for (int i = 0; i < 16; ++i) a[i] = __float_as_uint(v[i]);
       w.block(a, tok0 + k * 16, ntok - k * 16, 0, 0);
     }
+    return true;
   }
 };
 
@@ -236,10 +241,13 @@ __global__ void __launch_bounds__(64 + SPLIT_WARPS * 32) gemm_split_kernel(const
   float4 *part = reinterpret_cast<float4 *>(smem) + quarter * 32 + lane;     // [block of 16 tokens][4][128 threads]
   bool ok = true;
   if (warp >= 2) {
-    ok = mbar_wait_warp(tfull, 0, abort_flag);
+    auto wait = [&] {
+      const bool done = mbar_wait_warp(tfull, 0, abort_flag);
+      tc_fence_after_sync();
+      return done;
+    };
+    ok = splits > 1 ? wait() : epilogue_tile({p.epi, stage, taddr, half, SPLIT_WARPS / 4, lane, prow0, tok0, ntok}, wait, [] {});
     if (!ok) fail_code = ST_WAIT_TIMEOUT_EPILOGUE;
-    tc_fence_after_sync();
-    if (ok && splits == 1) epilogue_tile({p.epi, stage, taddr, half, SPLIT_WARPS / 4, lane, prow0, tok0, ntok}, [] {});
     if (ok && splits > 1) {
 #pragma unroll 1
       for (int k = half; k < (ntok + 15) / 16; k += 2) {
@@ -292,26 +300,40 @@ __global__ void __launch_bounds__(128 + TILES_WARPS * 32, 1) gemm_tiles_kernel(c
     fence_barrier_init();
     fence_proxy_async_smem();
   }
-  griddep_wait();                                             // (before tensor memory is taken, see gemm_split_kernel)
-  const int token_tiles = GROUPED ? *p.n_tiles : g.token_tiles;
-  if (GROUPED && threadIdx.x == 0) asm volatile("prefetch.global.L1 [%0];" ::"l"(p.tiles + blockIdx.x / CTAS / row_steps));
-  if (warp == 1) { if (PAIR) tmem_alloc2(tmem_slot, COLS); else tmem_alloc(tmem_slot, COLS); }
-  tc_fence_before_sync();
   __syncthreads();
-  if (PAIR) cluster_sync_all();
-  tc_fence_after_sync();
-  const uint32_t tmem = *tmem_slot;
-  griddep_launch_dependents();
+  if (PAIR) cluster_sync_all();                               // the barriers exist in both CTAs
+  // The producer of the weights starts at once, where these and the tiles are known before the kernel in front has ended.  The others
+  // wait for that; tensor memory is taken behind it, and the kernel behind may start when it has been (see gemm_split_kernel).
+  if (warp == 0 || warp == 2) {
+    if (PAIR) cluster_arrive();                               // (its wait is at the end)
+    if (warp == 2 || !g.early) griddep_wait();
+  } else {
+    griddep_wait();
+    if (warp == 1) { if (PAIR) tmem_alloc2(tmem_slot, COLS); else tmem_alloc(tmem_slot, COLS); }
+    tc_fence_before_sync();
+    if (PAIR) {
+      __syncwarp();
+      cluster_arrive();
+      cluster_wait();
+    } else if (warp != 3) {
+      named_bar_sync(1, (1 + TILES_WARPS) * 32);
+    }
+    tc_fence_after_sync();
+    if (warp == 1) griddep_launch_dependents();
+  }
+  const uint32_t tmem = warp == 0 || warp == 2 ? 0u : *tmem_slot;
+  // (from L2: a block that is early may meet lines of an earlier call in its SM's cache)
+  const int token_tiles = GROUPED ? __ldcg(p.n_tiles) : g.token_tiles;
   const int total = token_tiles * row_steps;
   const int first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
   struct Tile { int expert, row_tile, tok0, ntok; };
   auto tile_of = [&](int i) {
     Tile t;
     if (GROUPED) {
-      const GroupTile q = p.tiles[i / row_steps];
-      t.expert = q.expert;
-      t.tok0 = q.row0;
-      t.ntok = q.count;
+      const int4 q = __ldcg(reinterpret_cast<const int4 *>(p.tiles + i / row_steps));     // a GroupTile
+      t.expert = q.x;
+      t.tok0 = q.y;
+      t.ntok = q.z;
       t.row_tile = (i % row_steps) * CTAS + rank;
     } else {
       // bands of token tiles: inside one the walk goes down the rows, so that the CTAs at work share tokens and weights in L2
@@ -395,20 +417,25 @@ __global__ void __launch_bounds__(128 + TILES_WARPS * 32, 1) gemm_tiles_kernel(c
     for (int i = first; i < total; i += step, ++count) {
       const Tile t = tile_of(i);
       const uint32_t b = count & 1;
-      if (!mbar_wait_warp(&tfull[b], (count >> 1) & 1, abort_flag)) { fail_code = ST_WAIT_TIMEOUT_EPILOGUE; break; }
-      tc_fence_after_sync();
       const int prow0 = t.row_tile * GT_ROWS + quarter * 32;
-      epilogue_tile({p.epi, smem + L::EPI_OFF + (warp - 4) * EPI_STAGE, tmem + (static_cast<uint32_t>(quarter * 32) << 16) + b * ACC, part, TILES_WARPS / 4, lane,
-                     prow0, t.tok0, t.ntok},
-                    [&] {
-                      tc_fence_before_sync();
-                      __syncwarp();
-                      if (lane == 0) { if (PAIR) mbar_arrive_cluster(mapa_u32(&tempty[b], 0)); else mbar_arrive(&tempty[b]); }
-                    });
+      const bool ok = epilogue_tile({p.epi, smem + L::EPI_OFF + (warp - 4) * EPI_STAGE, tmem + (static_cast<uint32_t>(quarter * 32) << 16) + b * ACC, part,
+                                     TILES_WARPS / 4, lane, prow0, t.tok0, t.ntok},
+                                    [&] {
+                                      const bool done = mbar_wait_warp(&tfull[b], (count >> 1) & 1, abort_flag);
+                                      tc_fence_after_sync();
+                                      return done;
+                                    },
+                                    [&] {
+                                      tc_fence_before_sync();
+                                      __syncwarp();
+                                      if (lane == 0) { if (PAIR) mbar_arrive_cluster(mapa_u32(&tempty[b], 0)); else mbar_arrive(&tempty[b]); }
+                                    });
+      if (!ok) { fail_code = ST_WAIT_TIMEOUT_EPILOGUE; break; }
     }
   }
   __syncwarp();
   if (fail_code != 0) report_status(p.status, fail_code);
+  if (PAIR && (warp == 0 || warp == 2)) cluster_wait();
   tc_fence_before_sync();
   __syncthreads();
   if (PAIR) cluster_sync_all();
@@ -542,6 +569,7 @@ cudaError_t launch_gemm(const GemmParams &p, cudaStream_t s) {
   g.splits = 1;
   g.band = 8;
   g.box = 0;
+  g.early = !p.tiles || p.tiles_old;
   if (p.tiles) {
     g.token_tiles = p.max_tiles;
     g.tile_tokens = p.tile_tokens;

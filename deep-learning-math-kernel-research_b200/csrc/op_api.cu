@@ -651,6 +651,7 @@ int elb_experts_enqueue(elb_op_t *op, void *output, const void *input, const int
   q.row_tiles = (int)(up(d.ic, GT_ROWS) / GT_ROWS);
   q.w_stride = (size_t)q.row_tiles * q.kt * GT_BYTES;
   q.w_rows = (long long)d.experts * q.row_tiles * q.kt * GT_ROWS;
+  q.tiles_old = 1;
   q.epi.out = const_cast<float *>(e.y);
   q.epi.ld_out = e.pitch_y;
   q.epi.oc = (int)e.pitch_y;

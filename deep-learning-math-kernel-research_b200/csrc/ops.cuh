@@ -68,7 +68,7 @@ inline int packed_rows(int oc, bool gated) { return gated ? (oc + 7) / 8 * 16 : 
 constexpr int GT_ROWS = 128, GT_K = 64, GT_BYTES = GT_ROWS * GT_K * 2;
 
 // Rows of one expert: input rows [row0, row0 + count) of the sorted rows.
-struct GroupTile { int expert, row0, count, pad; };
+struct alignas(16) GroupTile { int expert, row0, count, pad; };
 
 struct GemmParams {
   const uint8_t *w;                 // packed weights; expert e at w + e * w_stride
@@ -79,6 +79,7 @@ struct GemmParams {
   int in_et;                        // ET_BF16 or ET_F16
   const GroupTile *tiles;           // grouped: the token tiles, *n_tiles of them; null: dense
   const int *n_tiles;
+  int tiles_old;                    // they were written before the kernel in front of this one started
   int max_tiles, tile_tokens;       // grouped: the most that *n_tiles can be; tokens of a tile (grouped_tile_tokens)
   long long w_rows;                 // rows of 128 bytes of the whole packed image
   int num_sms, max_pairs;

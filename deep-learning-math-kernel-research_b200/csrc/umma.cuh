@@ -344,6 +344,9 @@ __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// the two halves of it, for threads that have work between them (each must run both, in this order)
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // address of the same shared-memory object in CTA `rank` of the cluster
 __device__ __forceinline__ uint32_t mapa_u32(const void *p, uint32_t rank) {
   uint32_t r;
