@@ -112,7 +112,7 @@ __device__ __forceinline__ float row_sum(float v, float (&part)[4][32], int slot
 constexpr int WARP_ROWS = 4;    // rows of a block whose rows belong to warps
 
 // One row's arithmetic, on the values of its threads: v[i][j] is element c(i) + j, of which those outside the row are zero and stay
-// out of the sums.  `inside(i, j)` says whether an element exists, `some(i)` whether any of an item does.
+// out of the sums.  some(i) says whether an item has any inside; settle(i) clears those of a window's that lie outside.
 template <int VEC, int ITEMS, bool WARP, bool WINDOW>
 struct RowNorm {
   float (&v)[ITEMS][VEC];
@@ -120,7 +120,13 @@ struct RowNorm {
   int c0, step, channels;
   __device__ __forceinline__ int c(int i) const { return c0 + i * step; }
   __device__ __forceinline__ bool some(int i) const { return c(i) < channels && (!WINDOW || c(i) + VEC > 0); }
-  __device__ __forceinline__ bool inside(int i, int j) const { return !WINDOW || (c(i) + j >= 0 && c(i) + j < channels); }
+  __device__ __forceinline__ void settle(int i) {
+    if (WINDOW && (c(i) < 0 || c(i) + VEC > channels)) {          // (the first and the last of a row)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        if (c(i) + j < 0 || c(i) + j >= channels) v[i][j] = 0.0f;
+    }
+  }
   // w, b: at element 0 (or, with a window, at the row's copy of the vectors)
   __device__ __forceinline__ void operator()(int kind, float eps, const float *w, const float *b, int slot) {
     float mean = 0.0f, sq = 0.0f;
@@ -136,10 +142,10 @@ struct RowNorm {
     for (int i = 0; i < ITEMS; ++i)
       if (some(i)) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          v[i][j] = inside(i, j) ? v[i][j] - mean : 0.0f;
-          sq = fmaf(v[i][j], v[i][j], sq);
-        }
+        for (int j = 0; j < VEC; ++j) v[i][j] -= mean;
+        if (kind == 2) settle(i);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) sq = fmaf(v[i][j], v[i][j], sq);
       }
     const float by = 1.0f / sqrtf(row_sum<WARP>(sq, part, slot + 1) / channels + eps);
 #pragma unroll
@@ -148,12 +154,13 @@ struct RowNorm {
         float wv[VEC];
         load_w<VEC>(wv, w + c(i));
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) v[i][j] = inside(i, j) ? v[i][j] * by * wv[j] : 0.0f;
+        for (int j = 0; j < VEC; ++j) v[i][j] = v[i][j] * by * wv[j];
         if (b) {
           load_w<VEC>(wv, b + c(i));
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) v[i][j] += wv[j];         // (zero outside the row)
+          for (int j = 0; j < VEC; ++j) v[i][j] += wv[j];
         }
+        settle(i);
       }
   }
 };
