@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(128 + TILES_WARPS * 32, 1) gemm_tiles_kernel(c
     // stage's MMAs.
     const bool weights = warp == 0;
     const uint32_t el = elect_one();
-    int s = 0;
+    int s = 0, free_stages = weights && g.early ? STAGES : -1;
     uint32_t phase = 1;
     bool ok = true;
     for (int i = first; i < total && ok; i += step) {
@@ -365,6 +365,9 @@ __global__ void __launch_bounds__(128 + TILES_WARPS * 32, 1) gemm_tiles_kernel(c
       const int mine = columns(t.ntok) / CTAS, boxes = (mine + g.box - 1) / g.box, x0 = t.tok0 + rank * mine;
       const uint32_t bytes = CTAS * (GT_BYTES + boxes * g.box * 128);
       for (int k = 0; k < p.kt; ++k) {
+        // (a full ring empties when the kernel in front has ended, however long that takes; the wait behind this one has a limit)
+        if (free_stages == 0) griddep_wait();
+        --free_stages;
         if (!mbar_poll_warp(&empty[s], phase, abort_flag)) { ok = false; fail_code = ST_WAIT_TIMEOUT_PRODUCER; break; }
         uint8_t *dst = smem + s * L::STAGE;
         if (weights) {
@@ -525,7 +528,7 @@ cudaError_t launch_align_rows(void *dst, long long pitch, const void *src, long 
                            static_cast<const uint16_t *>(src), ld, rows, n);
 }
 
-// Kernel attributes are a device's: once for each plan.  max_pairs: the pairs of CTAs that the device holds at once (a
+// Kernel attributes are a device's: once for each of them.  max_pairs: the pairs of CTAs that the device holds at once (a
 // persistent kernel with more would have them run one after the other).
 cudaError_t init_gemm(int num_sms, int *max_pairs) {
   cudaError_t e = cudaSuccess;

@@ -111,6 +111,8 @@ void put_status(int *p) {
 
 }  // namespace
 
+constexpr int MAX_OLD = 40;
+
 struct elb_op {
   Kind kind;
   int device = 0, num_sms = 0, max_pairs = 0;
@@ -129,8 +131,10 @@ struct elb_op {
   };
   void *w[2] = {};            // packed weights: of the product, or into and out of the experts
   float *f[4] = {};           // bias, or the norms' weights and biases
-  void *ws = nullptr;         // the experts' workspace
+  void *ws = nullptr;         // the experts' workspace, or that of a product for inputs that are not aligned
   size_t ws_bytes = 0;
+  void *old[MAX_OLD] = {};    // workspaces that have become too small
+  int n_old = 0;
   ExpertsParams ep = {};
   bool count_stale = false;   // a call's launches failed half way: the experts' counts are not zero
   void *mid = nullptr;
@@ -141,6 +145,7 @@ struct elb_op {
     DeviceGuard guard(device);
     for (void *q : w) if (q) cudaFree(q);
     for (float *q : f) if (q) cudaFree(q);
+    for (int i = 0; i < n_old; ++i) cudaFree(old[i]);
     if (ws) cudaFree(ws);
     if (done) cudaEventDestroy(done);
     put_status(h_status);       // (behind the cudaFree above, which has waited for the plan's kernels)
@@ -241,15 +246,18 @@ int leave_workspace(elb_op &op, cudaStream_t s, bool capturing) {
   return ELB_OK;
 }
 
-// (cudaFree waits for the calls that still use the old one)
+// The old workspace stays with the plan: calls in flight and captured graphs may still use it.  It at least doubles, so that there
+// are few of them.
 int grow_workspace(elb_op &op, size_t bytes) {
   if (bytes <= op.ws_bytes) return ELB_OK;
+  if (op.ws && op.n_old == MAX_OLD) return op_fail(ELB_GENERAL_ERROR, "the workspace has grown too often");
+  const size_t want = bytes > 2 * op.ws_bytes ? bytes : 2 * op.ws_bytes;
   void *q = nullptr;
-  OP_TRY(cudaMalloc(&q, bytes));
-  if (op.ws) cudaFree(op.ws);
-  op.bytes += bytes - op.ws_bytes;
+  OP_TRY(cudaMalloc(&q, want));
+  if (op.ws) op.old[op.n_old++] = op.ws;
+  op.bytes += want;
   op.ws = q;
-  op.ws_bytes = bytes;
+  op.ws_bytes = want;
   return ELB_OK;
 }
 
@@ -296,7 +304,7 @@ int drop(elb_op &op, int rc) {
   cudaGetLastError();
   for (void *&q : op.w) if (q) { cudaFree(q); q = nullptr; }
   for (float *&q : op.f) if (q) { cudaFree(q); q = nullptr; }
-  op.bytes = op.ws_bytes;
+  op.bytes = op.ws_bytes;       // (a plan that is not prepared has made no call: no older workspaces)
   return rc;
 }
 
@@ -541,7 +549,7 @@ int elb_experts_create(const elb_experts_desc_t *desc, elb_op_t **out) {
   if (d.experts > 1024 || d.top_k > 32) return op_fail(ELB_UNIMPLEMENTED, "%d of %d experts: at most 32 of 1024", d.top_k, d.experts);
   if (d.dt != ELB_BF16 && d.dt != ELB_F16) return op_fail(ELB_UNIMPLEMENTED, "experts take bf16 and f16");
   if (d.activation < ELB_ACT_NONE || d.activation > ELB_ACT_SILU) return op_fail(ELB_GENERAL_ERROR, "activation %d", d.activation);
-  if (d.max_rows < 1 || d.max_rows * d.top_k > MAX_ROWS) return op_fail(ELB_GENERAL_ERROR, "max_rows %lld", (long long)d.max_rows);
+  if (d.max_rows < 1 || d.max_rows > MAX_ROWS / d.top_k) return op_fail(ELB_GENERAL_ERROR, "max_rows %lld", (long long)d.max_rows);
   int rc = check_ld("input", d.ld_input, d.ic);
   if (rc == ELB_OK) rc = check_ld("output", d.ld_output, d.ic);
   elb_op *op = nullptr;

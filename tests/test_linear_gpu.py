@@ -202,6 +202,32 @@ def test_streams_and_graphs(U):
         assert lin.device_status() == 0
 
 
+def test_a_captured_call_outlives_a_larger_workspace(U):
+    """Inputs that are not aligned go through the plan's workspace; a graph captured with a small one is right after larger calls."""
+    E = U.E
+    ic, oc = 333, 320
+    w = U.randn(oc, ic, dtype=torch.bfloat16, seed=2, scale=0.05)
+    lin = E.Linear(ic, oc)
+    assert lin.prepare(w) == 0
+    x, y = U.randn(300, ic, dtype=torch.bfloat16, seed=1), torch.empty(300, oc, dtype=torch.bfloat16, device="cuda")
+    assert lin.enqueue(y, x, rows=300) == 0
+    want = y.clone()
+    g, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(g, stream=s):
+        assert lin.enqueue(y, x, rows=300, stream=s.cuda_stream) == 0, E.last_error()
+    for rows in (900, 5000, 20000):
+        big, out = U.randn(rows, ic, dtype=torch.bfloat16, seed=rows), torch.empty(rows, oc, dtype=torch.bfloat16, device="cuda")
+        assert lin.enqueue(out, big, rows=rows) == 0
+        torch.cuda.synchronize()
+        filler = torch.full((rows, ic), float("nan"), dtype=torch.bfloat16, device="cuda")     # takes memory that was given back
+        y.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+        U.close(out, *U.linear64(big, w, None, None, "none", False, 1.0), E.bf16)
+        del filler
+
+
 def test_host_weights(U):
     E = U.E
     x, w = U.randn(10, 70, dtype=torch.float16, seed=1), U.randn(90, 70, dtype=torch.float16, seed=2)

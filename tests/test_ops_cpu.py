@@ -48,7 +48,7 @@ def test_route_refusals(pkg, kw, code, word):
 
 
 BAD_EXPERTS = [(dict(experts=0), 2, "experts"), (dict(experts=2000), 1, "1024"), (dict(top_k=33), 1, "32"), (dict(ic=0), 2, "channels"), (dict(mid=0), 2, "channels"), (dict(dtype=1), 1, "bf16"),
-               (dict(activation=-1), 2, "activation"), (dict(max_rows=0), 2, "max_rows"), (dict(max_rows=1 << 31), 2, "max_rows"), (dict(ld_input=1), 2, "apart")]
+               (dict(activation=-1), 2, "activation"), (dict(max_rows=0), 2, "max_rows"), (dict(max_rows=1 << 31), 2, "max_rows"), (dict(max_rows=1 << 62, top_k=4), 2, "max_rows"), (dict(ld_input=1), 2, "apart")]
 
 
 @pytest.mark.parametrize("kw,code,word", BAD_EXPERTS, ids=str)
