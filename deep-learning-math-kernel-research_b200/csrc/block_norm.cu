@@ -7,7 +7,7 @@
 // is HBM for long calls and the chain load -> reductions -> store for short ones.  Layer norm takes its variance around the
 // mean, from the registers, not from a difference of sums.
 //
-// Rows of up to 1024 channels belong to a warp (no block barriers), longer ones to a block.
+// Rows of up to 1024 channels belong to a warp (no block barriers), longer ones to a block, which in long calls walks several.
 // Rows that do not start at 16-byte boundaries (an odd number of channels) are taken in the aligned 8-element windows that cover
 // them, the first and last of which are partly outside; the weights exist once for each of the eight places a row can
 // start at (2500 x 1155, layer norms and gate, f16:
@@ -247,6 +247,77 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) block_norm_kernel(const NormP
   }
 }
 
+// Many aligned rows without a gate: blocks that walk them, a thread two vectors of each, the next row's input and residual on their
+// way in registers while this row's sums are joined.  A block that has one row idles at each sum's barrier, and other blocks of its SM fill that only as
+// far as registers go; with the loads in front it needs a third fewer threads for the same bytes in flight.  16384 x 4096 with two RMS
+// norms and an fp32 residual: 135 us, 6.0 TB/s of 6.6 that a copy reaches (a block a row 149).  One row ahead, three blocks of 256
+// threads on an SM: four leave too few registers (179), two too few warps (148), one vector a thread in 512 threads 145.
+template <typename T, typename TR, int MOST, int BLOCKS>
+__global__ void __launch_bounds__(MOST, BLOCKS) block_norm_walk_kernel(const NormParams p) {
+  constexpr int ITEMS = 2, VEC = 8;
+  __shared__ float part[2][4][32];                                // by the row's parity: one barrier lies between two rows' uses of a slot
+  griddep_launch_dependents();
+  griddep_wait();
+  const int c0 = threadIdx.x * VEC;
+  Raw<T, VEC> raw[ITEMS];
+  Raw<TR, VEC> res[ITEMS];
+  auto ask = [&](long long row) {
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int c = c0 + i * (int)blockDim.x * VEC;
+      if (c < p.channels) {
+        raw[i].load(static_cast<const T *>(p.x) + row * p.ld_x + c);
+        if (p.res) res[i].load(static_cast<const TR *>(p.res) + row * p.ld_res + c);
+      }
+    }
+  };
+  ask(blockIdx.x);
+  int odd = 0;
+  for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, odd ^= 1) {
+    float v[ITEMS][VEC];
+    Raw<TR, VEC> add[ITEMS];
+    RowNorm<VEC, ITEMS, false, false> norm{v, part[odd], c0, (int)blockDim.x * VEC, p.channels};
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      if (norm.some(i)) raw[i].get(v[i]);
+      else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[i][j] = 0.0f;
+      }
+      add[i] = res[i];
+    }
+    if (row + gridDim.x < p.rows) ask(row + gridDim.x);
+    if (p.post != 0) norm(p.post, p.post_eps, p.post_w, p.post_b, 0);
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int c = norm.c(i);
+      if (norm.some(i)) {
+        float o[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[i][j] *= p.scale;
+        if (p.res) {
+          add[i].get(o);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) v[i][j] += o[j];
+        }
+        if (p.sum) Raw<TR, VEC>::store(static_cast<TR *>(p.sum) + row * p.ld_sum + c, v[i]);
+      }
+    }
+    if (p.pre != 0 && p.y) {
+      norm(p.pre, p.pre_eps, p.pre_w, p.pre_b, 2);
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i)
+        if (norm.some(i)) Raw<T, VEC>::store(static_cast<T *>(p.y) + row * p.ld_y + norm.c(i), v[i]);
+    }
+  }
+}
+template <typename T, typename TR, int MOST, int BLOCKS>
+cudaError_t by_walk(const NormParams &p, int n, cudaStream_t s) {
+  const int threads = (n + 63) / 64 * 32;
+  const long long most = (long long)p.num_sms * (MOST * BLOCKS / threads);
+  return launch_overlapped(block_norm_walk_kernel<T, TR, MOST, BLOCKS>, dim3((unsigned)(p.rows < most ? p.rows : most)), dim3(threads), 0, s, p);
+}
+
 // Copy a of a vector has element c at index a + c: eight places that a row's first element can have in its window, zeros around.
 __global__ void norm_vector_kernel(float *dst, const void *src, int et, int n, long long pitch, float offset) {
   const long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x;
@@ -280,9 +351,21 @@ cudaError_t by_vectors(const NormParams &p, int n, cudaStream_t s) {
   if (few && n <= 1024) return by_blocks<T, TR, 8, 1, WINDOW>(p, n, s);
   if (n <= 64) return by_warps<T, TR, 8, 2, WINDOW>(p, s);
   if (n <= 128) return by_warps<T, TR, 8, 4, WINDOW>(p, s);
+  // Walked: rows with two sums or more, where a barrier's wait is what the loads ahead hide (us, walked / a block a row: 16384 x 4096,
+  // two RMS norms 102 / 113, a layer norm 78 / 92, but one RMS norm 91 / 82), and rows of more than 512 vectors, whose blocks are too
+  // large for several on an SM (one RMS norm: 9000 x 8192 100 / 103, 2400 x 6144 21.2 / 26.6; two: 9000 x 8192 169 / 193).  From two
+  // rows an SM on, behind `few` (300 x 4096 5.6 / 7.4, 500 8.6 / 7.9, 1100 15.1 / 16.7).  Not with a gate, whose rows are not loaded
+  // ahead (8000 x 4096, layer norms 85 / 78; 4000 x 8192, one RMS norm 61 / 52), and not up to 256 vectors, where enough blocks are
+  // resident (30000 x 1536 92.6 / 97.2, but 900 x 1600 5.5 / 5.2).
+  const int sums = p.post + (p.y ? p.pre : 0);                    // (ELB_NORM_RMS is one, ELB_NORM_LAYER two)
+  if (!WINDOW && !p.gate) {
+    if (n > 256 && n <= 512 && sums >= 2) return by_walk<T, TR, 256, 3>(p, n, s);
+    if (n > 512 && n <= 768) return by_walk<T, TR, 384, 2>(p, n, s);
+    if (n > 768 && n <= 1024) return by_walk<T, TR, 512, 1>(p, n, s);
+  }
   // (many short rows: ten blocks of 128 threads on an SM, 16384 x 1792 38.1 us, with one load per thread 43.4; 2500 x 1152 9.3 / 11.1)
   if (n <= 256) return p.rows < 32 * p.num_sms ? by_blocks<T, TR, 8, 1, WINDOW, 256>(p, n, s) : by_blocks<T, TR, 8, 2, WINDOW, 128, 10>(p, n, s);
-  // (five blocks of 256 threads on an SM: 16384 x 4096 with both norms, fp32 residual, 149.5 us, with four 162.6; one norm 80.9 / 87.4)
+  // (five blocks of 256 threads on an SM: 16384 x 4096 with one norm 80.9 us, with four 87.4)
   if (n <= 512) return by_blocks<T, TR, 8, 2, WINDOW, 256, 5>(p, n, s);
   if (n <= 1024) return by_blocks<T, TR, 8, 2, WINDOW, 512, 2>(p, n, s);
   if (n <= 2048) return by_blocks<T, TR, 8, 2, WINDOW>(p, n, s);

@@ -120,6 +120,29 @@ def test_long_calls(U, rows, n, types):
     _run(U, rows, n, *types, post="layer", pre="none", with_residual=False, pad=16)
 
 
+@pytest.mark.parametrize("rows,n", [(297, 1032), (890, 1544), (2700, 2824), (445, 4096), (447, 4104), (600, 6152), (299, 8192)])
+@pytest.mark.parametrize("types", [("bf16", "same"), ("f16", "f32"), ("f32", "same")], ids="-".join)
+def test_blocks_that_walk_rows(U, rows, n, types):
+    """Row counts around those of resident blocks: some blocks have one row more than others, or one alone."""
+    _run(U, rows, n, *types, post="rms", pre="rms", in_place=True)
+    _run(U, rows, n, *types, post="layer", pre="layer", gate_rows=rows - 1, pad=8, scale=-2.0, want_sum=False)
+    _run(U, rows, n, *types, post="none", pre="layer", with_residual=False)
+    _run(U, rows, n, *types, post="layer", pre="none", gate_rows=1)
+
+
+def test_walked_rows_that_are_not_finite_stay_alone(U):
+    E = U.E
+    rows, n = 1500, 4096
+    x = U.randn(rows, n, dtype=torch.bfloat16, seed=1)
+    odd = torch.arange(rows, device="cuda") % 7 == 3
+    x[odd, 5] = float("nan")
+    op = E.BlockNorm(n, post=E.NORM_RMS, pre=E.NORM_LAYER, with_residual=False)
+    y, s = torch.empty_like(x), torch.empty_like(x)
+    assert op.prepare() == 0 and op.enqueue(y, s, x, rows=rows) == 0
+    torch.cuda.synchronize()
+    assert bool(y[odd].isnan().all()) and bool(s[odd].isnan().all()) and bool(y[~odd].isfinite().all()) and bool(s[~odd].isfinite().all())
+
+
 @pytest.mark.parametrize("n", [9, 37, 250, 511, 1001, 1155, 1537, 2049, 4099, 9001, 16387])
 @pytest.mark.parametrize("types", [("bf16", "same"), ("f16", "f32"), ("f32", "same")], ids="-".join)
 @pytest.mark.parametrize("rows", [3, 9, 700])
