@@ -6,7 +6,7 @@
 // of a channel lie 8 lanes apart and so meet in one thread; two tokens of a channel become one word of 16-bit values, and
 // stmatrix.trans turns 8 channels by 8 tokens of those round, so that shared memory holds each token's channels in
 // order and global memory is written (and the residual read) 16 bytes per thread.  Measured for a tile of 128 channels
-// by 256 tokens, bf16, 12 warps, one CTA on every SM: 2700 cycles (gated silu 3500, silu 5800, gelu 7700, fp32 results 4900), bound by the
+// by 256 tokens, bf16, 12 warps, one CTA on every SM: 2700 cycles (gated silu 3700, silu with a bias 6000, gelu 7900, fp32 results 4800), bound by the
 // warps' instructions; with one lane of tensor memory per thread, neighbouring lanes trading values and 4-byte stores 6700.
 #pragma once
 #include "ops.cuh"
@@ -25,13 +25,14 @@ __device__ __forceinline__ float rcp(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// 1 / (1 + 2^t) for two values with one reciprocal.  The exponent is cut at 63, so that the product stays finite (and a NaN, which
-// min drops, stays out of the other value's factor: the caller multiplies it back in); values are then 2^-63 where they would be less.
+// 1 / (1 + 2^t) for two values with one reciprocal: 2^-t / (1 + 2^-t) where t > 0, so that the exponentials are at most 1 and the product of
+// the denominators at most 4, whatever t is (a sum of -1e20 gives a factor of 0; below 2^-126 it is flushed there).  min drops a NaN, which stays out of
+// the other value's factor: the caller multiplies it back in.  (silu with a bias 6000 cycles a tile; 2^t cut at 63 and 2^-t selected beyond it 6600.)
 __device__ __forceinline__ void logistic2(float t0, float t1, float &s0, float &s1) {
-  const float d0 = 1.0f + ex2(fminf(t0, 63.0f)), d1 = 1.0f + ex2(fminf(t1, 63.0f));
+  const float e0 = ex2(fminf(-fabsf(t0), 0.0f)), e1 = ex2(fminf(-fabsf(t1), 0.0f)), d0 = 1.0f + e0, d1 = 1.0f + e1;
   const float r = rcp(d0 * d1);
-  s0 = r * d1;
-  s1 = r * d0;
+  s0 = r * (t0 > 0.0f ? e0 * d1 : d1);
+  s1 = r * (t1 > 0.0f ? e1 * d0 : d0);
 }
 
 // v / (1 + 2^t(v)).  Values i and i + 4 are two channels of one token: what a value comes to depends on no other token.

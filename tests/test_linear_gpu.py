@@ -262,3 +262,63 @@ def test_refusals_of_calls(U):
     # a plan of another operator
     norm = E.BlockNorm(64)
     assert E.lib.elb_linear_enqueue(norm.h, x.data_ptr(), x.data_ptr(), None, 4, None) == E.ELB_GENERAL_ERROR
+
+
+@pytest.mark.parametrize("rows,ic", [(1, 64), (3, 64), (24, 4096), (90, 512), (700, 512)])
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
+@pytest.mark.parametrize("gated", [False, True], ids=["plain", "gated"])
+def test_activations_far_from_zero(U, rows, ic, act, gated):
+    """Sums of any size, the type's lowest value among them, on every route: one product with 1, the others with 0.
+
+    The logistic factor 1 / (1 + 2^t): t carries a relative 2^-22 (a constant, three products and sums), so the exponential 126 * 2^-22 * ln 2
+    at most before it is flushed to zero, which 2^-15 covers with the other roundings.  Behind t = 126 the factor is 0 for a value of 90 at
+    most (silu; the tanh form: 7), an error under 90 * 2^-126 < 2^-119."""
+    E = U.E
+    v = torch.tensor([-3.3895313892515355e38, -1e30, -1e20, -1e10, -40000.0, -300.0, -126.0, -90.0, -86.5, -64.0, -50.0, -44.0, -20.0, -11.0, -6.0, -4.5, -3.0,
+                      -1.0, -0.01, 0.0, 0.5, 3.0, 20.0, 70.0, 1e4, 1e20, 3e38, float("inf"), float("-inf"), float("nan")], device="cuda").to(torch.bfloat16)
+    if gated:
+        v = v[:-3]                                 # (the up row's product with 0 makes NaN of those)
+    rows = max(rows, 1)
+    oc = 150
+    x = torch.zeros(rows, ic, dtype=torch.bfloat16, device="cuda")
+    w = torch.zeros(2 * oc if gated else oc, ic, dtype=torch.bfloat16, device="cuda")
+    w[:oc, 5], w[oc:, 9] = 1.0, 1.0
+    x[:, 9] = 1.0
+    for out in (E.f32, E.bf16):
+        lin = E.Linear(ic, oc, out_dtype=out, activation=U.ACTS[act], gated=gated)
+        assert lin.prepare(w) == 0
+        for k in range(0, len(v), rows):           # every value in some row
+            x[:, 5] = v[(torch.arange(rows, device="cuda") + k) % len(v)]
+            y = torch.empty(rows, oc, dtype=U.TORCH[out], device="cuda")
+            assert lin.enqueue(y, x, rows=rows) == 0
+            torch.cuda.synchronize()
+            z = x[:, 5:6].double()
+            t = z if act == "silu" else 2 * math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3)
+            want = (z * torch.sigmoid(t)).expand(rows, oc)
+            odd = want.isnan()
+            assert bool(y[odd].isnan().all()), "an infinite sum times a factor of zero, and NaN, are NaN as in the formula"
+            U.close(y[~odd], want[~odd], 2.0 ** -15 * want[~odd].abs() + 2.0 ** -119, out)
+
+
+@pytest.mark.parametrize("rows", [1, 20, 300])
+@pytest.mark.parametrize("act", ["relu", "gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("gated", [False, True], ids=["plain", "gated"])
+def test_channels_that_are_not_finite_stay_alone(U, rows, act, gated):
+    """A NaN or an infinity in some channels of a token changes no bit of the others (two of them share a reciprocal)."""
+    E = U.E
+    ic, oc = 64, 96
+    x = U.randn(rows, ic, dtype=torch.bfloat16, seed=1)
+    w = U.randn(2 * oc if gated else oc, ic, dtype=torch.bfloat16, seed=2, scale=0.3)
+    odd = torch.zeros(oc, dtype=torch.bool, device="cuda")
+    odd[[0, 9, 18, 27, 37, 63, 95]] = True
+    ys = []
+    for value in (None, float("nan"), float("inf"), 3e38):
+        wv = w.clone()
+        if value is not None:
+            wv[:oc][odd] = value
+        lin, y = E.Linear(ic, oc, activation=U.ACTS[act], gated=gated), torch.empty(rows, oc, dtype=torch.bfloat16, device="cuda")
+        assert lin.prepare(wv) == 0 and lin.enqueue(y, x, rows=rows) == 0
+        torch.cuda.synchronize()
+        ys.append(y)
+        assert torch.equal(y[:, ~odd], ys[0][:, ~odd])
+    assert bool(ys[1][:, odd].isnan().all())
