@@ -19,6 +19,9 @@ __device__ __forceinline__ uint32_t order_key(float v) {
   return b ^ (static_cast<uint32_t>(static_cast<int>(b) >> 31) | 0x80000000u);      // larger than 0 for every value, -inf too
 }
 
+// The key of an expert of a closed group: below an open one's whose choice is -inf.  top_k is at most the open experts, so it is never taken.
+constexpr uint32_t SHUT_KEY = 1u;
+
 // the two best of (a, b) and (c, d), a >= b and c >= d
 __device__ __forceinline__ void merge2(float &a, float &b, float c, float d) {
   b = fmaxf(fminf(a, c), fmaxf(b, d));
@@ -138,7 +141,7 @@ __global__ void __launch_bounds__(WARPS * 32) route_kernel(const RouteParams p) 
   if (shut) {
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i)
-      if ((shut >> i) & 1u) key[i] = order_key(-INFINITY);
+      if ((shut >> i) & 1u) key[i] = SHUT_KEY;
   }
   if (!full) {
 #pragma unroll

@@ -183,3 +183,30 @@ def test_refusals_of_calls(U):
     assert op.enqueue(ids, None, None, rows=4) == E.ELB_GENERAL_ERROR
     assert op.enqueue(ids, None, z, rows=-3) == E.ELB_GENERAL_ERROR
     assert op.enqueue(ids, None, z, rows=0) == E.ELB_OK and op.launch_count() == 0
+
+
+@pytest.mark.parametrize("n,groups,top", [(64, 8, 2), (256, 8, 4), (60, 4, 2), (96, 32, 6), (40, 5, 3)])
+@pytest.mark.parametrize("sigmoid", [False, True], ids=["softmax", "sigmoid"])
+@pytest.mark.parametrize("shut", [float("-inf"), float("nan")], ids=["-inf", "nan"])
+def test_only_experts_of_open_groups(U, n, groups, top, sigmoid, shut):
+    """A bias that leaves each group one expert that counts: the others of the open groups come next, by their index, and no expert of a
+    closed group does, however low its index."""
+    E = U.E
+    size, rows = n // groups, 40
+    z = _spread(U, rows, n, n)
+    bias = torch.full((n,), shut, device="cuda")
+    bias[size - 1::size] = 0.0
+    k = min(8, size * top)
+    op = E.Route(n, k, score=E.SCORE_SIGMOID if sigmoid else E.SCORE_SOFTMAX, with_bias=True, groups=groups, top_groups=top, renormalise=False)
+    ids, w = torch.empty(rows, k, dtype=torch.int32, device="cuda"), torch.empty(rows, k, device="cuda")
+    assert op.prepare(bias) == 0 and op.enqueue(ids, w, z, rows=rows) == 0
+    torch.cuda.synchronize()
+    zd = z.double()
+    score = torch.sigmoid(zd) if sigmoid else torch.softmax(zd, 1)
+    for t in range(rows):
+        best = score[t, size - 1::size].sort(descending=True).indices[:top].tolist()
+        want = [g * size + size - 1 for g in best]
+        want += sorted(g * size + i for g in best for i in range(size - 1))
+        assert ids[t].tolist() == want[:k]
+    got = score.gather(1, ids.long())
+    assert bool(((w.double() - got).abs() <= 64 * 2.0 ** -24 * got).all())
