@@ -121,7 +121,7 @@ struct elb_op {
   int *h_status = nullptr, *d_status = nullptr;
   // Orders the calls of a plan with workspace across streams.
   cudaEvent_t done = nullptr;
-  cudaStream_t last = nullptr;
+  unsigned long long last = 0;      // the last call's stream, by its id
   bool pending = false;
   union {
     elb_linear_desc_t lin;
@@ -230,18 +230,22 @@ int check_ld(const char *what, int64_t &ld, int64_t dense) {
 
 bool finite(float v) { return v - v == 0.0f; }
 
-// The plan's workspace may still be in use by its last call, on another stream.
+// The plan's workspace may still be in use by its last call, on another stream.  Streams are told apart by their ids: cudaStreamPerThread is one
+// handle for a stream of each thread, and a destroyed stream's handle may come back while its work still runs.
 int enter_workspace(elb_op &op, cudaStream_t s, bool &capturing) {
   cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
   OP_TRY(cudaStreamIsCapturing(s, &st));
   capturing = st != cudaStreamCaptureStatusNone;
-  if (!capturing && op.pending && op.last != s) OP_TRY(cudaStreamWaitEvent(s, op.done, 0));
+  if (capturing) return ELB_OK;
+  unsigned long long id = 0;
+  OP_TRY(cudaStreamGetId(s, &id));
+  if (op.pending && op.last != id) OP_TRY(cudaStreamWaitEvent(s, op.done, 0));
+  op.last = id;
   return ELB_OK;
 }
 int leave_workspace(elb_op &op, cudaStream_t s, bool capturing) {
   if (capturing) return ELB_OK;
   OP_TRY(cudaEventRecord(op.done, s));
-  op.last = s;
   op.pending = true;
   return ELB_OK;
 }

@@ -322,3 +322,41 @@ def test_channels_that_are_not_finite_stay_alone(U, rows, act, gated):
         ys.append(y)
         assert torch.equal(y[:, ~odd], ys[0][:, ~odd])
     assert bool(ys[1][:, odd].isnan().all())
+
+
+def test_per_thread_streams_take_turns_in_the_workspace(U):
+    """cudaStreamPerThread is one handle for a stream of each thread: a call in one thread comes behind the other thread's call of the plan."""
+    import threading
+    E = U.E
+    rows, ic, oc, per_thread = 500, 333, 200, 2
+    w = U.randn(oc, ic, dtype=torch.bfloat16, seed=2, scale=0.05)
+    xs = [U.randn(rows, ic, dtype=torch.bfloat16, seed=k) for k in range(2)]
+    ys = [torch.empty(rows, oc, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    lin = E.Linear(ic, oc)
+    assert lin.prepare(w) == 0
+    first_done, results = torch.cuda.Event(), []
+    for x, y in zip(xs, ys):
+        assert lin.enqueue(y, x, rows=rows) == 0
+        y.zero_()
+    torch.cuda.synchronize()
+
+    def call(k):
+        stream = torch.cuda.ExternalStream(per_thread)
+        with torch.cuda.stream(stream):
+            if k == 0:
+                torch.cuda._sleep(200_000_000)             # 0.1 s in front of the first thread's call
+            results.append(lin.enqueue(ys[k], xs[k], rows=rows, stream=per_thread))
+            if k == 0:
+                first_done.record(stream)
+            else:
+                stream.synchronize()
+                results.append(first_done.query())
+
+    for k in range(2):
+        t = threading.Thread(target=call, args=(k,))
+        t.start()
+        t.join()
+    torch.cuda.synchronize()
+    assert results == [0, 0, True]
+    for x, y in zip(xs, ys):
+        U.close(y, *U.linear64(x, w, None, None, "none", False, 1.0), E.bf16)
