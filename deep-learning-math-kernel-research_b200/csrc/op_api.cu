@@ -232,23 +232,37 @@ bool finite(float v) { return v - v == 0.0f; }
 
 // The plan's workspace may still be in use by its last call, on another stream.  Streams are told apart by their ids: cudaStreamPerThread is one
 // handle for a stream of each thread, and a destroyed stream's handle may come back while its work still runs.
-int enter_workspace(elb_op &op, cudaStream_t s, bool &capturing) {
-  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
-  OP_TRY(cudaStreamIsCapturing(s, &st));
-  capturing = st != cudaStreamCaptureStatusNone;
-  if (capturing) return ELB_OK;
-  unsigned long long id = 0;
-  OP_TRY(cudaStreamGetId(s, &id));
-  if (op.pending && op.last != id) OP_TRY(cudaStreamWaitEvent(s, op.done, 0));
-  op.last = id;
-  return ELB_OK;
-}
-int leave_workspace(elb_op &op, cudaStream_t s, bool capturing) {
-  if (capturing) return ELB_OK;
-  OP_TRY(cudaEventRecord(op.done, s));
-  op.pending = true;
-  return ELB_OK;
-}
+// A call that fails half way has launched kernels that use it all the same: whatever way the call ends, its last launch is noted.
+class WorkspaceCall {
+ public:
+  bool capturing = false;
+  WorkspaceCall(elb_op &op, cudaStream_t s) : op_(op), s_(s) {}
+  int enter() {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    OP_TRY(cudaStreamIsCapturing(s_, &st));
+    capturing = st != cudaStreamCaptureStatusNone;
+    if (capturing) return ELB_OK;
+    unsigned long long id = 0;
+    OP_TRY(cudaStreamGetId(s_, &id));
+    if (op_.pending && op_.last != id) OP_TRY(cudaStreamWaitEvent(s_, op_.done, 0));
+    op_.last = id;
+    inside_ = true;
+    return ELB_OK;
+  }
+  int leave() {
+    if (!inside_) return ELB_OK;
+    inside_ = false;
+    OP_TRY(cudaEventRecord(op_.done, s_));
+    op_.pending = true;
+    return ELB_OK;
+  }
+  ~WorkspaceCall() { if (inside_ && cudaEventRecord(op_.done, s_) == cudaSuccess) op_.pending = true; }
+
+ private:
+  elb_op &op_;
+  cudaStream_t s_;
+  bool inside_ = false;
+};
 
 // The old workspace stays with the plan: calls in flight and captured graphs may still use it.  It at least doubles, so that there
 // are few of them.
@@ -400,8 +414,8 @@ int elb_linear_enqueue(elb_op_t *op, void *output, const void *input, const void
   }
   // rows that a tiled copy cannot read go through the plan's workspace
   const int64_t pitch = up(d.ic, 8);
-  bool capturing = false;
-  rc = enter_workspace(*op, s, capturing);
+  WorkspaceCall use(*op, s);
+  rc = use.enter();
   if (rc == ELB_OK) rc = grow_workspace(*op, (size_t)rows * pitch * 2);
   if (rc != ELB_OK) return rc;
   OP_TRY(launch_align_rows(op->ws, pitch, input, d.ld_input, (int)rows, d.ic, s));
@@ -409,7 +423,7 @@ int elb_linear_enqueue(elb_op_t *op, void *output, const void *input, const void
   p.ld_x = pitch;
   OP_TRY(launch_gemm(p, s));
   op->launches += 2;
-  return leave_workspace(*op, s, capturing);
+  return use.leave();
 }
 
 // ------------------------------------------------------------------------------------------- norm
@@ -616,8 +630,8 @@ int elb_experts_enqueue(elb_op_t *op, void *output, const void *input, const int
   if (!aligned(output, 2) || !aligned(input, 2) || !aligned(ids, 4) || !aligned(weights, 4)) return op_fail(ELB_GENERAL_ERROR, "misaligned tensor");
   DeviceGuard guard(op->device);
   const cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
-  bool capturing = false;
-  rc = enter_workspace(*op, s, capturing);
+  WorkspaceCall use(*op, s);
+  rc = use.enter();
   if (rc != ELB_OK) return rc;
   ExpertsParams e = op->ep;
   e.rows = (int)rows;
@@ -678,7 +692,7 @@ int elb_experts_enqueue(elb_op_t *op, void *output, const void *input, const int
     q.epi.out_et = e.et;
     OP_TRY(launch_gemv_experts(p, q, ids, weights, (int)rows, d.top_k, d.experts, s));
     op->launches += 2;
-    return leave_workspace(*op, s, capturing);
+    return use.leave();
   }
   const bool count = !experts_count_here(slots);
   e.clear = count;
@@ -693,7 +707,7 @@ int elb_experts_enqueue(elb_op_t *op, void *output, const void *input, const int
   OP_TRY(launch_experts_combine(e, s));
   if (count) op->count_stale = false;
   op->launches += count ? 5 : 4;
-  return leave_workspace(*op, s, capturing);
+  return use.leave();
 }
 
 // ------------------------------------------------------------------------------------------- all

@@ -203,12 +203,26 @@ void one_handle() {
   }
 }
 
+// A call whose launch fails half way leaves kernels in flight that use the workspace: a call on another stream comes behind them.
+template <typename Plan>
+void failed(std::vector<std::string> launches) {
+  Plan p;
+  need(p.call(5) == ELB_OK, "call");
+  for (const std::string &l : launches) {
+    g_fail = l;
+    need(p.call(6) != ELB_OK, "a call whose launch failed");
+    g_fail.clear();
+    need(p.call(7) == ELB_OK, "the call behind a failed one");
+  }
+}
+
 }  // namespace
 
 int main(int argc, char **argv) {
   const std::string what = argc > 1 ? argv[1] : "";
   if (what == "streams") { streams<Linear>(); g_users.clear(); streams<Experts>(); }
   else if (what == "one_handle") { one_handle<Linear>(); g_users.clear(); one_handle<Experts>(); }
+  else if (what == "failed") { failed<Linear>({"gemm"}); g_users.clear(); failed<Experts>({"gather", "gemm", "combine"}); }
   else { std::printf("no such case\n"); return 2; }
   if (g_bad == 0) std::printf("ok\n");
   return g_bad != 0;

@@ -31,3 +31,7 @@ def test_calls_on_several_streams_take_turns_in_the_workspace(check):
 def test_streams_that_share_a_handle_take_turns_in_the_workspace(check):
     """cudaStreamPerThread is one handle for a stream of each thread, and a destroyed stream's handle may come back."""
     check("one_handle")
+
+
+def test_a_call_that_failed_half_way_is_waited_for(check):
+    check("failed")
