@@ -136,7 +136,7 @@ struct elb_op {
   void *old[MAX_OLD] = {};    // workspaces that have become too small
   int n_old = 0;
   ExpertsParams ep = {};
-  bool count_stale = false;   // a call's launches failed half way: the experts' counts are not zero
+  bool count_stale = false;   // a call's launches failed half way and the experts' counts could not be cleared behind them
   void *mid = nullptr;
   int64_t pitch_mid = 0;
 
@@ -695,17 +695,20 @@ int elb_experts_enqueue(elb_op_t *op, void *output, const void *input, const int
     return use.leave();
   }
   const bool count = !experts_count_here(slots);
+  const size_t count_bytes = d.experts * sizeof(int);
   e.clear = count;
-  if (count) {
-    if (op->count_stale) OP_TRY(cudaMemsetAsync(e.count, 0, d.experts * sizeof(int), s));
-    op->count_stale = true;
-    OP_TRY(launch_experts_count(e, s));
+  if (count && op->count_stale) {
+    OP_TRY(cudaMemsetAsync(e.count, 0, count_bytes, s));
+    if (!use.capturing) op->count_stale = false;       // (what is captured has not run)
   }
-  OP_TRY(launch_experts_gather(e, op->num_sms, s));
-  OP_TRY(launch_gemm(p, s));
-  OP_TRY(launch_gemm(q, s));
-  OP_TRY(launch_experts_combine(e, s));
-  if (count) op->count_stale = false;
+  cudaError_t err = count ? launch_experts_count(e, s) : cudaSuccess;
+  if (err == cudaSuccess) err = launch_experts_gather(e, op->num_sms, s);
+  if (err == cudaSuccess) err = launch_gemm(p, s);
+  if (err == cudaSuccess) err = launch_gemm(q, s);
+  if (err == cudaSuccess) err = launch_experts_combine(e, s);
+  // The sum over a token's experts, which leaves zero counts, has not been launched
+  if (err != cudaSuccess && count && cudaMemsetAsync(e.count, 0, count_bytes, s) != cudaSuccess && !use.capturing) op->count_stale = true;
+  OP_TRY(err);
   op->launches += count ? 5 : 4;
   return use.leave();
 }

@@ -30,7 +30,7 @@ std::map<cudaStream_t, unsigned long long> g_ids;             // the id a handle
 std::map<cudaEvent_t, std::map<unsigned long long, int>> g_events;
 std::set<cudaStream_t> g_capturing;
 std::map<unsigned long long, int> g_users;                    // the last work of each stream in the plan's workspace
-std::string g_fail;                                           // the launch that fails
+std::string g_fail, g_fail_too;                               // the launches that fail
 int g_device = 0;
 std::map<const void *, int> g_on_device;                      // device pointers of the caller's, and where they lie
 std::map<int, int> g_waits;                                   // cudaDeviceSynchronize per device
@@ -82,7 +82,7 @@ cudaError_t cudaMemcpy(void *d, const void *s, size_t n, cudaMemcpyKind) { memcp
 cudaError_t cudaMemset(void *p, int v, size_t n) { memset(p, v, n); return cudaSuccess; }
 cudaError_t cudaMemsetAsync(void *p, int, size_t, cudaStream_t s) {
   g_log.push_back("memset");
-  if (g_fail == "memset") return cudaErrorInvalidValue;
+  if (g_fail == "memset" || g_fail_too == "memset") return cudaErrorInvalidValue;
   if (p == g_counts && !g_capturing.count(s)) g_counts_dirty = false;
   return cudaSuccess;
 }
@@ -216,6 +216,46 @@ void failed(std::vector<std::string> launches) {
   }
 }
 
+// The experts' counts are zero when a call begins to count, whatever came before: calls that failed behind the counting, captured calls in
+// between (which run later, or never), and calls of few slots, which count elsewhere.
+void counts() {
+  for (const char *launch : {"gather", "gemm", "combine"})
+    for (bool memset_fails : {false, true}) {
+      Experts p;
+      need(p.call(5) == ELB_OK && p.call(5, 10) == ELB_OK && p.call(5) == ELB_OK, "calls");
+      g_fail = launch;
+      if (!memset_fails) {
+        need(p.call(5) != ELB_OK, "a call whose launch failed");
+        g_fail.clear();
+        need(!g_counts_dirty, "a failed call leaves counts behind that a captured call adds to");
+      } else {
+        g_fail_too = "memset";
+        need(p.call(5) != ELB_OK, "a call whose launch failed, and the clearing behind it");
+        g_fail = "memset";
+        g_fail_too.clear();
+        need(p.call(5) != ELB_OK, "a call that could not clear the counts");
+        g_fail.clear();
+      }
+      g_capturing.insert(handle(6));
+      g_log.clear();
+      need(p.call(6) == ELB_OK, "a captured call");
+      need(!memset_fails || g_log[0] == "memset", "a captured call behind counts that are not zero clears them");
+      g_capturing.clear();
+      need(p.call(5) == ELB_OK, "the call behind them");
+      need(p.call(7) == ELB_OK && !g_counts_dirty, "calls");
+      g_users.clear();
+    }
+  // a capture that breaks off
+  Experts p;
+  g_capturing.insert(handle(6));
+  g_fail = "gemm";
+  need(p.call(6) != ELB_OK, "a captured call whose launch failed");
+  g_fail.clear();
+  need(g_log.back() == "memset", "the graph of a captured call that failed clears the counts");
+  g_capturing.clear();
+  need(p.call(5) == ELB_OK && p.call(5) == ELB_OK, "calls");
+}
+
 }  // namespace
 
 int main(int argc, char **argv) {
@@ -223,6 +263,7 @@ int main(int argc, char **argv) {
   if (what == "streams") { streams<Linear>(); g_users.clear(); streams<Experts>(); }
   else if (what == "one_handle") { one_handle<Linear>(); g_users.clear(); one_handle<Experts>(); }
   else if (what == "failed") { failed<Linear>({"gemm"}); g_users.clear(); failed<Experts>({"gather", "gemm", "combine"}); }
+  else if (what == "counts") counts();
   else { std::printf("no such case\n"); return 2; }
   if (g_bad == 0) std::printf("ok\n");
   return g_bad != 0;

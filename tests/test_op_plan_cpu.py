@@ -35,3 +35,7 @@ def test_streams_that_share_a_handle_take_turns_in_the_workspace(check):
 
 def test_a_call_that_failed_half_way_is_waited_for(check):
     check("failed")
+
+
+def test_experts_counts_start_from_zero_behind_failed_and_captured_calls(check):
+    check("counts")
