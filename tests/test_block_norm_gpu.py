@@ -214,3 +214,15 @@ def test_refusals_of_calls(U):
     assert op.enqueue(x, x, x, x, None, rows=4) == E.ELB_GENERAL_ERROR
     assert op.enqueue(x, x, x.data_ptr() + 1, x, x, rows=1) == E.ELB_GENERAL_ERROR
     assert op.enqueue(x, x, x, x, x, rows=0) == E.ELB_OK and op.launch_count() == 0
+
+
+@pytest.mark.parametrize("rows,n", [(297, 2064), (445, 4096), (900, 4088), (447, 4104), (600, 6144), (299, 8192), (1000, 8184)])
+@pytest.mark.parametrize("types", [("bf16", "same"), ("f16", "f32"), ("f32", "same")], ids="-".join)
+def test_walked_rows_without_a_gate(U, rows, n, types):
+    """Rows of 257 vectors and more without a gate: a scale, no sum, rows further apart, one output in the residual's place."""
+    _run(U, rows, n, *types, post="rms", pre="layer", scale=-2.0, want_sum=False)
+    _run(U, rows, n, *types, post="layer", pre="rms", scale=0.3, pad=8)
+    _run(U, rows, n, *types, post="rms", pre="rms", scale=-0.5, in_place=True, pad=24)
+    _run(U, rows, n, *types, post="layer", pre="layer", with_residual=False, want_sum=False)
+    _run(U, rows, n, *types, post="layer", pre="none", scale=-2.0)
+    _run(U, rows, n, *types, post="rms", pre="none")

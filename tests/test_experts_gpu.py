@@ -193,3 +193,71 @@ def test_the_four_together(U, rows, channels, dtype):
     torch.cuda.synchronize()
     y2.copy_(ff.out[:rows])
     assert torch.equal(y2, out) and torch.equal(s2, s)
+
+
+@pytest.mark.parametrize("rows", [513, 700, 3000])
+def test_loads_of_counted_calls(U, rows):
+    """More than 2048 slots, which a kernel of its own counts, over several of its blocks: all tokens to one expert, ids outside the experts,
+    experts that nobody wants, rows without any."""
+    k, experts = 4, 9
+    ids = torch.full((rows, k), 5, dtype=torch.int32, device="cuda")
+    _run(U, rows, experts, k, 96, 80, ids=ids)
+    g = torch.Generator().manual_seed(rows)
+    ids = torch.randint(-2, experts + 2, (rows, k), generator=g).to(torch.int32)
+    ids[(ids == 3) | (ids == 0)] = 8
+    ids[0] = -1
+    ids[1] = torch.tensor([2147483647, -2147483648, 9, 8], dtype=torch.int32)
+    ids[rows // 2:rows // 2 + 40] = -1
+    _, y = _run(U, rows, experts, k, 96, 80, ids=ids.cuda())
+    assert bool((y[0] == 0).all()) and bool((y[rows // 2:rows // 2 + 40] == 0).all())
+    _, y = _run(U, rows, experts, k, 96, 80, ids=torch.full((rows, k), -1, dtype=torch.int32, device="cuda"))
+    assert bool((y == 0).all())
+    ids = torch.full((rows, k), -1, dtype=torch.int32, device="cuda")
+    ids[rows - 1, k - 1] = 1                       # one slot, the last
+    _, y = _run(U, rows, experts, k, 96, 80, ids=ids)
+    assert bool((y[:rows - 1] == 0).all())
+
+
+def test_one_plan_counted_and_not(U):
+    """Calls of one plan on both sides of 2048 slots, in any order."""
+    op, _ = _run(U, 1500, 8, 2, 128, 96, max_rows=1500)
+    for n, rows in enumerate((1024, 1025, 3, 1400, 1500, 64, 1025, 1, 1024, 1499)):
+        g = torch.Generator().manual_seed(n)
+        _run(U, rows, 8, 2, 128, 96, plan=op, ids=torch.randint(-1, 9, (rows, 2), generator=g).to(torch.int32).cuda())
+
+
+def test_counted_calls_on_streams_and_in_graphs(U):
+    """One workspace and one set of counts: calls on four streams at once, long and short in turn, and a captured one between them."""
+    E = U.E
+    experts, k, ic, mid, sizes = 8, 3, 136, 104, (900, 50, 1200, 700)
+    w_in, w_out = U.randn(experts, 2 * mid, ic, dtype=torch.bfloat16, seed=1, scale=0.1), U.randn(experts, ic, mid, dtype=torch.bfloat16, seed=2, scale=0.1)
+    op = E.Experts(experts, k, ic, mid, max_rows=max(sizes))
+    assert op.prepare(w_in, w_out) == 0
+    data, outs = [], []
+    for s, rows in enumerate(sizes):
+        ids = U.randn(rows, experts, dtype=torch.float32, seed=20 + s).topk(k, dim=1).indices.to(torch.int32)
+        ids[::7, 1] = -1
+        data.append((U.randn(rows, ic, dtype=torch.bfloat16, seed=10 + s), ids, torch.softmax(U.randn(rows, k, dtype=torch.float32, seed=30 + s), 1)))
+        outs.append(torch.empty(rows, ic, dtype=torch.bfloat16, device="cuda"))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sizes]
+    for i in range(20):
+        x, ids, share = data[i % 4]
+        assert op.enqueue(outs[i % 4], x, ids, share, rows=sizes[i % 4], stream=streams[i % 4].cuda_stream) == 0, E.last_error()
+    torch.cuda.synchronize()
+    for o, (x, ids, share) in zip(outs, data):
+        U.close(o, *_want(U, x, ids, share, w_in, w_out, "silu", True, E.bf16), E.bf16)
+    y, g, s = torch.empty_like(outs[2]), torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    x, ids, share = (t.clone() for t in data[2])
+    with torch.cuda.graph(g, stream=s):
+        assert op.enqueue(y, x, ids, share, rows=sizes[2], stream=s.cuda_stream) == 0, E.last_error()
+    for n in range(3):
+        again = torch.empty_like(outs[n])
+        assert op.enqueue(again, *data[n], rows=sizes[n]) == 0
+        torch.cuda.synchronize()
+        assert torch.equal(again, outs[n])
+        y.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, outs[2])
+    assert op.device_status() == 0
