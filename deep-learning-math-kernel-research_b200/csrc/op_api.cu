@@ -195,20 +195,25 @@ int alloc(elb_op &op, T **p, size_t bytes) {
   return ELB_OK;
 }
 
-// A tensor of the caller's, host or device, as device memory for the time of a preparation.
+// A tensor of the caller's, in host memory or on any device, as memory of the plan's device (the current one) for the time of a preparation.
 struct Staged {
   const void *p = nullptr;
   void *own = nullptr;
   ~Staged() { if (own) cudaFree(own); }
-  int take(const void *src, size_t bytes) {
-    cudaPointerAttributes a;
-    if (cudaPointerGetAttributes(&a, src) == cudaSuccess && (a.type == cudaMemoryTypeDevice || a.type == cudaMemoryTypeManaged)) {
+  int take(const elb_op &op, const void *src, size_t bytes) {
+    cudaPointerAttributes a = {};
+    const bool known = cudaPointerGetAttributes(&a, src) == cudaSuccess;
+    if (known && (a.type == cudaMemoryTypeManaged || (a.type == cudaMemoryTypeDevice && a.device == op.device))) {
       p = src;
       return ELB_OK;
     }
     cudaGetLastError();
+    if (known && a.type == cudaMemoryTypeDevice) {     // whatever stream of that device it comes from
+      DeviceGuard guard(a.device);
+      OP_TRY(cudaDeviceSynchronize());
+    }
     OP_TRY(cudaMalloc(&own, bytes));
-    OP_TRY(cudaMemcpy(own, src, bytes, cudaMemcpyHostToDevice));
+    OP_TRY(cudaMemcpy(own, src, bytes, cudaMemcpyDefault));
     p = own;
     return ELB_OK;
   }
@@ -282,7 +287,7 @@ int grow_workspace(elb_op &op, size_t bytes) {
 // Weights [experts][rows][ic] -> packed image
 int pack(elb_op &op, void **dst, const void *src, int experts, int64_t rows, int ic, bool gated, bool hwio) {
   Staged st;
-  int rc = st.take(src, (size_t)experts * rows * ic * 2);
+  int rc = st.take(op, src, (size_t)experts * rows * ic * 2);
   if (rc != ELB_OK) return rc;
   const size_t bytes = (size_t)experts * (up(packed_rows(gated ? rows / 2 : rows, gated), GT_ROWS) / GT_ROWS) * (up(ic, GT_K) / GT_K) * GT_BYTES;
   rc = alloc(op, dst, bytes);
@@ -294,7 +299,7 @@ int pack(elb_op &op, void **dst, const void *src, int experts, int64_t rows, int
 
 int vector_f32(elb_op &op, float **dst, const void *src, int et, int n, int padded, bool gated) {
   Staged st;
-  int rc = st.take(src, n * et_bytes(et));
+  int rc = st.take(op, src, n * et_bytes(et));
   if (rc != ELB_OK) return rc;
   rc = alloc(op, dst, (size_t)padded * 4);
   if (rc != ELB_OK) return rc;
@@ -308,7 +313,7 @@ int64_t norm_pitch(int n) { return up(n + 16, 8); }
 // A norm's weights as fp32, offset included; null: ones (offset and all), or no vector for a bias
 int norm_vector(elb_op &op, float **dst, const void *src, int et, int n, float offset) {
   Staged st;
-  int rc = src ? st.take(src, n * et_bytes(et)) : ELB_OK;
+  int rc = src ? st.take(op, src, n * et_bytes(et)) : ELB_OK;
   if (rc == ELB_OK) rc = alloc(op, dst, (size_t)norm_pitch(n) * 8 * 4);
   if (rc != ELB_OK) return rc;
   OP_TRY(launch_norm_vector(*dst, st.p, et, n, norm_pitch(n), offset, nullptr));

@@ -346,7 +346,8 @@ ELB_API int elb_wino_f32_noalloc_status(void);
  * rows is a call that does nothing.  Rows of a tensor are ld elements apart (0 in the description: dense).
  * Tensors need the alignment of their type only; 16-byte aligned tensors whose rows are multiples of
  * 16 bytes are read without a copy.  An output may be the residual's tensor (the same address and ld);
- * no other tensors of a call may overlap an output.  prepare: host or device tensors; it waits for the device.
+ * no other tensors of a call may overlap an output.  prepare: tensors in host memory or on any device; it waits for the
+ * devices.
  * Calls may be captured in a CUDA graph if the plan is prepared and a call of as many rows has been
  * made before.  A plan with workspace orders its own calls across streams (not inside a capture, nor between a
  * captured graph and other calls: those the caller orders). */

@@ -256,6 +256,42 @@ void counts() {
   need(p.call(5) == ELB_OK && p.call(5) == ELB_OK, "calls");
 }
 
+// Weights on another device than the plan's: its work is waited for, and the kernels read a copy on the plan's own.
+void devices() {
+  std::vector<char> buf(4 * 64 * 64 * 2);
+  for (int where : {1, 0, -1})                             // the other device, the plan's, the host
+    for (int current : {0, 1}) {
+      g_on_device.erase(buf.data());
+      if (where >= 0) g_on_device[buf.data()] = where;
+      g_device = current;
+      g_waits.clear();
+      elb_op_t *op[4] = {};
+      elb_linear_desc_t l = {};
+      l.ic = l.oc = 64; l.dt_input = l.dt_output = ELB_BF16; l.dt_bias = ELB_F32; l.fmt_weights = ELB_OIHW; l.with_bias = 1; l.scale = 1.0f;
+      elb_norm_desc_t n = {};
+      n.channels = 64; n.dt = n.dt_residual = ELB_BF16; n.dt_weights = ELB_F32; n.post = ELB_NORM_RMS; n.pre = ELB_NORM_LAYER; n.scale = 1.0f;
+      elb_route_desc_t r = {};
+      r.experts = 64; r.top_k = 2; r.dt_logits = ELB_F32; r.with_bias = 1; r.groups = r.top_groups = r.group_best = 1; r.scale = 1.0f;
+      elb_experts_desc_t e = {};
+      e.experts = 4; e.top_k = 2; e.ic = e.mid = 64; e.dt = ELB_BF16; e.max_rows = 4;
+      need(elb_linear_create(&l, &op[0]) == ELB_OK && elb_norm_create(&n, &op[1]) == ELB_OK && elb_route_create(&r, &op[2]) == ELB_OK &&
+           elb_experts_create(&e, &op[3]) == ELB_OK, "create");
+      g_waits.clear();
+      const void *b = buf.data();
+      need(elb_linear_prepare(op[0], b, b) == ELB_OK, "linear");
+      need(where != 1 || g_waits[1] > 0, "the weights' device was not waited for");
+      need(elb_norm_prepare(op[1], b, b, b, b) == ELB_OK, "norm");
+      need(elb_route_prepare(op[2], static_cast<const float *>(b)) == ELB_OK, "route");
+      need(elb_experts_prepare(op[3], b, b) == ELB_OK, "experts");
+      need(g_device == current, "the current device has changed");
+      for (elb_op_t *o : op) elb_op_destroy(o);
+      g_on_device.erase(buf.data());
+      size_t left = 0;
+      for (auto &m : g_on_device) left += m.first != nullptr;
+      need(left == 0, "memory was not freed");
+    }
+}
+
 }  // namespace
 
 int main(int argc, char **argv) {
@@ -264,6 +300,7 @@ int main(int argc, char **argv) {
   else if (what == "one_handle") { one_handle<Linear>(); g_users.clear(); one_handle<Experts>(); }
   else if (what == "failed") { failed<Linear>({"gemm"}); g_users.clear(); failed<Experts>({"gather", "gemm", "combine"}); }
   else if (what == "counts") counts();
+  else if (what == "devices") devices();
   else { std::printf("no such case\n"); return 2; }
   if (g_bad == 0) std::printf("ok\n");
   return g_bad != 0;

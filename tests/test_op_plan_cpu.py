@@ -39,3 +39,7 @@ def test_a_call_that_failed_half_way_is_waited_for(check):
 
 def test_experts_counts_start_from_zero_behind_failed_and_captured_calls(check):
     check("counts")
+
+
+def test_weights_on_another_device_are_copied(check):
+    check("devices")
