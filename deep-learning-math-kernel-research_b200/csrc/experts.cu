@@ -45,7 +45,7 @@ __global__ void __launch_bounds__(COUNT_THREADS) experts_count_kernel(const Expe
 // COUNT: few slots, which every block counts for itself, places and all, in the slots' order; there is no kernel before it.
 constexpr int GATHER_THREADS = 256, COUNT_HERE = 2048;
 template <bool WORDS, bool COUNT>                      // WORDS: rows in 16-byte words
-__global__ void __launch_bounds__(GATHER_THREADS) experts_gather_kernel(const ExpertsParams p, int per_block) {
+__global__ void __launch_bounds__(GATHER_THREADS) experts_gather_kernel(const ExpertsParams p, const SlotShare share) {
   __shared__ int row0[MAX_EXPERTS];
   __shared__ int2 part[GATHER_THREADS / 32];
   __shared__ short ids[COUNT ? COUNT_HERE : 1];
@@ -97,8 +97,8 @@ __global__ void __launch_bounds__(GATHER_THREADS) experts_gather_kernel(const Ex
   if (blockIdx.x == 0 && tid == GATHER_THREADS - 1) *p.n_tiles = t;
   __syncthreads();
   // a warp per slot
-  const int end = min(slots, (int)(blockIdx.x + 1) * per_block);
-  for (int i = blockIdx.x * per_block + warp; i < end; i += GATHER_THREADS / 32) {
+  const int end = share.end(blockIdx.x, slots);
+  for (int i = share.first(blockIdx.x) + warp; i < end; i += GATHER_THREADS / 32) {
     const int e = COUNT ? ids[i] : p.ids[i];
     if (e < 0 || e >= p.experts) continue;
     int place = 0;
@@ -177,14 +177,13 @@ cudaError_t launch_experts_count(const ExpertsParams &p, cudaStream_t s) {
   return launch_overlapped(experts_count_kernel, dim3((slots + COUNT_SLOTS - 1) / COUNT_SLOTS), dim3(COUNT_THREADS), 0, s, p);
 }
 cudaError_t launch_experts_gather(const ExpertsParams &p, int num_sms, cudaStream_t s) {
-  const int slots = p.rows * p.top_k, most = num_sms * 8;
-  const int warps = GATHER_THREADS / 32, blocks = (slots + warps - 1) / warps < most ? (slots + warps - 1) / warps : most;
-  const int per = (slots + blocks - 1) / blocks;
+  const int slots = p.rows * p.top_k;
+  const SlotShare share = share_slots(slots, GATHER_THREADS / 32, num_sms * 8);
   const bool words = (reinterpret_cast<uintptr_t>(p.x) & 15) == 0 && p.ld_x % 8 == 0 && p.ic % 8 == 0;
   const bool here = experts_count_here(slots);
   auto k = words ? (here ? experts_gather_kernel<true, true> : experts_gather_kernel<true, false>)
                  : (here ? experts_gather_kernel<false, true> : experts_gather_kernel<false, false>);
-  return launch_overlapped(k, dim3((slots + per - 1) / per), dim3(GATHER_THREADS), 0, s, p, per);
+  return launch_overlapped(k, dim3(share.blocks), dim3(GATHER_THREADS), 0, s, p, share);
 }
 cudaError_t launch_experts_combine(const ExpertsParams &p, cudaStream_t s) {
   const bool words = (reinterpret_cast<uintptr_t>(p.out) & 7) == 0 && p.ld_out % 4 == 0 && p.ic % 4 == 0;

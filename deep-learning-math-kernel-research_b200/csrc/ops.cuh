@@ -121,6 +121,19 @@ struct ExpertsParams {
   int clear;                        // the combine kernel leaves zero counts
   int rows, top_k, experts, ic, et, tile_tokens;    // tile_tokens: the most that a token tile holds
 };
+// Slots of the gather kernel's blocks, `per` each (the last one fewer).  In 64 bits: the last block's end may pass 2^31 before it is cut.
+struct SlotShare {
+  int per, blocks;
+  __host__ __device__ int first(int block) const { return block * per; }
+  __host__ __device__ int end(int block, int slots) const {
+    const long long e = (block + 1ll) * per;
+    return e < slots ? (int)e : slots;
+  }
+};
+inline SlotShare share_slots(int slots, int warps, int most) {
+  const int blocks = (slots + warps - 1) / warps < most ? (slots + warps - 1) / warps : most, per = (slots + blocks - 1) / blocks;
+  return {per, (int)(((long long)slots + per - 1) / per)};
+}
 bool experts_count_here(int slots);      // the gather kernel counts few slots itself
 cudaError_t launch_experts_count(const ExpertsParams &p, cudaStream_t s);
 cudaError_t launch_experts_gather(const ExpertsParams &p, int num_sms, cudaStream_t s);

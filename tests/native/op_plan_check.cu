@@ -15,6 +15,8 @@
 #include "ops.cuh"
 
 #ifndef __CUDA_ARCH__       // (host code alone)
+using namespace elb;
+
 namespace {
 
 int g_bad = 0;
@@ -292,6 +294,23 @@ void devices() {
     }
 }
 
+// Every slot belongs to one block of the gather kernel, up to the most that a plan takes (2^31 - 4096).
+void shares() {
+  for (int warps : {8})
+    for (int most : {148 * 8, 16})
+      for (int slots : {1, 7, 8, 9, 1000, 9471, 9472, 9473, 12345678, 0x7FFFFFFF - 2000000, 0x7FFFFFFF - 4096, 0x7FFFF000}) {
+        const SlotShare s = share_slots(slots, warps, most);
+        long long at = 0;
+        bool fine = s.per >= 1 && s.blocks >= 1 && s.blocks <= most;
+        for (int b = 0; b < s.blocks && fine; ++b) {
+          fine = s.first(b) == at && s.end(b, slots) > at;
+          at = s.end(b, slots);
+        }
+        if (!(fine && at == slots)) std::printf("%d slots, %d blocks of %d: ", slots, s.blocks, s.per);
+        need(fine && at == slots, "slots without a block of their own");
+      }
+}
+
 }  // namespace
 
 int main(int argc, char **argv) {
@@ -301,6 +320,7 @@ int main(int argc, char **argv) {
   else if (what == "failed") { failed<Linear>({"gemm"}); g_users.clear(); failed<Experts>({"gather", "gemm", "combine"}); }
   else if (what == "counts") counts();
   else if (what == "devices") devices();
+  else if (what == "shares") shares();
   else { std::printf("no such case\n"); return 2; }
   if (g_bad == 0) std::printf("ok\n");
   return g_bad != 0;

@@ -43,3 +43,7 @@ def test_experts_counts_start_from_zero_behind_failed_and_captured_calls(check):
 
 def test_weights_on_another_device_are_copied(check):
     check("devices")
+
+
+def test_slots_up_to_the_most_of_a_plan_are_shared_out(check):
+    check("shares")
