@@ -1250,8 +1250,7 @@ struct LaunchConfig {
     cfg.blockDim = dim3(hp.kind == HALO_F32 ? THREADS_F32 : THREADS_I8);
     cfg.dynamicSmemBytes = hp.smem_bytes;
     cfg.stream = s;
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[0] = overlap_attribute();
     at[1].id = cudaLaunchAttributeClusterDimension;
     at[1].val.clusterDim.x = hp.p.pair ? 2 : hp.p.split; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
     cfg.attrs = at;

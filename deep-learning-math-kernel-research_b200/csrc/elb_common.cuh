@@ -31,6 +31,14 @@ inline int tune_env(const char *name, int dflt) {
 __device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void griddep_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// What lets a launch do so.  ELB_NO_OVERLAP in a tuning build turns it off in every kernel, to tell an ordering fault from others.
+inline cudaLaunchAttribute overlap_attribute() {
+  cudaLaunchAttribute at = {};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = tune_env("ELB_NO_OVERLAP", 0) ? 0 : 1;
+  return at;
+}
+
 // Launch a kernel that may overlap its set-up with the tail of the kernel before it in the stream
 // (the kernel must contain griddep_wait).  Captured into a CUDA graph the
 // dependency becomes a programmatic edge.  The INT8 tensor-core kernels are launched this way:
@@ -46,10 +54,8 @@ inline cudaError_t launch_overlapped(void (*kernel)(KArgs...), dim3 grid, dim3 b
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = tune_env("ELB_NO_OVERLAP", 0) ? 0 : 1;
-  cfg.attrs = at;
+  cudaLaunchAttribute at = overlap_attribute();
+  cfg.attrs = &at;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }

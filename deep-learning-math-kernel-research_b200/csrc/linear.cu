@@ -473,8 +473,7 @@ cudaError_t launch_gemm_kernel(K kern, const GemmLaunch &g, int grid, int thread
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[0] = overlap_attribute();
   at[1].id = cudaLaunchAttributeClusterDimension;
   at[1].val.clusterDim.x = cluster; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
