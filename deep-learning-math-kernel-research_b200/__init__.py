@@ -471,13 +471,57 @@ class MultiConv:
             pass
 
 
+_DTYPE_NAMES = {f32: "float32", f16: "float16", bf16: "bfloat16", s32: "int32"}
+
+
 def _dev(x):
-    """Address of a device tensor (torch tensor, raw address or None): what the operators' enqueue calls take."""
+    """Address of a device tensor (torch tensor, raw address or None) that a call does not use."""
     if x is None or type(x) is int:
         return x
     if not x.is_cuda:
         raise ValueError("the operators' enqueue calls take device tensors")
     return x.data_ptr()
+
+
+class _Spec:
+    """What a plan wants of a tensor: rows of ``n`` elements of an ELB type, ``ld`` apart."""
+    __slots__ = ("type", "n", "ld", "what", "dtype", "row_bytes")
+
+    def __init__(self, type, n, ld, what):
+        self.type, self.n, self.ld, self.what = type, n, ld or n, what
+        self.dtype = None                                                # the tensors' own name for the type, once one has been met
+        self.row_bytes = n * (2 if type in (f16, bf16) else 4) if self.ld == n else float("inf")
+
+
+def _rows(x, spec, rows):
+    """Address of a device tensor of which a call reads or writes ``rows`` rows: a torch tensor that holds them, a raw address, which is taken as it
+    is, or None.  (A property of a tensor costs 30 to 70 ns here, beside a call's 4 us: dense tensors are looked at three times.)"""
+    if x is None or type(x) is int:
+        return x
+    if not (x.dtype is spec.dtype and x.is_contiguous() and x.nbytes >= rows * spec.row_bytes) and rows > 0:
+        _check_rows(x, spec, rows)
+    if not x.is_cuda:
+        raise ValueError("the operators' enqueue calls take device tensors")
+    return x.data_ptr()
+
+
+def _check_rows(x, spec, rows):
+    """As ``_rows``, for any tensor: a dense one of enough elements where rows are dense or it has one dimension; otherwise the last dimension holds
+    a row, and the others, taken together, ``rows`` of them, ``ld`` elements apart."""
+    n, ld = spec.n, spec.ld
+    name, shape, stride = str(x.dtype).replace("torch.", ""), tuple(x.shape), tuple(x.stride())
+    if x.is_contiguous() and (ld == n or len(shape) == 1):
+        fits = x.numel() >= (rows - 1) * ld + n
+    else:
+        fits = bool(shape) and shape[-1] >= n and (n == 1 or stride[-1] == 1)
+        held = 1
+        for size, step in zip(reversed(shape[:-1]), reversed(stride[:-1])):
+            fits = fits and (size == 1 or step == held * ld)
+            held *= size
+        fits = fits and held >= rows
+    if not fits or name != _DTYPE_NAMES[spec.type]:
+        raise ValueError(f"{spec.what}: {rows} rows of {n} elements in {_DTYPE_NAMES[spec.type]}, {ld} apart, are wanted, got {shape} with strides {stride} in {name}")
+    spec.dtype = x.dtype
 
 
 def _dense(x, shape, dtypes, what):
@@ -497,13 +541,11 @@ def _dense(x, shape, dtypes, what):
     return _ptr(x)
 
 
-_DTYPE_NAMES = {f32: "float32", f16: "float16", bf16: "bfloat16"}
-
-
 class _Op:
     """A plan of one of the operators of transformer blocks (``elb_op_t``).  ``prepare`` copies the weights (host or
-    device tensors, read once; later calls do nothing), ``enqueue`` runs on ``stream`` (None: the default stream) and
-    returns an ELB_* code; rows of tensors are ``ld_*`` elements apart (0: dense)."""
+    device tensors, read once; later calls do nothing), ``enqueue`` runs on ``stream`` (a cudaStream_t; None: the legacy default stream, not
+    torch's current one) and returns an ELB_* code; rows of tensors are ``ld_*`` elements apart (0: dense).  Torch tensors must hold the call's
+    rows in the plan's types, or ``enqueue`` raises ValueError; raw addresses are taken as they are."""
     h = None
 
     def _create(self, create, desc):
@@ -547,12 +589,16 @@ class Linear(_Op):
         wide = 2 * oc if gated else oc
         self._weights = ((wide, ic) if weights_format == oihw else (ic, wide), (dtype,))
         self._bias = ((wide,), (bias_dtype,))
+        out = dtype if out_dtype is None else out_dtype
+        self._output, self._input = _Spec(out, oc, ld_output, "output"), _Spec(dtype, ic, ld_input, "input")
+        self._residual = _Spec(out, oc, ld_residual, "residual") if with_residual else None
 
     def prepare(self, weights, bias=None) -> int:
         return lib.elb_linear_prepare(self.h, _dense(weights, *self._weights, "weights"), _dense(bias, *self._bias, "bias"))
 
     def enqueue(self, output, input, residual=None, *, rows: int, stream=None) -> int:
-        return lib.elb_linear_enqueue(self.h, _dev(output), _dev(input), _dev(residual), rows, stream)
+        return lib.elb_linear_enqueue(self.h, _rows(output, self._output, rows), _rows(input, self._input, rows),
+                                      _rows(residual, self._residual, rows) if self._residual else _dev(residual), rows, stream)
 
 
 class BlockNorm(_Op):
@@ -567,12 +613,20 @@ class BlockNorm(_Op):
                                                       post_eps, pre_eps, weight_offset, scale, int(with_residual), gate_rows, device,
                                                       ld_input, ld_residual, ld_gate, ld_sum, ld_output))
         self._vector = ((channels,), (weights_dtype,), "weights")
+        stream = dtype if residual_dtype is None else residual_dtype
+        self._output = _Spec(dtype, channels, ld_output, "output") if pre != NORM_NONE else None
+        self._sum, self._input = _Spec(stream, channels, ld_sum, "sum"), _Spec(dtype, channels, ld_input, "input")
+        self._residual = _Spec(stream, channels, ld_residual, "residual") if with_residual else None
+        self._gate = _Spec(dtype, channels, ld_gate, "gate") if gate_rows else None
+        self._gate_rows = gate_rows
 
     def prepare(self, post_weight=None, post_bias=None, pre_weight=None, pre_bias=None) -> int:
         return lib.elb_norm_prepare(self.h, *(_dense(v, *self._vector) for v in (post_weight, post_bias, pre_weight, pre_bias)))
 
     def enqueue(self, output, sum, input, residual=None, gate=None, *, rows: int, stream=None) -> int:
-        return lib.elb_norm_enqueue(self.h, _dev(output), _dev(sum), _dev(input), _dev(residual), _dev(gate), rows, stream)
+        return lib.elb_norm_enqueue(self.h, _rows(output, self._output, rows) if self._output else _dev(output), _rows(sum, self._sum, rows),
+                                    _rows(input, self._input, rows), _rows(residual, self._residual, rows) if self._residual else _dev(residual),
+                                    _rows(gate, self._gate, -(-rows // self._gate_rows)) if self._gate else _dev(gate), rows, stream)
 
 
 class Route(_Op):
@@ -584,13 +638,14 @@ class Route(_Op):
         self._create(lib.elb_route_create, ElbRouteDesc(experts, top_k, dtype, score, int(with_bias), groups, top_groups, group_best,
                                                         int(renormalise), scale, device, ld_logits))
         self._bias = ((experts,), (f32,), "bias")
+        self._ids, self._weights, self._logits = _Spec(s32, top_k, 0, "ids"), _Spec(f32, top_k, 0, "weights"), _Spec(dtype, experts, ld_logits, "logits")
 
     def prepare(self, bias=None) -> int:
         return lib.elb_route_prepare(self.h, _dense(bias, *self._bias))
 
     def enqueue(self, ids, weights, logits, *, rows: int, stream=None) -> int:
         """ids: int32 [rows, top_k], weights: float32 [rows, top_k] or None, both dense."""
-        return lib.elb_route_enqueue(self.h, _dev(ids), _dev(weights), _dev(logits), rows, stream)
+        return lib.elb_route_enqueue(self.h, _rows(ids, self._ids, rows), _rows(weights, self._weights, rows), _rows(logits, self._logits, rows), rows, stream)
 
 
 class Experts(_Op):
@@ -603,9 +658,12 @@ class Experts(_Op):
                                                             ld_input, ld_output))
         self._in = ((experts, 2 * mid if gated else mid, ic), (dtype,), "w_in")
         self._out = ((experts, ic, mid), (dtype,), "w_out")
+        self._output, self._input = _Spec(dtype, ic, ld_output, "output"), _Spec(dtype, ic, ld_input, "input")
+        self._ids, self._weights = _Spec(s32, top_k, 0, "ids"), _Spec(f32, top_k, 0, "weights")
 
     def prepare(self, w_in, w_out) -> int:
         return lib.elb_experts_prepare(self.h, _dense(w_in, *self._in), _dense(w_out, *self._out))
 
     def enqueue(self, output, input, ids, weights, *, rows: int, stream=None) -> int:
-        return lib.elb_experts_enqueue(self.h, _dev(output), _dev(input), _dev(ids), _dev(weights), rows, stream)
+        return lib.elb_experts_enqueue(self.h, _rows(output, self._output, rows), _rows(input, self._input, rows), _rows(ids, self._ids, rows),
+                                       _rows(weights, self._weights, rows), rows, stream)
