@@ -360,3 +360,25 @@ def test_per_thread_streams_take_turns_in_the_workspace(U):
     assert results == [0, 0, True]
     for x, y in zip(xs, ys):
         U.close(y, *U.linear64(x, w, None, None, "none", False, 1.0), E.bf16)
+
+
+@pytest.mark.parametrize("rows", [1, 20, 300, 700])
+@pytest.mark.parametrize("gated", [False, True], ids=["plain", "gated"])
+def test_gelu_keeps_its_relative_precision(U, rows, gated):
+    """fp32 results of gelu's erf form, of both signs until they vanish: each sum is one product with 1.
+
+    Relative error: the fit of erfc, its evaluation, a reciprocal (2^-23), an exponential (2^-22) and three products, 2^-19 together; the exponential's
+    argument z^2 / 2 is 2.5 * 2^-24 off, relatively, which 2^-23 z^2 covers.  Flushed to zero below 2^-126, with |z| under 14."""
+    E = U.E
+    ic, oc = 64, 1801
+    z = torch.linspace(-14.0, 14.0, oc, device="cuda").to(torch.bfloat16)
+    x = torch.zeros(rows, ic, dtype=torch.bfloat16, device="cuda")
+    w = torch.zeros(2 * oc if gated else oc, ic, dtype=torch.bfloat16, device="cuda")
+    x[:, 5] = x[:, 9] = 1.0
+    w[:oc, 5], w[oc:, 9] = z, 1.0
+    lin, y = E.Linear(ic, oc, out_dtype=E.f32, activation=E.ACT_GELU, gated=gated), torch.empty(rows, oc, device="cuda")
+    assert lin.prepare(w) == 0 and lin.enqueue(y, x, rows=rows) == 0
+    torch.cuda.synchronize()
+    zd = z.double()
+    want = (zd * 0.5 * torch.erfc(-zd / math.sqrt(2.0))).expand(rows, oc)
+    U.close(y, want, want.abs() * (2.0 ** -19 + 2.0 ** -23 * zd * zd) + 14 * 2.0 ** -126, E.f32)
