@@ -11,6 +11,11 @@ namespace elb {
 // Bytes of the operand rings.  The kernel of few tiles with few tokens and shared channels leaves room for a second CTA on its
 // SM (the next launch's weights arrive while this one ends, and a cluster finds its SMs); a CTA that streams a whole row tile
 // wants all of the SM's memory for loads in flight (24 x 4096 -> 16384 23.4 us, 29.0 with the small ring).
+//
+// Clusters on several streams: a CTA of one that holds tensor memory while its partner elsewhere waits for some must not meet a CTA of another in the
+// reverse position.  Kernels of the small ring take 32 columns, two of them on an SM; every other cluster's kernel fills an SM by its
+// shared memory or registers; the nearest to leaving room is the fp32 direct convolution (all 512 columns), whose 512 threads of 80 registers and
+// 320 of 80 here would be 66560 of 65536.  Whoever changes these counts has to look at that again.
 constexpr int SMALL_RING = 110 * 1024, LARGE_RING = 224 * 1024;
 constexpr int TILES_RING = 192 * 1024;
 

@@ -672,7 +672,7 @@ int elb_experts_enqueue(elb_op_t *op, void *output, const void *input, const int
   p.epi.oc = (int)op->pitch_mid;          // (channels past the end are products with rows of zeros)
   p.epi.act = d.activation;
   p.epi.gated = d.gated;
-  p.epi.out_et = e.et;
+  p.epi.out_et = e.et;                    // the middle is a 16-bit operand of the second product: one rounding, as large as the output's
   q.w = static_cast<const uint8_t *>(op->w[1]);
   q.x = op->mid;
   q.ld_x = op->pitch_mid;

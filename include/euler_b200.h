@@ -361,7 +361,9 @@ enum { ELB_SCORE_SOFTMAX = 0, ELB_SCORE_SIGMOID = 1 };
 
 /* output[t][o] = residual[t][o] + scale * act(z[t][o]),  z[t][o] = bias[o] + sum_i input[t][i] * weights[o][i]
  * gated: weights and bias hold 2 * oc rows, z of the gate in the first oc, u in the others: scale * act(z) * u.
- * Products are accumulated in 32 bits, everything up to the output's one rounding is done in 32 bits. */
+ * Products are accumulated in 32 bits, everything up to the output's one rounding is done in 32 bits (activations to a relative
+ * 2^-19 plus what rounding the exponential's argument costs, results below 2^-126 flushed; sums of one row are added on CUDA cores, of many rows in tensor
+ * memory, which cuts partial sums off). */
 typedef struct elb_linear_desc {
   int32_t ic, oc;                                 /* input and output channels */
   int32_t dt_input;                               /* ELB_BF16 or ELB_F16; the weights' type too */
@@ -407,6 +409,7 @@ ELB_API int elb_norm_enqueue(elb_op_t *op, void *output, void *sum, const void *
  *   score = softmax(logits) or sigmoid(logits); choice = score + bias (bias is for the choice alone)
  *   groups > 1: an expert is open if its group is among the top_groups best by the sum of its group_best best
  *   choices; ids = the top_k open experts of the largest choice, ties to the lowest index (groups as well)
+ *   (a choice that is NaN counts as -inf; an expert of a closed group is never chosen)
  *   weights = scale * score[ids], divided by their sum first where renormalise is set (a sum of 0 gives weights of 0)
  * A NaN among the logits counts as -inf; +inf takes softmax's whole weight (shared with others of its row).  Without a bias softmax chooses by
  * exp(logit - max), which has the order of the scores. */
@@ -426,15 +429,18 @@ ELB_API int elb_route_prepare(elb_op_t *op, const float *bias);
 ELB_API int elb_route_enqueue(elb_op_t *op, int32_t *ids, float *weights, const void *logits, int64_t rows, void *cuda_stream);
 
 /* The experts' products:  output[t] = sum_j weights[t][j] * W_out[e] * f(W_in[e] * input[t]),  e = ids[t][j]
- * f is the activation of mid channels; gated: W_in has 2 * mid rows, gate first, as in elb_linear.  The middle
- * tensor is held in dt, the sum over j in 32 bits.  An id outside 0 .. experts - 1 is a slot that adds nothing. */
+ * f is the activation of mid channels; gated: W_in has 2 * mid rows, gate first, as in elb_linear.  The sum over j is held in 32
+ * bits.  The middle tensor is rounded to dt, the second product's operand (its error is about the output's own rounding; an f16 value past
+ * 65504 becomes infinite), but calls of few slots, which run on CUDA cores (256 slots at most, fewer where experts are large), keep it in 32
+ * bits: a token's result may differ by that rounding between calls of different lengths.  An id outside 0 .. experts - 1 is a slot that adds nothing. */
 typedef struct elb_experts_desc {
   int32_t experts, top_k;                         /* 1 .. 1024; 1 .. 32 */
   int32_t ic, mid;
   int32_t dt;                                     /* ELB_BF16 or ELB_F16: input, both weights, middle, output */
   int32_t activation, gated;
   int32_t device;
-  int64_t max_rows;                               /* the workspace is made for calls of so many rows */
+  int64_t max_rows;                               /* the plan's workspace is made for calls of so many rows: of each slot about
+                                                     6 * ic + 2 * mid bytes (4096 rows of 2048, 8 slots each of 1024: 0.47 GB) */
   int64_t ld_input, ld_output;
 } elb_experts_desc_t;
 ELB_API int elb_experts_create(const elb_experts_desc_t *desc, elb_op_t **op);
