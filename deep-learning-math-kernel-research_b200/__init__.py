@@ -153,6 +153,7 @@ def _load():
         "elb_experts_prepare": (i32, [vp, vp, vp]),
         "elb_experts_enqueue": (i32, [vp, vp, vp, vp, vp, C.c_int64, vp]),
         "elb_op_device_status": (i32, [vp]),
+        "elb_op_device": (i32, [vp]),
         "elb_op_launch_count": (u64, [vp]),
         "elb_op_workspace_bytes": (u64, [vp]),
         "elb_op_destroy": (None, [vp]),
@@ -176,7 +177,7 @@ EXPORTED_SYMBOLS = ["elb_conv_sizes", "elb_conv_create", "elb_conv_info", "elb_c
                     "elb_conv_input_step_supported", "elb_conv_enqueue_strided",
                     "elb_linear_create", "elb_linear_prepare", "elb_linear_enqueue", "elb_norm_create", "elb_norm_prepare",
                     "elb_norm_enqueue", "elb_route_create", "elb_route_prepare", "elb_route_enqueue", "elb_experts_create",
-                    "elb_experts_prepare", "elb_experts_enqueue", "elb_op_device_status", "elb_op_launch_count",
+                    "elb_experts_prepare", "elb_experts_enqueue", "elb_op_device_status", "elb_op_device", "elb_op_launch_count",
                     "elb_op_workspace_bytes", "elb_op_destroy"]
 
 
@@ -474,21 +475,21 @@ class MultiConv:
 _DTYPE_NAMES = {f32: "float32", f16: "float16", bf16: "bfloat16", s32: "int32"}
 
 
-def _dev(x):
-    """Address of a device tensor (torch tensor, raw address or None) that a call does not use."""
+def _dev(x, device):
+    """Address of a tensor of ``device`` (torch tensor, raw address or None) that a call does not use."""
     if x is None or type(x) is int:
         return x
-    if not x.is_cuda:
-        raise ValueError("the operators' enqueue calls take device tensors")
+    if x.get_device() != device:
+        raise ValueError(f"the plan's enqueue calls take tensors of device {device}")
     return x.data_ptr()
 
 
 class _Spec:
-    """What a plan wants of a tensor: rows of ``n`` elements of an ELB type, ``ld`` apart."""
-    __slots__ = ("type", "n", "ld", "what", "dtype", "row_bytes")
+    """What a plan wants of a tensor: rows of ``n`` elements of an ELB type, ``ld`` apart, on the plan's device."""
+    __slots__ = ("type", "n", "ld", "what", "device", "dtype", "row_bytes")
 
-    def __init__(self, type, n, ld, what):
-        self.type, self.n, self.ld, self.what = type, n, ld or n, what
+    def __init__(self, type, n, ld, what, device):
+        self.type, self.n, self.ld, self.what, self.device = type, n, ld or n, what, device
         self.dtype = None                                                # the tensors' own name for the type, once one has been met
         self.row_bytes = n * (2 if type in (f16, bf16) else 4) if self.ld == n else float("inf")
 
@@ -500,8 +501,8 @@ def _rows(x, spec, rows):
         return x
     if not (x.dtype is spec.dtype and x.is_contiguous() and x.nbytes >= rows * spec.row_bytes) and rows > 0:
         _check_rows(x, spec, rows)
-    if not x.is_cuda:
-        raise ValueError("the operators' enqueue calls take device tensors")
+    if x.get_device() != spec.device:
+        raise ValueError(f"{spec.what}: the plan's enqueue calls take tensors of device {spec.device}")
     return x.data_ptr()
 
 
@@ -545,7 +546,7 @@ class _Op:
     """A plan of one of the operators of transformer blocks (``elb_op_t``).  ``prepare`` copies the weights (host or
     device tensors, read once; later calls do nothing), ``enqueue`` runs on ``stream`` (a cudaStream_t; None: the legacy default stream, not
     torch's current one) and returns an ELB_* code; rows of tensors are ``ld_*`` elements apart (0: dense).  Torch tensors must hold the call's
-    rows in the plan's types, or ``enqueue`` raises ValueError; raw addresses are taken as they are."""
+    rows in the plan's types, on its device, or ``enqueue`` raises ValueError; raw addresses are taken as they are."""
     h = None
 
     def _create(self, create, desc):
@@ -554,6 +555,10 @@ class _Op:
         if rc != ELB_OK:
             raise RuntimeError(f"rc={rc}: {last_error()}")
         self.h = h
+        self.device = lib.elb_op_device(h)
+
+    def _spec(self, type, n, ld, what):
+        return _Spec(type, n, ld, what, self.device)
 
     def device_status(self) -> int:
         return lib.elb_op_device_status(self.h)
@@ -590,15 +595,15 @@ class Linear(_Op):
         self._weights = ((wide, ic) if weights_format == oihw else (ic, wide), (dtype,))
         self._bias = ((wide,), (bias_dtype,))
         out = dtype if out_dtype is None else out_dtype
-        self._output, self._input = _Spec(out, oc, ld_output, "output"), _Spec(dtype, ic, ld_input, "input")
-        self._residual = _Spec(out, oc, ld_residual, "residual") if with_residual else None
+        self._output, self._input = self._spec(out, oc, ld_output, "output"), self._spec(dtype, ic, ld_input, "input")
+        self._residual = self._spec(out, oc, ld_residual, "residual") if with_residual else None
 
     def prepare(self, weights, bias=None) -> int:
         return lib.elb_linear_prepare(self.h, _dense(weights, *self._weights, "weights"), _dense(bias, *self._bias, "bias"))
 
     def enqueue(self, output, input, residual=None, *, rows: int, stream=None) -> int:
         return lib.elb_linear_enqueue(self.h, _rows(output, self._output, rows), _rows(input, self._input, rows),
-                                      _rows(residual, self._residual, rows) if self._residual else _dev(residual), rows, stream)
+                                      _rows(residual, self._residual, rows) if self._residual else _dev(residual, self.device), rows, stream)
 
 
 class BlockNorm(_Op):
@@ -614,19 +619,19 @@ class BlockNorm(_Op):
                                                       ld_input, ld_residual, ld_gate, ld_sum, ld_output))
         self._vector = ((channels,), (weights_dtype,), "weights")
         stream = dtype if residual_dtype is None else residual_dtype
-        self._output = _Spec(dtype, channels, ld_output, "output") if pre != NORM_NONE else None
-        self._sum, self._input = _Spec(stream, channels, ld_sum, "sum"), _Spec(dtype, channels, ld_input, "input")
-        self._residual = _Spec(stream, channels, ld_residual, "residual") if with_residual else None
-        self._gate = _Spec(dtype, channels, ld_gate, "gate") if gate_rows else None
+        self._output = self._spec(dtype, channels, ld_output, "output") if pre != NORM_NONE else None
+        self._sum, self._input = self._spec(stream, channels, ld_sum, "sum"), self._spec(dtype, channels, ld_input, "input")
+        self._residual = self._spec(stream, channels, ld_residual, "residual") if with_residual else None
+        self._gate = self._spec(dtype, channels, ld_gate, "gate") if gate_rows else None
         self._gate_rows = gate_rows
 
     def prepare(self, post_weight=None, post_bias=None, pre_weight=None, pre_bias=None) -> int:
         return lib.elb_norm_prepare(self.h, *(_dense(v, *self._vector) for v in (post_weight, post_bias, pre_weight, pre_bias)))
 
     def enqueue(self, output, sum, input, residual=None, gate=None, *, rows: int, stream=None) -> int:
-        return lib.elb_norm_enqueue(self.h, _rows(output, self._output, rows) if self._output else _dev(output), _rows(sum, self._sum, rows),
-                                    _rows(input, self._input, rows), _rows(residual, self._residual, rows) if self._residual else _dev(residual),
-                                    _rows(gate, self._gate, -(-rows // self._gate_rows)) if self._gate else _dev(gate), rows, stream)
+        return lib.elb_norm_enqueue(self.h, _rows(output, self._output, rows) if self._output else _dev(output, self.device), _rows(sum, self._sum, rows),
+                                    _rows(input, self._input, rows), _rows(residual, self._residual, rows) if self._residual else _dev(residual, self.device),
+                                    _rows(gate, self._gate, -(-rows // self._gate_rows)) if self._gate else _dev(gate, self.device), rows, stream)
 
 
 class Route(_Op):
@@ -638,7 +643,7 @@ class Route(_Op):
         self._create(lib.elb_route_create, ElbRouteDesc(experts, top_k, dtype, score, int(with_bias), groups, top_groups, group_best,
                                                         int(renormalise), scale, device, ld_logits))
         self._bias = ((experts,), (f32,), "bias")
-        self._ids, self._weights, self._logits = _Spec(s32, top_k, 0, "ids"), _Spec(f32, top_k, 0, "weights"), _Spec(dtype, experts, ld_logits, "logits")
+        self._ids, self._weights, self._logits = self._spec(s32, top_k, 0, "ids"), self._spec(f32, top_k, 0, "weights"), self._spec(dtype, experts, ld_logits, "logits")
 
     def prepare(self, bias=None) -> int:
         return lib.elb_route_prepare(self.h, _dense(bias, *self._bias))
@@ -658,8 +663,8 @@ class Experts(_Op):
                                                             ld_input, ld_output))
         self._in = ((experts, 2 * mid if gated else mid, ic), (dtype,), "w_in")
         self._out = ((experts, ic, mid), (dtype,), "w_out")
-        self._output, self._input = _Spec(dtype, ic, ld_output, "output"), _Spec(dtype, ic, ld_input, "input")
-        self._ids, self._weights = _Spec(s32, top_k, 0, "ids"), _Spec(f32, top_k, 0, "weights")
+        self._output, self._input = self._spec(dtype, ic, ld_output, "output"), self._spec(dtype, ic, ld_input, "input")
+        self._ids, self._weights = self._spec(s32, top_k, 0, "ids"), self._spec(f32, top_k, 0, "weights")
 
     def prepare(self, w_in, w_out) -> int:
         return lib.elb_experts_prepare(self.h, _dense(w_in, *self._in), _dense(w_out, *self._out))

@@ -725,6 +725,7 @@ int elb_op_device_status(elb_op_t *op) {
   if (cudaDeviceSynchronize() != cudaSuccess) return -1;
   return *reinterpret_cast<volatile int *>(op->h_status);
 }
+int elb_op_device(const elb_op_t *op) { return op ? op->device : -1; }
 uint64_t elb_op_launch_count(const elb_op_t *op) { return op ? op->launches : 0; }
 uint64_t elb_op_workspace_bytes(const elb_op_t *op) { return op ? op->bytes : 0; }
 void elb_op_destroy(elb_op_t *op) { delete op; }

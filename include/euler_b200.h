@@ -452,6 +452,7 @@ ELB_API int elb_experts_enqueue(elb_op_t *op, void *output, const void *input, c
 /* 0 = every finished call of the plan was well; otherwise the code of the bounded wait that gave up (see
  * elb_conv_device_status).  Waits for the device; -1: it could not. */
 ELB_API int elb_op_device_status(elb_op_t *op);
+ELB_API int elb_op_device(const elb_op_t *op);                 /* the CUDA device ordinal whose tensors enqueue takes */
 ELB_API uint64_t elb_op_launch_count(const elb_op_t *op);
 ELB_API uint64_t elb_op_workspace_bytes(const elb_op_t *op);   /* device memory the plan holds, weights included */
 ELB_API void elb_op_destroy(elb_op_t *op);

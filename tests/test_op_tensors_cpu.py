@@ -21,8 +21,11 @@ class Tensor:
     """A CPU tensor that says it is a GPU's."""
     is_cuda = True
 
-    def __init__(self, t):
-        self.t = t
+    def __init__(self, t, device=0):
+        self.t, self.device = t, device
+
+    def get_device(self):
+        return self.device
 
     def __getattr__(self, name):
         return getattr(self.t, name)
@@ -69,8 +72,9 @@ def test_tensors_that_do_not_hold_the_rows_are_refused(E, kind, argument):
     for b in bad:
         with pytest.raises(ValueError, match=argument):
             plan.enqueue(**{**good, argument: Tensor(b)}, rows=6)
-    with pytest.raises(ValueError, match="device tensors"):
-        plan.enqueue(**{**good, argument: t}, rows=6)
+    for elsewhere in (t, Tensor(t, device=1)):
+        with pytest.raises(ValueError, match="device 0"):
+            plan.enqueue(**{**good, argument: elsewhere}, rows=6)
     assert len(E.lib.calls) == 1
     # what holds them in another shape, more of them, an address, and calls without rows, which use none
     for fine in (torch.empty(2, t.shape[0] // 2, n, dtype=t.dtype), torch.empty(t.numel() + 5, dtype=t.dtype), torch.empty(t.shape[0] + 3, n, dtype=t.dtype)):
