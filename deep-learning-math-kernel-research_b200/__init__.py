@@ -3,8 +3,8 @@
 This package is the Python door to the C-ABI library ``lib/libeuler_b200.so`` (sources in
 ``csrc/``, interface in ``include/euler_b200.h``).  It mirrors the reference's public surface
 (``include/euler.hpp``): an ``eld_conv_t`` descriptor with the same field names, ``setup()`` and
-``elx_conv(desc, output, input, weights, bias)``.  ``Linear``, ``BlockNorm``, ``Route`` and ``Experts`` are the
-operators of transformer blocks, with the same describe / prepare / enqueue protocol.
+``elx_conv(desc, output, input, weights, bias)``.  ``Linear``, ``BlockNorm``, ``Route``, ``Experts``, ``Rotary``,
+``CacheAppend`` and ``Attention`` are the operators of transformer blocks, with the same describe / prepare / enqueue protocol.
 
 There is no CPU implementation here.  Importing works without a GPU (the library loads and its
 symbols can be inspected), but every compute call needs an sm_100 device and fails loudly
@@ -36,6 +36,8 @@ FINE, COARSE, CALIBRATED = range(3)
 ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU = range(5)
 NORM_NONE, NORM_RMS, NORM_LAYER = range(3)
 SCORE_SOFTMAX, SCORE_SIGMOID = range(2)
+ROTARY_HALVES, ROTARY_NEIGHBOURS = range(2)
+SCALE_NONE, SCALE_LINEAR, SCALE_BY_PARTS = range(3)
 EL_NO_CALI = 3.4028234663852886e38
 KERNEL_NAMES = {0: "none", 1: "i8_gemm_umma", 2: "i8_conv_umma", 3: "i8_simt", 4: "wino_f32_umma",
                 5: "wino_i8_umma", 6: "i8_depthwise", 7: "f32_direct_umma", 8: "f32_small_ic", 9: "conv_halo"}
@@ -91,6 +93,23 @@ class ElbRouteDesc(C.Structure):
 class ElbExpertsDesc(C.Structure):
     _fields_ = [(k, C.c_int32) for k in ("experts", "top_k", "ic", "mid", "dt", "activation", "gated", "device")] + \
                [(k, C.c_int64) for k in ("max_rows", "ld_input", "ld_output")]
+
+
+class ElbRotaryDesc(C.Structure):
+    _fields_ = [(k, C.c_int32) for k in ("heads", "kv_heads", "head_dim", "rotary_dim", "dt", "layout", "scaling", "inverse")] + \
+               [(k, C.c_float) for k in ("base", "factor", "slow", "fast", "magnitude")] + [("original", C.c_int32), ("device", C.c_int32)] + \
+               [(k, C.c_int64) for k in ("ld_q", "ld_k", "ld_q_out", "ld_k_out")]
+
+
+class ElbAppendDesc(C.Structure):
+    _fields_ = [("rotary", ElbRotaryDesc), ("page_size", C.c_int32), ("reserved", C.c_int32)] + \
+               [(k, C.c_int64) for k in ("ld_v", "ld_page", "ld_head", "ld_token")]
+
+
+class ElbAttentionDesc(C.Structure):
+    _fields_ = [(k, C.c_int32) for k in ("heads", "kv_heads", "head_dim", "dt", "page_size", "causal")] + \
+               [("scale", C.c_float), ("device", C.c_int32)] + \
+               [(k, C.c_int64) for k in ("ld_input", "ld_output", "ld_page", "ld_head", "ld_token")]
 
 
 def _load():
@@ -152,6 +171,14 @@ def _load():
         "elb_experts_create": (i32, [C.POINTER(ElbExpertsDesc), C.POINTER(vp)]),
         "elb_experts_prepare": (i32, [vp, vp, vp]),
         "elb_experts_enqueue": (i32, [vp, vp, vp, vp, vp, C.c_int64, vp]),
+        "elb_rotary_create": (i32, [C.POINTER(ElbRotaryDesc), C.POINTER(vp)]),
+        "elb_rotary_prepare": (i32, [vp, vp]),
+        "elb_rotary_enqueue": (i32, [vp, vp, vp, vp, vp, vp, C.c_int64, vp]),
+        "elb_append_create": (i32, [C.POINTER(ElbAppendDesc), C.POINTER(vp)]),
+        "elb_append_prepare": (i32, [vp, vp]),
+        "elb_append_enqueue": (i32, [vp] * 10 + [C.c_int64] * 4 + [vp]),
+        "elb_attention_create": (i32, [C.POINTER(ElbAttentionDesc), C.POINTER(vp)]),
+        "elb_attention_enqueue": (i32, [vp] * 8 + [C.c_int64] * 4 + [vp]),
         "elb_op_device_status": (i32, [vp]),
         "elb_op_device": (i32, [vp]),
         "elb_op_launch_count": (u64, [vp]),
@@ -177,7 +204,8 @@ EXPORTED_SYMBOLS = ["elb_conv_sizes", "elb_conv_create", "elb_conv_info", "elb_c
                     "elb_conv_input_step_supported", "elb_conv_enqueue_strided",
                     "elb_linear_create", "elb_linear_prepare", "elb_linear_enqueue", "elb_norm_create", "elb_norm_prepare",
                     "elb_norm_enqueue", "elb_route_create", "elb_route_prepare", "elb_route_enqueue", "elb_experts_create",
-                    "elb_experts_prepare", "elb_experts_enqueue", "elb_op_device_status", "elb_op_device", "elb_op_launch_count",
+                    "elb_experts_prepare", "elb_experts_enqueue", "elb_rotary_create", "elb_rotary_prepare", "elb_rotary_enqueue",
+                    "elb_append_create", "elb_append_prepare", "elb_append_enqueue", "elb_attention_create", "elb_attention_enqueue", "elb_op_device_status", "elb_op_device", "elb_op_launch_count",
                     "elb_op_workspace_bytes", "elb_op_destroy"]
 
 
@@ -672,3 +700,209 @@ class Experts(_Op):
     def enqueue(self, output, input, ids, weights, *, rows: int, stream=None) -> int:
         return lib.elb_experts_enqueue(self.h, _rows(output, self._output, rows), _rows(input, self._input, rows), _rows(ids, self._ids, rows),
                                        _rows(weights, self._weights, rows), rows, stream)
+
+
+class Rotary(_Op):
+    """Queries and keys turned by their positions: pairs (i, i + r/2) or (2i, 2i + 1) of the first r = ``rotary_dim`` channels (None: all) of each
+    head.  Either may have no heads; outputs may be their inputs' tensors.  ``prepare`` takes frequencies of its own, float32 [r / 2]."""
+
+    def __init__(self, heads: int, kv_heads: int, head_dim: int, rotary_dim: int | None = None, dtype: int = bf16, layout: int = ROTARY_HALVES,
+                 scaling: int = SCALE_NONE, inverse: bool = False, base: float = 10000.0, factor: float = 1.0, slow: float = 1.0, fast: float = 4.0,
+                 magnitude: float = 1.0, original: int = 8192, ld_q: int = 0, ld_k: int = 0, ld_q_out: int = 0, ld_k_out: int = 0, device: int = -1):
+        turn = head_dim if rotary_dim is None else rotary_dim
+        self._create(lib.elb_rotary_create, ElbRotaryDesc(heads, kv_heads, head_dim, turn, dtype, layout, scaling, int(inverse), base, factor, slow,
+                                                          fast, magnitude, original, device, ld_q, ld_k, ld_q_out, ld_k_out))
+        self._frequencies = ((turn // 2,), (f32,), "frequencies")
+        wide = ((heads, ld_q, "q"), (kv_heads, ld_k, "k"), (heads, ld_q_out, "q_out"), (kv_heads, ld_k_out, "k_out"))
+        self._q, self._k, self._q_out, self._k_out = (self._spec(dtype, h * head_dim, ld, what) if h else None for h, ld, what in wide)
+        self._positions = self._spec(s32, 1, 0, "positions")
+
+    def prepare(self, frequencies=None) -> int:
+        return lib.elb_rotary_prepare(self.h, _dense(frequencies, *self._frequencies))
+
+    def enqueue(self, q_out, k_out, q, k, positions, *, rows: int, stream=None) -> int:
+        return lib.elb_rotary_enqueue(self.h, _heads(q_out, self._q_out, rows, self.device), _heads(k_out, self._k_out, rows, self.device),
+                                      _heads(q, self._q, rows, self.device), _heads(k, self._k, rows, self.device), _flat(positions, rows, self._positions),
+                                      rows, stream)
+
+
+class _Cache:
+    """What a plan wants of a cache's tensor: [pages, kv_heads, page_size, head_dim], the middle two in either order, as its strides say."""
+    __slots__ = ("type", "shape", "strides", "middle", "device", "dtype", "dense")
+
+    def __init__(self, type, kv_heads, page_size, head_dim, ld_page, ld_head, ld_token, device):
+        token = ld_token or head_dim
+        head = ld_head or page_size * token
+        page = ld_page or (kv_heads * head if head > token else page_size * token)
+        self.type, self.device, self.dtype = type, device, None
+        self.shape, self.strides = (kv_heads, page_size, head_dim), (page, head, token, 1)
+        self.dense = self.strides == (kv_heads * page_size * head_dim, page_size * head_dim, head_dim, 1)
+
+    def take(self, x, what, pages):
+        """(address, pages) of a cache"""
+        if x is None or type(x) is int:
+            if pages is None:
+                raise ValueError(f"{what}: pages are wanted beside an address")
+            return x, pages
+        shape = tuple(x.shape)
+        if not (self.dense and x.dtype is self.dtype and shape[1:] == self.shape and x.is_contiguous()):
+            self.check(x, what, shape)
+        if x.get_device() != self.device:
+            raise ValueError(f"{what}: the plan's enqueue calls take tensors of device {self.device}")
+        if pages is None:
+            pages = shape[0]
+        elif pages > shape[0]:
+            raise ValueError(f"{what}: {pages} pages are wanted, got {shape[0]}")
+        return x.data_ptr(), pages
+
+    def check(self, x, what, shape):
+        name, stride, (heads, tokens, dim) = str(x.dtype).replace("torch.", ""), tuple(x.stride()), self.shape
+        page, head, token, _ = self.strides
+
+        def lies(a, b, sa, sb):
+            return len(shape) == 4 and shape[1:] == (a, b, dim) and all(n == 1 or s == w for n, s, w in zip(shape, stride, (page, sa, sb, 1)))
+        if name != _DTYPE_NAMES[self.type] or not (lies(heads, tokens, head, token) or lies(tokens, heads, token, head)):
+            raise ValueError(f"{what}: pages of {heads} heads and {tokens} tokens of {dim} channels in {_DTYPE_NAMES[self.type]}, strides {self.strides} of page, "
+                             f"head and token, are wanted, got {shape} with strides {stride} in {name}")
+        self.dtype = x.dtype
+
+
+def _heads(x, spec, rows, device):
+    """Address of a tensor of which a call uses ``rows`` rows of heads: [rows, heads, channels] or [rows, heads * channels]; without heads, none."""
+    if spec is None:
+        return _dev(x, device)
+    if x is None or type(x) is int:
+        return x
+    if x.dtype is spec.dtype and x.is_contiguous() and x.nbytes >= rows * spec.row_bytes and x.get_device() == spec.device:
+        return x.data_ptr()
+    if len(x.shape) == 3 and x.shape[2] != spec.n and not x.is_contiguous():
+        (held, heads, dim), (row, head, one) = x.shape, x.stride()
+        if not (heads * dim == spec.n and held >= rows and (held == 1 or row == spec.ld) and (heads == 1 or head == dim) and (dim == 1 or one == 1)) or \
+                str(x.dtype).replace("torch.", "") != _DTYPE_NAMES[spec.type]:
+            raise ValueError(f"{spec.what}: {rows} rows of {spec.n} elements in {_DTYPE_NAMES[spec.type]}, {spec.ld} apart, are wanted, got {tuple(x.shape)} with "
+                             f"strides {tuple(x.stride())} in {x.dtype}")
+        if x.get_device() != device:
+            raise ValueError(f"{spec.what}: the plan's enqueue calls take tensors of device {device}")
+        return x.data_ptr()
+    return _rows(x, spec, rows)
+
+
+def _flat(x, n, spec):
+    """Address of a dense vector of at least n elements."""
+    if x is None or type(x) is int:
+        return x
+    if x.dtype is not spec.dtype or not x.is_contiguous() or x.numel() < n:
+        if str(x.dtype).replace("torch.", "") != _DTYPE_NAMES[spec.type] or not x.is_contiguous() or x.numel() < n:
+            raise ValueError(f"{spec.what}: a dense tensor of {n} elements in {_DTYPE_NAMES[spec.type]} is wanted, got {tuple(x.shape)} in {x.dtype}")
+        spec.dtype = x.dtype
+    if x.get_device() != spec.device:
+        raise ValueError(f"{spec.what}: the plan's enqueue calls take tensors of device {spec.device}")
+    return x.data_ptr()
+
+
+class _OverSequences(_Op):
+    """A plan whose calls go over a batch of sequences: ``table`` [seqs, width], ``lengths`` [seqs] and ``starts`` [seqs + 1], all int32."""
+
+    def _sequences(self):
+        self._table, self._lengths, self._starts = (self._spec(s32, 1, 0, what) for what in ("table", "lengths", "starts"))
+
+    def _batch(self, table, lengths, starts, seqs, width):
+        """(table, lengths, starts, width)"""
+        if table is not None and type(table) is not int:
+            shape = tuple(table.shape)
+            if len(shape) != 2 or shape[0] < seqs:
+                raise ValueError(f"table: {seqs} rows of pages are wanted, got {shape}")
+            if width is None:
+                width = shape[1]
+            elif width != shape[1]:
+                raise ValueError(f"table: rows of {width} pages are wanted, got {shape}")
+        if width is None:
+            raise ValueError("table: width is wanted beside an address")
+        return _flat(table, seqs * width, self._table), _flat(lengths, seqs, self._lengths), _flat(starts, seqs + 1, self._starts), width
+
+
+class CacheAppend(_OverSequences):
+    """New tokens come into a cache of pages: q turned into ``q_out``, k turned into its place in ``k_cache``, v copied to its place in ``v_cache``.
+    Caches are [pages, kv_heads, page_size, head_dim], or as ``ld_*`` say; ``rotary_dim`` 0: nothing turns."""
+
+    def __init__(self, heads: int, kv_heads: int, head_dim: int, page_size: int, rotary_dim: int | None = None, dtype: int = bf16, layout: int = ROTARY_HALVES,
+                 scaling: int = SCALE_NONE, base: float = 10000.0, factor: float = 1.0, slow: float = 1.0, fast: float = 4.0, magnitude: float = 1.0,
+                 original: int = 8192, ld_q: int = 0, ld_k: int = 0, ld_v: int = 0, ld_q_out: int = 0, ld_page: int = 0, ld_head: int = 0, ld_token: int = 0,
+                 device: int = -1):
+        turn = head_dim if rotary_dim is None else rotary_dim
+        self._create(lib.elb_append_create, ElbAppendDesc(ElbRotaryDesc(heads, kv_heads, head_dim, turn, dtype, layout, scaling, 0, base, factor, slow, fast,
+                                                                        magnitude, original, device, ld_q, ld_k, ld_q_out, 0),
+                                                          page_size, 0, ld_v, ld_page, ld_head, ld_token))
+        self._frequencies = ((turn // 2,), (f32,), "frequencies")
+        wide = ((heads, ld_q, "q"), (kv_heads, ld_k, "k"), (kv_heads, ld_v, "v"), (heads, ld_q_out, "q_out"))
+        self._q, self._k, self._v, self._q_out = (self._spec(dtype, h * head_dim, ld, what) if h else None for h, ld, what in wide)
+        self._cache = _Cache(dtype, kv_heads, page_size, head_dim, ld_page, ld_head, ld_token, self.device)
+        self._sequences()
+
+    def prepare(self, frequencies=None) -> int:
+        return lib.elb_append_prepare(self.h, _dense(frequencies, *self._frequencies))
+
+    def enqueue(self, q_out, k_cache, v_cache, q, k, v, table, lengths, starts=None, *, rows: int, seqs: int, pages: int | None = None, width: int | None = None,
+                stream=None) -> int:
+        dev, cache = self.device, self._cache
+        kc, pages = cache.take(k_cache, "k_cache", pages)
+        vc, pages = cache.take(v_cache, "v_cache", pages)
+        table, lengths, starts, width = self._batch(table, lengths, starts, seqs, width)
+        return lib.elb_append_enqueue(self.h, _heads(q_out, self._q_out, rows, dev), kc, vc, _heads(q, self._q, rows, dev), _heads(k, self._k, rows, dev),
+                                      _heads(v, self._v, rows, dev), table, lengths, starts, rows, seqs, pages, width, stream)
+
+
+class Attention(_OverSequences):
+    """output[t] = sum_j softmax_j(scale * q[t] k[j]) v[j] over the keys that token t sees.  k and v: a cache of pages of ``page_size`` tokens, as
+    CacheAppend writes it, with ``table`` and ``lengths``; or, ``page_size`` 0, tensors [seqs, keys, kv_heads, head_dim] (strides as ``ld_*`` say), of which
+    ``lengths`` may leave the last keys out.  ``causal``: a sequence's new tokens are its last ones.  Nothing to prepare."""
+
+    def __init__(self, heads: int, kv_heads: int, head_dim: int, dtype: int = bf16, page_size: int = 0, causal: bool = True, scale: float = 0.0, ld_input: int = 0,
+                 ld_output: int = 0, ld_page: int = 0, ld_head: int = 0, ld_token: int = 0, device: int = -1):
+        self._create(lib.elb_attention_create, ElbAttentionDesc(heads, kv_heads, head_dim, dtype, page_size, int(causal), scale, device, ld_input, ld_output,
+                                                                ld_page, ld_head, ld_token))
+        self._input, self._output = self._spec(dtype, heads * head_dim, ld_input, "input"), self._spec(dtype, heads * head_dim, ld_output, "output")
+        self._cache = _Cache(dtype, kv_heads, page_size, head_dim, ld_page, ld_head, ld_token, self.device) if page_size else None
+        head = ld_head or head_dim
+        self._dense, self._dtype = (kv_heads, head_dim, ld_page, head, ld_token or kv_heads * head, dtype), None
+        self._sequences()
+
+    def _keys(self, x, what, seqs, width):
+        """(address, keys of a sequence) of dense keys or values"""
+        if x is None or type(x) is int:
+            if width is None:
+                raise ValueError(f"{what}: width is wanted beside an address")
+            return x, width
+        kv_heads, dim, ld_page, head, token, kind = self._dense
+        shape, stride, name = tuple(x.shape), tuple(x.stride()), str(x.dtype).replace("torch.", "")
+
+        def lies(keys, heads, sk, sh, rest):
+            return heads == kv_heads and rest == dim and (keys <= 1 or sk == token) and (heads == 1 or sh == head) and (dim == 1 or stride[3] == 1) and \
+                (shape[0] <= 1 or keys == 0 or stride[0] == (ld_page or keys * token)) and (width is None or keys == width)
+        keys = None
+        if len(shape) == 4 and name == _DTYPE_NAMES[kind] and shape[0] >= seqs:
+            if lies(shape[1], shape[2], stride[1], stride[2], shape[3]):
+                keys = shape[1]
+            elif lies(shape[2], shape[1], stride[2], stride[1], shape[3]):
+                keys = shape[2]
+        if keys is None:
+            raise ValueError(f"{what}: {seqs} sequences of {'keys' if width is None else width}, {kv_heads} heads of {dim} channels in {_DTYPE_NAMES[kind]}, strides "
+                             f"{(ld_page or 'dense', token, head)} of sequence, key and head, are wanted, got {shape} with strides {stride} in {name}")
+        if x.get_device() != self.device:
+            raise ValueError(f"{what}: the plan's enqueue calls take tensors of device {self.device}")
+        return x.data_ptr(), keys
+
+    def enqueue(self, output, input, k, v, table=None, lengths=None, starts=None, *, rows: int, seqs: int, pages: int | None = None, width: int | None = None,
+                stream=None) -> int:
+        if self._cache:
+            k, pages = self._cache.take(k, "k", pages)
+            v, pages = self._cache.take(v, "v", pages)
+            table, lengths, starts, width = self._batch(table, lengths, starts, seqs, width)
+        else:
+            k, width = self._keys(k, "k", seqs, width)
+            v, width = self._keys(v, "v", seqs, width)
+            if table is not None:
+                raise ValueError("table: the plan's keys and values are dense")
+            lengths, starts, pages = _flat(lengths, seqs, self._lengths), _flat(starts, seqs + 1, self._starts), 0
+        return lib.elb_attention_enqueue(self.h, _heads(output, self._output, rows, self.device), _heads(input, self._input, rows, self.device), k, v, table, lengths,
+                                         starts, rows, seqs, pages, width, stream)

@@ -1,0 +1,66 @@
+// Parameter blocks and launchers of the attention operators (elb_rotary_*, elb_append_*, elb_attention_*).
+#pragma once
+#include "ops.cuh"
+
+namespace elb {
+
+// The sequences of a call: rows [first, first + n) of its new tokens, `length` tokens in all.  Whatever starts and lengths hold, rows lie in the
+// call and the length in what table or tensor can hold.
+struct Sequences {
+  const int *table, *lengths, *starts;
+  long long rows, seqs, width, pages;
+  int each;                         // rows of every sequence, where starts is null
+  int capacity;                     // tokens that a sequence can hold
+};
+struct Sequence { int first, n, length; };
+__device__ __forceinline__ Sequence sequence_of(const Sequences &b, int s) {
+  Sequence q;
+  if (b.starts) {
+    const int end = min(max(b.starts[s + 1], 0), (int)b.rows);
+    q.first = min(max(b.starts[s], 0), (int)b.rows);
+    q.n = max(end - q.first, 0);
+  } else {
+    q.first = s * b.each;
+    q.n = b.each;
+  }
+  q.length = b.lengths ? min(max(b.lengths[s], 0), b.capacity) : b.capacity;
+  return q;
+}
+// The sequence of a row, found by a warp: the starts behind the first that are not behind the row.  seqs or more, or -1: none.
+__device__ __forceinline__ int sequence_of_row(const Sequences &b, int row, int lane) {
+  if (!b.starts) return row / b.each;
+  int before = 0;
+  for (long long s = lane; s <= b.seqs; s += 32) before += b.starts[s] <= row;
+  return __reduce_add_sync(0xFFFFFFFFu, before) - 1;
+}
+
+struct RotaryParams {
+  const void *q, *k, *v;
+  void *q_out, *k_out, *v_out;      // append: the caches
+  const int *positions;             // null: of the sequences' tokens (append)
+  Sequences seq;
+  long long rows;
+  long long ld_q, ld_k, ld_v, ld_q_out, ld_k_out;
+  long long ld_page, ld_head, ld_token;
+  const unsigned long long *steps;  // of each pair: turns per position, modulo 1, times 2^64
+  int heads, kv_heads, head_dim, rotary, neighbours, inverse, page_size, et;
+  float magnitude;
+  int words;                        // everything lies in whole 16-byte words
+  int *status;
+};
+cudaError_t launch_rotary(const RotaryParams &p, cudaStream_t s);
+
+struct AttentionParams {
+  void *out;
+  const void *q, *k, *v;
+  Sequences seq;
+  long long ld_q, ld_out, ld_page, ld_head, ld_token;
+  int heads, kv_heads, head_dim, et, page_size, causal;
+  float scale;
+  int words;                        // what tiled copies ask for: 16-byte aligned tensors, strides and head_dim of whole 16 bytes
+  int num_sms;
+  int *status;
+};
+cudaError_t launch_attention_any(const AttentionParams &p, cudaStream_t s);
+
+}  // namespace elb

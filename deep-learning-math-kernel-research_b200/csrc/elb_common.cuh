@@ -66,7 +66,8 @@ enum : int {
   ST_WAIT_TIMEOUT_PRODUCER = 101,   // producer waited too long for a free shared-memory stage
   ST_WAIT_TIMEOUT_MMA = 102,        // MMA issuer waited too long for operands or a free accumulator
   ST_WAIT_TIMEOUT_EPILOGUE = 103,   // epilogue waited too long for an accumulator
-  ST_WAIT_TIMEOUT_TEST = 104        // the deliberate give-up of the wait self-test
+  ST_WAIT_TIMEOUT_TEST = 104,       // the deliberate give-up of the wait self-test
+  ST_BAD_PAGE = 105                 // a table names a page outside the pool, or a new token has no place in it
 };
 
 // The status word of a plan lies in host memory that the device maps: a kernel that gives up a wait leaves its code

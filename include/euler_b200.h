@@ -449,6 +449,82 @@ ELB_API int elb_experts_prepare(elb_op_t *op, const void *w_in, const void *w_ou
 ELB_API int elb_experts_enqueue(elb_op_t *op, void *output, const void *input, const int32_t *ids, const float *weights,
                                 int64_t rows, void *cuda_stream);
 
+/* ---- Attention -----------------------------------------------------------------------------------
+ * The attention half of a transformer block, for inference: positions, a cache of keys and values in pages, and
+ * attention over it or over dense tensors.  The protocol is the operators' above; a plan of attention has nothing to prepare.
+ *
+ * A batch is `seqs` sequences of which a call brings `rows` new tokens, one row each, those of a sequence behind one another:
+ *   starts    int32 [seqs + 1], the first row of each sequence and the end of the last; NULL: every sequence brings rows / seqs
+ *             (no remainder).  Rows behind the last sequence are left as they are.
+ *   lengths   int32 [seqs], the tokens that a sequence holds, the new ones included: new token i of n stands at length - n + i
+ *   table     int32 [seqs][width], the page that holds tokens p * page_size .. of a sequence; entries behind its length are not
+ *             read.  A page outside 0 .. pages - 1 is not touched: its keys and values count as zeros, nothing is written to it, and
+ *             elb_op_device_status tells (105).  Sequences may share pages that are read.
+ * Cache: pages of page_size tokens, element (page, head, token, channel) at page * ld_page + head * ld_head + token * ld_token +
+ * channel; all three 0: [pages][kv_heads][page_size][head_dim]. */
+enum { ELB_ROTARY_HALVES = 0 /* channels i and i + r/2 turn together */, ELB_ROTARY_NEIGHBOURS = 1 /* 2i and 2i + 1 */ };
+enum { ELB_SCALE_NONE = 0, ELB_SCALE_LINEAR = 1, ELB_SCALE_BY_PARTS = 2 };
+
+/* Rotary positions: channels a, b of pair i of the first r = rotary_dim channels of each head become
+ *   magnitude * (a cos x - b sin x), magnitude * (b cos x + a sin x),  x = position * f_i  (inverse: -x, so that magnitude 1 undoes it)
+ *   f_i = base^(-2i/r); linear: f_i / factor; by parts: with t = original * f_i / (2 pi) turns over the original length and
+ *   s = (t - slow) / (fast - slow) cut to 0 .. 1: s * f_i + (1 - s) * f_i / factor
+ * or any f_i that prepare is given.  The other channels are copied.  x is reduced exactly for every 32-bit position; the turn itself is done in 32 bits. */
+typedef struct elb_rotary_desc {
+  int32_t heads, kv_heads, head_dim;              /* of q and of k (either may be 0); head_dim up to 1024 */
+  int32_t rotary_dim;                             /* even, 2 .. head_dim (elb_append: 0 as well, nothing turns) */
+  int32_t dt;                                     /* ELB_F32, ELB_F16 or ELB_BF16 */
+  int32_t layout, scaling, inverse;               /* ELB_ROTARY_*, ELB_SCALE_* */
+  float base, factor, slow, fast, magnitude;      /* factor: linear and by parts; slow, fast: by parts */
+  int32_t original;                               /* by parts: the length that the frequencies were made for */
+  int32_t device;
+  int64_t ld_q, ld_k, ld_q_out, ld_k_out;         /* elements from one token to the next, its heads head_dim apart; 0 = dense */
+} elb_rotary_desc_t;
+ELB_API int elb_rotary_create(const elb_rotary_desc_t *desc, elb_op_t **op);
+/* frequencies: float [rotary_dim / 2], NULL: as the description says */
+ELB_API int elb_rotary_prepare(elb_op_t *op, const float *frequencies);
+/* positions: int32 [rows].  An output may be its input's tensor. */
+ELB_API int elb_rotary_enqueue(elb_op_t *op, void *q_out, void *k_out, const void *q, const void *k, const int32_t *positions, int64_t rows,
+                               void *cuda_stream);
+
+/* New tokens come into the cache: q is turned into q_out, k turned into its place in k_cache, v copied to its place in v_cache.  A row
+ * whose place has no page (before the sequence's start, past the table, a page outside the pool) is left out, its q_out too, and
+ * elb_op_device_status tells (105).  Two rows of a call must not have the same place. */
+typedef struct elb_append_desc {
+  elb_rotary_desc_t rotary;                       /* kv_heads at least 1; ld_k_out is not used */
+  int32_t page_size, reserved;
+  int64_t ld_v;                                   /* elements from one token's values to the next's; 0 = dense */
+  int64_t ld_page, ld_head, ld_token;
+} elb_append_desc_t;
+ELB_API int elb_append_create(const elb_append_desc_t *desc, elb_op_t **op);
+ELB_API int elb_append_prepare(elb_op_t *op, const float *frequencies);
+ELB_API int elb_append_enqueue(elb_op_t *op, void *q_out, void *k_cache, void *v_cache, const void *q, const void *k, const void *v,
+                               const int32_t *table, const int32_t *lengths, const int32_t *starts, int64_t rows, int64_t seqs, int64_t pages,
+                               int64_t width, void *cuda_stream);
+
+/* output[t][h] = sum_j softmax_j(scale * input[t][h] . k[j][h / g]) v[j][h / g],  g = heads / kv_heads, over the keys j that token t sees:
+ * those below its sequence's length and, causal, not behind its own place.  A token that sees none gets zeros.  Scores, sums and the result are
+ * held in 32 bits; the softmax's terms are rounded to dt, the second product's operand, except on CUDA cores.  Keys and values behind a sequence's length are not
+ * looked at, whatever they hold; a value that some token of a call sees and another of its sequence does not has to be finite for both.
+ * dense (table NULL): k and v are [seqs][width][kv_heads][head_dim], page_size 0, lengths may be NULL (all `width` keys), `pages` is not used; ld_page
+ * is then a sequence's.
+ * Tensor cores run head_dim up to 128, multiples of 8, 16-byte aligned tensors with strides of multiples of 8 elements, pages of a multiple of 8 tokens, up
+ * to 128 heads that share a key head; everything else runs on CUDA cores, many times slower. */
+typedef struct elb_attention_desc {
+  int32_t heads, kv_heads, head_dim;              /* kv_heads divides heads; head_dim 1 .. 256 */
+  int32_t dt;                                     /* ELB_BF16 or ELB_F16 */
+  int32_t page_size;                              /* tokens of a page, 0: dense */
+  int32_t causal;
+  float scale;                                    /* 0: 1 / sqrt(head_dim) */
+  int32_t device;
+  int64_t ld_input, ld_output;                    /* elements from one token to the next, its heads head_dim apart; 0 = dense */
+  int64_t ld_page, ld_head, ld_token;             /* of k and v; 0: as above (dense: ld_page = width * ld_token) */
+} elb_attention_desc_t;
+ELB_API int elb_attention_create(const elb_attention_desc_t *desc, elb_op_t **op);
+ELB_API int elb_attention_enqueue(elb_op_t *op, void *output, const void *input, const void *k, const void *v, const int32_t *table,
+                                  const int32_t *lengths, const int32_t *starts, int64_t rows, int64_t seqs, int64_t pages, int64_t width,
+                                  void *cuda_stream);
+
 /* 0 = every finished call of the plan was well; otherwise the code of the bounded wait that gave up (see
  * elb_conv_device_status).  Waits for the device; -1: it could not. */
 ELB_API int elb_op_device_status(elb_op_t *op);
