@@ -1,5 +1,6 @@
 // Parameter blocks and launchers of the attention operators (elb_rotary_*, elb_append_*, elb_attention_*).
 #pragma once
+#include "elb_common.cuh"
 #include "ops.cuh"
 
 namespace elb {
@@ -61,6 +62,42 @@ struct AttentionParams {
   int num_sms;
   int *status;
 };
+// Keys in tiles of up to TILE rows, as tiled copies bring them: whole pages where some fit, otherwise (and dense) parts of a page.
+template <int TILE>
+struct KeyTiles {
+  int page;                         // tokens of a page; 0: dense, a sequence is one
+  int pages;                        // whole pages of a tile; 0: parts of a page
+  int rows;                         // tokens of a tile (of the last part of a page: at most)
+  int parts;                        // of a page
+  __host__ __device__ explicit KeyTiles(int page_size) : page(page_size) {
+    pages = page_size > 0 && page_size <= TILE ? TILE / page_size : 0;
+    rows = pages ? pages * page_size : TILE;
+    parts = page_size > TILE ? (page_size + TILE - 1) / TILE : 1;
+  }
+  __host__ __device__ int box() const { return pages ? page : TILE; }
+  __host__ __device__ int count(int keys) const {
+    return page > TILE ? keys / page * parts + (keys % page + TILE - 1) / TILE : (keys + rows - 1) / rows;
+  }
+  // the first key of a tile, and how many rows of it are keys, of `keys` in all
+  __device__ __forceinline__ int first(int t) const { return page > TILE ? t / parts * page + t % parts * TILE : t * rows; }
+  __device__ __forceinline__ int held(int t, int keys) const {
+    const int here = page > TILE ? min(TILE, page - t % parts * TILE) : rows;
+    return min(here, keys - first(t));
+  }
+};
+
+// A tiled copy's view of keys or values: 64 channels x `rows` tokens, with the 128-byte swizzle; what lies outside arrives as zeros
+bool encode_keys(CUtensorMap *m, const AttentionParams &p, const void *base, int rows);
+
+// Where a call's partial results lie, and the counters of their joining; zero between calls.
+struct AttentionWorkspace { float *partial; int *arrived; };
+constexpr int PARTIAL_ROWS = 32, PARTIAL_FLOATS = PARTIAL_ROWS * (128 + 2);        // one partial result
+inline size_t attention_workspace_bytes(int num_sms) { return (size_t)num_sms * (2 * PARTIAL_FLOATS + 64) * 4; }
+
+// Few rows to a key head, over pages or dense tensors that tiled copies can read
+bool attention_token_takes(const AttentionParams &p);
+cudaError_t init_attention();                         // kernel attributes of the current device
+cudaError_t launch_attention_token(const AttentionParams &p, const AttentionWorkspace &w, cudaStream_t s);
 cudaError_t launch_attention_any(const AttentionParams &p, cudaStream_t s);
 
 }  // namespace elb

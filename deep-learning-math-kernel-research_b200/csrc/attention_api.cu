@@ -1,6 +1,7 @@
 // C-ABI of the attention operators (include/euler_b200.h, "Attention"): descriptions are checked when a plan is made, a call checks
 // its arguments and enqueues.
 #include <cmath>
+#include <mutex>
 
 #include "attention.cuh"
 #include "op_plan.cuh"
@@ -112,6 +113,16 @@ int check_cache(int64_t &ld_page, int64_t &ld_head, int64_t &ld_token, int64_t k
   const int64_t last = (kv_heads - 1) * ld_head + (page_size - 1) * ld_token + head_dim;
   const bool apart = ld_token >= head_dim && (kv_heads == 1 || (ld_head >= head_dim && (ld_head >= (page_size - 1) * ld_token + head_dim || ld_token >= (kv_heads - 1) * ld_head + head_dim)));
   if (!apart || ld_page < last) return op_fail(ELB_GENERAL_ERROR, "pages of %lld heads and %lld tokens overlap", (long long)kv_heads, (long long)page_size);
+  return ELB_OK;
+}
+
+// Kernel attributes are a device's: once for each of them.
+int init_device(int device) {
+  static std::mutex mutex;
+  static bool known[64];
+  std::lock_guard<std::mutex> lock(mutex);
+  if (!known[device]) OP_TRY(init_attention());                // (make_op has refused larger ordinals)
+  known[device] = true;
   return ELB_OK;
 }
 
@@ -233,6 +244,15 @@ int elb_attention_create(const elb_attention_desc_t *desc, elb_op_t **out) {
   if (rc == ELB_OK) rc = make_op(ATTENTION, d.device, &op);
   if (rc != ELB_OK) return rc;
   op->att = d;
+  DeviceGuard guard(op->device);
+  rc = init_device(op->device);
+  op->ws_bytes = attention_workspace_bytes(op->num_sms);
+  if (rc == ELB_OK) rc = alloc(*op, &op->ws, op->ws_bytes);
+  if (rc == ELB_OK && (cudaMemset(op->ws, 0, op->ws_bytes) != cudaSuccess || cudaDeviceSynchronize() != cudaSuccess)) {
+    cudaGetLastError();
+    rc = op_fail(ELB_GENERAL_ERROR, "the workspace could not be cleared");
+  }
+  if (rc != ELB_OK) { delete op; return rc; }
   op->prepared = true;
   *out = op;
   return ELB_OK;
@@ -263,9 +283,19 @@ int elb_attention_enqueue(elb_op_t *op, void *output, const void *input, const v
             (d.head_dim | d.ld_input | d.ld_output | p.ld_page | p.ld_head | p.ld_token) % 8 == 0;
   p.num_sms = op->num_sms;
   p.status = op->d_status;
-  OP_TRY(launch_attention_any(p, static_cast<cudaStream_t>(cuda_stream)));
+  const cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
+  if (!attention_token_takes(p)) {
+    OP_TRY(launch_attention_any(p, s));
+    ++op->launches;
+    return ELB_OK;
+  }
+  WorkspaceCall use(*op, s);
+  rc = use.enter();
+  if (rc != ELB_OK) return rc;
+  float *partial = static_cast<float *>(op->ws);
+  OP_TRY(launch_attention_token(p, {partial, reinterpret_cast<int *>(partial + (size_t)op->num_sms * 2 * PARTIAL_FLOATS)}, s));
   ++op->launches;
-  return ELB_OK;
+  return use.leave();
 }
 
 }  // extern "C"
