@@ -293,7 +293,7 @@ int elb_attention_enqueue(elb_op_t *op, void *output, const void *input, const v
   rc = use.enter();
   if (rc != ELB_OK) return rc;
   float *partial = static_cast<float *>(op->ws);
-  OP_TRY(launch_attention_token(p, {partial, reinterpret_cast<int *>(partial + (size_t)op->num_sms * 2 * PARTIAL_FLOATS)}, s));
+  OP_TRY(launch_attention_token(p, {partial, reinterpret_cast<int *>(partial + attention_partial_floats(op->num_sms))}, s));
   ++op->launches;
   return use.leave();
 }

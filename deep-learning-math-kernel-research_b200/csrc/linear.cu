@@ -92,14 +92,6 @@ struct alignas(64) GemmLaunch {
 
 __device__ __forceinline__ uint8_t *smem_1k(uint8_t *base) { return base + ((1024u - (smem_u32(base) & 1023u)) & 1023u); }
 
-// As mbar_wait_warp, but every lane tests the barrier, some 400 times, before lane 0 suspends: what a role waits for comes at every
-// step, and a branch to one lane and the shuffle behind it cost the role loops 5 to 12 % (1024 x 4096 -> 4096 31.1 -> 28.8 us).
-__device__ __forceinline__ bool mbar_poll_warp(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
-  bool ok = false;
-  for (int i = 0; i < 400 && !ok; ++i) ok = mbar_test_wait(bar, parity);
-  return __all_sync(0xFFFFFFFFu, ok) || mbar_wait_warp(bar, parity, abort_flag);
-}
-
 struct EpilogueTile {
   const Epilogue &e;
   uint8_t *stage;

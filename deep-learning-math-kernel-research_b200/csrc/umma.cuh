@@ -146,6 +146,14 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t *bar, uint32_t parity, v
   return ok != 0;
 }
 
+// As mbar_wait_warp, but every lane tests the barrier, some 400 times, before lane 0 suspends: what a role waits for comes at every
+// step, and a branch to one lane and the shuffle behind it cost the role loops 5 to 12 % (1024 x 4096 -> 4096 31.1 -> 28.8 us).
+__device__ __forceinline__ bool mbar_poll_warp(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
+  bool ok = false;
+  for (int i = 0; i < 400 && !ok; ++i) ok = mbar_test_wait(bar, parity);
+  return __all_sync(0xFFFFFFFFu, ok) || mbar_wait_warp(bar, parity, abort_flag);
+}
+
 // ------------------------------------------------------------------------------------ TMA
 // 1-D bulk copy global -> shared, completion counted in bytes on an mbarrier.
 // Both addresses must be 16-byte aligned and bytes a multiple of 16.
