@@ -2,8 +2,8 @@
 //
 // What it is made of is reading K and V once.  All rows of a key head (its g heads times the sequence's new tokens) share a tile of
 // 32 keys; the call's tiles, of all sequences and key heads in order, are dealt out evenly to two or three CTAs per SM, whatever their lengths, so a
-// sequence's length is split wherever that falls.  A CTA's producer keeps 32 to 64 KB of tiled copies in flight, and four warps take a tile each, in
-// turns, with a running maximum, sum and result of their own, so that they meet only at the end of a piece.  Then their results are joined,
+// sequence's length is split wherever that falls.  Four warps of a CTA take a tile each, in turns, with a running maximum, sum and result of their own, so
+// that they meet only at the end of a piece; four others bring the tiles, in turns too, since each takes about 1100 cycles to issue one.  Then their results are joined,
 // written out if the piece is all of its key head's keys, and left in the workspace otherwise, where the last CTA of those that share it joins
 // them in the order of the keys: no result depends on timing.  While one CTA of an SM does that, the others read.
 //
@@ -19,26 +19,31 @@ namespace elb {
 
 namespace {
 
-constexpr int TILE = 32, WARPS = 4, THREADS = WARPS * 32 + 32;
+constexpr int TILE = 32, WARPS = 4, PRODUCERS = 4, THREADS = (WARPS + PRODUCERS) * 32;
 constexpr int BOX_BYTES = TILE * 128;                           // the keys of a tile, 64 channels each
 
 // CB: boxes of 64 channels; MB: blocks of 16 rows, each a warp's.  The warps of a block take turns in TURNS.
 template <int CB, int MB>
 struct Smem {
   static constexpr int CTAS = CB == 1 ? 3 : 2;                  // per SM
+  static constexpr int REGS = CB == 1 ? 120 : 208, REGS_PRODUCER = 40;      // of threads, of (80 or 128) * 256 that a CTA has
   static constexpr int TURNS = WARPS / MB, NB = CB * 8;
   static constexpr int STAGE = 2 * CB * BOX_BYTES;
-  // A multiple of the turns: the same warps then come back to a stage, and see each of its phases.  (One bit of parity does not tell a stage that has
+  // A multiple of the turns, also of the producers: the same warps then come back to a stage, and see each of its phases.  (One bit of parity does not tell a stage that has
   // not been filled from one that has been twice.)
-  static constexpr int STAGES = (CB == 1 && MB == 2 ? 6 : 4) / TURNS * TURNS;
-  static constexpr int Q_BYTES = CB * MB * 16 * 128, Q_OFF = STAGES * STAGE;       // two slots
+  static constexpr int STAGES = 4;
+  static_assert(STAGES % TURNS == 0 && STAGES % PRODUCERS == 0, "");
+  static constexpr int Q_BYTES = CB * MB * 16 * 128, Q_OFF = STAGES * STAGE;       // two slots, of a piece's queries and the next one's
+  static constexpr int PITCH = CB * 64 + 8;                     // floats of a warp's row among the results (8: its lanes' banks)
   static constexpr int MERGE_OFF = Q_OFF + 2 * Q_BYTES;
-  static constexpr int MERGE = WARPS / 2 * NB * 32 * 16;        // the results of half of the warps
+  static constexpr int COPIES = MB > 1 ? 1 : WARPS;             // results of a block that lie there at the end; two blocks: a warp's, joined with its partner's
+  static constexpr int MERGE = COPIES * MB * 16 * PITCH * 4;
   static constexpr int ML_OFF = MERGE_OFF + MERGE;              // maxima and sums, [WARPS][16]
-  static constexpr int BAR_OFF = ML_OFF + WARPS * 16 * 8;       // full[S], empty[S], qfull[2], qempty[2]
-  static constexpr int MISC_OFF = BAR_OFF + (2 * STAGES + 4) * 8;
-  static constexpr int TOTAL = MISC_OFF + 128 + 1024;
+  static constexpr int BAR_OFF = ML_OFF + WARPS * 16 * 8;       // full[S], empty[S], qfull[2]
+  static constexpr int MISC_OFF = BAR_OFF + (2 * STAGES + 2) * 8;
+  static constexpr int TOTAL = MISC_OFF + 16 + 1024;           // (room to align)
   static constexpr int PARTIAL = MB * 16 * (CB * 64 + 2);       // floats of a partial result: rows, then their maxima and sums
+  static_assert(CTAS * (TOTAL + 1024) <= 228 * 1024, "");
 };
 
 struct alignas(64) TokenLaunch {
@@ -78,7 +83,7 @@ struct Deal {
   long long each, more;
   int ctas;
   __device__ __forceinline__ Deal(long long total) {
-    ctas = (int)min((long long)gridDim.x, total);
+    ctas = (int)min((long long)gridDim.x, (total + WARPS - 1) / WARPS);      // (a CTA takes no longer for a tile of each warp than for one)
     each = quotient(total, ctas);
     more = total - each * ctas;
   }
@@ -88,70 +93,66 @@ struct Deal {
     return (int)(tile < of_more ? quotient(tile, each + 1) : more + quotient(tile - of_more, each));
   }
 };
-// Where a CTA is: tile t of `tiles` of key head `head` of sequence s
-struct Walk {
-  const AttentionParams &p;
-  const KeyTiles<TILE> kt;
-  Sequence q;
-  int s, head, tiles, t;
-  __device__ __forceinline__ Walk(const AttentionParams &p, long long at, int s, long long base) : p(p), kt(p.page_size), s(s) {
-    read();
-    head = (int)quotient(at - base, tiles);
-    t = (int)(at - base - (long long)head * tiles);
-  }
-  __device__ __forceinline__ void read() {
-    q = sequence_of(p.seq, s);
-    tiles = max(1, kt.count(q.length));
-  }
-  // behind the last tile of a key head, to the next one's first (the call has another tile)
-  __device__ __forceinline__ void wrap() {
-    if (t < tiles) return;
-    t = 0;
-    if (++head < p.kv_heads) return;
-    head = 0;
-    ++s;
-    read();
-  }
-};
-
-// The tiles of a call and, of CTA `cta` of its deal, the first sequence and where that begins, from the sequences' lengths, by all threads of the block.
-__device__ __forceinline__ Deal find_start(const AttentionParams &p, long long *shared, int cta, int &s, long long &base) {
-  // shared: [0, 5) the warps' sums, 6: sequence, 7: base
+// The deal of a call and where this CTA starts, from the sequences' lengths, by a warp.
+struct Start { Sequence q; long long base; int s; };
+__device__ __forceinline__ Deal find_start(const AttentionParams &p, int cta, Start &start) {
   const KeyTiles<TILE> kt(p.page_size);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int per = (int)((p.seq.seqs + THREADS - 1) / THREADS), s0 = threadIdx.x * per, s1 = (int)min((long long)s0 + per, p.seq.seqs);
-  auto tiles = [&](int i) { return (long long)max(1, kt.count(sequence_of(p.seq, i).length)) * p.kv_heads; };
+  const int lane = threadIdx.x & 31, per = (int)((p.seq.seqs + 31) / 32), s0 = lane * per, s1 = (int)min((long long)s0 + per, p.seq.seqs);
+  auto tiles = [&](const Sequence &q) { return (long long)max(1, kt.count(q.length)) * p.kv_heads; };
+  Sequence q = {0, 0, 0};
   long long sum = 0;
-  for (int i = s0; i < s1; ++i) sum += tiles(i);
+  if (per == 1) {
+    if (s0 < s1) {
+      q = sequence_of(p.seq, s0);
+      sum = tiles(q);
+    }
+  } else {
+#pragma unroll 4
+    for (int i = s0; i < s1; ++i) sum += tiles(sequence_of(p.seq, i));
+  }
   long long scan = sum;
 #pragma unroll
   for (int b = 1; b < 32; b <<= 1) {
     const long long v = __shfl_up_sync(0xFFFFFFFFu, scan, b);
     if (lane >= b) scan += v;
   }
-  if (lane == 31) shared[warp] = scan;
-  __syncthreads();
-  long long before = 0, total = 0;
-#pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) {
-    if (w < warp) before += shared[w];
-    total += shared[w];
+  const Deal deal(__shfl_sync(0xFFFFFFFFu, scan, 31));
+  const long long at = cta < deal.ctas ? deal.begin(cta) : 0;
+  long long here = scan - sum;
+  const int mine = __ffs(__ballot_sync(0xFFFFFFFFu, at >= here && at < here + sum)) - 1;
+  int i = s0;
+  if (per > 1 && lane == mine) {
+    q = sequence_of(p.seq, i);
+    for (long long t = tiles(q); at >= here + t; t = tiles(q)) { here += t; q = sequence_of(p.seq, ++i); }
   }
-  const Deal deal(total);
-  const long long at = cta < deal.ctas ? deal.begin(cta) : -1;
-  long long here = before + scan - sum;
-  if (at >= here && at < here + sum) {
-    int i = s0;
-    if (per > 1)
-      for (long long t = tiles(i); at >= here + t; t = tiles(i)) { here += t; ++i; }
-    shared[6] = i;
-    shared[7] = here;
-  }
-  __syncthreads();
-  s = (int)shared[6];
-  base = shared[7];
+  start.s = __shfl_sync(0xFFFFFFFFu, i, mine);
+  start.base = __shfl_sync(0xFFFFFFFFu, here, mine);
+  start.q.first = __shfl_sync(0xFFFFFFFFu, q.first, mine);
+  start.q.n = __shfl_sync(0xFFFFFFFFu, q.n, mine);
+  start.q.length = __shfl_sync(0xFFFFFFFFu, q.length, mine);
   return deal;
 }
+
+// Where a CTA is: tile t of `tiles` of key head `head` of sequence s
+struct Walk {
+  const AttentionParams &p;
+  const KeyTiles<TILE> kt;
+  Sequence q;
+  int s, head, tiles, t;
+  __device__ __forceinline__ Walk(const AttentionParams &p, long long at, const Start &start) : p(p), kt(p.page_size), q(start.q), s(start.s) {
+    tiles = max(1, kt.count(q.length));
+    head = (int)quotient(at - start.base, tiles);
+    t = (int)(at - start.base - (long long)head * tiles);
+  }
+  // from behind the last tile of a key head to the next one (the call has more)
+  __device__ __forceinline__ void wrap() {
+    t -= tiles;
+    if (++head < p.kv_heads) return;
+    head = 0;
+    q = sequence_of(p.seq, ++s);
+    tiles = max(1, kt.count(q.length));
+  }
+};
 
 template <typename T, int CB, int MB>
 __global__ void __launch_bounds__(THREADS, Smem<CB, MB>::CTAS) attention_token_kernel(const __grid_constant__ TokenLaunch g) {
@@ -159,10 +160,9 @@ __global__ void __launch_bounds__(THREADS, Smem<CB, MB>::CTAS) attention_token_k
   constexpr int STAGES = L::STAGES, NB = L::NB;                 // NB: blocks of 8 channels
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::BAR_OFF), *empty = full + STAGES, *qfull = empty + STAGES, *qempty = qfull + 2;
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::BAR_OFF), *empty = full + STAGES, *qfull = empty + STAGES;
   volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::MISC_OFF);
   int *verdict = reinterpret_cast<int *>(smem + L::MISC_OFF + 4);
-  long long *found = reinterpret_cast<long long *>(smem + L::MISC_OFF + 8);
   const AttentionParams &p = g.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = p.heads / p.kv_heads;
   if (threadIdx.x == 0) {
@@ -170,71 +170,67 @@ __global__ void __launch_bounds__(THREADS, Smem<CB, MB>::CTAS) attention_token_k
     tma_prefetch_desc(&g.vmap);
     tma_prefetch_desc(&g.qmap);
     for (int i = 0; i < STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], MB); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&qfull[i], 1); mbar_init(&qempty[i], WARPS); }
+    for (int i = 0; i < 2; ++i) mbar_init(&qfull[i], 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
   // rows of queries that no copy fills
   for (int i = threadIdx.x; i < 2 * L::Q_BYTES / 16; i += THREADS) reinterpret_cast<uint4 *>(smem + L::Q_OFF)[i] = make_uint4(0, 0, 0, 0);
   fence_proxy_async_smem();
+  __syncthreads();
   griddep_launch_dependents();
   griddep_wait();
-  int s0;
-  long long base0;
-  const Deal deal = find_start(p, found, blockIdx.x, s0, base0);       // (its barriers order the initialisation above)
+  Start start;
+  const Deal deal = find_start(p, blockIdx.x, start);
   if ((int)blockIdx.x >= deal.ctas) return;
   const long long first = deal.begin(blockIdx.x), end = deal.begin(blockIdx.x + 1);
-  Walk walk(p, first, s0, base0);
+  Walk walk(p, first, start);
   const KeyTiles<TILE> &kt = walk.kt;
   int fail_code = 0;
 
-  if (warp == WARPS) {
-    // ---- the producer: a lane per copy, [K or V][64 channels][page of the tile]
+  if (warp >= WARPS) {
+    // ---- a producer: a lane per copy, [K or V][64 channels][page of the tile]
+    reg_dealloc<L::REGS_PRODUCER>();
     const int boxes = kt.pages ? kt.pages : 1, bytes = 2 * CB * boxes * kt.box() * 128;
     const int which = lane / boxes, page_in_tile = lane - which * boxes, cb = which % CB;
     const bool mine = lane < 2 * CB * boxes, values = which >= CB;
     const CUtensorMap *map = values ? &g.vmap : &g.kmap;
     uint8_t *dst = smem + which * BOX_BYTES + page_in_tile * kt.page * 128;
-    // What this lane copies for a tile.  Tables are read some tiles ahead and looked at when the copies are issued: a read takes as long as a tile does.
-    constexpr int AHEAD = 4;
-    struct { int page, token, head, row; } next[AHEAD];           // row: of the queries, in front of a piece's first tile
-    auto read = [&](int j, bool piece) {
-      walk.wrap();
+    // What this lane copies for a tile.  Tables are read a tile ahead and looked at when the copies are issued.
+    constexpr int AHEAD = 2;
+    struct { int page, token, head; } next[AHEAD];
+    auto read = [&](int j) {
+      while (walk.t >= walk.tiles) walk.wrap();
       next[j].head = walk.head;
-      next[j].row = piece || walk.t == 0 ? walk.q.first : -1;
       next[j].token = 0;
       next[j].page = (int)p.seq.pages;                          // one outside the map: zeros
       if (!kt.page) {
         next[j].page = walk.s;
         next[j].token = walk.t * TILE;
       } else if (mine) {
-        const int i = kt.pages ? walk.t * kt.pages + page_in_tile : walk.t / kt.parts;
-        if (!kt.pages) next[j].token = walk.t % kt.parts * TILE;
+        int i = walk.t * kt.pages + page_in_tile;
+        if (!kt.pages) {
+          i = walk.t / kt.parts;
+          next[j].token = (walk.t - i * kt.parts) * TILE;
+        }
         if ((long long)i * kt.page < walk.q.length) next[j].page = p.seq.table[walk.s * p.seq.width + i];
         else next[j].token = -1;                                // behind the sequence's end
       }
-      ++walk.t;
+      walk.t += PRODUCERS;
     };
-    int stage = 0, issued = 0, pieces = 0;
-    uint32_t phase = 1;
     const int tiles = (int)min(end - first, 0x7FFFFFFFll);
+    int i = warp - WARPS;
+    walk.t += i;
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j)
-      if (j < tiles) read(j, j == 0);
+      if (i + j * PRODUCERS < tiles) read(j);
     bool ok = true;
-    for (int i = 0; i < tiles && ok; i += AHEAD) {
+    while (i < tiles && ok) {
 #pragma unroll
       for (int j = 0; j < AHEAD; ++j) {
-        if (i + j >= tiles || !ok) break;
-        if (next[j].row >= 0) {
-          uint64_t *bar = &qfull[pieces & 1];
-          if (!mbar_poll_warp(&qempty[pieces & 1], ((pieces >> 1) & 1) ^ 1, abort_flag)) { ok = false; break; }
-          if (lane == 0) mbar_arrive_expect_tx(bar, CB * g.box * group * 128);
-          __syncwarp();
-          if (lane < CB) tma_tile_3d(smem + L::Q_OFF + (pieces & 1) * L::Q_BYTES + lane * MB * 16 * 128, &g.qmap, lane * 64, next[j].head * group, next[j].row, bar);
-          ++pieces;
-        }
-        if (!mbar_poll_warp(&empty[stage], phase, abort_flag)) { ok = false; break; }
+        if (i >= tiles || !ok) break;
+        const int stage = i % STAGES;
+        if (!mbar_poll_warp(&empty[stage], ((i / STAGES) & 1) ^ 1, abort_flag)) { ok = false; break; }
         if (lane == 0) mbar_arrive_expect_tx(&full[stage], bytes);
         __syncwarp();
         if (mine) {
@@ -245,46 +241,56 @@ __global__ void __launch_bounds__(THREADS, Smem<CB, MB>::CTAS) attention_token_k
           }
           tma_tile_4d(dst + stage * L::STAGE, map, cb * 64, max(next[j].token, 0), next[j].head, page, &full[stage]);
         }
-        if (++stage == STAGES) { stage = 0; phase ^= 1; }
-        if (i + j + AHEAD < tiles) read(j, false);
-        ++issued;
+        if (i + AHEAD * PRODUCERS < tiles) read(j);
+        i += PRODUCERS;
       }
     }
     if (!ok) fail_code = ST_WAIT_TIMEOUT_PRODUCER;
     // no copy is in flight when the block ends, however its other warps end
-    for (int i = max(0, issued - STAGES); i < issued; ++i) mbar_wait_warp(&full[i % STAGES], (i / STAGES) & 1, abort_flag);
-    for (int i = max(0, pieces - 2); i < pieces; ++i) mbar_wait_warp(&qfull[i & 1], (i >> 1) & 1, abort_flag);
+    static_assert(STAGES == PRODUCERS, "a stage is one producer's");
+    if (i >= PRODUCERS) mbar_wait_warp(&full[(i - PRODUCERS) % STAGES], ((i - PRODUCERS) / STAGES) & 1, abort_flag);
   } else {
+    reg_alloc<L::REGS>();
     // ---- the consumers.  Accumulators of a lane: rows lane / 4 and lane / 4 + 8 of a block, channels 2 * (lane % 4) and the next of eight
     const int quad = lane & 3, ksteps = (p.head_dim + 15) / 16, block = warp % MB, turn = warp / MB;
     const float c = fabsf(p.scale) * 1.4426950408889634f;
     const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u;    // a negative scale goes to the queries, so that the largest product has the largest score
-    float4 *merge = reinterpret_cast<float4 *>(smem + L::MERGE_OFF);
+    float *merge = reinterpret_cast<float *>(smem + L::MERGE_OFF);     // [WARPS][16][PITCH]
     float2 *ml = reinterpret_cast<float2 *>(smem + L::ML_OFF);
     const int kid = lane >> 3, krow = lane & 7;
     const uint32_t k_off = ((kid >> 1) * 8 + krow) * 128, v_off = ((kid & 1) * 8 + krow) * 128;
+    // the queries of the next piece are on their way while one is worked on: its slot was read in the piece before, which all warps have left
+    auto fetch = [&](int piece, int head, int row) {
+      if (lane == 0) mbar_arrive_expect_tx(&qfull[piece & 1], CB * g.box * group * 128);
+      __syncwarp();
+      if (lane < CB) tma_tile_3d(smem + L::Q_OFF + (piece & 1) * L::Q_BYTES + lane * MB * 16 * 128, &g.qmap, lane * 64, head * group, row, &qfull[piece & 1]);
+    };
+    if (warp == 0) fetch(0, walk.head, walk.q.first);
     int index = 0, pieces = 0;                                  // index: of a piece's first tile among this CTA's
     for (long long at = first; at < end; ++pieces) {
-      walk.wrap();
+      if (walk.t >= walk.tiles) walk.wrap();
       const int t0 = walk.t, t1 = (int)min((long long)walk.tiles, t0 + (end - at)), rows = walk.q.n * group, length = walk.q.length;
       const long long item = at - t0, item_end = item + walk.tiles;
       at += t1 - t0;
+      if (warp == 0 && at < end) {
+        if (walk.head + 1 < p.kv_heads) fetch(pieces + 1, walk.head + 1, walk.q.first);
+        else fetch(pieces + 1, 0, sequence_of(p.seq, walk.s + 1).first);
+      }
       int seen[2];                                              // the first key that a row does not see
 #pragma unroll
       for (int half = 0; half < 2; ++half) seen[half] = p.causal ? length - walk.q.n + (block * 16 + half * 8 + (lane >> 2)) / group + 1 : length;
       const int seen_by_all = p.causal ? length - walk.q.n + 1 : length;
       // Q of this key head's rows, in the products' own order
       uint32_t q[CB * 4][4];
-      if (!mbar_poll_warp(&qfull[pieces & 1], (pieces >> 1) & 1, abort_flag)) fail_code = ST_WAIT_TIMEOUT_MMA;
-      const uint32_t qb = smem_u32(smem + L::Q_OFF + (pieces & 1) * L::Q_BYTES) + (block * 16 + (kid & 1) * 8 + krow) * 128;
+      const int slot = pieces & 1;
+      if (!mbar_poll_warp(&qfull[slot], (pieces >> 1) & 1, abort_flag)) fail_code = ST_WAIT_TIMEOUT_MMA;
+      const uint32_t qb = smem_u32(smem + L::Q_OFF + slot * L::Q_BYTES) + (block * 16 + (kid & 1) * 8 + krow) * 128;
 #pragma unroll
       for (int k = 0; k < CB * 4; ++k) {
         ldmatrix4(q[k], qb + (k >> 2) * MB * 16 * 128 + ((((k & 3) * 2 + (kid >> 1)) ^ krow) << 4));
 #pragma unroll
         for (int i = 0; i < 4; ++i) q[k][i] ^= flip;
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&qempty[pieces & 1]);
       float o[NB][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 #pragma unroll
       for (int n = 0; n < NB; ++n)
@@ -376,147 +382,164 @@ __global__ void __launch_bounds__(THREADS, Smem<CB, MB>::CTAS) attention_token_k
         if (lane == 0) mbar_arrive(&empty[stage]);
       }
       index += t1 - t0;
-      // ---- The warps' results together: the second two hand theirs to the first two, whose results all four then join, a quarter of the channels each.
+      // ---- The warps' results together.  From here on a row is a warp's, a lane has 2 * CB of its channels.
+      float own[2] = {1.0f, 1.0f}, add[2] = {0.0f, 0.0f};
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         l[half] += __shfl_xor_sync(0xFFFFFFFFu, l[half], 1);
         l[half] += __shfl_xor_sync(0xFFFFFFFFu, l[half], 2);
         m[half] *= c;
       }
-      constexpr int HALF = WARPS / 2;
-      if (warp >= HALF) {
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-          if (quad == 0) ml[warp * 16 + half * 8 + (lane >> 2)] = make_float2(m[half], l[half]);
-#pragma unroll
-        for (int n = 0; n < NB; ++n) merge[((warp - HALF) * NB + n) * 32 + lane] = make_float4(o[n][0], o[n][1], o[n][2], o[n][3]);
-      }
-      named_bar_sync(1, WARPS * 32);
-      if (warp < HALF) {
-        float mine[2], theirs[2];
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const float2 x = ml[(warp + HALF) * 16 + half * 8 + (lane >> 2)];
-          const float top = fmaxf(m[half], x.x), from = top == -INFINITY ? 0.0f : top;
-          mine[half] = exp2_approx(m[half] - from);
-          theirs[half] = exp2_approx(x.x - from);
-          if (quad == 0) ml[warp * 16 + half * 8 + (lane >> 2)] = make_float2(top, l[half] * mine[half] + x.y * theirs[half]);
-        }
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-          float4 &at = merge[(warp * NB + n) * 32 + lane];
-          const float4 x = at;
-          at = make_float4(o[n][0] * mine[0] + x.x * theirs[0], o[n][1] * mine[0] + x.y * theirs[0], o[n][2] * mine[1] + x.z * theirs[1],
-                           o[n][3] * mine[1] + x.w * theirs[1]);
-        }
-      }
-      named_bar_sync(1, WARPS * 32);
-      // A warp takes every fourth block of channels.  Piece of a whole item: out; otherwise to the workspace, and the last one there joins all of them.
-      const int c0 = deal.owner(item), c1 = deal.owner(item_end - 1);
-      const bool alone = c0 == c1;
-      constexpr int PER = NB / WARPS, COPIES = HALF / MB;
-      auto part = [&](int cta) { return g.w.partial + ((size_t)cta * 2 + (cta == c0 ? 1 : 0)) * L::PARTIAL; };     // (its last piece, or its first)
-      float *mine = part(blockIdx.x);
-      float4 sum[MB][PER];
-      float lsum[MB][2];
-#pragma unroll
-      for (int b = 0; b < MB; ++b) {
-        float weight[COPIES][2];
+      float *place = merge + ((MB > 1 ? block : warp) * 16 + (lane >> 2)) * L::PITCH + quad * 2;
+      auto leave_rows = [&](bool joining) {
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const int r = half * 8 + (lane >> 2);
-          float2 x[COPIES];
-          float top = -INFINITY;
-          lsum[b][half] = 0.0f;
-#pragma unroll
-          for (int w = 0; w < COPIES; ++w) { x[w] = ml[(MB > 1 ? b : w) * 16 + r]; top = fmaxf(top, x[w].x); }
-          const float from = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-          for (int w = 0; w < COPIES; ++w) {
-            weight[w][half] = exp2_approx(x[w].x - from);
-            lsum[b][half] += x[w].y * weight[w][half];
+          if (joining) {
+            const float2 x = ml[(warp + MB) * 16 + r];
+            const float top = fmaxf(m[half], x.x), from = top == -INFINITY ? 0.0f : top;
+            own[half] = exp2_approx(m[half] - from);
+            add[half] = exp2_approx(x.x - from);
+            m[half] = top;
+            l[half] = l[half] * own[half] + x.y * add[half];
           }
-          if (!alone && warp == 0 && quad == 0 && b * 16 + r < rows)
-            *reinterpret_cast<float2 *>(mine + MB * 16 * CB * 64 + (b * 16 + r) * 2) = make_float2(top, lsum[b][half]);
-        }
+          if (quad == 0) ml[warp * 16 + r] = make_float2(m[half], l[half]);
+          if (block * 16 + r < rows) {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          const int n = i * WARPS + warp;
-          float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-          for (int w = 0; w < COPIES; ++w) {
-            const float4 x = merge[((MB > 1 ? b : w) * NB + n) * 32 + lane];
-            v.x += x.x * weight[w][0]; v.y += x.y * weight[w][0];
-            v.z += x.z * weight[w][1]; v.w += x.w * weight[w][1];
+            for (int n = 0; n < NB; ++n) {
+              float2 &at = *reinterpret_cast<float2 *>(place + half * 8 * L::PITCH + n * 8);
+              float2 v = make_float2(o[n][half * 2] * own[half], o[n][half * 2 + 1] * own[half]);
+              if (joining) { v.x += at.x * add[half]; v.y += at.y * add[half]; }
+              at = v;
+            }
           }
-          sum[b][i] = v;
-          if (!alone && b * 16 + (lane >> 2) < rows) reinterpret_cast<float4 *>(mine)[(b * NB + n) * 32 + lane] = v;
         }
+      };
+      if (MB == 1 || turn > 0) leave_rows(false);
+      named_bar_sync(1, WARPS * 32);
+      if (MB > 1) {
+        if (turn == 0) leave_rows(true);
+        named_bar_sync(1, WARPS * 32);
       }
-      bool write = alone;
-      if (!alone) {
+      const int c0 = deal.owner(item), c1 = deal.owner(item_end - 1), sharers = c1 - c0 + 1;
+      constexpr int PER = 2 * CB, WIDE = CB * 64, GROUP = 32;
+      struct Row { float v[PER], top, l; };
+      auto part = [&](int cta) { return g.w.partial + ((size_t)cta * 2 + (cta == c0 ? 1 : 0)) * L::PARTIAL; };     // (its last piece, or its first)
+      auto base_of = [](float top) { return top == -INFINITY ? 0.0f : top; };
+      // a row of all of the warps that had its block
+      auto row_here = [&](int r) {
+        Row x;
+        float2 y[L::COPIES];
+        x.top = -INFINITY;
+        x.l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) x.v[i] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < L::COPIES; ++w) { y[w] = ml[w * 16 + r]; x.top = fmaxf(x.top, y[w].x); }
+#pragma unroll
+        for (int w = 0; w < L::COPIES; ++w) {
+          const float k = exp2_approx(y[w].x - base_of(x.top));
+          const float *src = merge + (w * 16 + r) * L::PITCH + lane * PER;
+          x.l += y[w].y * k;
+#pragma unroll
+          for (int i = 0; i < PER; ++i) x.v[i] += src[i] * k;
+        }
+        return x;
+      };
+      // a row of n CTAs' results, in their order
+      auto row_of = [&](int r, auto cta_of, int n) {
+        Row x;
+        x.top = -INFINITY;
+        x.l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) x.v[i] = 0.0f;
+#pragma unroll 1
+        for (int k0 = 0; k0 < n; k0 += 32) {                    // a lane looks at one maximum and sum
+          const int here = min(32, n - k0);
+          const float2 y = lane < here ? __ldcg(reinterpret_cast<const float2 *>(part(cta_of(k0 + lane)) + MB * 16 * WIDE) + r) : make_float2(-INFINITY, 0.0f);
+          float top = fmaxf(x.top, y.x);
+#pragma unroll
+          for (int b = 16; b > 0; b >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, b));
+          const float keep = exp2_approx(x.top - base_of(top)), weight = exp2_approx(y.x - base_of(top));
+          float sum = y.y * weight;
+#pragma unroll
+          for (int b = 16; b > 0; b >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, b);
+          x.top = top;
+          x.l = x.l * keep + sum;
+#pragma unroll
+          for (int i = 0; i < PER; ++i) x.v[i] *= keep;
+          constexpr int BATCH = 16;                             // results on their way at once
+#pragma unroll 1
+          for (int k = 0; k < here; k += BATCH) {
+            float z[BATCH][PER];
+#pragma unroll
+            for (int j = 0; j < BATCH; ++j) {
+              const float *src = part(cta_of(k0 + min(k + j, here - 1))) + r * WIDE + lane * PER;
+              if constexpr (CB == 2) *reinterpret_cast<float4 *>(z[j]) = __ldcg(reinterpret_cast<const float4 *>(src));
+              else *reinterpret_cast<float2 *>(z[j]) = __ldcg(reinterpret_cast<const float2 *>(src));
+            }
+#pragma unroll
+            for (int j = 0; j < BATCH; ++j) {
+              const float w = k + j < here ? __shfl_sync(0xFFFFFFFFu, weight, k + j) : 0.0f;
+#pragma unroll
+              for (int i = 0; i < PER; ++i) x.v[i] += k + j < here ? z[j][i] * w : 0.0f;
+            }
+          }
+        }
+        return x;
+      };
+      auto leave = [&](int cta, int r, const Row &x) {
+        float *dst = part(cta);
+        if constexpr (CB == 2) *reinterpret_cast<float4 *>(dst + r * WIDE + lane * PER) = make_float4(x.v[0], x.v[1], x.v[2], x.v[3]);
+        else *reinterpret_cast<float2 *>(dst + r * WIDE + lane * PER) = make_float2(x.v[0], x.v[1]);
+        if (lane == 0) reinterpret_cast<float2 *>(dst + MB * 16 * WIDE)[r] = make_float2(x.top, x.l);
+      };
+      // whether this CTA is the last of n that have left their rows; the others' can then be read
+      auto last_of = [&](int *arrived, int n) {
         named_bar_sync(1, WARPS * 32);
         // (released and acquired by one thread for the block, whose other threads are ordered by the barriers)
         if (threadIdx.x == 0) {
           int before;
-          asm volatile("atom.acq_rel.gpu.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(g.w.arrived + c0) : "memory");
-          if (before == c1 - c0) g.w.arrived[c0] = 0;
-          *verdict = before == c1 - c0;
+          asm volatile("atom.acq_rel.gpu.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(arrived) : "memory");
+          if (before == n - 1) *arrived = 0;
+          *verdict = before == n - 1;
         }
         named_bar_sync(1, WARPS * 32);
-        write = *verdict != 0;
-        if (write) {
-#pragma unroll
-          for (int b = 0; b < MB; ++b) {
-            if (b * 16 + (lane >> 2) >= rows) continue;
-            float top[2] = {-INFINITY, -INFINITY};
-            auto stats = [&](int cta, int half) {
-              const int r = min(b * 16 + half * 8 + (lane >> 2), rows - 1);
-              return __ldcg(reinterpret_cast<const float2 *>(part(cta) + MB * 16 * CB * 64 + r * 2));
-            };
-#pragma unroll 8
-            for (int cta = c0; cta <= c1; ++cta)
-#pragma unroll
-              for (int half = 0; half < 2; ++half) top[half] = fmaxf(top[half], stats(cta, half).x);
-#pragma unroll
-            for (int i = 0; i < PER; ++i) sum[b][i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            lsum[b][0] = lsum[b][1] = 0.0f;
-#pragma unroll 8
-            for (int cta = c0; cta <= c1; ++cta) {
-              const float *from = part(cta);
-              float weight[2];
-#pragma unroll
-              for (int half = 0; half < 2; ++half) {
-                const float2 x = stats(cta, half);
-                weight[half] = exp2_approx(x.x - (top[half] == -INFINITY ? 0.0f : top[half]));
-                lsum[b][half] += x.y * weight[half];
-              }
-#pragma unroll
-              for (int i = 0; i < PER; ++i) {
-                const float4 x = __ldcg(reinterpret_cast<const float4 *>(from) + (b * NB + i * WARPS + warp) * 32 + lane);
-                sum[b][i].x += x.x * weight[0]; sum[b][i].y += x.y * weight[0];
-                sum[b][i].z += x.z * weight[1]; sum[b][i].w += x.w * weight[1];
-              }
-            }
+        return *verdict != 0;
+      };
+      auto write = [&](int r, const Row &x) {
+        const float inv = x.l == 0.0f ? 0.0f : 1.0f / x.l;
+        const int token = r / group, ch = lane * PER;
+        T *out = static_cast<T *>(p.out) + (long long)(walk.q.first + token) * p.ld_out + (long long)(walk.head * group + r - token * group) * p.head_dim + ch;
+        if (ch >= p.head_dim) return;
+        if constexpr (CB == 2) *reinterpret_cast<uint2 *>(out) = make_uint2(pack2<T>(x.v[0] * inv, x.v[1] * inv), pack2<T>(x.v[2] * inv, x.v[3] * inv));
+        else *reinterpret_cast<uint32_t *>(out) = pack2<T>(x.v[0] * inv, x.v[1] * inv);
+      };
+      // Piece of a whole item: out; otherwise to the workspace, where the last one there joins all of them.  Where more than two groups of CTAs share an
+      // item, the last of each group joins that first, and the last of these the groups.
+      if (sharers == 1) {
+#pragma unroll 1
+        for (int r = warp; r < rows; r += WARPS) write(r, row_here(r));
+      } else {
+#pragma unroll 1
+        for (int r = warp; r < rows; r += WARPS) leave(blockIdx.x, r, row_here(r));
+        int *arrived = g.w.arrived + c0, n = sharers, stride = 1, at = c0;
+        bool last = true;
+        if (sharers > 2 * GROUP) {
+          const int begin = c0 + ((int)blockIdx.x - c0) / GROUP * GROUP, final = min(begin + GROUP - 1, c1);
+          last = last_of(g.w.arrived + gridDim.x + final, final - begin + 1);
+          if (last) {
+#pragma unroll 1
+            for (int r = warp; r < rows; r += WARPS) leave(final, r, row_of(r, [&](int k) { return begin + k; }, final - begin + 1));
           }
+          n = (sharers + GROUP - 1) / GROUP;
+          stride = GROUP;
+          at = c0 + GROUP - 1;
         }
-      }
-      if (write) {
-#pragma unroll
-        for (int b = 0; b < MB; ++b)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const int r = b * 16 + half * 8 + (lane >> 2), token = r / group;
-            if (r >= rows) continue;
-            const float total = lsum[b][half], inv = total == 0.0f ? 0.0f : 1.0f / total;
-            T *out = static_cast<T *>(p.out) + (long long)(walk.q.first + token) * p.ld_out + (long long)(walk.head * group + r - token * group) * p.head_dim;
-#pragma unroll
-            for (int i = 0; i < PER; ++i) {
-              const int ch = (i * WARPS + warp) * 8 + quad * 2;
-              const float4 v = sum[b][i];
-              if (ch < p.head_dim) *reinterpret_cast<uint32_t *>(out + ch) = half ? pack2<T>(v.z * inv, v.w * inv) : pack2<T>(v.x * inv, v.y * inv);
-            }
-          }
+        if (last && last_of(arrived, n)) {
+#pragma unroll 1
+          for (int r = warp; r < rows; r += WARPS) write(r, row_of(r, [&](int k) { return min(at + k * stride, c1); }, n));
+        }
       }
       walk.t = t1;
       named_bar_sync(1, WARPS * 32);                            // the merge area may be written again
