@@ -17,7 +17,7 @@ HOST_LIB_PATH = PKG_DIR / "lib" / "libel.so"
 CSRC = PKG_DIR / "csrc"
 CU_SOURCES = ["elb_api.cu", "int8_conv.cu", "int8_conv2.cu", "wino.cu", "conv_halo.cu", "host_pipe.cu", "depthwise.cu", "misc.cu", "elb_multi.cu", "f32_small_ic.cu", "f32_rgb_umma.cu",
               "op_api.cu", "linear.cu", "gemv.cu", "block_norm.cu", "route.cu", "experts.cu",
-              "attention_api.cu", "rotary.cu", "attention.cu", "attention_token.cu"]
+              "attention_api.cu", "rotary.cu", "attention.cu", "attention_token.cu", "attention_prompt.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC,-fvisibility=hidden", "-shared"]
 

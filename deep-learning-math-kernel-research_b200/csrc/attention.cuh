@@ -35,6 +35,15 @@ __device__ __forceinline__ int sequence_of_row(const Sequences &b, int row, int 
   return __reduce_add_sync(0xFFFFFFFFu, before) - 1;
 }
 
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
 struct RotaryParams {
   const void *q, *k, *v;
   void *q_out, *k_out, *v_out;      // append: the caches
@@ -102,6 +111,10 @@ inline size_t attention_workspace_bytes(int num_sms) { return (attention_partial
 bool attention_token_takes(const AttentionParams &p);
 cudaError_t init_attention();                         // kernel attributes of the current device
 cudaError_t launch_attention_token(const AttentionParams &p, const AttentionWorkspace &w, cudaStream_t s);
+// Prompts, in tiles of 128 rows
+bool attention_prompt_takes(const AttentionParams &p);
+cudaError_t init_attention_prompt();
+cudaError_t launch_attention_prompt(const AttentionParams &p, cudaStream_t s);
 cudaError_t launch_attention_any(const AttentionParams &p, cudaStream_t s);
 
 }  // namespace elb

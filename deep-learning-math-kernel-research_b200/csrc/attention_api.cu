@@ -121,7 +121,10 @@ int init_device(int device) {
   static std::mutex mutex;
   static bool known[64];
   std::lock_guard<std::mutex> lock(mutex);
-  if (!known[device]) OP_TRY(init_attention());                // (make_op has refused larger ordinals)
+  if (!known[device]) {                                         // (make_op has refused larger ordinals)
+    OP_TRY(init_attention());
+    OP_TRY(init_attention_prompt());
+  }
   known[device] = true;
   return ELB_OK;
 }
@@ -285,7 +288,7 @@ int elb_attention_enqueue(elb_op_t *op, void *output, const void *input, const v
   p.status = op->d_status;
   const cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
   if (!attention_token_takes(p)) {
-    OP_TRY(launch_attention_any(p, s));
+    OP_TRY(attention_prompt_takes(p) ? launch_attention_prompt(p, s) : launch_attention_any(p, s));
     ++op->launches;
     return ELB_OK;
   }

@@ -53,11 +53,6 @@ struct alignas(64) TokenLaunch {
   int box;                          // new tokens of a copy of queries
 };
 
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
@@ -74,9 +69,6 @@ template <> __device__ __forceinline__ void mma16816<__half>(float (&c)[4], cons
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ long long quotient(long long a, long long b) {
-  return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
-}
 // The call's tiles in order: sequences, their key heads, their tiles (one at least, so that every row is written).  The first `more` CTAs take
 // each + 1 of them, the others `each`.
 struct Deal {
