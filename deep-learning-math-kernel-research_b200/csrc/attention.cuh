@@ -101,11 +101,12 @@ bool encode_keys(CUtensorMap *m, const AttentionParams &p, const void *base, int
 // and of the queries: 64 channels x `heads` heads that share a key head x `tokens` tokens
 bool encode_queries(CUtensorMap *m, const AttentionParams &p, int heads, int tokens);
 
-// Where a call's partial results lie, and the counters of their joining (two of each CTA), zero between calls.  Per SM: CTAs, and floats of one partial result of each.
-struct AttentionWorkspace { float *partial; int *arrived; };
-constexpr int TOKEN_CTAS = 3, TOKEN_PARTIAL = 2 * 32 * (128 + 2);
-inline size_t attention_partial_floats(int num_sms) { return (size_t)num_sms * 2 * TOKEN_PARTIAL; }
-inline size_t attention_workspace_bytes(int num_sms) { return (attention_partial_floats(num_sms) + (size_t)num_sms * TOKEN_CTAS * 2) * 4; }
+// Where a call's partial results lie, the counters of their joining (two of each CTA), and that of the items taken, zero between calls.  Per SM, for few tokens: CTAs, and floats of
+// one partial result of each (each has up to two); for prompts: floats of a CTA's.
+struct AttentionWorkspace { float *partial; int *arrived, *next; };
+constexpr int TOKEN_CTAS = 3, TOKEN_PARTIAL = 2 * 32 * (128 + 2), PROMPT_PARTIAL = 2 * 128 * (128 + 2);
+inline size_t attention_partial_floats(int num_sms) { return (size_t)num_sms * (2 * TOKEN_PARTIAL > PROMPT_PARTIAL ? 2 * TOKEN_PARTIAL : PROMPT_PARTIAL); }
+inline size_t attention_workspace_bytes(int num_sms) { return (attention_partial_floats(num_sms) + (size_t)num_sms * TOKEN_CTAS * 2 + 32) * 4; }
 
 // Few rows to a key head, over pages or dense tensors that tiled copies can read
 bool attention_token_takes(const AttentionParams &p);
@@ -114,7 +115,7 @@ cudaError_t launch_attention_token(const AttentionParams &p, const AttentionWork
 // Prompts, in tiles of 128 rows
 bool attention_prompt_takes(const AttentionParams &p);
 cudaError_t init_attention_prompt();
-cudaError_t launch_attention_prompt(const AttentionParams &p, cudaStream_t s);
+cudaError_t launch_attention_prompt(const AttentionParams &p, const AttentionWorkspace &w, cudaStream_t s);
 cudaError_t launch_attention_any(const AttentionParams &p, cudaStream_t s);
 
 }  // namespace elb

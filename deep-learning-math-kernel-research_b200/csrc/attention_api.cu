@@ -287,8 +287,9 @@ int elb_attention_enqueue(elb_op_t *op, void *output, const void *input, const v
   p.num_sms = op->num_sms;
   p.status = op->d_status;
   const cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
-  if (!attention_token_takes(p)) {
-    OP_TRY(attention_prompt_takes(p) ? launch_attention_prompt(p, s) : launch_attention_any(p, s));
+  const bool token = attention_token_takes(p);
+  if (!token && !attention_prompt_takes(p)) {
+    OP_TRY(launch_attention_any(p, s));
     ++op->launches;
     return ELB_OK;
   }
@@ -296,7 +297,9 @@ int elb_attention_enqueue(elb_op_t *op, void *output, const void *input, const v
   rc = use.enter();
   if (rc != ELB_OK) return rc;
   float *partial = static_cast<float *>(op->ws);
-  OP_TRY(launch_attention_token(p, {partial, reinterpret_cast<int *>(partial + attention_partial_floats(op->num_sms))}, s));
+  int *arrived = reinterpret_cast<int *>(partial + attention_partial_floats(op->num_sms));
+  const AttentionWorkspace w = {partial, arrived, arrived + (size_t)op->num_sms * TOKEN_CTAS * 2};
+  OP_TRY(token ? launch_attention_token(p, w, s) : launch_attention_prompt(p, w, s));
   ++op->launches;
   return use.leave();
 }

@@ -154,6 +154,30 @@ __device__ __forceinline__ bool mbar_poll_warp(uint64_t *bar, uint32_t parity, v
   return __all_sync(0xFFFFFFFFu, ok) || mbar_wait_warp(bar, parity, abort_flag);
 }
 
+// As mbar_wait_warp, but all lanes wait together, and suspended: in a kernel where many warps wait, polling keeps the barrier unit, and so every other
+// wait, busy.  A wait that is over costs a test, a branch and a vote.
+__device__ __forceinline__ bool mbar_wait_uniform(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred P, Q;\n\t"
+      ".reg .u32 n;\n\t"
+      "mov.u32 n, 0;\n\t"
+      "WAIT_%=:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2, %3;\n\t"
+      "@P bra DONE_%=;\n\t"
+      "add.u32 n, n, 1;\n\t"
+      "setp.lt.u32 Q, n, 16;\n\t"
+      "@Q bra WAIT_%=;\n\t"
+      "DONE_%=:\n\t"
+      "selp.u32 %0, 1, 0, P;\n\t"
+      "}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(WAIT_SUSPEND_NS)
+      : "memory");
+  return __all_sync(0xFFFFFFFFu, ok) || mbar_wait_warp(bar, parity, abort_flag);
+}
+
 // ------------------------------------------------------------------------------------ TMA
 // 1-D bulk copy global -> shared, completion counted in bytes on an mbarrier.
 // Both addresses must be 16-byte aligned and bytes a multiple of 16.
