@@ -43,6 +43,21 @@ __device__ __forceinline__ float exp2_approx(float x) {
 __device__ __forceinline__ long long quotient(long long a, long long b) {
   return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
 }
+// A call's tiles, dealt out in order: the first `more` CTAs take each + 1 of them, the others `each`.
+struct Deal {
+  long long each = 0, more = 0;
+  int ctas = 0;
+  Deal() = default;
+  __device__ __forceinline__ Deal(long long total, long long most) : ctas((int)min(most, total)) {
+    each = quotient(total, ctas);
+    more = total - each * ctas;
+  }
+  __device__ __forceinline__ long long begin(int c) const { return c * each + min((long long)c, more); }
+  __device__ __forceinline__ int owner(long long tile) const {
+    const long long of_more = more * (each + 1);
+    return (int)(tile < of_more ? quotient(tile, each + 1) : more + quotient(tile - of_more, each));
+  }
+};
 
 struct RotaryParams {
   const void *q, *k, *v;
@@ -85,6 +100,7 @@ struct KeyTiles {
   }
   __host__ __device__ int box() const { return pages ? page : TILE; }
   __host__ __device__ int count(int keys) const {
+    if (rows == TILE && page <= TILE) return (keys + TILE - 1) / TILE;
     return page > TILE ? keys / page * parts + (keys % page + TILE - 1) / TILE : (keys + rows - 1) / rows;
   }
   // the first key of a tile, and how many rows of it are keys, of `keys` in all
@@ -101,8 +117,9 @@ bool encode_keys(CUtensorMap *m, const AttentionParams &p, const void *base, int
 // and of the queries: 64 channels x `heads` heads that share a key head x `tokens` tokens
 bool encode_queries(CUtensorMap *m, const AttentionParams &p, int heads, int tokens);
 
-// Where a call's partial results lie, the counters of their joining (two of each CTA), and that of the items taken, zero between calls.  Per SM, for few tokens: CTAs, and floats of
-// one partial result of each (each has up to two); for prompts: floats of a CTA's.
+// Where a call's partial results lie, the counters of their joining (two of each CTA), and that of the items taken, zero between calls.  Per SM: for few
+// tokens CTAs, and floats of one partial result of each; of which a CTA has up to two, its first
+// piece's and its last's; for prompts floats of one.
 struct AttentionWorkspace { float *partial; int *arrived, *next; };
 constexpr int TOKEN_CTAS = 3, TOKEN_PARTIAL = 2 * 32 * (128 + 2), PROMPT_PARTIAL = 2 * 128 * (128 + 2);
 inline size_t attention_partial_floats(int num_sms) { return (size_t)num_sms * (2 * TOKEN_PARTIAL > PROMPT_PARTIAL ? 2 * TOKEN_PARTIAL : PROMPT_PARTIAL); }

@@ -7,9 +7,10 @@
 // its 16384 exponentials the SM's 16 special-function lanes 1024, and the way round of scores, softmax and results about 3400 a tile: 8192 tokens of 32 heads
 // over 8, causal, 448 us, 1230 TFLOP/s.
 //
-// A CTA per SM goes over the items, those that see the most keys first, each the next that nobody has taken; one warp does nothing but find them (a dozen
-// divisions, 3 to 8 k cycles between items when every role did it). The next one's queries, keys and scores are on their way while the last one's
-// results are written, through shared memory, since a row per thread makes 32 lines of each store.  Where there are fewer items than half of the SMs, their keys are split, and the last CTA of those that share a tile joins the results in order.
+// A CTA per SM goes over the items, each the next that nobody has taken, those of the longest sequences first; one warp does nothing but find them (3 to 8 k cycles
+// between items when every role did it).  The next one's queries, keys and scores are on their way while the last one's results are written, exchanged among
+// four lanes first, since a row per thread makes 32 lines of each store.  Where there are fewer items than half of the SMs, their keys are split, and the last CTA
+// of those that share a tile joins the results in the order of the keys.
 //
 // The maximum that the terms are relative to may stay 8 powers of two behind: P then reaches 256, O and l are in 32 bits, and scaling O again, a round trip
 // through registers, is left out for nearly every tile.  When the scores of a tile are there, so is O's last product: both are the same thread's, in order.
@@ -34,10 +35,9 @@ constexpr float SLACK = 8.0f;                                   // powers of two
 template <int CB>
 struct Smem {
   static constexpr int Q_BYTES = CB * BOX_BYTES, STAGE = CB * BOX_BYTES;
-  static constexpr int STAGES = CB == 1 ? 8 : 4;                // of K or V
+  static constexpr int STAGES = CB == 1 ? 8 : 5;                // of K or V
   static constexpr int RING_OFF = 2 * Q_BYTES;
-  static constexpr int OUT_OFF = RING_OFF + STAGES * STAGE;     // of each warp of rows, 32 rows of 64 channels of the result
-  static constexpr int BAR_OFF = OUT_OFF + 8 * 32 * 128;        // full[S], empty[S], qfull[2], qempty[2], sfull[2], phalf[2], pfull[2], ofull[2], oempty[2], ifull[2], iempty[2]
+  static constexpr int BAR_OFF = RING_OFF + STAGES * STAGE;     // full[S], empty[S], qfull[2], qempty[2], sfull[2], phalf[2], pfull[2], ofull[2], oempty[2], ifull[2], iempty[2]
   static constexpr int MISC_OFF = BAR_OFF + (2 * STAGES + 18) * 8;
   static constexpr int ITEMS_OFF = (MISC_OFF + 16 + 63) / 64 * 64;             // (misc: tmem slot, abort flag, verdicts)
   static constexpr int TOTAL = ITEMS_OFF + 2 * 64 + 1024;       // (room to align)
@@ -48,7 +48,6 @@ struct alignas(64) PromptLaunch {
   AttentionParams p;
   AttentionWorkspace w;
   int tokens;                       // of a row tile
-  int blocks;                       // of two row tiles, of all sequences (ragged: at most)
   int splits;                       // CTAs that share an item's keys; above 1: no CTA has two items
 };
 
@@ -72,73 +71,76 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 // A matrix descriptor whose low word, the address and the distance along M or N, is worked out in 32 bits
 __device__ __forceinline__ uint64_t with_low(uint64_t desc, uint32_t low) { return (desc & 0xFFFFFFFF00000000ull) | low; }
 
-// The block of two row tiles that a CTA has, by a warp: the last blocks first, which see the most keys
-struct Block { int s, index; Sequence q; };
-__device__ __forceinline__ bool find_block(const PromptLaunch &g, int at, Block &b) {
-  const Sequences &q = g.p.seq;
-  const int per_block = 2 * g.tokens;
-  if (!q.starts) {
-    const int per = (q.each + per_block - 1) / per_block, seqs = (int)q.seqs, turn = at / seqs;
-    b.index = per - 1 - turn;
-    b.s = at - turn * seqs;
-    b.q = sequence_of(q, b.s);
-    return true;
-  }
-  const int lane = threadIdx.x & 31, per = (int)((q.seqs + 31) / 32), s0 = lane * per, s1 = (int)min((long long)s0 + per, q.seqs);
-  auto blocks = [&](int s) { return (sequence_of(q, s).n + per_block - 1) / per_block; };
-  int sum = 0;
-#pragma unroll 4
-  for (int s = s0; s < s1; ++s) sum += blocks(s);
-  int scan = sum;
-#pragma unroll
-  for (int k = 1; k < 32; k <<= 1) {
-    const int v = __shfl_up_sync(0xFFFFFFFFu, scan, k);
-    if (lane >= k) scan += v;
-  }
-  int here = scan - sum;
-  const uint32_t who = __ballot_sync(0xFFFFFFFFu, at >= here && at < scan);
-  if (who == 0) return false;
-  int s = s0, n = 0;
-  if (at >= here && at < scan) {
-    for (n = blocks(s); at >= here + n; n = blocks(s)) { here += n; ++s; }
-  }
-  const int mine = __ffs(who) - 1;
-  b.s = __shfl_sync(0xFFFFFFFFu, s, mine);
-  b.index = __shfl_sync(0xFFFFFFFFu, n - 1 - (at - here), mine);
-  b.q = sequence_of(q, b.s);
-  return true;
-}
-
-// An item, and of its tiles of keys those that this CTA has: [t0, t1), of which row tile i sees those below end[i].  at: -1 behind the last
+// An item, and of its tiles of keys those that this CTA has: [t0, t1), of which row tile i sees those below end[i].  place: of its partial result in the
+// workspace, where those of an item that is split begin at `places`.  s: -1 behind the last item
 struct alignas(64) Item {
-  int at, index, head, s, first, n, length, row0, t0, t1, end[2];
+  int s, head, first, n, length, row0, t0, t1, end[2], place, places;
 };
-__device__ __forceinline__ bool find_item(const PromptLaunch &g, const KeyTiles<TILE> &kt, int at, Item &it) {
-  const AttentionParams &p = g.p;
-  it.at = at;
-  it.index = at / g.splits;
-  const int split = at - it.index * g.splits, block_at = it.index / p.kv_heads;
-  it.head = it.index - block_at * p.kv_heads;
-  Block block;
-  if (!find_block(g, block_at, block)) return false;
-  it.s = block.s;
-  it.first = block.q.first;
-  it.n = block.q.n;
-  it.length = block.q.length;
-  it.row0 = block.index * 2 * g.tokens;
-  int seen[2];
+
+// The items of a call in order, by one warp: sequences (up to 32 of them the longest first), their blocks of two row tiles from the last, which sees the most keys,
+// their key heads, their splits.
+struct Finder {
+  const PromptLaunch &g;
+  const KeyTiles<TILE> kt;
+  const int lane, per_block;
+  int total;                        // items
+  int own, upto;                    // sequence of this lane (of the first of several); blocks of the call up to the end of this lane's sequences
+  __device__ __forceinline__ int blocks_of(int s) const { return (sequence_of(g.p.seq, s).n + per_block - 1) / per_block; }
+  __device__ __forceinline__ Finder(const PromptLaunch &g) : g(g), kt(g.p.page_size), lane(threadIdx.x & 31), per_block(2 * g.tokens) {
+    const int seqs = (int)g.p.seq.seqs, per = (seqs + 31) / 32;
+    own = lane * per;
+    int blocks = 0;
+    if (per == 1) {
+      int length = lane < seqs ? sequence_of(g.p.seq, lane).length : -1, rank = 0;
+      for (int j = 0; j < seqs; ++j) {
+        const int other = __shfl_sync(0xFFFFFFFFu, length, j);
+        rank += other > length || (other == length && j < lane);
+      }
+      for (int j = 0; j < seqs; ++j) {
+        const int at = __shfl_sync(0xFFFFFFFFu, rank, j);
+        if (at == lane) own = j;
+      }
+      if (lane < seqs) blocks = blocks_of(own);
+    } else {
+      for (int s = own; s < min(own + per, seqs); ++s) blocks += blocks_of(s);
+    }
+    upto = blocks;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int first = it.row0 + i * g.tokens, last = min(first + g.tokens, it.n) - 1;
-    seen[i] = first >= it.n ? 0 : kt.count(max(0, p.causal ? min(it.length, it.length - it.n + last + 1) : it.length));
+    for (int k = 1; k < 32; k <<= 1) {
+      const int v = __shfl_up_sync(0xFFFFFFFFu, upto, k);
+      if (lane >= k) upto += v;
+    }
+    total = __shfl_sync(0xFFFFFFFFu, upto, 31) * g.p.kv_heads * g.splits;
   }
-  const long long most = max(seen[0], seen[1]);
-  it.t0 = (int)(most * split / g.splits);
-  it.t1 = (int)(most * (split + 1) / g.splits);
+  __device__ __forceinline__ void find(int at, Item &it) const {
+    const AttentionParams &p = g.p;
+    const int item = at / g.splits, split = at - item * g.splits, block_at = item / p.kv_heads;
+    it.head = item - block_at * p.kv_heads;
+    it.places = item * g.splits;
+    it.place = at;
+    const int mine = __ffs(__ballot_sync(0xFFFFFFFFu, block_at < upto)) - 1;
+    int s = __shfl_sync(0xFFFFFFFFu, own, mine), before = mine > 0 ? __shfl_sync(0xFFFFFFFFu, upto, mine > 0 ? mine - 1 : 0) : 0;
+    int blocks = blocks_of(s);
+    while (block_at >= before + blocks) { before += blocks; blocks = blocks_of(++s); }        // (several sequences a lane)
+    const Sequence q = sequence_of(p.seq, s);
+    it.s = s;
+    it.first = q.first;
+    it.n = q.n;
+    it.length = q.length;
+    it.row0 = (blocks - 1 - (block_at - before)) * per_block;
+    int seen[2];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) it.end[i] = max(it.t0, min(it.t1, seen[i]));
-  return true;
-}
+    for (int i = 0; i < 2; ++i) {
+      const int from = it.row0 + i * g.tokens, last = min(from + g.tokens, q.n) - 1;
+      seen[i] = from >= q.n ? 0 : kt.count(max(0, p.causal ? min(q.length, q.length - q.n + last + 1) : q.length));
+    }
+    const long long most = max(seen[0], seen[1]);
+    it.t0 = (int)quotient(most * split, g.splits);
+    it.t1 = (int)quotient(most * (split + 1), g.splits);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) it.end[i] = max(it.t0, min(it.t1, seen[i]));
+  }
+};
 
 template <typename T, int CB>
 __global__ void __launch_bounds__(THREADS, 1) attention_prompt_kernel(const __grid_constant__ PromptLaunch g) {
@@ -189,14 +191,16 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prompt_kernel(const __gr
   const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
   int fail_code = 0;
   // the next item of a role, which the finding warp has put down; false: there is none
-  auto next_item = [&](uint32_t &count, Item &it) {
-    const uint32_t slot = count & 1;
-    if (!mbar_wait_uniform(&ifull[slot], (count >> 1) & 1, abort_flag)) return false;
-    it = slots[slot];
+  auto done_item = [&](uint32_t &count) {
     __syncwarp();
-    if (lane == 0) mbar_arrive(&iempty[slot]);
+    if (lane == 0) mbar_arrive(&iempty[count & 1]);
     ++count;
-    return it.at >= 0;
+  };
+  auto next_item = [&](uint32_t &count, Item &it) {
+    if (!mbar_wait_uniform(&ifull[count & 1], (count >> 1) & 1, abort_flag)) return false;
+    it = slots[count & 1];
+    done_item(count);
+    return it.s >= 0;
   };
 
   if (warp < 4) {
@@ -213,6 +217,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prompt_kernel(const __gr
       uint32_t count = 0;
       for (Item it; ok && next_item(count, it);) {
         if (it.t1 == it.t0) continue;
+        // (the queries' place is free when the item in front has had its last scores: until then they come as far as L2)
+        if (lane < 2 * CB && it.end[lane / CB] > it.t0) tma_prefetch_3d(&g.qmap, lane % CB * 64, it.head * group, it.first + it.row0 + lane / CB * g.tokens);
         int next_page = 0, next_token = 0;
         auto read = [&](int t) {
           next_page = (int)p.seq.pages;                         // one outside the map: zeros
@@ -367,17 +373,15 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prompt_kernel(const __gr
     } else if (warp == 2) {
       // ---- items: the CTA's own first one, then the next that nobody has taken.  Every CTA counts once past the last, so the counter sees as many
       // counts as there are items, and the last of them leaves it at zero.
-      const int total = g.blocks * p.kv_heads * g.splits, ctas = gridDim.x;
+      const Finder finder(g);
+      const int ctas = gridDim.x;
       uint32_t count = 0;
       bool ok = true;
-      for (int at = blockIdx.x; at >= 0;) {
+      for (int at = blockIdx.x;;) {
         Item it;
-        bool put = at < total && find_item(g, kt, at, it);
-        if (at >= total) {
-          it.at = at = -1;
-          put = true;
-        }
-        if (put && ok) {                                        // (on, where the others have given up: the counter has to come to its end)
+        if (at < finder.total) finder.find(at, it);
+        else it.s = -1;
+        if (ok) {                                               // (on, where the others have given up: the counter has to come to its end)
           ok = mbar_wait_uniform(&iempty[count & 1], ((count >> 1) & 1) ^ 1, abort_flag);
           if (ok && lane == 0) {
             slots[count & 1] = it;
@@ -385,17 +389,16 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prompt_kernel(const __gr
           }
           ++count;
         }
-        if (at < 0) break;
-        int next = total;
-        if (total > ctas) {
+        if (at >= finder.total) break;
+        at = finder.total;
+        if (finder.total > ctas) {
+          int taken = 0;
           if (lane == 0) {
-            const int taken = atomicAdd(g.w.next, 1);
-            if (taken == total - 1) *g.w.next = 0;
-            next = ctas + taken;
+            taken = atomicAdd(g.w.next, 1);
+            if (taken == finder.total - 1) *g.w.next = 0;
           }
-          next = __shfl_sync(0xFFFFFFFFu, next, 0);
+          at = ctas + __shfl_sync(0xFFFFFFFFu, taken, 0);
         }
-        at = next;
       }
       if (!ok) fail_code = ST_WAIT_TIMEOUT_PRODUCER;
     }
@@ -406,11 +409,12 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prompt_kernel(const __gr
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16, s_at = tmem + lanes + S_COL + i * TILE, o_at = tmem + lanes + O_COL + i * CB * 64;
     const float c = fabsf(p.scale) * 1.4426950408889634f, slack = SLACK / c;
     uint32_t items = 0, terms = 0, count = 0;
-    for (Item it; next_item(count, it);) {
-      const int length = it.length, n = it.n, t0 = it.t0, end = i ? it.end[1] : it.end[0], token = it.row0 + i * g.tokens + in_tile, tiles = end - t0;
-      if (it.row0 + i * g.tokens >= n) continue;                // no rows in this tile
-      const bool mine = in_tile < g.tokens && token < n;
-      const int seen = p.causal ? min(length, length - n + token + 1) : length;
+    // (an item is read again where its results are written, which keeps it out of the registers of the loop)
+    for (; mbar_wait_uniform(&ifull[count & 1], (count >> 1) & 1, abort_flag) && slots[count & 1].s >= 0; done_item(count)) {
+      volatile Item &it = slots[count & 1];
+      const int length = it.length, t0 = it.t0, end = it.end[i], tiles = end - t0;
+      if (it.row0 + i * g.tokens >= it.n) continue;             // no rows in this tile
+      const int seen = p.causal ? min(length, length - it.n + it.row0 + i * g.tokens + in_tile + 1) : length;
       float m = -INFINITY, l = 0.0f;
       for (int t = t0; t < end; ++t, ++terms) {
         if (!mbar_wait_uniform(&sfull[i], terms & 1, abort_flag)) { fail_code = ST_WAIT_TIMEOUT_EPILOGUE; break; }
@@ -485,35 +489,43 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prompt_kernel(const __gr
       }
       if (tiles > 0 && !mbar_wait_uniform(&ofull[i], items & 1, abort_flag)) fail_code = ST_WAIT_TIMEOUT_EPILOGUE;
       tc_fence_after_sync();
+      const int token = it.row0 + i * g.tokens + in_tile;
+      const bool mine = in_tile < g.tokens && token < it.n;
       T *out = static_cast<T *>(p.out) + (long long)(it.first + token) * p.ld_out + (long long)(it.head * group + r - in_tile * group) * p.head_dim;
       const uint32_t rows_here = __ballot_sync(0xFFFFFFFFu, mine);
-      // 32 channels of a warp's 32 rows to its place in shared memory, a row per lane, 16-byte chunk x of row y at x ^ (y & 7); then, 64 channels at a time, to the
-      // rows in memory, eight lanes to a row
-      uint4 *stage = reinterpret_cast<uint4 *>(smem + L::OUT_OFF + (warp - 4) * 32 * 128);
+      // 32 channels of a row are four words of 16 bytes; four lanes exchange theirs, so that a store has 64 bytes of each of eight rows
       auto write = [&](const float (&v)[32], int q, float inv) {
+        uint4 w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          w[k] = make_uint4(pack2<T>(v[k * 8] * inv, v[k * 8 + 1] * inv), pack2<T>(v[k * 8 + 2] * inv, v[k * 8 + 3] * inv),
+                            pack2<T>(v[k * 8 + 4] * inv, v[k * 8 + 5] * inv), pack2<T>(v[k * 8 + 6] * inv, v[k * 8 + 7] * inv));
+        auto trade = [&](uint4 &a, uint4 &b, int with) {        // the lane whose bit is clear gives b and takes the other's a in its place
+          const bool upper = (lane & with) != 0;
+          uint4 x = upper ? a : b;
+          x.x = __shfl_xor_sync(0xFFFFFFFFu, x.x, with);
+          x.y = __shfl_xor_sync(0xFFFFFFFFu, x.y, with);
+          x.z = __shfl_xor_sync(0xFFFFFFFFu, x.z, with);
+          x.w = __shfl_xor_sync(0xFFFFFFFFu, x.w, with);
+          if (upper) a = x;
+          else b = x;
+        };
+        trade(w[0], w[1], 1);
+        trade(w[2], w[3], 1);
+        trade(w[0], w[2], 2);
+        trade(w[1], w[3], 2);
+        const int ch = q * 32 + (lane & 3) * 8;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          uint32_t w[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) w[j] = pack2<T>(v[k * 8 + 2 * j] * inv, v[k * 8 + 2 * j + 1] * inv);
-          stage[lane * 8 + (((q & 1) * 4 + k) ^ (lane & 7))] = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-        if ((q & 1) == 0) return;
-        __syncwarp();
-        const int chunk = lane & 7, ch = (q >> 1) * 64 + chunk * 8;
-#pragma unroll
-        for (int y0 = 0; y0 < 32; y0 += 4) {
-          const int y = y0 + (lane >> 3);
+          const int y = (lane & ~3) + k;
           T *to = reinterpret_cast<T *>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(out), y));
-          const uint4 x = stage[y * 8 + (chunk ^ (y & 7))];
-          if (((rows_here >> y) & 1) && ch < p.head_dim) *reinterpret_cast<uint4 *>(to + ch) = x;
+          if (((rows_here >> y) & 1) && ch < p.head_dim) *reinterpret_cast<uint4 *>(to + ch) = w[k];
         }
-        __syncwarp();
       };
       // a partial result: [4 channels][row], then the rows' maxima and sums
       constexpr int WIDE = CB * 64;
-      auto part = [&](int split) { return g.w.partial + ((size_t)(it.index * g.splits + split) * 2 + i) * (TILE * (WIDE + 2)); };
-      float *mine_part = part(it.at - it.index * g.splits);
+      auto part = [&](int place) { return g.w.partial + ((size_t)place * 2 + i) * (TILE * (WIDE + 2)); };
+      float *mine_part = part(it.place);
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll 1
       for (int q = 0; q < 2 * CB; ++q) {
@@ -545,18 +557,19 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prompt_kernel(const __gr
         named_bar_sync(1 + i, 128);
         // (released and acquired by one thread for the row tile's four warps, which the barriers order)
         if (r == 0) {
-          int before, *arrived = g.w.arrived + it.index * 2 + i;
+          int before, *arrived = g.w.arrived + it.places * 2 + i;
           asm volatile("atom.acq_rel.gpu.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(arrived) : "memory");
           if (before == g.splits - 1) *arrived = 0;
           verdict[i] = before == g.splits - 1;
         }
         named_bar_sync(1 + i, 128);
         if (verdict[i] != 0) {                                  // (rows that are not there read what others left and write nothing)
+          const int places = it.places;
           float top = -INFINITY, whole = 0.0f;
-          for (int k = 0; k < g.splits; ++k) top = fmaxf(top, __ldcg(reinterpret_cast<const float2 *>(part(k) + TILE * WIDE) + r).x);
+          for (int k = 0; k < g.splits; ++k) top = fmaxf(top, __ldcg(reinterpret_cast<const float2 *>(part(places + k) + TILE * WIDE) + r).x);
           const float from = top == -INFINITY ? 0.0f : top;
           for (int k = 0; k < g.splits; ++k) {
-            const float2 x = __ldcg(reinterpret_cast<const float2 *>(part(k) + TILE * WIDE) + r);
+            const float2 x = __ldcg(reinterpret_cast<const float2 *>(part(places + k) + TILE * WIDE) + r);
             whole += x.y * exp2_approx(x.x - from);
           }
           const float inv = whole == 0.0f ? 0.0f : 1.0f / whole;
@@ -567,10 +580,10 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prompt_kernel(const __gr
             for (int k = 0; k < 32; ++k) v[k] = 0.0f;
 #pragma unroll 2
             for (int k = 0; k < g.splits; ++k) {
-              const float w = exp2_approx(__ldcg(reinterpret_cast<const float2 *>(part(k) + TILE * WIDE) + r).x - from);
+              const float w = exp2_approx(__ldcg(reinterpret_cast<const float2 *>(part(places + k) + TILE * WIDE) + r).x - from);
 #pragma unroll
               for (int j = 0; j < 8; ++j) {
-                const float4 x = __ldcg(reinterpret_cast<const float4 *>(part(k)) + (q * 8 + j) * TILE + r);
+                const float4 x = __ldcg(reinterpret_cast<const float4 *>(part(places + k)) + (q * 8 + j) * TILE + r);
                 v[4 * j] += x.x * w; v[4 * j + 1] += x.y * w; v[4 * j + 2] += x.z * w; v[4 * j + 3] += x.w * w;
               }
             }
@@ -588,19 +601,19 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prompt_kernel(const __gr
 }
 
 template <typename T, int CB>
-cudaError_t go(const PromptLaunch &g, cudaStream_t s) {
+cudaError_t go(const PromptLaunch &g, long long items, cudaStream_t s) {
   static_assert(2 * TILE * (CB * 64 + 2) <= PROMPT_PARTIAL, "");
-  const int total = g.blocks * g.p.kv_heads * g.splits;
-  return launch_overlapped(attention_prompt_kernel<T, CB>, dim3(total < g.p.num_sms ? total : g.p.num_sms), dim3(THREADS), Smem<CB>::TOTAL, s, g);
+  return launch_overlapped(attention_prompt_kernel<T, CB>, dim3((unsigned)(items < g.p.num_sms ? items : g.p.num_sms)), dim3(THREADS), Smem<CB>::TOTAL, s, g);
 }
 template <typename T>
-cudaError_t go(const PromptLaunch &g, cudaStream_t s) { return g.p.head_dim <= 64 ? go<T, 1>(g, s) : go<T, 2>(g, s); }
+cudaError_t go(const PromptLaunch &g, long long items, cudaStream_t s) { return g.p.head_dim <= 64 ? go<T, 1>(g, items, s) : go<T, 2>(g, items, s); }
 template <typename K>
 cudaError_t allow(K kern, int smem) { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); }
 
-long long blocks_of(const AttentionParams &p, int tokens) {
-  if (!p.seq.starts) return p.seq.seqs * ((p.seq.each + 2ll * tokens - 1) / (2 * tokens));
-  return p.seq.rows / (2 * tokens) + p.seq.seqs;
+// Items before splitting; of ragged sequences the most that there can be
+long long items_of(const AttentionParams &p) {
+  const long long block = 2 * (TILE / (p.heads / p.kv_heads)), blocks = p.seq.starts ? p.seq.rows / block + p.seq.seqs : p.seq.seqs * ((p.seq.each + block - 1) / block);
+  return blocks * p.kv_heads;
 }
 
 }  // namespace
@@ -615,8 +628,7 @@ cudaError_t init_attention_prompt() {
 
 bool attention_prompt_takes(const AttentionParams &p) {
   const int group = p.heads / p.kv_heads;
-  return p.words && p.head_dim <= 128 && group <= TILE && p.page_size % 8 == 0 && p.seq.width > 0 && p.seq.pages > 0 &&
-         blocks_of(p, TILE / group) * p.kv_heads <= INT32_MAX / 2;
+  return p.words && p.head_dim <= 128 && group <= TILE && p.page_size % 8 == 0 && p.seq.width > 0 && p.seq.pages > 0 && items_of(p) <= INT32_MAX;
 }
 
 // Keys are split where that fills the SMs, into no fewer than three tiles each of what the sequences can hold.
@@ -625,13 +637,12 @@ cudaError_t launch_attention_prompt(const AttentionParams &p, const AttentionWor
   const int rows = KeyTiles<TILE>(p.page_size).box(), group = p.heads / p.kv_heads;
   g.p = p;
   g.tokens = TILE / group;
-  g.blocks = (int)blocks_of(p, g.tokens);
   g.w = w;
-  const int fit = p.num_sms / (g.blocks * p.kv_heads < p.num_sms ? g.blocks * p.kv_heads : p.num_sms), worth = p.seq.capacity / (3 * TILE);
-  g.splits = fit < worth ? fit : worth;
+  const long long items = items_of(p), fit = p.num_sms / items, worth = p.seq.capacity / (3 * TILE);
+  g.splits = (int)(fit < worth ? fit : worth);
   if (g.splits < 1) g.splits = 1;
   if (!encode_keys(&g.kmap, p, p.k, rows) || !encode_keys(&g.vmap, p, p.v, rows) || !encode_queries(&g.qmap, p, group, g.tokens)) return cudaErrorInvalidValue;
-  return p.et == ET_BF16 ? go<__nv_bfloat16>(g, s) : go<__half>(g, s);
+  return p.et == ET_BF16 ? go<__nv_bfloat16>(g, items * g.splits, s) : go<__half>(g, items * g.splits, s);
 }
 
 }  // namespace elb

@@ -69,23 +69,8 @@ template <> __device__ __forceinline__ void mma16816<__half>(float (&c)[4], cons
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// The call's tiles in order: sequences, their key heads, their tiles (one at least, so that every row is written).  The first `more` CTAs take
-// each + 1 of them, the others `each`.
-struct Deal {
-  long long each, more;
-  int ctas;
-  __device__ __forceinline__ Deal(long long total) {
-    ctas = (int)min((long long)gridDim.x, (total + WARPS - 1) / WARPS);      // (a CTA takes no longer for a tile of each warp than for one)
-    each = quotient(total, ctas);
-    more = total - each * ctas;
-  }
-  __device__ __forceinline__ long long begin(int c) const { return c * each + min((long long)c, more); }
-  __device__ __forceinline__ int owner(long long tile) const {
-    const long long of_more = more * (each + 1);
-    return (int)(tile < of_more ? quotient(tile, each + 1) : more + quotient(tile - of_more, each));
-  }
-};
-// The deal of a call and where this CTA starts, from the sequences' lengths, by a warp.
+// The call's tiles lie in order: sequences, their key heads, their tiles (one at least, so that every row is written).
+// Their deal and where this CTA starts, from the sequences' lengths, by a warp.
 struct Start { Sequence q; long long base; int s; };
 __device__ __forceinline__ Deal find_start(const AttentionParams &p, int cta, Start &start) {
   const KeyTiles<TILE> kt(p.page_size);
@@ -108,7 +93,9 @@ __device__ __forceinline__ Deal find_start(const AttentionParams &p, int cta, St
     const long long v = __shfl_up_sync(0xFFFFFFFFu, scan, b);
     if (lane >= b) scan += v;
   }
-  const Deal deal(__shfl_sync(0xFFFFFFFFu, scan, 31));
+  // (a CTA takes no longer for a tile of each warp than for one)
+  const long long total = __shfl_sync(0xFFFFFFFFu, scan, 31);
+  const Deal deal(total, min((long long)gridDim.x, (total + WARPS - 1) / WARPS));
   const long long at = cta < deal.ctas ? deal.begin(cta) : 0;
   long long here = scan - sum;
   const int mine = __ffs(__ballot_sync(0xFFFFFFFFu, at >= here && at < here + sum)) - 1;
