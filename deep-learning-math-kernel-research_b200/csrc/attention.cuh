@@ -117,13 +117,13 @@ bool encode_keys(CUtensorMap *m, const AttentionParams &p, const void *base, int
 // and of the queries: 64 channels x `heads` heads that share a key head x `tokens` tokens
 bool encode_queries(CUtensorMap *m, const AttentionParams &p, int heads, int tokens);
 
-// Where a call's partial results lie, the counters of their joining (two of each CTA), and that of the items taken, zero between calls.  Per SM: for few
+// Where a call's partial results lie, the counters of their joining (two of each CTA), zero between calls.  Per SM: for few
 // tokens CTAs, and floats of one partial result of each; of which a CTA has up to two, its first
 // piece's and its last's; for prompts floats of one.
-struct AttentionWorkspace { float *partial; int *arrived, *next; };
+struct AttentionWorkspace { float *partial; int *arrived; };
 constexpr int TOKEN_CTAS = 3, TOKEN_PARTIAL = 2 * 32 * (128 + 2), PROMPT_PARTIAL = 2 * 128 * (128 + 2);
 inline size_t attention_partial_floats(int num_sms) { return (size_t)num_sms * (2 * TOKEN_PARTIAL > PROMPT_PARTIAL ? 2 * TOKEN_PARTIAL : PROMPT_PARTIAL); }
-inline size_t attention_workspace_bytes(int num_sms) { return (attention_partial_floats(num_sms) + (size_t)num_sms * TOKEN_CTAS * 2 + 32) * 4; }
+inline size_t attention_workspace_bytes(int num_sms) { return (attention_partial_floats(num_sms) + (size_t)num_sms * TOKEN_CTAS * 2) * 4; }
 
 // Few rows to a key head, over pages or dense tensors that tiled copies can read
 bool attention_token_takes(const AttentionParams &p);

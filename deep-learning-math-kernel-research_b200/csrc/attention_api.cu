@@ -297,8 +297,7 @@ int elb_attention_enqueue(elb_op_t *op, void *output, const void *input, const v
   rc = use.enter();
   if (rc != ELB_OK) return rc;
   float *partial = static_cast<float *>(op->ws);
-  int *arrived = reinterpret_cast<int *>(partial + attention_partial_floats(op->num_sms));
-  const AttentionWorkspace w = {partial, arrived, arrived + (size_t)op->num_sms * TOKEN_CTAS * 2};
+  const AttentionWorkspace w = {partial, reinterpret_cast<int *>(partial + attention_partial_floats(op->num_sms))};
   OP_TRY(token ? launch_attention_token(p, w, s) : launch_attention_prompt(p, w, s));
   ++op->launches;
   return use.leave();
