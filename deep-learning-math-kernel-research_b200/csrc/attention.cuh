@@ -93,20 +93,32 @@ struct KeyTiles {
   int pages;                        // whole pages of a tile; 0: parts of a page
   int rows;                         // tokens of a tile (of the last part of a page: at most)
   int parts;                        // of a page
+  int shift;                        // parts are 1 << shift; -1: no power of two
+  bool flat;                        // tile t holds keys t * TILE and on, as where pages and tiles are multiples of one another
   __host__ __device__ explicit KeyTiles(int page_size) : page(page_size) {
     pages = page_size > 0 && page_size <= TILE ? TILE / page_size : 0;
     rows = pages ? pages * page_size : TILE;
     parts = page_size > TILE ? (page_size + TILE - 1) / TILE : 1;
+    flat = page_size > TILE ? page_size % TILE == 0 : rows == TILE;
+    shift = -1;
+    if ((parts & (parts - 1)) == 0)
+      for (shift = 0; 1 << shift < parts;) ++shift;
   }
   __host__ __device__ int box() const { return pages ? page : TILE; }
   __host__ __device__ int count(int keys) const {
-    if (rows == TILE && page <= TILE) return (keys + TILE - 1) / TILE;
+    if (flat) return (keys + TILE - 1) / TILE;
     return page > TILE ? keys / page * parts + (keys % page + TILE - 1) / TILE : (keys + rows - 1) / rows;
   }
+  // the page that a tile is a part of
+  __device__ __forceinline__ int page_of(int t) const { return shift >= 0 ? t >> shift : t / parts; }
   // the first key of a tile, and how many rows of it are keys, of `keys` in all
-  __device__ __forceinline__ int first(int t) const { return page > TILE ? t / parts * page + t % parts * TILE : t * rows; }
+  __device__ __forceinline__ int first(int t) const {
+    if (flat) return t * TILE;
+    return page > TILE ? page_of(t) * page + (t - page_of(t) * parts) * TILE : t * rows;
+  }
   __device__ __forceinline__ int held(int t, int keys) const {
-    const int here = page > TILE ? min(TILE, page - t % parts * TILE) : rows;
+    if (flat) return min(TILE, keys - t * TILE);
+    const int here = page > TILE ? min(TILE, page - (t - page_of(t) * parts) * TILE) : rows;
     return min(here, keys - first(t));
   }
 };

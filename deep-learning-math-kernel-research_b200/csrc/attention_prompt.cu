@@ -149,12 +149,17 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prompt_kernel(const __gr
   const int item = blockIdx.x / g.splits, split = blockIdx.x - item * g.splits, head = item % p.kv_heads;
   Block block;
   if (!find_block(g, item / p.kv_heads, block)) return;         // (the same for all warps)
-  if (warp == 1) tmem_alloc(tmem_slot, COLS);
-  tc_fence_before_sync();
-  __syncthreads();
-  tc_fence_after_sync();
-  griddep_launch_dependents();
-  const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
+  // (the copies start without tensor memory, which is taken when the kernel in front has ended; the kernel behind may start when it has been)
+  if (warp == 1 || warp >= 4) {
+    if (warp == 1) {
+      tmem_alloc(tmem_slot, COLS);
+      griddep_launch_dependents();
+    }
+    tc_fence_before_sync();
+    named_bar_sync(3, 9 * 32);
+    tc_fence_after_sync();
+  }
+  const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);        // (nothing yet in the other warps)
   // The tiles of keys that this CTA has, [t0, t1), of which the row tiles see those below n0 and n1
   const int length = block.q.length, n = block.q.n, row0 = block.index * 2 * g.tokens;
   auto seen_by = [&](int i) {
@@ -183,7 +188,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prompt_kernel(const __gr
         } else if (mine) {
           int i = t * kt.pages + page_in_tile;
           if (!kt.pages) {
-            i = t / kt.parts;
+            i = kt.page_of(t);
             next_token = (t - i * kt.parts) * TILE;
           }
           if ((long long)i * kt.page < length) next_page = p.seq.table[block.s * p.seq.width + i];

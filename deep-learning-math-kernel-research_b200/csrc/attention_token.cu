@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(THREADS, Smem<CB, MB>::CTAS) attention_token_k
       } else if (mine) {
         int i = walk.t * kt.pages + page_in_tile;
         if (!kt.pages) {
-          i = walk.t / kt.parts;
+          i = kt.page_of(walk.t);
           next[j].token = (walk.t - i * kt.parts) * TILE;
         }
         if ((long long)i * kt.page < walk.q.length) next[j].page = p.seq.table[walk.s * p.seq.width + i];
@@ -403,7 +403,7 @@ __global__ void __launch_bounds__(THREADS, Smem<CB, MB>::CTAS) attention_token_k
       const int c0 = deal.owner(item), c1 = deal.owner(item_end - 1), sharers = c1 - c0 + 1;
       constexpr int PER = 2 * CB, WIDE = CB * 64, GROUP = 32;
       struct Row { float v[PER], top, l; };
-      auto part = [&](int cta) { return g.w.partial + ((size_t)cta * 2 + (cta == c0 ? 1 : 0)) * L::PARTIAL; };     // (its last piece, or its first)
+      auto part = [&](int cta) { return g.w.partial + (cta * 2 + (cta == c0 ? 1 : 0)) * L::PARTIAL; };     // (its last piece, or its first)
       auto base_of = [](float top) { return top == -INFINITY ? 0.0f : top; };
       // a row of all of the warps that had its block
       auto row_here = [&](int r) {
