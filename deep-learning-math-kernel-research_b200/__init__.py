@@ -728,13 +728,13 @@ class Rotary(_Op):
 
 class _Cache:
     """What a plan wants of a cache's tensor: [pages, kv_heads, page_size, head_dim], the middle two in either order, as its strides say."""
-    __slots__ = ("type", "shape", "strides", "middle", "device", "dtype", "dense")
+    __slots__ = ("type", "shape", "strides", "device", "dtype", "dense", "seen")
 
     def __init__(self, type, kv_heads, page_size, head_dim, ld_page, ld_head, ld_token, device):
         token = ld_token or head_dim
         head = ld_head or page_size * token
         page = ld_page or (kv_heads * head if head > token else page_size * token)
-        self.type, self.device, self.dtype = type, device, None
+        self.type, self.device, self.dtype, self.seen = type, device, None, None         # seen: the last whole shape that has been found right
         self.shape, self.strides = (kv_heads, page_size, head_dim), (page, head, token, 1)
         self.dense = self.strides == (kv_heads * page_size * head_dim, page_size * head_dim, head_dim, 1)
 
@@ -744,9 +744,10 @@ class _Cache:
             if pages is None:
                 raise ValueError(f"{what}: pages are wanted beside an address")
             return x, pages
-        shape = tuple(x.shape)
-        if not (self.dense and x.dtype is self.dtype and shape[1:] == self.shape and x.is_contiguous()):
-            self.check(x, what, shape)
+        shape = x.shape
+        if not (shape == self.seen and x.dtype is self.dtype and x.is_contiguous()):
+            self.check(x, what, tuple(shape))
+            self.seen = shape if self.dense and x.is_contiguous() and tuple(shape[1:]) == self.shape else None
         if x.get_device() != self.device:
             raise ValueError(f"{what}: the plan's enqueue calls take tensors of device {self.device}")
         if pages is None:
@@ -809,13 +810,13 @@ class _OverSequences(_Op):
     def _batch(self, table, lengths, starts, seqs, width):
         """(table, lengths, starts, width)"""
         if table is not None and type(table) is not int:
-            shape = tuple(table.shape)
+            shape = table.shape
             if len(shape) != 2 or shape[0] < seqs:
-                raise ValueError(f"table: {seqs} rows of pages are wanted, got {shape}")
+                raise ValueError(f"table: {seqs} rows of pages are wanted, got {tuple(shape)}")
             if width is None:
                 width = shape[1]
             elif width != shape[1]:
-                raise ValueError(f"table: rows of {width} pages are wanted, got {shape}")
+                raise ValueError(f"table: rows of {width} pages are wanted, got {tuple(shape)}")
         if width is None:
             raise ValueError("table: width is wanted beside an address")
         return _flat(table, seqs * width, self._table), _flat(lengths, seqs, self._lengths), _flat(starts, seqs + 1, self._starts), width
