@@ -99,7 +99,7 @@ int check_sequences(Sequences &b, const int32_t *table, const int32_t *lengths, 
   b.rows = rows; b.seqs = seqs; b.width = width; b.pages = pages;
   b.each = starts || seqs == 0 ? 0 : (int)(rows / seqs);
   const int64_t capacity = page_size ? width * page_size : width;
-  b.capacity = (int)(capacity < INT32_MAX ? capacity : INT32_MAX);
+  b.capacity = (int)(capacity < INT32_MAX - 255 ? capacity : INT32_MAX - 255);     // (a tile's end is a number too)
   return ELB_OK;
 }
 

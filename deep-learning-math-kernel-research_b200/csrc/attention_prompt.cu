@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prompt_kernel(const __gr
     const int i = (warp - 4) >> 2, r = (warp & 3) * 32 + lane, in_tile = r / group, token = row0 + i * g.tokens + in_tile, end = i ? n1 : n0, tiles = end - t0;
     const bool mine = in_tile < g.tokens && token < n;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16, s_at = tmem + lanes + S_COL + i * TILE, o_at = tmem + lanes + O_COL + i * CB * 64;
-    const float c = fabsf(p.scale) * 1.4426950408889634f, slack = SLACK / c;
+    const float c = fabsf(p.scale) * 1.4426950408889634f, slack = fminf(SLACK / c, 3e38f);
     const int seen = p.causal ? min(length, length - n + token + 1) : length;
     float m = -INFINITY, l = 0.0f;
     uint32_t parity = 0;
@@ -402,10 +402,13 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prompt_kernel(const __gr
     tc_fence_after_sync();
     T *out = static_cast<T *>(p.out) + (long long)(block.q.first + token) * p.ld_out + (long long)(head * group + r - in_tile * group) * p.head_dim;
     const uint32_t rows_here = __ballot_sync(0xFFFFFFFFu, mine);
+    float finite = 0.0f;                                        // 0 while the row's results are
     // A row per thread would make 32 lines of each store: 64 channels of a warp's rows go through the place of its queries, which nothing reads any more, 16-byte word x
     // of row y at x ^ (y & 7), and on to memory eight lanes to a row.
     uint4 *stage = reinterpret_cast<uint4 *>(smem + i * L::Q_BYTES + (warp & 3) * 32 * 128);
     auto write = [&](const float (&v)[32], int q, float inv) {
+#pragma unroll
+      for (int k = 0; k < 32; ++k) finite = fmaf(v[k], 0.0f, finite);
 #pragma unroll
       for (int k = 0; k < 4; ++k)
         stage[lane * 8 + (((q & 1) * 4 + k) ^ (lane & 7))] =
@@ -483,6 +486,13 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prompt_kernel(const __gr
             }
             write(v, q, inv);
           }
+        }
+      }
+      // A value that is not finite, of a token that a row does not see and others do, has been multiplied by 0: such rows are worked out again without it
+      if (p.causal) {
+        for (uint32_t again = __ballot_sync(0xFFFFFFFFu, mine && finite != 0.0f); again != 0; again &= again - 1) {
+          const int y = __ffs(again) - 1, row = block.q.first + __shfl_sync(0xFFFFFFFFu, token, y);
+          attend_row<T, CB * 2>(p, block.s, block.q, row, head * group + __shfl_sync(0xFFFFFFFFu, r - in_tile * group, y), lane);
         }
       }
     }

@@ -69,13 +69,15 @@ template <> __device__ __forceinline__ void mma16816<__half>(float (&c)[4], cons
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// The call's tiles lie in order: sequences, their key heads, their tiles (one at least, so that every row is written).
+// A key head's tiles: one at least, so that every row is written, and no more for sequences without new tokens
+__device__ __forceinline__ int tiles_of(const KeyTiles<TILE> &kt, const Sequence &q) { return q.n > 0 ? max(1, kt.count(q.length)) : 1; }
+// The call's tiles lie in order: sequences, their key heads, their tiles.
 // Their deal and where this CTA starts, from the sequences' lengths, by a warp.
 struct Start { Sequence q; long long base; int s; };
 __device__ __forceinline__ Deal find_start(const AttentionParams &p, int cta, Start &start) {
   const KeyTiles<TILE> kt(p.page_size);
   const int lane = threadIdx.x & 31, per = (int)((p.seq.seqs + 31) / 32), s0 = lane * per, s1 = (int)min((long long)s0 + per, p.seq.seqs);
-  auto tiles = [&](const Sequence &q) { return (long long)max(1, kt.count(q.length)) * p.kv_heads; };
+  auto tiles = [&](const Sequence &q) { return (long long)tiles_of(kt, q) * p.kv_heads; };
   Sequence q = {0, 0, 0};
   long long sum = 0;
   if (per == 1) {
@@ -119,7 +121,7 @@ struct Walk {
   Sequence q;
   int s, head, tiles, t;
   __device__ __forceinline__ Walk(const AttentionParams &p, long long at, const Start &start) : p(p), kt(p.page_size), q(start.q), s(start.s) {
-    tiles = max(1, kt.count(q.length));
+    tiles = tiles_of(kt, q);
     head = (int)quotient(at - start.base, tiles);
     t = (int)(at - start.base - (long long)head * tiles);
   }
@@ -129,7 +131,7 @@ struct Walk {
     if (++head < p.kv_heads) return;
     head = 0;
     q = sequence_of(p.seq, ++s);
-    tiles = max(1, kt.count(q.length));
+    tiles = tiles_of(kt, q);
   }
 };
 
@@ -490,6 +492,14 @@ __global__ void __launch_bounds__(THREADS, Smem<CB, MB>::CTAS) attention_token_k
         const float inv = x.l == 0.0f ? 0.0f : 1.0f / x.l;
         const int token = r / group, ch = lane * PER;
         T *out = static_cast<T *>(p.out) + (long long)(walk.q.first + token) * p.ld_out + (long long)(walk.head * group + r - token * group) * p.head_dim + ch;
+        // A value that is not finite, of a token that this row does not see and another does, has been multiplied by 0: such a row is worked out again without it
+        float all = 0.0f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) all = fmaf(x.v[i], 0.0f, all);
+        if (p.causal && walk.q.n > 1 && __any_sync(0xFFFFFFFFu, all != 0.0f)) {
+          attend_row<T, CB * 2>(p, walk.s, walk.q, walk.q.first + token, walk.head * group + r - token * group, lane);
+          return;
+        }
         if (ch >= p.head_dim) return;
         if constexpr (CB == 2) *reinterpret_cast<uint2 *>(out) = make_uint2(pack2<T>(x.v[0] * inv, x.v[1] * inv), pack2<T>(x.v[2] * inv, x.v[3] * inv));
         else *reinterpret_cast<uint32_t *>(out) = pack2<T>(x.v[0] * inv, x.v[1] * inv);

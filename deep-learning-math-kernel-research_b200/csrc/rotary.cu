@@ -39,12 +39,12 @@ __global__ void __launch_bounds__(WARPS * 32, 4) rotary_kernel(const RotaryParam
       const int s = sequence_of_row(p.seq, (int)row, lane);
       if (s >= 0 && s < p.seq.seqs) {
         const Sequence q = sequence_of(p.seq, s);
-        position = q.length - q.n + ((int)row - q.first);
+        position = max(p.seq.lengths[s], 0) - q.n + ((int)row - q.first);     // (a length past the table is none that it can hold: no place)
         int page = -1, offset = 0;
         if (position >= 0 && (int)row < q.first + q.n) {
           const int i = position / p.page_size;
           offset = position - i * p.page_size;
-          page = p.seq.table[s * p.seq.width + i];
+          if (i < p.seq.width) page = p.seq.table[s * p.seq.width + i];
         }
         if (page >= 0 && page < p.seq.pages) at = page * p.ld_page + offset * p.ld_token;
         else if (lane == 0) report_status(p.status, ST_BAD_PAGE);
