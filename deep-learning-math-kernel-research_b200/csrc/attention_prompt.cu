@@ -408,7 +408,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prompt_kernel(const __gr
     uint4 *stage = reinterpret_cast<uint4 *>(smem + i * L::Q_BYTES + (warp & 3) * 32 * 128);
     auto write = [&](const float (&v)[32], int q, float inv) {
 #pragma unroll
-      for (int k = 0; k < 32; ++k) finite = fmaf(v[k], 0.0f, finite);
+      for (int k = 0; k < 32; ++k)
+        if (q * 32 + (k & ~7) < p.head_dim) finite = fmaf(v[k], 0.0f, finite);        // (no product has written the columns behind)
 #pragma unroll
       for (int k = 0; k < 4; ++k)
         stage[lane * 8 + (((q & 1) * 4 + k) ^ (lane & 7))] =

@@ -157,6 +157,24 @@ def test_plans_and_graphs_beside_one_another(new):
     assert all(torch.equal(r, out) for r in results) and all(c[0].device_status() == 0 for c in cases)
 
 
+@pytest.mark.parametrize("d", [96, 104, 56])
+def test_what_lay_in_tensor_memory_does_not_matter(d):
+    """Calls behind ones whose results are NaN in all of their channels give the bits that they give behind others."""
+    b = A.batch([200] * 3, [700, 900, 800], 16)
+    before, q0, k0, v0, _ = paged(b, 8, 2, 128 if d > 64 else 64)
+    plan, q, k, v, _ = paged(b, 8, 2, d, seed=9)
+    outs, rest = [A.poisoned(b.rows, 8, d, dt=E.bf16) for _ in range(2)], torch.empty_like(q0)
+    torch.cuda.synchronize()
+    for out in outs:
+        for _ in range(3):
+            run(before, b, rest, q0, k0, v0)
+        run(plan, b, out, q, k, v)
+        torch.cuda.synchronize()
+        q0.fill_(A.NAN)
+    assert bool(rest.isnan().all()) and torch.equal(*outs)
+    assert plan.device_status() == before.device_status() == 0
+
+
 def test_refused_calls():
     """Arguments that a call refuses, with the code and a word of the message; nothing is written."""
     b = A.batch([1, 1], [20, 20], 16)
