@@ -10,6 +10,7 @@
 // Products are mma.sync m16n8k16: 16 rows are the least a matrix instruction takes, and at HBM's rate (23 bytes per SM and cycle) one of them is wanted
 // every 22 cycles, far below what it can do; tcgen05 would pad 128 rows and bring each score through tensor memory.
 #include <cmath>
+#include <type_traits>
 
 #include "attention.cuh"
 #include "elb_common.cuh"
@@ -427,47 +428,63 @@ __global__ void __launch_bounds__(THREADS, Smem<CB, MB>::CTAS) attention_token_k
         }
         return x;
       };
-      // a row of n CTAs' results, in their order
-      auto row_of = [&](int r, auto cta_of, int n) {
-        Row x;
-        x.top = -INFINITY;
-        x.l = 0.0f;
+      // Rows of n CTAs' results, in their order.  R rows of a warp at once, WARPS apart (where there are as many, otherwise the first again): each is little work
+      // behind two round trips to L2.
+      auto nth = [&](int r, int a) { return r + a * WARPS < rows ? r + a * WARPS : r; };
+      auto rows_of = [&](auto &x, int r, auto cta_of, int n) {
+        constexpr int R = sizeof(x) / sizeof(Row);
 #pragma unroll
-        for (int i = 0; i < PER; ++i) x.v[i] = 0.0f;
+        for (int a = 0; a < R; ++a) {
+          x[a].top = -INFINITY;
+          x[a].l = 0.0f;
+#pragma unroll
+          for (int i = 0; i < PER; ++i) x[a].v[i] = 0.0f;
+        }
 #pragma unroll 1
         for (int k0 = 0; k0 < n; k0 += 32) {                    // a lane looks at one maximum and sum
           const int here = min(32, n - k0);
-          const float2 y = lane < here ? __ldcg(reinterpret_cast<const float2 *>(part(cta_of(k0 + lane)) + MB * 16 * WIDE) + r) : make_float2(-INFINITY, 0.0f);
-          float top = fmaxf(x.top, y.x);
+          float2 y[R];
+          float weight[R];
 #pragma unroll
-          for (int b = 16; b > 0; b >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, b));
-          const float keep = exp2_approx(x.top - base_of(top)), weight = exp2_approx(y.x - base_of(top));
-          float sum = y.y * weight;
+          for (int a = 0; a < R; ++a)
+            y[a] = lane < here ? __ldcg(reinterpret_cast<const float2 *>(part(cta_of(k0 + lane)) + MB * 16 * WIDE) + nth(r, a)) : make_float2(-INFINITY, 0.0f);
 #pragma unroll
-          for (int b = 16; b > 0; b >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, b);
-          x.top = top;
-          x.l = x.l * keep + sum;
+          for (int a = 0; a < R; ++a) {
+            float top = fmaxf(x[a].top, y[a].x);
 #pragma unroll
-          for (int i = 0; i < PER; ++i) x.v[i] *= keep;
-          constexpr int BATCH = 16;                             // results on their way at once
+            for (int b = 16; b > 0; b >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, b));
+            const float keep = exp2_approx(x[a].top - base_of(top));
+            weight[a] = exp2_approx(y[a].x - base_of(top));
+            float sum = y[a].y * weight[a];
+#pragma unroll
+            for (int b = 16; b > 0; b >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, b);
+            x[a].top = top;
+            x[a].l = x[a].l * keep + sum;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) x[a].v[i] *= keep;
+          }
+          constexpr int BATCH = 16 / R;                         // results on their way at once, of each row
 #pragma unroll 1
           for (int k = 0; k < here; k += BATCH) {
-            float z[BATCH][PER];
+            float z[R][BATCH][PER];
 #pragma unroll
-            for (int j = 0; j < BATCH; ++j) {
-              const float *src = part(cta_of(k0 + min(k + j, here - 1))) + r * WIDE + lane * PER;
-              if constexpr (CB == 2) *reinterpret_cast<float4 *>(z[j]) = __ldcg(reinterpret_cast<const float4 *>(src));
-              else *reinterpret_cast<float2 *>(z[j]) = __ldcg(reinterpret_cast<const float2 *>(src));
-            }
+            for (int j = 0; j < BATCH; ++j)
 #pragma unroll
-            for (int j = 0; j < BATCH; ++j) {
-              const float w = k + j < here ? __shfl_sync(0xFFFFFFFFu, weight, k + j) : 0.0f;
+              for (int a = 0; a < R; ++a) {
+                const float *src = part(cta_of(k0 + min(k + j, here - 1))) + nth(r, a) * WIDE + lane * PER;
+                if constexpr (CB == 2) *reinterpret_cast<float4 *>(z[a][j]) = __ldcg(reinterpret_cast<const float4 *>(src));
+                else *reinterpret_cast<float2 *>(z[a][j]) = __ldcg(reinterpret_cast<const float2 *>(src));
+              }
 #pragma unroll
-              for (int i = 0; i < PER; ++i) x.v[i] += k + j < here ? z[j][i] * w : 0.0f;
-            }
+            for (int j = 0; j < BATCH; ++j)
+#pragma unroll
+              for (int a = 0; a < R; ++a) {
+                const float w = k + j < here ? __shfl_sync(0xFFFFFFFFu, weight[a], k + j) : 0.0f;
+#pragma unroll
+                for (int i = 0; i < PER; ++i) x[a].v[i] += k + j < here ? z[a][j][i] * w : 0.0f;
+              }
           }
         }
-        return x;
       };
       auto leave = [&](int cta, int r, const Row &x) {
         float *dst = part(cta);
@@ -506,29 +523,46 @@ __global__ void __launch_bounds__(THREADS, Smem<CB, MB>::CTAS) attention_token_k
       };
       // Piece of a whole item: out; otherwise to the workspace, where the last one there joins all of them.  Where more than two groups of CTAs share an
       // item, the last of each group joins that first, and the last of these the groups.
-      if (sharers == 1) {
+      auto finish = [&](auto of_warp) {
+        constexpr int R = decltype(of_warp)::value;
+        Row x[R];
 #pragma unroll 1
-        for (int r = warp; r < rows; r += WARPS) write(r, row_here(r));
-      } else {
-#pragma unroll 1
-        for (int r = warp; r < rows; r += WARPS) leave(blockIdx.x, r, row_here(r));
+        for (int r = warp; r < rows; r += R * WARPS) {
+#pragma unroll
+          for (int a = 0; a < R; ++a) x[a] = row_here(nth(r, a));
+#pragma unroll
+          for (int a = 0; a < R; ++a) leave(blockIdx.x, nth(r, a), x[a]);
+        }
         int *arrived = g.w.arrived + c0, n = sharers, stride = 1, at = c0;
-        bool last = true;
         if (sharers > 2 * GROUP) {
           const int begin = c0 + ((int)blockIdx.x - c0) / GROUP * GROUP, final = min(begin + GROUP - 1, c1);
-          last = last_of(g.w.arrived + gridDim.x + final, final - begin + 1);
-          if (last) {
+          if (!last_of(g.w.arrived + gridDim.x + final, final - begin + 1)) return;
 #pragma unroll 1
-            for (int r = warp; r < rows; r += WARPS) leave(final, r, row_of(r, [&](int k) { return begin + k; }, final - begin + 1));
+          for (int r = warp; r < rows; r += R * WARPS) {
+            rows_of(x, r, [&](int k) { return begin + k; }, final - begin + 1);
+#pragma unroll
+            for (int a = 0; a < R; ++a) leave(final, nth(r, a), x[a]);
           }
           n = (sharers + GROUP - 1) / GROUP;
           stride = GROUP;
           at = c0 + GROUP - 1;
         }
-        if (last && last_of(arrived, n)) {
+        if (!last_of(arrived, n)) return;
 #pragma unroll 1
-          for (int r = warp; r < rows; r += WARPS) write(r, row_of(r, [&](int k) { return min(at + k * stride, c1); }, n));
+        for (int r = warp; r < rows; r += R * WARPS) {
+          rows_of(x, r, [&](int k) { return min(at + k * stride, c1); }, n);
+#pragma unroll
+          for (int a = 0; a < R; ++a)
+            if (r + a * WARPS < rows) write(r + a * WARPS, x[a]);
         }
+      };
+      if (sharers == 1) {
+#pragma unroll 1
+        for (int r = warp; r < rows; r += WARPS) write(r, row_here(r));
+      } else if (rows <= WARPS) {
+        finish(std::integral_constant<int, 1>());
+      } else {
+        finish(std::integral_constant<int, 4>());
       }
       walk.t = t1;
       named_bar_sync(1, WARPS * 32);                            // the merge area may be written again
@@ -589,6 +623,9 @@ cudaError_t init_attention() {
   return e == cudaSuccess ? allow_all<__half>() : e;
 }
 
+// Up to 16 rows to a key head a warp's matrix instruction is as long whatever they are; with up to 32 two warps share a tile of keys.  (32 heads of 128 over 8, us
+// here / with the prompts' kernel: 1 x 1 token behind 4000 15/33, 64 x 1 175/219, 8 x 4 36/42, 8 x 8 43/42, 24 x 8 84/113, 64 x 8 196/221, 8 x 5 of 40 heads behind 1000 to
+// 7000 46/62; behind 1000, where that starts and joins sooner, 8 x 8 25/19, 64 x 8 69/78.)
 bool attention_token_takes(const AttentionParams &p) {
   return p.words && p.head_dim <= 128 && p.page_size % 8 == 0 && p.seq.width > 0 && p.seq.pages > 0 && most_rows(p) <= 32;
 }
