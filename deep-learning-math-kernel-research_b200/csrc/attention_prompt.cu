@@ -15,6 +15,7 @@
 // Measured and not taken (8192 tokens of 32 heads over 8, causal: 450 us so): two warpgroups a row tile 468 us; an issuer for each row tile 589; P handed over in
 // quarters 520, whole 462; 1 to 4 of 8 exponentials from a polynomial on the multiply-add pipe 453 to 500; a CTA per SM that goes over the blocks, the next one's
 // first scores beside the last one's results, 469, with tiles of keys dealt out evenly over the CTAs 478.
+// With 64 channels (377 us so): P beside the scores, so that the next ones wait for nothing, 381; a row tile a CTA, two CTAs an SM, 410.
 #include <cmath>
 
 #include "attention.cuh"

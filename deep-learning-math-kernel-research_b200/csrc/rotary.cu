@@ -126,7 +126,8 @@ __global__ void __launch_bounds__(WARPS * 32, 4) rotary_kernel(const RotaryParam
 
 template <typename T, int VEC, bool NEAR>
 cudaError_t go(const RotaryParams &p, cudaStream_t s) {
-  // A token per block is done sooner, a token per warp needs no barrier: the block's where it has the SMs to itself.
+  // A token per block is done sooner, a token per warp needs no barrier: the block's where it has the SMs to itself.  (32 + 8 heads of 128, us, block / warp: 64 rows
+  // 3.2/5.8, 200 4.0/5.8, 592 4.4/6.6, 1184 7.7/6.1, 2400 13.9/10.7, 4700 28/15.)
   const bool team = p.rows < 148 * WARPS;
   const dim3 grid((unsigned)(team ? p.rows : (p.rows + WARPS - 1) / WARPS));
   const size_t smem = (size_t)(team ? 1 : WARPS) * (p.rotary / 2) * sizeof(float2);

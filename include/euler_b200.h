@@ -510,7 +510,7 @@ ELB_API int elb_append_enqueue(elb_op_t *op, void *q_out, void *k_cache, void *v
  * dense (table NULL): k and v are [seqs][width][kv_heads][head_dim], page_size 0, lengths may be NULL (all `width` keys), `pages` is not used; ld_page
  * is then a sequence's.
  * Tensor cores run head_dim up to 128, multiples of 8, 16-byte aligned tensors with strides of multiples of 8 elements, pages of a multiple of 8 tokens, up
- * to 128 heads that share a key head; everything else runs on CUDA cores, many times slower. */
+ * to 128 heads that share a key head; everything else runs on CUDA cores, many times slower.  A plan holds 20 MB for partial results. */
 typedef struct elb_attention_desc {
   int32_t heads, kv_heads, head_dim;              /* kv_heads divides heads; head_dim 1 .. 256 */
   int32_t dt;                                     /* ELB_BF16 or ELB_F16 */
@@ -527,7 +527,7 @@ ELB_API int elb_attention_enqueue(elb_op_t *op, void *output, const void *input,
                                   void *cuda_stream);
 
 /* 0 = every finished call of the plan was well; otherwise the code of the bounded wait that gave up (see
- * elb_conv_device_status).  Waits for the device; -1: it could not. */
+ * elb_conv_device_status), or 105: a table named a page outside the pool, or a token has no place.  Waits for the device; -1: it could not. */
 ELB_API int elb_op_device_status(elb_op_t *op);
 ELB_API int elb_op_device(const elb_op_t *op);                 /* the CUDA device ordinal whose tensors enqueue takes */
 ELB_API uint64_t elb_op_launch_count(const elb_op_t *op);
