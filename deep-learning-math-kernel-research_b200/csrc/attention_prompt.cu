@@ -472,6 +472,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prompt_kernel(const __gr
             whole += x.y * exp2_approx(x.x - from);
           }
           const float inv = whole == 0.0f ? 0.0f : 1.0f / whole;
+          l = whole;
 #pragma unroll 1
           for (int q = 0; q < 2 * CB; ++q) {
             float v[32];
@@ -490,9 +491,10 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prompt_kernel(const __gr
           }
         }
       }
-      // A value that is not finite, of a token that a row does not see and others do, has been multiplied by 0: such rows are worked out again without it
+      // A value that is not finite, of a token that a row does not see and others do, has been multiplied by 0: such rows are worked out again without it.  (Where the
+      // sum is not finite either, what the row sees is not.)
       if (p.causal) {
-        for (uint32_t again = __ballot_sync(0xFFFFFFFFu, mine && finite != 0.0f); again != 0; again &= again - 1) {
+        for (uint32_t again = __ballot_sync(0xFFFFFFFFu, mine && finite != 0.0f && l - l == 0.0f); again != 0; again &= again - 1) {
           const int y = __ffs(again) - 1, row = block.q.first + __shfl_sync(0xFFFFFFFFu, token, y);
           attend_row<T, CB * 2>(p, block.s, block.q, row, head * group + __shfl_sync(0xFFFFFFFFu, r - in_tile * group, y), lane);
         }

@@ -512,11 +512,12 @@ __global__ void __launch_bounds__(THREADS, Smem<CB, MB>::CTAS) attention_token_k
         const float inv = x.l == 0.0f ? 0.0f : 1.0f / x.l;
         const int token = r / group, ch = lane * PER;
         T *out = static_cast<T *>(p.out) + (long long)(walk.q.first + token) * p.ld_out + (long long)(walk.head * group + r - token * group) * p.head_dim + ch;
-        // A value that is not finite, of a token that this row does not see and another does, has been multiplied by 0: such a row is worked out again without it
+        // A value that is not finite, of a token that this row does not see and another does, has been multiplied by 0: such a row is worked out again without it.  (Where
+        // the sum is not finite either, what the row sees is not.)
         float all = 0.0f;
 #pragma unroll
         for (int i = 0; i < PER; ++i) all = fmaf(x.v[i], 0.0f, all);
-        if (p.causal && walk.q.n > 1 && __any_sync(0xFFFFFFFFu, all != 0.0f)) {
+        if (p.causal && walk.q.n > 1 && x.l - x.l == 0.0f && __any_sync(0xFFFFFFFFu, all != 0.0f)) {
           attend_row<T, CB * 2>(p, walk.s, walk.q, walk.q.first + token, walk.head * group + r - token * group, lane);
           return;
         }
