@@ -38,9 +38,12 @@ int make_steps(elb_op &op, const elb_rotary_desc_t &d, const float *frequencies)
   const int n = d.rotary_dim / 2;
   unsigned long long steps[512];
   float given[512];
-  if (frequencies) {
+  if (frequencies && n > 0) {
     if (!aligned(frequencies, 4)) return op_fail(ELB_GENERAL_ERROR, "misaligned frequencies");
-    OP_TRY(cudaMemcpy(given, frequencies, n * sizeof(float), cudaMemcpyDefault));
+    Staged st;                                                 // (waits for another device's work)
+    const int rc = st.take(op, frequencies, n * sizeof(float));
+    if (rc != ELB_OK) return rc;
+    OP_TRY(cudaMemcpy(given, st.p, n * sizeof(float), cudaMemcpyDefault));
   }
   const double two_pi = 6.283185307179586476925;
   for (int i = 0; i < n; ++i) {
@@ -62,6 +65,7 @@ int make_steps(elb_op &op, const elb_rotary_desc_t &d, const float *frequencies)
   if (rc != ELB_OK) return rc;
   op.w[0] = dst;
   OP_TRY(cudaMemcpy(dst, steps, n * sizeof(unsigned long long), cudaMemcpyHostToDevice));
+  OP_TRY(cudaDeviceSynchronize());                             // (that copy returns when it has read its source; streams that wait for no other come next)
   return ELB_OK;
 }
 
