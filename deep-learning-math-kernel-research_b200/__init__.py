@@ -776,7 +776,7 @@ def _heads(x, spec, rows, device):
         return x
     if x.dtype is spec.dtype and x.is_contiguous() and x.nbytes >= rows * spec.row_bytes and x.get_device() == spec.device:
         return x.data_ptr()
-    if len(x.shape) == 3 and x.shape[2] != spec.n and not x.is_contiguous():
+    if len(x.shape) == 3 and x.shape[2] != spec.n and (spec.ld != spec.n or not x.is_contiguous()):        # (one row is contiguous wherever the next would lie)
         (held, heads, dim), (row, head, one) = x.shape, x.stride()
         if not (heads * dim == spec.n and held >= rows and (held == 1 or row == spec.ld) and (heads == 1 or head == dim) and (dim == 1 or one == 1)) or \
                 str(x.dtype).replace("torch.", "") != _DTYPE_NAMES[spec.type]:
