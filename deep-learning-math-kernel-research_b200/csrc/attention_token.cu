@@ -30,7 +30,7 @@ constexpr int BOX_BYTES = TILE * 128;                           // the keys of a
 template <int CB, int MB>
 struct Smem {
   static constexpr int CTAS = CB == 1 ? 3 : 2;                  // per SM (64 channels with 2: 24 x 1 token of 12 heads 29 -> 31.5 us, 64 x 1 of 16 140 -> 155)
-  static constexpr int REGS = CB == 1 ? 120 : 208, REGS_PRODUCER = 40;      // of threads, of (80 or 128) * 256 that a CTA has
+  static constexpr int REGS = CB == 1 ? 112 : 208, REGS_PRODUCER = CB == 1 ? 48 : 40;      // of threads, of (80 or 128) * 256 that a CTA has (no spills; 120 and 40: a producer's)
   static constexpr int TURNS = WARPS / MB, NB = CB * 8;
   static constexpr int STAGE = 2 * CB * BOX_BYTES;
   // A multiple of the turns, also of the producers: the same warps then come back to a stage, and see each of its phases.  (One bit of parity does not tell a stage that has
