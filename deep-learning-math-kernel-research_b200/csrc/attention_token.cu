@@ -363,6 +363,9 @@ __global__ void __launch_bounds__(THREADS, Smem<CB, MB>::CTAS) attention_token_k
           mma16816<T>(o[n], pf[1], v1[0], v1[1]);
           mma16816<T>(o[n + 1], pf[1], v1[2], v1[3]);
         }
+        // The next tile's copy, of the other proxy, comes behind the last read of this one.  (Without the fence some of the values' ldmatrix were found behind the arrival: in two
+        // calls of 100 of 64 x 1 tokens behind 500 to 16000 a few of a tile's values were those of the tile that comes to the same stage next.)
+        fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[stage]);
       }
