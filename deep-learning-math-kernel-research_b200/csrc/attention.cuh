@@ -1,5 +1,7 @@
 // Parameter blocks and launchers of the attention operators (elb_rotary_*, elb_append_*, elb_attention_*).
 #pragma once
+#include <type_traits>
+
 #include "elb_common.cuh"
 #include "ops.cuh"
 
@@ -87,6 +89,13 @@ struct AttentionParams {
   int *status;
 };
 
+// Where key j of sequence s lies in k and v (of key head 0); -1: in a page outside the pool
+__device__ __forceinline__ long long place_of_key(const AttentionParams &p, int s, int j) {
+  if (!p.page_size) return s * p.ld_page + j * p.ld_token;
+  const int page = p.seq.table[s * p.seq.width + j / p.page_size];
+  return page >= 0 && page < p.seq.pages ? page * p.ld_page + j % p.page_size * p.ld_token : -1;
+}
+
 // One head of one row by a warp, lanes the channels, in fp32 on CUDA cores: with the running maximum m and sum l of the softmax and
 // m' = max(m, s), l = l e^(m - m') + e^(s - m') and the same for the weighted sum of values.
 // CHUNKS: of 32 channels
@@ -103,16 +112,9 @@ __device__ __forceinline__ void attend_row(const AttentionParams &p, int s, cons
   }
 #pragma unroll 1
   for (int j = 0; j < keys; ++j) {
-    long long at;
-    bool there = true;
-    if (p.page_size) {
-      const int page = p.seq.table[s * p.seq.width + j / p.page_size];
-      there = page >= 0 && page < p.seq.pages;
-      if (!there && lane == 0) report_status(p.status, ST_BAD_PAGE);
-      at = page * p.ld_page + j % p.page_size * p.ld_token + head;
-    } else {
-      at = s * p.ld_page + j * p.ld_token + head;
-    }
+    const long long place = place_of_key(p, s, j), at = place + head;
+    const bool there = place >= 0;
+    if (!there && lane == 0) report_status(p.status, ST_BAD_PAGE);
     const T *k = static_cast<const T *>(p.k) + at, *v = static_cast<const T *>(p.v) + at;
     float z = 0.0f;
 #pragma unroll
@@ -133,6 +135,42 @@ __device__ __forceinline__ void attend_row(const AttentionParams &p, int s, cons
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c)
     if (lane + 32 * c < p.head_dim) out[lane + 32 * c] = from_f32<T>(o[c] * r);
+}
+
+// Values that are not finite, of keys that only some of a tile's rows see: 0, the term of a row that does not see them, times that would not be 0.  The products take
+// 0 in their place, and the rows that see them add them when they are done.
+// Here a warp looks at rows [from, to) of a tile as copies have brought it, CB boxes of 64 channels (UNROLL words of each at once).  Where there are such values it clears
+// them: true.
+template <typename T, int CB, int BOX_BYTES, int UNROLL>
+__device__ __forceinline__ bool clear_not_finite(uint8_t *tile, int from, int to) {
+  constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
+  constexpr uint32_t EXPONENTS = BF ? 0x7F807F80u : 0x7C007C00u;
+  const int begin = from * 8 + (threadIdx.x & 31), end = to * 8;
+  uint32_t zeros[4] = {0, 0, 0, 0};                             // a value times 0, not 0 where it is not finite
+  auto times_zero = [](uint32_t &sum, uint32_t w) {
+    if (BF) asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum) : "r"(w), "r"(0));
+    else asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(sum) : "r"(w), "r"(0));
+  };
+#pragma unroll UNROLL
+  for (int j = begin; j < end; j += 32)
+#pragma unroll
+    for (int c = 0; c < CB; ++c) {
+      const uint4 x = reinterpret_cast<const uint4 *>(tile + c * BOX_BYTES)[j];
+      times_zero(zeros[0], x.x);
+      times_zero(zeros[1], x.y);
+      times_zero(zeros[2], x.z);
+      times_zero(zeros[3], x.w);
+    }
+  if (!__any_sync(0xFFFFFFFFu, ((zeros[0] | zeros[1] | zeros[2] | zeros[3]) & 0x7FFF7FFFu) != 0)) return false;
+  auto cleared = [](uint32_t w) { return w & ~__vcmpeq2(w & EXPONENTS, EXPONENTS); };
+#pragma unroll 1
+  for (int j = begin; j < end; j += 32)
+#pragma unroll 1
+    for (int c = 0; c < CB; ++c) {
+      uint4 &x = reinterpret_cast<uint4 *>(tile + c * BOX_BYTES)[j];
+      x = make_uint4(cleared(x.x), cleared(x.y), cleared(x.z), cleared(x.w));
+    }
+  return true;
 }
 
 // Keys in tiles of up to TILE rows, as tiled copies bring them: whole pages where some fit, otherwise (and dense) parts of a page.

@@ -30,7 +30,7 @@ constexpr int BOX_BYTES = TILE * 128;                           // the keys of a
 template <int CB, int MB>
 struct Smem {
   static constexpr int CTAS = CB == 1 ? 3 : 2;                  // per SM (64 channels with 2: 24 x 1 token of 12 heads 29 -> 31.5 us, 64 x 1 of 16 140 -> 155)
-  static constexpr int REGS = CB == 1 ? 112 : 208, REGS_PRODUCER = CB == 1 ? 48 : 40;      // of threads, of (80 or 128) * 256 that a CTA has (no spills; 120 and 40: a producer's)
+  static constexpr int REGS = CB == 1 ? 112 : 208, REGS_PRODUCER = 48;      // of threads, together the (80 or 128) * 256 that a CTA has
   static constexpr int TURNS = WARPS / MB, NB = CB * 8;
   static constexpr int STAGE = 2 * CB * BOX_BYTES;
   // A multiple of the turns, also of the producers: the same warps then come back to a stage, and see each of its phases.  (One bit of parity does not tell a stage that has
@@ -43,9 +43,13 @@ struct Smem {
   static constexpr int COPIES = MB > 1 ? 1 : WARPS;             // results of a block that lie there at the end; two blocks: a warp's, joined with its partner's
   static constexpr int MERGE = COPIES * MB * 16 * PITCH * 4;
   static constexpr int ML_OFF = MERGE_OFF + MERGE;              // maxima and sums, [WARPS][16]
-  static constexpr int BAR_OFF = ML_OFF + WARPS * 16 * 8;       // full[S], empty[S], qfull[2]
-  static constexpr int MISC_OFF = BAR_OFF + (2 * STAGES + 2) * 8;
-  static constexpr int TOTAL = MISC_OFF + 16 + 1024;           // (room to align)
+  static constexpr int BAR_OFF = ML_OFF + WARPS * 16 * 8;       // full[S], empty[S], landed[S], qfull[2]
+  static constexpr int MISC_OFF = BAR_OFF + (3 * STAGES + 2) * 8;
+  // The pieces in whose values some were cleared, each at its number modulo SPOILT (copies are a ring of tiles ahead, and a piece has one at least), as the number's lower
+  // bits and 1.  (A piece that is taken for another has none to add.)
+  static constexpr int SPOILT = 8, PIECE_BITS = 0x7FFF;
+  static_assert(SPOILT > STAGES, "");
+  static constexpr int TOTAL = MISC_OFF + 8 + SPOILT * 4 + 1024;       // (room to align)
   static constexpr int PARTIAL = MB * 16 * (CB * 64 + 2);       // floats of a partial result: rows, then their maxima and sums
   static_assert(CTAS * (TOTAL + 1024) <= 228 * 1024, "");
 };
@@ -145,20 +149,22 @@ __global__ void __launch_bounds__(THREADS, Smem<CB, MB>::CTAS) attention_token_k
   constexpr int STAGES = L::STAGES, NB = L::NB;                 // NB: blocks of 8 channels
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::BAR_OFF), *empty = full + STAGES, *qfull = empty + STAGES;
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::BAR_OFF), *empty = full + STAGES, *landed = empty + STAGES, *qfull = landed + STAGES;
   volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::MISC_OFF);
   int *verdict = reinterpret_cast<int *>(smem + L::MISC_OFF + 4);
+  volatile int *spoilt = reinterpret_cast<volatile int *>(smem + L::MISC_OFF + 8);
   const AttentionParams &p = g.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = p.heads / p.kv_heads;
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&g.kmap);
     tma_prefetch_desc(&g.vmap);
     tma_prefetch_desc(&g.qmap);
-    for (int i = 0; i < STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], MB); }
+    for (int i = 0; i < STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], MB); mbar_init(&landed[i], 1); }
     for (int i = 0; i < 2; ++i) mbar_init(&qfull[i], 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
+  if (threadIdx.x >= 32 && threadIdx.x < 32 + L::SPOILT) spoilt[threadIdx.x - 32] = 0;
   // rows of queries that no copy fills
   for (int i = threadIdx.x; i < 2 * L::Q_BYTES / 16; i += THREADS) reinterpret_cast<uint4 *>(smem + L::Q_OFF)[i] = make_uint4(0, 0, 0, 0);
   fence_proxy_async_smem();
@@ -183,10 +189,16 @@ __global__ void __launch_bounds__(THREADS, Smem<CB, MB>::CTAS) attention_token_k
     uint8_t *dst = smem + which * BOX_BYTES + page_in_tile * kt.page * 128;
     // What this lane copies for a tile.  Tables are read a tile ahead and looked at when the copies are issued.
     constexpr int AHEAD = 2;
-    struct { int page, token, head; } next[AHEAD];
+    struct { int page, token, head, look; } next[AHEAD];
+    int piece = 0;
     auto read = [&](int j) {
-      while (walk.t >= walk.tiles) walk.wrap();
+      for (; walk.t >= walk.tiles; ++piece) walk.wrap();
       next[j].head = walk.head;
+      next[j].look = 0;                                         // or the tile's rows that some of the new tokens do not see, [lowest byte, the next) of a piece
+      if (p.causal && walk.q.n > 1) {
+        const int from = max(walk.q.length - walk.q.n + 1 - kt.first(walk.t), 0), to = kt.held(walk.t, walk.q.length);
+        if (from < to) next[j].look = from | to << 8 | (piece & L::PIECE_BITS) << 16;
+      }
       next[j].token = 0;
       next[j].page = (int)p.seq.pages;                          // one outside the map: zeros
       if (!kt.page) {
@@ -210,13 +222,16 @@ __global__ void __launch_bounds__(THREADS, Smem<CB, MB>::CTAS) attention_token_k
     for (int j = 0; j < AHEAD; ++j)
       if (i + j * PRODUCERS < tiles) read(j);
     bool ok = true;
+    uint32_t landed_phase = 0;
     while (i < tiles && ok) {
 #pragma unroll
       for (int j = 0; j < AHEAD; ++j) {
         if (i >= tiles || !ok) break;
         const int stage = i % STAGES;
         if (!mbar_poll_warp(&empty[stage], ((i / STAGES) & 1) ^ 1, abort_flag)) { ok = false; break; }
-        if (lane == 0) mbar_arrive_expect_tx(&full[stage], bytes);
+        const int look = next[j].look;
+        uint64_t *bar = look != 0 ? &landed[stage] : &full[stage];
+        if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
         __syncwarp();
         if (mine) {
           int page = next[j].page;
@@ -224,7 +239,16 @@ __global__ void __launch_bounds__(THREADS, Smem<CB, MB>::CTAS) attention_token_k
             if (next[j].token >= 0) report_status(p.status, ST_BAD_PAGE);
             page = (int)p.seq.pages;
           }
-          tma_tile_4d(dst + stage * L::STAGE, map, cb * 64, max(next[j].token, 0), next[j].head, page, &full[stage]);
+          tma_tile_4d(dst + stage * L::STAGE, map, cb * 64, max(next[j].token, 0), next[j].head, page, bar);
+        }
+        if (look != 0) {                                        // their values are looked at before the tile is handed on
+          ok = mbar_poll_warp(bar, landed_phase, abort_flag);
+          landed_phase ^= 1;
+          if (clear_not_finite<T, CB, BOX_BYTES, 1>(smem + stage * L::STAGE + CB * BOX_BYTES, look & 255, look >> 8 & 255))
+            spoilt[look >> 16 & (L::SPOILT - 1)] = (look >> 16) + 1;
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&full[stage]);
         }
         if (i + AHEAD * PRODUCERS < tiles) read(j);
         i += PRODUCERS;
@@ -409,6 +433,20 @@ __global__ void __launch_bounds__(THREADS, Smem<CB, MB>::CTAS) attention_token_k
         if (turn == 0) leave_rows(true);
         named_bar_sync(1, WARPS * 32);
       }
+      // of the values that were cleared those that a row sees, to one of its results, by the lanes that will join these
+      if (spoilt[pieces & (L::SPOILT - 1)] == (pieces & L::PIECE_BITS) + 1) {
+#pragma unroll 1
+        for (int r = warp; r < rows; r += WARPS) {
+          const int end = min(length, length - walk.q.n + r / group + 1);
+#pragma unroll 1
+          for (int j = max(seen_by_all, 0); j < end; ++j) {
+            const long long at = place_of_key(p, walk.s, j);
+            const T *v = static_cast<const T *>(p.v) + at + walk.head * p.ld_head;
+            for (int ch = lane * 2 * CB; ch < (at < 0 ? 0 : min((lane + 1) * 2 * CB, p.head_dim)); ++ch)
+              if (!isfinite(to_f32(v[ch]))) merge[r * L::PITCH + ch] += to_f32(v[ch]);
+          }
+        }
+      }
       const int c0 = deal.owner(item), c1 = deal.owner(item_end - 1), sharers = c1 - c0 + 1;
       constexpr int PER = 2 * CB, WIDE = CB * 64, GROUP = 32;
       struct Row { float v[PER], top, l; };
@@ -515,15 +553,6 @@ __global__ void __launch_bounds__(THREADS, Smem<CB, MB>::CTAS) attention_token_k
         const float inv = x.l == 0.0f ? 0.0f : 1.0f / x.l;
         const int token = r / group, ch = lane * PER;
         T *out = static_cast<T *>(p.out) + (long long)(walk.q.first + token) * p.ld_out + (long long)(walk.head * group + r - token * group) * p.head_dim + ch;
-        // A value that is not finite, of a token that this row does not see and another does, has been multiplied by 0: such a row is worked out again without it.  (Where
-        // the sum is not finite either, what the row sees is not.)
-        float all = 0.0f;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) all = fmaf(x.v[i], 0.0f, all);
-        if (p.causal && walk.q.n > 1 && x.l - x.l == 0.0f && __any_sync(0xFFFFFFFFu, all != 0.0f)) {
-          attend_row<T, CB * 2>(p, walk.s, walk.q, walk.q.first + token, walk.head * group + r - token * group, lane);
-          return;
-        }
         if (ch >= p.head_dim) return;
         if constexpr (CB == 2) *reinterpret_cast<uint2 *>(out) = make_uint2(pack2<T>(x.v[0] * inv, x.v[1] * inv), pack2<T>(x.v[2] * inv, x.v[3] * inv));
         else *reinterpret_cast<uint32_t *>(out) = pack2<T>(x.v[0] * inv, x.v[1] * inv);

@@ -84,3 +84,89 @@ def test_the_same_bits_at_the_memory_s_full_rate(heads, kv_heads, d, dt):
         call()
         differ += (out != first).any()
     assert int(differ) == 0 and plan.device_status() == 0
+
+
+# ------------------------------------------------------------------------------------------- values that are not finite
+def filled(new, lengths, heads, kv_heads, d, page_size, dt=E.bf16, seed=1, causal=True, bad=(), width=None):
+    """(call, out, want, bound, rows that no value spoils): a plan over a cache, or dense keys with ``page_size`` 0, whose values have ``bad`` (sequence, key, head, channel, value)."""
+    b = A.batch(new, lengths, page_size or 16, seed, width=width)
+    q, kv = A.inputs(b, heads, kv_heads, d, dt, seed)
+    want, err, _ = A.wanted(b, q, kv, causal, d ** -0.5, dt)
+    spoilt = torch.zeros(want.shape, dtype=torch.bool, device="cuda")
+    group = heads // kv_heads
+    for s, j, h, c, what in bad:
+        kv[s][1][j, h, c] = what
+        for i in range(b.new[s]):
+            if not causal or j <= lengths[s] - b.new[s] + i:
+                spoilt[b.starts[s] + i, h * group:(h + 1) * group, c] = True
+    if page_size:
+        (k, k_view, ld), (v, v_view, _) = A.cache(b, kv_heads, d, dt), A.cache(b, kv_heads, d, dt)
+        for s, (ks, vs) in enumerate(kv):
+            A.put(b, k_view, s, ks)
+            A.put(b, v_view, s, vs)
+        rest = (b.table, b.lengths_t, b.starts_t)
+    else:
+        k = torch.full((b.seqs, max(lengths), kv_heads, d), A.NAN, dtype=q.dtype, device="cuda")
+        v, ld, rest = k.clone(), {}, (None, b.lengths_t, b.starts_t)
+        for s, (ks, vs) in enumerate(kv):
+            k[s, :lengths[s]], v[s, :lengths[s]] = ks, vs
+    plan, out = E.Attention(heads, kv_heads, d, dtype=dt, page_size=page_size, causal=causal, **ld), A.poisoned(b.rows, heads, d, dt=dt)
+
+    def call():
+        assert plan.enqueue(out, q, k, v, *rest, rows=b.rows, seqs=b.seqs) == 0, E.last_error()
+        return plan
+    torch.cuda.synchronize()
+    return call, out, want, err, spoilt
+
+
+SHAPES = [([5, 5], [5, 200], 8, 2, 128), ([8], [3001], 4, 4, 64), ([2, 7, 32], [40, 1000, 32], 2, 2, 96), ([16, 16], [16, 90], 2, 1, 64), ([200], [200], 8, 2, 128), ([130, 300], [700, 300], 6, 2, 64),
+          ([300], [4100], 4, 1, 128), ([40, 3], [33, 3], 5, 1, 80), ([260], [20000], 2, 2, 64)]
+
+
+@pytest.mark.parametrize("new,lengths,heads,kv_heads,d", SHAPES, ids=str)
+@pytest.mark.parametrize("page_size", [16, 24, 72, 136, 0])
+@pytest.mark.parametrize("dt", [E.bf16, E.f16])
+def test_values_that_are_not_finite_reach_the_rows_that_see_them(new, lengths, heads, kv_heads, d, page_size, dt):
+    """Some thirty values anywhere among the last keys, of which rows see some, all or none: a channel that a row sees one in is not finite, every other is right."""
+    g = torch.Generator().manual_seed(7)
+    draw = lambda n: int(torch.randint(0, n, (1,), generator=g))                                                         # noqa: E731
+    bad = []
+    for s, (n, m) in enumerate(zip(new, lengths)):
+        places = [m - 1, max(0, m - n), max(0, m - n - 1)] + [m - 1 - draw(min(m, 2 * n)) for _ in range(8)]
+        bad += [(s, j, draw(kv_heads), draw(d), [A.NAN, float("inf"), -float("inf")][draw(3)]) for j in places]
+    call, out, want, err, spoilt = filled(new, lengths, heads, kv_heads, d, page_size, dt, bad=bad)
+    plan = call()
+    assert plan.device_status() == 0
+    assert not bool(out[spoilt].isfinite().any())
+    out[spoilt], want[spoilt] = 0, 0
+    close(out, want, err, dt)
+    first = out.clone()
+    call()
+    torch.cuda.synchronize()
+    out[spoilt] = 0
+    assert torch.equal(out, first)
+
+
+def milliseconds(call):
+    begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    call()
+    torch.cuda.synchronize()
+    begin.record()
+    call()
+    end.record()
+    torch.cuda.synchronize()
+    return begin.elapsed_time(end)
+
+
+@pytest.mark.parametrize("new,length,heads,kv_heads,d", [(8, 100000, 4, 1, 128), (8, 100000, 4, 1, 64)])
+@pytest.mark.parametrize("place", ["seen", "half"])
+def test_a_value_that_is_not_finite_costs_little(new, length, heads, kv_heads, d, place):
+    """A row worked out again by a warp takes half a microsecond for each of its keys: 50 ms here for one of these rows, and seconds for longer ones."""
+    bad = [(0, 5 if place == "seen" else length - new // 2, 0, 3, float("inf"))]
+    call, out, want, err, spoilt = filled([new], [length], heads, kv_heads, d, 16, bad=bad)
+    clean, _, _, _, _ = filled([new], [length], heads, kv_heads, d, 16)
+    took, usual = milliseconds(call), milliseconds(clean)
+    assert not bool(out[spoilt].isfinite().any())
+    out[spoilt], want[spoilt] = 0, 0
+    close(out, want, err, E.bf16)
+    assert took <= 3 * usual + 2.0, (took, usual)
