@@ -36,9 +36,9 @@ struct Smem {
   static constexpr int Q_BYTES = CB * BOX_BYTES, STAGE = CB * BOX_BYTES;
   static constexpr int STAGES = CB == 1 ? 8 : 5;                // of K or V
   static constexpr int RING_OFF = 2 * Q_BYTES;
-  static constexpr int BAR_OFF = RING_OFF + STAGES * STAGE;     // full[S], empty[S], qfull, sfull[2], phalf[2], pfull[2], ofull[2]
-  static constexpr int MISC_OFF = BAR_OFF + (2 * STAGES + 9) * 8;
-  static constexpr int TOTAL = MISC_OFF + 16 + 1024;            // tmem slot, abort flag, verdicts; room to align
+  static constexpr int BAR_OFF = RING_OFF + STAGES * STAGE;     // full[S], empty[S], qfull, sfull[2], phalf[2], pfull[2], ofull[2], clean[4]
+  static constexpr int MISC_OFF = BAR_OFF + (2 * STAGES + 13) * 8;
+  static constexpr int TOTAL = MISC_OFF + 32 + 1024;            // tmem slot, abort flag, verdicts, whether values were left out; room to align
 };
 
 struct alignas(64) PromptLaunch {
@@ -124,9 +124,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prompt_kernel(const __gr
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::BAR_OFF), *empty = full + STAGES, *qfull = empty + STAGES, *sfull = qfull + 1, *phalf = sfull + 2,
-           *pfull = phalf + 2, *ofull = pfull + 2;
+           *pfull = phalf + 2, *ofull = pfull + 2, *clean = ofull + 2;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + L::MISC_OFF);
-  volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::MISC_OFF + 4), *verdict = abort_flag + 1;
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::MISC_OFF + 4), *verdict = abort_flag + 1, *spoilt = abort_flag + 3;
   const AttentionParams &p = g.p;
   // (from lane 0: what is known to be the same in all lanes goes to the tensor cores without a move each)
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, group = p.heads / p.kv_heads;
@@ -136,8 +136,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prompt_kernel(const __gr
     tma_prefetch_desc(&g.qmap);
     for (int i = 0; i < STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
     mbar_init(qfull, 1);
-    for (int i = 0; i < 2; ++i) { mbar_init(&sfull[i], 1); mbar_init(&phalf[i], 4); mbar_init(&pfull[i], 4); mbar_init(&ofull[i], 1); }
-    *abort_flag = 0;
+    for (int i = 0; i < 4; ++i) mbar_init(&clean[i], 1);
+    for (int i = 0; i < 2; ++i) { mbar_init(&sfull[i], 1); mbar_init(&phalf[i], 4); mbar_init(&pfull[i], 4); mbar_init(&ofull[i], 2); }
+    *abort_flag = *spoilt = 0;
     fence_barrier_init();
   }
   const KeyTiles<TILE> kt(p.page_size);
@@ -170,6 +171,10 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prompt_kernel(const __gr
   const int seen0 = seen_by(0), seen1 = seen_by(1), all = max(seen0, seen1);
   const int t0 = g.splits > 1 ? (int)((long long)all * split / g.splits) : 0, t1 = g.splits > 1 ? (int)((long long)all * (split + 1) / g.splits) : all;
   const int n0 = max(t0, min(t1, seen0)), n1 = max(t0, min(t1, seen1));
+  const int edge = p.causal ? max(length - n + row0 + 1, 0) : length;      // the first key that not all rows see
+  // Values behind the sequence's end may be anything, and 0 times anything is not always 0; those of keys that not all rows see may not be finite (clear_not_finite).
+  // The tile in which the sequence ends and those from the edge on, a few of a block's, are looked at by the warp that copies: it has nothing else to do by then.
+  const int last = kt.count(length) - 1, looked_at = edge < length ? kt.count(edge + 1) - 1 : kt.held(last, length) < TILE ? last : INT32_MAX;
   int fail_code = 0;
 
   if (warp < 4) {
@@ -205,6 +210,19 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prompt_kernel(const __gr
       }
       int issued = 0;
       bool ok = true;
+      auto look_at = [&](int t) {
+        const int fill = (t - t0) * 2 + 1, begin = max(edge - kt.first(t), 0), end = kt.held(t, length);
+        uint8_t *rows = smem + L::RING_OFF + fill % STAGES * L::STAGE;
+        ok = ok && mbar_wait_uniform(&full[fill % STAGES], (fill / STAGES) & 1, abort_flag);
+        if (ok && t == last)
+          for (int j = end * 8 + lane; j < TILE * 8; j += 32)
+#pragma unroll
+            for (int c = 0; c < CB; ++c) reinterpret_cast<uint4 *>(rows + c * BOX_BYTES)[j] = make_uint4(0, 0, 0, 0);
+        if (ok && begin < end && clear_not_finite<T, CB, BOX_BYTES, 4>(rows, begin, end)) *spoilt = 1;
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0 && ok) mbar_arrive(&clean[(t - max(looked_at, t0)) & 3]);
+      };
       for (int t = t0; t < t1 && ok; ++t) {
         int page = next_page;
         const int token = max(next_token, 0);
@@ -224,7 +242,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prompt_kernel(const __gr
                         &full[stage]);
           ++issued;
         }
+        if (ok && t > t0 && t - 1 >= looked_at) look_at(t - 1);   // (behind the copies of the next tile, in front of those that wait for the products with this one)
       }
+      if (ok && t1 > t0 && t1 - 1 >= looked_at) look_at(t1 - 1);
       if (!ok) fail_code = ST_WAIT_TIMEOUT_PRODUCER;
       // no copy is in flight when the block ends, however its other warps end
       for (int i = max(0, issued - STAGES); i < issued; ++i) mbar_wait_warp(&full[i % STAGES], (i / STAGES) & 1, abort_flag);
@@ -257,18 +277,11 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prompt_kernel(const __gr
         }
         umma_commit_el(&sfull[i], el);
       };
-      // the tile in which the sequence ends: values behind its end may be anything, and 0 times anything is not always 0
-      const int last = kt.count(length) - 1, held = kt.held(last, length);
+      // (four barriers in turns: tile t + 4's values are not copied before tile t's have been multiplied)
+      static_assert(STAGES <= 8, "");
       auto next_values = [&](int t) {
-        const int at = next_full();
-        if (t == last && held < TILE && ok) {
-          uint8_t *rows = smem + L::RING_OFF + at * L::STAGE;
-          for (int j = held * 8 + lane; j < TILE * 8; j += 32)
-#pragma unroll
-            for (int c = 0; c < CB; ++c) reinterpret_cast<uint4 *>(rows + c * BOX_BYTES)[j] = make_uint4(0, 0, 0, 0);
-          fence_proxy_async_smem();
-          __syncwarp();
-        }
+        const int at = next_full(), k = t - max(looked_at, t0);
+        if (k >= 0) ok = ok && mbar_wait_uniform(&clean[k & 3], (k >> 2) & 1, abort_flag);
         return at;
       };
       int keys_at = next_full();
@@ -300,7 +313,10 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prompt_kernel(const __gr
             }
             if (!ok) break;
             if (t + 1 < end) scores(i, keys_at);
-            else umma_commit_el(&ofull[i], el);
+            else {
+              umma_commit_el(&ofull[i], el);
+              if (lane == 0) mbar_arrive(&ofull[i]);            // (and what this warp has written)
+            }
           }
         }
         umma_commit_el(&empty[values_at], el);
@@ -401,16 +417,34 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prompt_kernel(const __gr
     // (the queries' place is written below: where nothing was computed, their copy has to have landed first)
     if (tiles == 0 && t1 > t0 && !mbar_wait_uniform(qfull, 0, abort_flag)) fail_code = ST_WAIT_TIMEOUT_EPILOGUE;
     tc_fence_after_sync();
+    if (__any_sync(0xFFFFFFFFu, tiles > 0 && *spoilt != 0)) {     // values that are not finite: those that the row sees
+#pragma unroll 1
+      for (int q = 0; q < 2 * CB; ++q) {
+        uint32_t o[32];
+        tmem_ld32(o_at + q * 32, o);
+        tmem_ld_wait();
+        tmem_arrived32(o);
+#pragma unroll 1
+        for (int j = edge; j < (mine ? seen : 0); ++j) {
+          const long long at = place_of_key(p, block.s, j);
+          const T *v = static_cast<const T *>(p.v) + at + head * p.ld_head + q * 32;
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            const float x = at >= 0 && q * 32 + k < p.head_dim ? to_f32(v[k]) : 0.0f;
+            if (!isfinite(x)) o[k] = __float_as_uint(__uint_as_float(o[k]) + x);
+          }
+        }
+        __syncwarp();
+        tmem_st32(o_at + q * 32, o);
+      }
+      tmem_st_wait();
+    }
     T *out = static_cast<T *>(p.out) + (long long)(block.q.first + token) * p.ld_out + (long long)(head * group + r - in_tile * group) * p.head_dim;
     const uint32_t rows_here = __ballot_sync(0xFFFFFFFFu, mine);
-    float finite = 0.0f;                                        // 0 while the row's results are
     // A row per thread would make 32 lines of each store: 64 channels of a warp's rows go through the place of its queries, which nothing reads any more, 16-byte word x
     // of row y at x ^ (y & 7), and on to memory eight lanes to a row.
     uint4 *stage = reinterpret_cast<uint4 *>(smem + i * L::Q_BYTES + (warp & 3) * 32 * 128);
     auto write = [&](const float (&v)[32], int q, float inv) {
-#pragma unroll
-      for (int k = 0; k < 32; ++k)
-        if (q * 32 + (k & ~7) < p.head_dim) finite = fmaf(v[k], 0.0f, finite);        // (no product has written the columns behind)
 #pragma unroll
       for (int k = 0; k < 4; ++k)
         stage[lane * 8 + (((q & 1) * 4 + k) ^ (lane & 7))] =
@@ -472,7 +506,6 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prompt_kernel(const __gr
             whole += x.y * exp2_approx(x.x - from);
           }
           const float inv = whole == 0.0f ? 0.0f : 1.0f / whole;
-          l = whole;
 #pragma unroll 1
           for (int q = 0; q < 2 * CB; ++q) {
             float v[32];
@@ -489,14 +522,6 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prompt_kernel(const __gr
             }
             write(v, q, inv);
           }
-        }
-      }
-      // A value that is not finite, of a token that a row does not see and others do, has been multiplied by 0: such rows are worked out again without it.  (Where the
-      // sum is not finite either, what the row sees is not.)
-      if (p.causal) {
-        for (uint32_t again = __ballot_sync(0xFFFFFFFFu, mine && finite != 0.0f && l - l == 0.0f); again != 0; again &= again - 1) {
-          const int y = __ffs(again) - 1, row = block.q.first + __shfl_sync(0xFFFFFFFFu, token, y);
-          attend_row<T, CB * 2>(p, block.s, block.q, row, head * group + __shfl_sync(0xFFFFFFFFu, r - in_tile * group, y), lane);
         }
       }
     }

@@ -505,7 +505,7 @@ ELB_API int elb_append_enqueue(elb_op_t *op, void *q_out, void *k_cache, void *v
 /* output[t][h] = sum_j softmax_j(scale * input[t][h] . k[j][h / g]) v[j][h / g],  g = heads / kv_heads, over the keys j that token t sees:
  * those below its sequence's length and, causal, not behind its own place.  A token that sees none gets zeros.  Scores, sums and the result are
  * held in 32 bits; the softmax's terms are rounded to dt, the second product's operand, except on CUDA cores.  Keys and values that a token does not see do not enter its
- * result, whatever they hold (where they lie within the sequence's length and are not finite, the call takes much longer).  A length past what the table, or `width`,
+ * result, whatever they hold; a value that is not finite makes its channel so in the results of all tokens that see it.  A length past what the table, or `width`,
  * can hold counts as that.
  * dense (table NULL): k and v are [seqs][width][kv_heads][head_dim], page_size 0, lengths may be NULL (all `width` keys), `pages` is not used; ld_page
  * is then a sequence's.

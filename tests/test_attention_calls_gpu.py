@@ -158,7 +158,7 @@ def milliseconds(call):
     return begin.elapsed_time(end)
 
 
-@pytest.mark.parametrize("new,length,heads,kv_heads,d", [(8, 100000, 4, 1, 128), (8, 100000, 4, 1, 64)])
+@pytest.mark.parametrize("new,length,heads,kv_heads,d", [(8, 100000, 4, 1, 128), (8, 100000, 4, 1, 64), (4096, 4096, 8, 2, 128), (4096, 4096, 4, 2, 64)])
 @pytest.mark.parametrize("place", ["seen", "half"])
 def test_a_value_that_is_not_finite_costs_little(new, length, heads, kv_heads, d, place):
     """A row worked out again by a warp takes half a microsecond for each of its keys: 50 ms here for one of these rows, and seconds for longer ones."""
