@@ -287,7 +287,8 @@ int elb_attention_enqueue(elb_op_t *op, void *output, const void *input, const v
   p.causal = d.causal != 0;
   p.scale = d.scale;
   p.words = aligned(output, 16) && aligned(input, 16) && aligned(k, 16) && aligned(v, 16) &&
-            (d.head_dim | d.ld_input | d.ld_output | p.ld_page | p.ld_head | p.ld_token) % 8 == 0;
+            (d.head_dim | d.ld_input | d.ld_output | p.ld_page | p.ld_head | p.ld_token) % 8 == 0 &&
+            (d.ld_input | p.ld_page | p.ld_head | p.ld_token) < 1ll << 39;          // (a tiled copy's strides are below 2^40 bytes)
   p.num_sms = op->num_sms;
   p.status = op->d_status;
   const cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);

@@ -67,10 +67,10 @@ def test_the_same_bits_at_the_memory_s_full_rate(heads, kv_heads, d, dt):
         table[s, :n] = order[sum(held[:s]):sum(held[:s]) + n]
     q = randn(seqs, heads, d, dtype=A.TORCH[dt], seed=1, scale=1.5)
     k, v = (randn(sum(held), kv_heads, page, d, dtype=A.TORCH[dt], seed=i) for i in (2, 3))
-    plan, out = E.Attention(heads, kv_heads, d, dtype=dt, page_size=page), A.poisoned(seqs, heads, d, dt=dt)
+    plan, out, held_t = E.Attention(heads, kv_heads, d, dtype=dt, page_size=page), A.poisoned(seqs, heads, d, dt=dt), A.ints(lengths)
 
     def call():
-        assert plan.enqueue(out, q, k, v, table, A.ints(lengths), rows=seqs, seqs=seqs) == 0, E.last_error()
+        assert plan.enqueue(out, q, k, v, table, held_t, rows=seqs, seqs=seqs) == 0, E.last_error()
     call()
     torch.cuda.synchronize()
     first = out.clone()
@@ -170,3 +170,27 @@ def test_a_value_that_is_not_finite_costs_little(new, length, heads, kv_heads, d
     out[spoilt], want[spoilt] = 0, 0
     close(out, want, err, E.bf16)
     assert took <= 3 * usual + 2.0, (took, usual)
+
+
+# ------------------------------------------------------------------------------------------- strides and batches
+@pytest.mark.parametrize("n", [1, 40])
+@pytest.mark.parametrize("what", ["page", "row", "dense"])
+def test_strides_that_no_tiled_copy_takes(n, what):
+    """Rows and pages of which there is one may lie as far apart as the description takes."""
+    far, d, dt = 1 << 40, 64, E.bf16
+    q, k, v = (randn(m, 1, d, dtype=A.TORCH[dt], seed=m) for m in (n, 50, 51))
+    v = v[:50].contiguous()
+    out = A.poisoned(n, 1, d, dt=dt)
+    rows, table, lengths = 1 if what == "row" else n, A.ints([[0]]), A.ints([50])
+    if what == "page":
+        plan = E.Attention(1, 1, d, page_size=64, ld_page=far)
+        kc, vc = (torch.cat([x, x.new_zeros(14, 1, d)]).permute(1, 0, 2)[None].contiguous() for x in (k, v))
+        args = (kc.data_ptr(), vc.data_ptr(), table.data_ptr(), lengths.data_ptr(), None, rows, 1, 1, 1)
+    else:
+        plan = E.Attention(1, 1, d, **(dict(ld_page=far) if what == "dense" else dict(ld_input=far, ld_output=far)))
+        args = (k.data_ptr(), v.data_ptr(), None, None, None, rows, 1, 1, 50)
+    torch.cuda.synchronize()
+    assert E.lib.elb_attention_enqueue(plan.h, out.data_ptr(), q.data_ptr(), *args, None) == 0, E.last_error()
+    assert plan.device_status() == 0
+    want, err = A.attention64(q[:rows], k, v, rows, True, d ** -0.5, dt)
+    close(out[:rows], want, err, dt)
