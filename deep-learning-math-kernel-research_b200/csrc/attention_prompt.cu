@@ -67,6 +67,28 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+// What a row's terms are relative to, once its maximum so far is m: 2^(s c - m c), c the scale in powers of two, is one fused multiply-add of s, `step` = c and -`from` =
+// -m c.  m c is rounded, by up to 2^-25 of it, for all terms alike, and past 2^128 none of fp32's numbers.  From 2^27 on the next smaller score's term is below 2^-7, most are
+// below 2^-126, and `step` is the power of two above c, with which nothing is rounded.
+struct Reference { float step, from; };
+__device__ __forceinline__ float power_above(float c) { return __uint_as_float((__float_as_uint(c) + 0x007FFFFFu) & 0x7F800000u); }
+__device__ __forceinline__ bool is_large(const Reference &r) { return !(fabsf(r.from) < 0x1p27f); }
+__device__ __forceinline__ Reference reference(float m, float c) { return {c, m == -INFINITY ? 0.0f : __fmul_rn(m, c)}; }
+__device__ __forceinline__ Reference large_reference(float m, float c) {
+  const float step = power_above(c), from = m * step;
+  return isinf(from) ? Reference{1.0f, m} : Reference{step, from};
+}
+// The factor of what is relative to the old maximum
+__device__ __forceinline__ float to_reference(float old, float m, float c) {
+  const Reference was = reference(old, c), is = reference(m, c);
+  return old == -INFINITY ? 0.0f : exp2_approx(is_large(was) || is_large(is) ? (old - m) * c : was.from - is.from);
+}
+// What a partial result says that it is relative to, in powers of two times unit_of(c), which rounds nothing and keeps it in fp32's range; or -inf.
+__device__ __forceinline__ float unit_of(float c) { return fmaxf(power_above(c), 1.0f); }
+__device__ __forceinline__ float left_reference(float m, float c) {
+  const Reference r = reference(m, c);
+  return m == -INFINITY ? m : is_large(r) ? m * fminf(power_above(c), 1.0f) : r.from / unit_of(c);
+}
 // A matrix descriptor whose low word, the address and the distance along M or N, is worked out in 32 bits
 __device__ __forceinline__ uint64_t with_low(uint64_t desc, uint32_t low) { return (desc & 0xFFFFFFFF00000000ull) | low; }
 
@@ -336,7 +358,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prompt_kernel(const __gr
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16, s_at = tmem + lanes + S_COL + i * TILE, o_at = tmem + lanes + O_COL + i * CB * 64;
     const float c = fabsf(p.scale) * 1.4426950408889634f, slack = fminf(SLACK / c, 3e38f);
     const int seen = p.causal ? min(length, length - n + token + 1) : length;
-    float m = -INFINITY, l = 0.0f;
+    float l = 0.0f;
+    float m = -INFINITY;
+    Reference ref = reference(m, c);
     uint32_t parity = 0;
     for (int t = t0; t < end; ++t, parity ^= 1) {
       if (!mbar_wait_uniform(&sfull[i], parity, abort_flag)) { fail_code = ST_WAIT_TIMEOUT_EPILOGUE; break; }
@@ -364,7 +388,10 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prompt_kernel(const __gr
       }
       const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
       if (__any_sync(0xFFFFFFFFu, top > m + slack)) {
-        const float to = top > m + slack ? top : m, scale = m == -INFINITY ? 0.0f : exp2_approx((m - to) * c);
+        const float to = top > m + slack ? top : m, scale = to_reference(m, to, c);
+        m = to;
+        ref = reference(m, c);
+        if (is_large(ref)) ref = large_reference(m, c);
         if (t > t0) {
 #pragma unroll 1
           for (int q = 0; q < 2 * CB; ++q) {
@@ -378,17 +405,15 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prompt_kernel(const __gr
           }
         }
         l *= scale;
-        m = to;
       }
-      const float from = m == -INFINITY ? 0.0f : m * c;
-      const uint64_t c2 = pair(c, c), from2 = pair(-from, -from);
+      const uint64_t step2 = pair(ref.step, ref.step), from2 = pair(-ref.from, -ref.from);
       uint64_t sum[2] = {0, 0};
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         uint32_t w[16];
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
-          const uint64_t z = fma2(pair(__uint_as_float(s[q][2 * k]), __uint_as_float(s[q][2 * k + 1])), c2, from2);
+          const uint64_t z = fma2(pair(__uint_as_float(s[q][2 * k]), __uint_as_float(s[q][2 * k + 1])), step2, from2);
           float a, b;
           unpair(z, a, b);
           a = exp2_approx(a);
@@ -483,11 +508,12 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prompt_kernel(const __gr
         } else if (mine) {
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            reinterpret_cast<float4 *>(part(split))[(q * 8 + k) * TILE + r] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+            reinterpret_cast<float4 *>(part(split))[(q * 8 + k) * TILE + r] =
+                make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
         }
       }
       if (g.splits > 1) {
-        if (mine) reinterpret_cast<float2 *>(part(split) + TILE * WIDE)[r] = make_float2(m * c, l);
+        if (mine) reinterpret_cast<float2 *>(part(split) + TILE * WIDE)[r] = make_float2(left_reference(m, c), l);
         named_bar_sync(1 + i, 128);
         // (released and acquired by one thread for the row tile's four warps, which the barriers order)
         if (r == 0) {
@@ -498,12 +524,13 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prompt_kernel(const __gr
         }
         named_bar_sync(1 + i, 128);
         if (verdict[i] != 0) {                                  // (rows that are not there read what others left, and write nothing)
+          const float unit = unit_of(c);
           float top = -INFINITY, whole = 0.0f;
           for (int k = 0; k < g.splits; ++k) top = fmaxf(top, __ldcg(reinterpret_cast<const float2 *>(part(k) + TILE * WIDE) + r).x);
           const float from = top == -INFINITY ? 0.0f : top;
           for (int k = 0; k < g.splits; ++k) {
             const float2 x = __ldcg(reinterpret_cast<const float2 *>(part(k) + TILE * WIDE) + r);
-            whole += x.y * exp2_approx(x.x - from);
+            whole += x.y * exp2_approx((x.x - from) * unit);
           }
           const float inv = whole == 0.0f ? 0.0f : 1.0f / whole;
 #pragma unroll 1
@@ -513,7 +540,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prompt_kernel(const __gr
             for (int k = 0; k < 32; ++k) v[k] = 0.0f;
 #pragma unroll 2
             for (int k = 0; k < g.splits; ++k) {
-              const float w = exp2_approx(__ldcg(reinterpret_cast<const float2 *>(part(k) + TILE * WIDE) + r).x - from);
+              const float w = exp2_approx((__ldcg(reinterpret_cast<const float2 *>(part(k) + TILE * WIDE) + r).x - from) * unit);
 #pragma unroll
               for (int j = 0; j < 8; ++j) {
                 const float4 x = __ldcg(reinterpret_cast<const float4 *>(part(k)) + (q * 8 + j) * TILE + r);

@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(THREADS, Smem<CB, MB>::CTAS) attention_token_k
             if (key >= here || key0 + key >= seen[(i >> 1) & 1]) sc[i >> 2][i & 3] = -INFINITY;
           }
         }
-        float keep[2], from[2];
+        float keep[2], base[2];
         bool moved = false;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
@@ -343,11 +343,14 @@ __global__ void __launch_bounds__(THREADS, Smem<CB, MB>::CTAS) attention_token_k
           for (int n = 0; n < 4; ++n) top = fmaxf(top, fmaxf(sc[n][half * 2], sc[n][half * 2 + 1]));
           top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
           top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-          from[half] = top == -INFINITY ? 0.0f : top * c;
-          keep[half] = exp2_approx(m[half] * c - from[half]);
+          base[half] = top == -INFINITY ? 0.0f : top;
+          keep[half] = exp2_approx((m[half] - base[half]) * c);
           moved |= top > m[half];
           m[half] = top;
         }
+        // (Their distances from the largest, then times c: products of large scores with c are rounded, by more than one from 2^25 on, and past 2^128 none of fp32's numbers.)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[i >> 2][i & 3] -= base[(i >> 1) & 1];
         if (__any_sync(0xFFFFFFFFu, moved)) {
 #pragma unroll
           for (int half = 0; half < 2; ++half) l[half] *= keep[half];
@@ -361,7 +364,7 @@ __global__ void __launch_bounds__(THREADS, Smem<CB, MB>::CTAS) attention_token_k
         for (int n = 0; n < 4; ++n)
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            const float w0 = exp2_approx(fmaf(sc[n][half * 2], c, -from[half])), w1 = exp2_approx(fmaf(sc[n][half * 2 + 1], c, -from[half]));
+            const float w0 = exp2_approx(sc[n][half * 2] * c), w1 = exp2_approx(sc[n][half * 2 + 1] * c);
             l[half] += w0 + w1;                                 // (of this lane's keys: the four lanes of a row meet at the end)
             pf[n >> 1][half + 2 * (n & 1)] = pack2<T>(w0, w1);  // the second product's operand has 16 bits
           }
@@ -400,7 +403,6 @@ __global__ void __launch_bounds__(THREADS, Smem<CB, MB>::CTAS) attention_token_k
       for (int half = 0; half < 2; ++half) {
         l[half] += __shfl_xor_sync(0xFFFFFFFFu, l[half], 1);
         l[half] += __shfl_xor_sync(0xFFFFFFFFu, l[half], 2);
-        m[half] *= c;
       }
       float *place = merge + ((MB > 1 ? block : warp) * 16 + (lane >> 2)) * L::PITCH + quad * 2;
       auto leave_rows = [&](bool joining) {
@@ -410,8 +412,8 @@ __global__ void __launch_bounds__(THREADS, Smem<CB, MB>::CTAS) attention_token_k
           if (joining) {
             const float2 x = ml[(warp + MB) * 16 + r];
             const float top = fmaxf(m[half], x.x), from = top == -INFINITY ? 0.0f : top;
-            own[half] = exp2_approx(m[half] - from);
-            add[half] = exp2_approx(x.x - from);
+            own[half] = exp2_approx((m[half] - from) * c);
+            add[half] = exp2_approx((x.x - from) * c);
             m[half] = top;
             l[half] = l[half] * own[half] + x.y * add[half];
           }
@@ -464,7 +466,7 @@ __global__ void __launch_bounds__(THREADS, Smem<CB, MB>::CTAS) attention_token_k
         for (int w = 0; w < L::COPIES; ++w) { y[w] = ml[w * 16 + r]; x.top = fmaxf(x.top, y[w].x); }
 #pragma unroll
         for (int w = 0; w < L::COPIES; ++w) {
-          const float k = exp2_approx(y[w].x - base_of(x.top));
+          const float k = exp2_approx((y[w].x - base_of(x.top)) * c);
           const float *src = merge + (w * 16 + r) * L::PITCH + lane * PER;
           x.l += y[w].y * k;
 #pragma unroll
@@ -497,8 +499,8 @@ __global__ void __launch_bounds__(THREADS, Smem<CB, MB>::CTAS) attention_token_k
             float top = fmaxf(x[a].top, y[a].x);
 #pragma unroll
             for (int b = 16; b > 0; b >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, b));
-            const float keep = exp2_approx(x[a].top - base_of(top));
-            weight[a] = exp2_approx(y[a].x - base_of(top));
+            const float keep = exp2_approx((x[a].top - base_of(top)) * c);
+            weight[a] = exp2_approx((y[a].x - base_of(top)) * c);
             float sum = y[a].y * weight[a];
 #pragma unroll
             for (int b = 16; b > 0; b >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, b);

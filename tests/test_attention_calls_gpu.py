@@ -194,3 +194,64 @@ def test_strides_that_no_tiled_copy_takes(n, what):
     assert plan.device_status() == 0
     want, err = A.attention64(q[:rows], k, v, rows, True, d ** -0.5, dt)
     close(out[:rows], want, err, dt)
+
+
+# ------------------------------------------------------------------------------------------- the largest scores
+@pytest.mark.parametrize("n,length", [(1, 700), (3, 500), (1, 40000), (90, 300), (130, 20000)])
+@pytest.mark.parametrize("d,scale", [(64, 1.0), (128, 1.0), (64, 0.125), (64, 0.01), (128, 60.0)])
+@pytest.mark.parametrize("scores", ["lowest", "lowest but one", "highest", "rising", "both"])
+def test_scores_up_to_the_ends_of_fp32(n, length, d, scale, scores):
+    """Scores of up to 1.75 * 2^127, whose products with log2 e are rounded to far more than one, or are none of fp32's numbers: the largest share the sum alone."""
+    size, dt = 1.75 * 2.0 ** 63, E.bf16
+    k0 = torch.full((length,), {"lowest": -size, "lowest but one": -size, "highest": size, "rising": 0.0, "both": -size}[scores], dtype=torch.float64, device="cuda")
+    if scores == "lowest but one":
+        k0[length // 3] = 0.0
+    if scores == "rising":
+        k0 = torch.linspace(-1.0, 1.0, length, dtype=torch.float64, device="cuda") * size
+    if scores == "both":
+        k0[::5] = size
+    k0 = k0.to(A.TORCH[dt])
+    k = torch.zeros(1, length, 2, d, dtype=A.TORCH[dt], device="cuda")
+    k[0, :, :, 5] = k0[:, None]
+    q = torch.zeros(n, 4, d, dtype=A.TORCH[dt], device="cuda")
+    q[..., 5] = 2.0 ** 64
+    v = randn(1, length, 2, d, dtype=A.TORCH[dt], seed=4)
+    plan, out = E.Attention(4, 2, d, dtype=dt, causal=False, scale=scale), A.poisoned(n, 4, d, dt=dt)
+    torch.cuda.synchronize()
+    assert plan.enqueue(out, q, k, v, rows=n, seqs=1) == 0, E.last_error()
+    assert plan.device_status() == 0
+    top = k0 == k0.max()
+    mean, size = (f(v[0].double()[top]).mean(0).repeat_interleave(2, 0).expand(n, -1, -1) for f in (lambda x: x, torch.abs))
+    close(out, mean, (2.0 ** -17 + (4 * int(top.sum()) ** 0.5 + 8) * 2.0 ** -23) * 2 * size, dt)
+
+
+@pytest.mark.parametrize("n", [1, 3, 90])
+@pytest.mark.parametrize("power", [10, 20, 24, 27, 28, 31, 40, 60])
+@pytest.mark.parametrize("dt", [E.bf16, E.f16])
+def test_large_scores_that_are_near_one_another(n, power, dt):
+    """Scores of 2^power and a few of their own last places below it, exact in 32 bits: the definition's weights, whatever the product with log2 e is rounded to."""
+    if dt == E.f16 and power > 28:
+        return
+    length, d = 300, 64
+    half = power // 2
+    scale = 1.0 if power > 20 else 0.75
+    k = torch.zeros(1, length, 1, d, dtype=A.TORCH[dt], device="cuda")
+    q = torch.zeros(n, 2, d, dtype=A.TORCH[dt], device="cuda")
+    steps = torch.arange(length, device="cuda") % 5                                      # 0, 1, 2, 3, 4 last places (of 2^(power - 22)) below the largest
+    last = 2.0 ** max(power - 22, -3)
+    q[..., 0], q[..., 1] = 2.0 ** half, -2.0 ** min(half, 10)
+    k[..., 0] = 2.0 ** (power - half)
+    k[0, :, 0, 1] = (steps * last / 2.0 ** min(half, 10)).to(k.dtype)
+    v = randn(1, length, 1, d, dtype=A.TORCH[dt], seed=4)
+    plan, out = E.Attention(2, 1, d, dtype=dt, causal=False, scale=scale), A.poisoned(n, 2, d, dt=dt)
+    torch.cuda.synchronize()
+    assert plan.enqueue(out, q, k, v, rows=n, seqs=1) == 0, E.last_error()
+    assert plan.device_status() == 0
+    s = (q[0, 0].double() @ k[0, :, 0].double().T) * scale
+    w = torch.softmax(s, -1)
+    want = (w @ v[0, :, 0].double()).expand(n, 2, -1)
+    size = (w @ v[0, :, 0].double().abs()).expand(n, 2, -1)
+    # the terms' rounding and the exponential's; above 2^27 the power of two above scale * log2 e stands in for it: a last place is then 8 or more of its powers of two, and a term
+    # of 2^-8 / 2^-11.5 at most the other
+    off = 2.0 ** -16 + {E.bf16: 2.0 ** -8, E.f16: 2.0 ** -11}[dt] + (2.0 ** -8 if power >= 27 else 0.0)
+    close(out, want, off * 2 * size, dt)
