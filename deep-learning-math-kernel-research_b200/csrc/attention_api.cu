@@ -33,7 +33,8 @@ int check_rotary(elb_rotary_desc_t &d, bool append) {
   return rc;
 }
 
-// Turns per position of each pair, modulo 1, as 64-bit fractions
+// Turns per position of each pair, modulo 1, as 64-bit fractions, worked out in the long double's 64 bits: 53 of them would leave the angle of position 2^31 wrong by
+// 2^-20 times the frequency in radians.
 int make_steps(elb_op &op, const elb_rotary_desc_t &d, const float *frequencies) {
   const int n = d.rotary_dim / 2;
   unsigned long long steps[512];
@@ -45,20 +46,20 @@ int make_steps(elb_op &op, const elb_rotary_desc_t &d, const float *frequencies)
     if (rc != ELB_OK) return rc;
     OP_TRY(cudaMemcpy(given, st.p, n * sizeof(float), cudaMemcpyDefault));
   }
-  const double two_pi = 6.283185307179586476925;
+  const long double two_pi = 6.283185307179586476925286766559005768L;
   for (int i = 0; i < n; ++i) {
-    double f = std::pow((double)d.base, -2.0 * i / d.rotary_dim);
+    long double f = std::pow((long double)d.base, -2.0L * i / d.rotary_dim);
     if (d.scaling == ELB_SCALE_LINEAR) f /= d.factor;
     if (d.scaling == ELB_SCALE_BY_PARTS) {
-      double s = (d.original * f / two_pi - d.slow) / ((double)d.fast - d.slow);
-      s = s < 0.0 ? 0.0 : s > 1.0 ? 1.0 : s;
-      f = s * f + (1.0 - s) * f / d.factor;
+      long double s = (d.original * f / two_pi - d.slow) / ((long double)d.fast - d.slow);
+      s = s < 0.0L ? 0.0L : s > 1.0L ? 1.0L : s;
+      f = s * f + (1.0L - s) * f / d.factor;
     }
     if (frequencies) f = given[i];
     if (!std::isfinite(f)) return op_fail(ELB_GENERAL_ERROR, "frequency %d is not finite", i);
-    double turn = f / two_pi;
+    long double turn = f / two_pi;
     turn -= std::floor(turn);
-    steps[i] = turn >= 1.0 ? 0ull : (unsigned long long)std::ldexp(turn, 64);
+    steps[i] = turn >= 1.0L ? 0ull : (unsigned long long)std::ldexp(turn, 64);
   }
   unsigned long long *dst = nullptr;
   const int rc = alloc(op, &dst, (n > 0 ? n : 1) * sizeof(unsigned long long));

@@ -1,7 +1,7 @@
 // Rotary positions, of queries and keys or on the way into a cache of pages.
 //
 // (a, b) -> magnitude * (a cos x - b sin x, b cos x + a sin x), x = position * f.  An angle of 10^5 radians has no fraction left in 32 bits, so a plan holds
-// f / (2 pi) modulo 1 as a 64-bit fraction: its product with the position, modulo 2^64, is the turn without a rounding, and its upper 32
+// f / (2 pi) modulo 1 as a 64-bit fraction: its product with the position, modulo 2^64, is taken without a rounding, and its upper 32
 // bits are the argument of sincospi.
 //
 // A warp takes a token where there are many, the warps of a block its heads where there are few.  A lane has one 16-byte word of a head, or two words that turn

@@ -469,7 +469,8 @@ enum { ELB_SCALE_NONE = 0, ELB_SCALE_LINEAR = 1, ELB_SCALE_BY_PARTS = 2 };
  *   magnitude * (a cos x - b sin x), magnitude * (b cos x + a sin x),  x = position * f_i  (inverse: -x, so that magnitude 1 undoes it)
  *   f_i = base^(-2i/r); linear: f_i / factor; by parts: with t = original * f_i / (2 pi) turns over the original length and
  *   s = (t - slow) / (fast - slow) cut to 0 .. 1: s * f_i + (1 - s) * f_i / factor
- * or any f_i that prepare is given.  The other channels are copied.  x is reduced exactly for every 32-bit position; the turn itself is done in 32 bits. */
+ * or any f_i that prepare is given.  The other channels are copied.  f_i is held in 64 bits and x reduced without a rounding, for every 32-bit position; the turn itself is
+ * done in 32 bits. */
 typedef struct elb_rotary_desc {
   int32_t heads, kv_heads, head_dim;              /* of q and of k (either may be 0); head_dim up to 1024 */
   int32_t rotary_dim;                             /* even, 2 .. head_dim (elb_append: 0 as well, nothing turns) */

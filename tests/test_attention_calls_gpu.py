@@ -255,3 +255,22 @@ def test_large_scores_that_are_near_one_another(n, power, dt):
     # of 2^-8 / 2^-11.5 at most the other
     off = 2.0 ** -16 + {E.bf16: 2.0 ** -8, E.f16: 2.0 ** -11}[dt] + (2.0 ** -8 if power >= 27 else 0.0)
     close(out, want, off * 2 * size, dt)
+
+
+# ------------------------------------------------------------------------------------------- far positions
+def test_fast_frequencies_at_the_farthest_positions():
+    """Angles of up to 10^13 radians against their definition in rational numbers: the bound of every other position."""
+    from fractions import Fraction
+    turns = Fraction(15915494309189533576888376337251436203445964574045644874766734405889, 10 ** 68)     # 1 / (2 pi)
+    f = torch.tensor([1.0, 1000.0, -777.7, 333.3, 7.5, 5000.0, 0.1, 62.83], dtype=torch.float32)
+    pos = A.ints([2 ** 31 - 1, 2 ** 31 - 2, -(2 ** 31), 2 ** 30 + 12345, 10 ** 9 + 7, 10 ** 6 + 3, -1999999999])
+    x = randn(len(pos), 2, 16, dtype=torch.float32, seed=1)
+    plan, out = E.Rotary(2, 0, 16, dtype=E.f32), torch.empty_like(x)
+    assert plan.prepare(f) == 0, E.last_error()
+    assert plan.enqueue(out, None, x, None, pos, rows=len(pos)) == 0, E.last_error()
+    assert plan.device_status() == 0
+    angle = torch.tensor([[float((Fraction(p) * Fraction(w) * turns) % 1) for w in f.tolist()] for p in pos.tolist()], dtype=torch.float64, device="cuda")[:, None] * 2.0 * torch.pi
+    a, b = x.double().chunk(2, -1)
+    want = torch.cat((a * angle.cos() - b * angle.sin(), b * angle.cos() + a * angle.sin()), -1)
+    off = (a.abs() + b.abs()).repeat(1, 1, 2) * 2.0 ** -20                                                # (as turn64's)
+    close(out, want, off, E.f32)
