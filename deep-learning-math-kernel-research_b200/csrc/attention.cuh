@@ -29,12 +29,22 @@ __device__ __forceinline__ Sequence sequence_of(const Sequences &b, int s) {
   q.length = b.lengths ? min(max(b.lengths[s], 0), b.capacity) : b.capacity;
   return q;
 }
-// The sequence of a row, found by a warp: the starts behind the first that are not behind the row.  seqs or more, or -1: none.
+// The last i of 0 .. n - 1 whose value(i) is not above x, by a warp, a lane a value: values do not fall.  (They are the caller's tensors': where they do, some i.)  -1: none
+template <typename F>
+__device__ __forceinline__ long long last_up_to(long long n, int x, int lane, F value) {
+  long long at = 0;                                             // value(i) <= x below it; n more are not known
+  while (n > 0) {
+    const long long step = (n + 31) / 32, mine = (lane + 1) * step - 1;
+    const int below = __popc(__ballot_sync(0xFFFFFFFFu, mine < n && value(at + mine) <= x));
+    at += below * step;
+    n = min(step - 1, n - below * step);                        // (of the step that ends above x, or of what is left behind the last whole one)
+  }
+  return at - 1;
+}
+// The sequence of a row, found by a warp.  seqs, or -1: none.
 __device__ __forceinline__ int sequence_of_row(const Sequences &b, int row, int lane) {
   if (!b.starts) return row / b.each;
-  int before = 0;
-  for (long long s = lane; s <= b.seqs; s += 32) before += b.starts[s] <= row;
-  return __reduce_add_sync(0xFFFFFFFFu, before) - 1;
+  return (int)last_up_to(b.seqs + 1, row, lane, [&](long long s) { return b.starts[s]; });
 }
 
 __device__ __forceinline__ float exp2_approx(float x) {

@@ -6,7 +6,7 @@
 // O0 S0' O1 S1', so that one tile's products run while the other's softmax does.  With 128 channels a tile's products take the tensor cores 512 cycles each,
 // its 16384 exponentials the SM's 16 special-function lanes 1024, and the way round of scores, softmax and results some 3400 for both tiles.
 //
-// Blocks come in the order of their work, those of the longest sequences first and of each the last, which see the most keys.  Where there are fewer of them than
+// Blocks of up to 32 sequences come in the order of their work, those of the longest first and of each the last, which see the most keys.  Where there are fewer of them than
 // half of the SMs, their keys are split, and the last CTA of those that share a tile joins the results in the order of the keys.
 //
 // The maximum that the terms are relative to may stay 8 powers of two behind: P then reaches 256, O and l are in 32 bits, and scaling O again, a round trip
@@ -92,29 +92,33 @@ __device__ __forceinline__ float left_reference(float m, float c) {
 // A matrix descriptor whose low word, the address and the distance along M or N, is worked out in 32 bits
 __device__ __forceinline__ uint64_t with_low(uint64_t desc, uint32_t low) { return (desc & 0xFFFFFFFF00000000ull) | low; }
 
-// The `at`-th block of two row tiles of a call, by a warp: up to 32 sequences in the order of their lengths, of each the last block first.  false: there are fewer
+// The `at`-th block of two row tiles of a call, by a warp.  false: there is none.  Of up to 32 sequences the longest come first; of more, each has as many places as it has blocks,
+// or one more: the first at its first row over a block's, plus its number, so that it is found by a search.  Of each sequence the last block is the first.
 struct Block { int s, index; Sequence q; };
 __device__ __forceinline__ bool find_block(const PromptLaunch &g, int at, Block &b) {
   const Sequences &batch = g.p.seq;
-  const int lane = threadIdx.x & 31, per_block = 2 * g.tokens, seqs = (int)batch.seqs, per = (seqs + 31) / 32;
-  int s = lane * per, blocks = 0;
-  Sequence own = {0, 0, -1};
+  const int lane = threadIdx.x & 31, per_block = 2 * g.tokens, seqs = (int)batch.seqs;
   auto blocks_of = [&](const Sequence &q) { return (q.n + per_block - 1) / per_block; };
-  if (per == 1) {
-    if (lane < seqs) own = sequence_of(batch, lane);
-    int rank = 0;
-    for (int j = 0; j < seqs; ++j) {
-      const int other = __shfl_sync(0xFFFFFFFFu, own.length, j);
-      rank += other > own.length || (other == own.length && j < lane);
-    }
-    for (int j = 0; j < seqs; ++j)
-      if (__shfl_sync(0xFFFFFFFFu, rank, j) == lane) s = j;
-    own = {__shfl_sync(0xFFFFFFFFu, own.first, s), __shfl_sync(0xFFFFFFFFu, own.n, s), __shfl_sync(0xFFFFFFFFu, own.length, s)};
-    if (lane < seqs) blocks = blocks_of(own);
-  } else {
-#pragma unroll 4
-    for (int i = s; i < min(s + per, seqs); ++i) blocks += blocks_of(sequence_of(batch, i));
+  if (seqs > 32) {
+    const int each = (batch.each + per_block - 1) / per_block;
+    auto place = [&](long long s) { return batch.starts ? min(max(batch.starts[s], 0), (int)batch.rows) / per_block + (int)s : (int)s * each; };
+    b.s = batch.starts ? (int)last_up_to(seqs, at, lane, place) : at / each;
+    if (b.s < 0) return false;
+    b.q = sequence_of(batch, b.s);
+    const int behind = at - place(b.s), blocks = blocks_of(b.q);
+    b.index = blocks - 1 - behind;
+    return behind >= 0 && behind < blocks;                      // (whatever starts hold)
   }
+  const Sequence own = lane < seqs ? sequence_of(batch, lane) : Sequence{0, 0, -1};
+  int rank = 0, s = lane;
+  for (int j = 0; j < seqs; ++j) {
+    const int other = __shfl_sync(0xFFFFFFFFu, own.length, j);
+    rank += other > own.length || (other == own.length && j < lane);
+  }
+  for (int j = 0; j < seqs; ++j)
+    if (__shfl_sync(0xFFFFFFFFu, rank, j) == lane) s = j;
+  const Sequence q = {__shfl_sync(0xFFFFFFFFu, own.first, s), __shfl_sync(0xFFFFFFFFu, own.n, s), __shfl_sync(0xFFFFFFFFu, own.length, s)};
+  const int blocks = lane < seqs ? blocks_of(q) : 0;
   int upto = blocks;
 #pragma unroll
   for (int k = 1; k < 32; k <<= 1) {
@@ -124,17 +128,9 @@ __device__ __forceinline__ bool find_block(const PromptLaunch &g, int at, Block 
   const uint32_t who = __ballot_sync(0xFFFFFFFFu, at < upto);
   if (who == 0) return false;
   const int mine = __ffs(who) - 1;
-  int before = upto - blocks;
-  if (per > 1 && lane == mine) {
-    own = sequence_of(batch, s);
-    for (blocks = blocks_of(own); at >= before + blocks; blocks = blocks_of(own)) {
-      before += blocks;
-      own = sequence_of(batch, ++s);
-    }
-  }
   b.s = __shfl_sync(0xFFFFFFFFu, s, mine);
-  b.index = __shfl_sync(0xFFFFFFFFu, blocks - 1 - (at - before), mine);
-  b.q = {__shfl_sync(0xFFFFFFFFu, own.first, mine), __shfl_sync(0xFFFFFFFFu, own.n, mine), __shfl_sync(0xFFFFFFFFu, own.length, mine)};
+  b.index = __shfl_sync(0xFFFFFFFFu, upto - 1 - at, mine);
+  b.q = {__shfl_sync(0xFFFFFFFFu, q.first, mine), __shfl_sync(0xFFFFFFFFu, q.n, mine), __shfl_sync(0xFFFFFFFFu, q.length, mine)};
   return true;
 }
 

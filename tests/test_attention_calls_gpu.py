@@ -274,3 +274,79 @@ def test_fast_frequencies_at_the_farthest_positions():
     want = torch.cat((a * angle.cos() - b * angle.sin(), b * angle.cos() + a * angle.sin()), -1)
     off = (a.abs() + b.abs()).repeat(1, 1, 2) * 2.0 ** -20                                                # (as turn64's)
     close(out, want, off, E.f32)
+
+
+# ------------------------------------------------------------------------------------------- many sequences
+def many(new, lengths, heads, kv_heads, d, causal=True, aligned=True):
+    """Sequences of up to 16 tokens over one page each, against the definition for those that have new tokens."""
+    seqs, rows, dt = len(new), int(new.sum()), E.bf16
+    starts = torch.zeros(seqs + 1, dtype=torch.int32, device="cuda")
+    starts[1:] = new.cumsum(0)
+    some = new.nonzero()[:, 0]
+    pages = len(some) + 1
+    table = torch.full((seqs, 1), A.FAR_PAGE, dtype=torch.int32, device="cuda")
+    table[some, 0] = torch.randperm(pages, device="cuda")[:len(some)].to(torch.int32)
+    k, v = (randn(pages, kv_heads, 16, d, dtype=A.TORCH[dt], seed=i) for i in (1, 2))
+    q = randn(rows, heads, d, dtype=A.TORCH[dt], seed=3)
+    plan = E.Attention(heads, kv_heads, d, page_size=16, causal=causal, **({} if aligned else dict(ld_input=heads * d + 4)))
+    if not aligned:
+        wide = torch.empty(rows, heads * d + 4, dtype=q.dtype, device="cuda")
+        wide[:, :heads * d] = q.flatten(1)
+        q_in = wide[:, :heads * d]
+    else:
+        q_in = q
+    out = A.poisoned(rows, heads, d, dt=dt)
+    torch.cuda.synchronize()
+    assert plan.enqueue(out, q_in, k, v, table, lengths, starts, rows=rows, seqs=seqs) == 0, E.last_error()
+    assert plan.device_status() == 0
+    where = torch.repeat_interleave(torch.arange(seqs, device="cuda"), new)
+    place = torch.arange(rows, device="cuda") - starts[where]
+    group, at = heads // kv_heads, table[where, 0].long()
+    s = torch.einsum("rhd,rhmd->rhm", q.double(), k[at].double().repeat_interleave(group, 1)) * d ** -0.5
+    seen = lengths[where] - (new[where] - 1 - place if causal else 0)
+    s = s.masked_fill(torch.arange(16, device="cuda") >= seen[:, None, None], -float("inf"))
+    w = torch.softmax(s, -1).nan_to_num(0.0)
+    want, size = (torch.einsum("rhm,rhmd->rhd", w, x.repeat_interleave(group, 1)) for x in (v[at].double(), v[at].double().abs()))
+    close(out, want, (2.0 ** -8 + 2.0 ** -16) * 1.1 * size, dt)
+
+
+@pytest.mark.parametrize("seqs", [33, 64, 1000, 5000])
+@pytest.mark.parametrize("heads,kv_heads,d,aligned", [(4, 4, 64, True), (8, 1, 128, True), (3, 1, 64, True), (2, 2, 64, False)])
+def test_many_ragged_sequences(seqs, heads, kv_heads, d, aligned):
+    g = torch.Generator(device="cuda").manual_seed(seqs)
+    new = torch.randint(0, 17, (seqs,), generator=g, device="cuda") * (torch.rand(seqs, generator=g, device="cuda") < 0.6)
+    lengths = (new + torch.randint(0, 17, (seqs,), generator=g, device="cuda")).clamp(max=16).to(torch.int32)
+    many(new, lengths, heads, kv_heads, d, True, aligned)
+    many(new, lengths, heads, kv_heads, d, False, aligned)
+
+
+@pytest.mark.parametrize("count", [7, 4000])
+@pytest.mark.parametrize("aligned", [True, False])
+def test_a_few_of_a_million_sequences(count, aligned):
+    """A call's CTAs find their sequences by searching: looked at one after the other, 2^20 of them would cost each CTA some milliseconds, and a call of 2^20 CTAs half a
+    minute."""
+    seqs = 1 << 20
+    g = torch.Generator(device="cuda").manual_seed(count)
+    new = torch.zeros(seqs, dtype=torch.int64, device="cuda")
+    some = torch.randperm(seqs, generator=g, device="cuda")[:count]
+    new[some] = torch.randint(1, 4, (count,), generator=g, device="cuda")
+    lengths = torch.where(new > 0, new + 9, 0).to(torch.int32)
+    many(new, lengths, 2, 1, 64, True, aligned)
+    # and into the cache
+    rows = int(new.sum())
+    starts = torch.zeros(seqs + 1, dtype=torch.int32, device="cuda")
+    starts[1:] = new.cumsum(0)
+    table = torch.full((seqs, 1), A.FAR_PAGE, dtype=torch.int32, device="cuda")
+    some = new.nonzero()[:, 0]
+    table[some, 0] = torch.arange(count, dtype=torch.int32, device="cuda")
+    k, v = (torch.zeros(count, 1, 16, 64, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    q, nk, nv = (randn(rows, h, 64, dtype=torch.bfloat16, seed=i) for i, h in enumerate((2, 1, 1)))
+    plan, q_out = E.CacheAppend(2, 1, 64, 16, rotary_dim=0), torch.empty_like(q)
+    assert plan.prepare() == 0
+    torch.cuda.synchronize()
+    assert plan.enqueue(q_out, k, v, q, nk, nv, table, lengths, starts, rows=rows, seqs=seqs) == 0, E.last_error()
+    assert plan.device_status() == 0
+    where = torch.repeat_interleave(torch.arange(seqs, device="cuda"), new)
+    at = lengths[where].long() - new[where] + torch.arange(rows, device="cuda") - starts[where]
+    page = table[where, 0].long()
+    assert torch.equal(q_out, q) and torch.equal(k[page, :, at], nk) and torch.equal(v[page, :, at], nv)
