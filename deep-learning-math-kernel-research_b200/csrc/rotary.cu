@@ -37,9 +37,10 @@ __global__ void __launch_bounds__(WARPS * 32, 4) rotary_kernel(const RotaryParam
       position = p.positions[row];
     } else {
       const int s = sequence_of_row(p.seq, (int)row, lane);
-      if (s >= 0 && s < p.seq.seqs) {
+      const int length = s >= 0 && s < p.seq.seqs ? p.seq.lengths[s] : 0;
+      if (length > 0) {                                         // (an empty sequence's rows fill a batch up)
         const Sequence q = sequence_of(p.seq, s);
-        position = max(p.seq.lengths[s], 0) - q.n + ((int)row - q.first);     // (a length past the table is none that it can hold: no place)
+        position = length - q.n + ((int)row - q.first);         // (a length past the table is none that it can hold: no place)
         int page = -1, offset = 0;
         if (position >= 0 && (int)row < q.first + q.n) {
           const int i = position / p.page_size;

@@ -490,7 +490,8 @@ ELB_API int elb_rotary_enqueue(elb_op_t *op, void *q_out, void *k_out, const voi
 
 /* New tokens come into the cache: q is turned into q_out, k turned into its place in k_cache, v copied to its place in v_cache.  A row
  * whose place has no page (before the sequence's start, past the table, a page outside the pool) is left out, its q_out too, and
- * elb_op_device_status tells (105).  Two rows of a call must not have the same place. */
+ * elb_op_device_status tells (105).  Rows of a sequence of length 0, an empty slot of a padded batch, are left out too, which is no error.  Two rows of a call must not have the
+ * same place. */
 typedef struct elb_append_desc {
   elb_rotary_desc_t rotary;                       /* kv_heads at least 1; ld_k_out is not used */
   int32_t page_size, reserved;

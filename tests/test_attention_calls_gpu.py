@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import attentionutil as A
-from oputil import E, close, randn
+from oputil import E, POISON, close, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -350,3 +350,39 @@ def test_a_few_of_a_million_sequences(count, aligned):
     at = lengths[where].long() - new[where] + torch.arange(rows, device="cuda") - starts[where]
     page = table[where, 0].long()
     assert torch.equal(q_out, q) and torch.equal(k[page, :, at], nk) and torch.equal(v[page, :, at], nv)
+
+
+@pytest.mark.parametrize("new", [1, 3])
+@pytest.mark.parametrize("empty", [0, -7])
+def test_empty_slots_of_a_padded_batch(new, empty):
+    """A step of answers, captured once, in which some places of the batch hold no sequence: nothing is written for them, attention gives them zeros, and nothing is wrong."""
+    seqs, d = 6, 64
+    rows, lengths = seqs * new, A.ints([empty if i in (1, 4) else 20 + i for i in range(seqs)])
+    table = A.ints([[-1, -1] if i in (1, 4) else [2 * i, 2 * i + 1] for i in range(seqs)])
+    k, v = (torch.zeros(2 * seqs, 2, 16, d, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    q, nk, nv = (randn(rows, h, d, dtype=torch.bfloat16, seed=h) for h in (4, 2, 3))
+    nv = nv[:, :2].contiguous()
+    q_out, out = torch.full_like(q, POISON), A.poisoned(rows, 4, d, dt=E.bf16)
+    append, attention, s = E.CacheAppend(4, 2, d, 16, rotary_dim=0), E.Attention(4, 2, d, page_size=16), torch.cuda.Stream()
+    assert append.prepare() == 0
+
+    def step():
+        assert append.enqueue(q_out, k, v, q, nk, nv, table, lengths, rows=rows, seqs=seqs, stream=s.cuda_stream) == 0, E.last_error()
+        assert attention.enqueue(out, q_out, k, v, table, lengths, rows=rows, seqs=seqs, stream=s.cuda_stream) == 0, E.last_error()
+    torch.cuda.synchronize()
+    step()
+    s.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        step()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert append.device_status() == attention.device_status() == 0
+    for i in range(seqs):
+        r = slice(i * new, (i + 1) * new)
+        if i in (1, 4):
+            assert bool((q_out[r] == POISON).all()) and bool((out[r] == 0).all())
+            continue
+        at = torch.arange(20 + i - new, 20 + i, device="cuda")
+        assert torch.equal(q_out[r], q[r]) and torch.equal(k[2 * i + at // 16, :, at % 16], nk[r]) and torch.equal(v[2 * i + at // 16, :, at % 16], nv[r])
+    assert not bool(k[[2, 3, 8, 9]].any()) and not bool(v[[2, 3, 8, 9]].any())
