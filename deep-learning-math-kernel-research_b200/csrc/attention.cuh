@@ -83,6 +83,7 @@ struct RotaryParams {
   int heads, kv_heads, head_dim, rotary, neighbours, inverse, page_size, et;
   float magnitude;
   int words;                        // everything lies in whole 16-byte words
+  int num_sms;
   int *status;
 };
 cudaError_t launch_rotary(const RotaryParams &p, cudaStream_t s);

@@ -89,6 +89,7 @@ RotaryParams rotary_params(const elb_op &op, const elb_rotary_desc_t &d) {
   p.inverse = d.inverse != 0;
   p.et = et_of(d.dt);
   p.magnitude = d.magnitude;
+  p.num_sms = op.num_sms;
   p.status = op.d_status;
   return p;
 }

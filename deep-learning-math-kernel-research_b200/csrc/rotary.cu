@@ -127,9 +127,11 @@ __global__ void __launch_bounds__(WARPS * 32, 4) rotary_kernel(const RotaryParam
 
 template <typename T, int VEC, bool NEAR>
 cudaError_t go(const RotaryParams &p, cudaStream_t s) {
-  // A token per block is done sooner, a token per warp needs no barrier: the block's where it has the SMs to itself.  (32 + 8 heads of 128, us, block / warp: 64 rows
-  // 3.2/5.8, 200 4.0/5.8, 592 4.4/6.6, 1184 7.7/6.1, 2400 13.9/10.7, 4700 28/15.)
-  const bool team = p.rows < 148 * WARPS;
+  // A token per block is done sooner, a token per warp needs no barrier and no second wave: blocks' while warps' would not fill the SMs with a block each.  (us, block / warp, in a
+  // graph: 32 + 8 heads of 128: 64 rows 3.3/5.7, 592 4.2/6.0, 1036 6.9/10.0, 1600 9.6/10.4, 2400 13.3/11.0; 16 + 16 of 80: 1036 5.7/7.9, 2400 11.3/8.3; 1 + 1 of 128: 296 2.5/2.6,
+  // 1036 4.6/3.9.  Warps' grids of half of the SMs or just all of them are quicker than their neighbours: 1184 rows of 32 + 8 heads 7.4/5.9.  By rows alone the limit is a
+  // compromise: the two cross near 500 rows of 2 heads, 1700 of 40.)
+  const bool team = p.rows < (long long)p.num_sms * WARPS;
   const dim3 grid((unsigned)(team ? p.rows : (p.rows + WARPS - 1) / WARPS));
   const size_t smem = (size_t)(team ? 1 : WARPS) * (p.rotary / 2) * sizeof(float2);
   return team ? launch_overlapped(rotary_kernel<T, VEC, NEAR, true>, grid, dim3(WARPS * 32), smem, s, p)

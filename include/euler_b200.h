@@ -339,7 +339,7 @@ ELB_API int elb_wino_f32_noalloc_status(void);
  * feed-forward half of a transformer block, dense or routed to experts, for inference: four operators
  * with one protocol, the convolution plans' own: create from a description, prepare once (weights are
  * copied, converted and laid out; the caller's tensors are not read again, a second prepare does
- * nothing), enqueue often.  One opaque object serves all four.
+ * nothing), enqueue often.  One opaque object serves all of them, and those of attention below.
  *
  * enqueue: tensors are DEVICE memory of the plan's device, output first; work is enqueued on
  * cuda_stream (NULL = default stream) and not waited for; rows may differ from call to call, and 0
