@@ -210,8 +210,8 @@ __global__ void __launch_bounds__(THREADS, Smem<CB, MB>::CTAS) attention_token_k
           i = kt.page_of(walk.t);
           next[j].token = (walk.t - i * kt.parts) * TILE;
         }
-        if ((long long)i * kt.page < walk.q.length) next[j].page = p.seq.table[walk.s * p.seq.width + i];
-        else next[j].token = -1;                                // behind the sequence's end
+        if ((long long)i * kt.page < walk.q.length && walk.q.n > 0) next[j].page = p.seq.table[walk.s * p.seq.width + i];
+        else next[j].token = -1;                                // behind the sequence's end, or of one that nobody asks for
       }
       walk.t += PRODUCERS;
     };

@@ -457,8 +457,8 @@ ELB_API int elb_experts_enqueue(elb_op_t *op, void *output, const void *input, c
  *   starts    int32 [seqs + 1], the first row of each sequence and the end of the last; NULL: every sequence brings rows / seqs
  *             (no remainder).  Rows behind the last sequence are left as they are.
  *   lengths   int32 [seqs], the tokens that a sequence holds, the new ones included: new token i of n stands at length - n + i
- *   table     int32 [seqs][width], the page that holds tokens p * page_size .. of a sequence; entries behind its length are not
- *             read.  A page outside 0 .. pages - 1 is not touched: its keys and values count as zeros, nothing is written to it, and
+ *   table     int32 [seqs][width], the page that holds tokens p * page_size .. of a sequence; entries behind its length, and those of
+ *             sequences without new tokens, are not read.  A page outside 0 .. pages - 1 is not touched: its keys and values count as zeros, nothing is written to it, and
  *             elb_op_device_status tells (105).  Sequences may share pages that are read.
  * Cache: pages of page_size tokens, element (page, head, token, channel) at page * ld_page + head * ld_head + token * ld_token +
  * channel; all three 0: [pages][kv_heads][page_size][head_dim]. */

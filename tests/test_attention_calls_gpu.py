@@ -386,3 +386,28 @@ def test_empty_slots_of_a_padded_batch(new, empty):
         at = torch.arange(20 + i - new, 20 + i, device="cuda")
         assert torch.equal(q_out[r], q[r]) and torch.equal(k[2 * i + at // 16, :, at % 16], nk[r]) and torch.equal(v[2 * i + at // 16, :, at % 16], nv[r])
     assert not bool(k[[2, 3, 8, 9]].any()) and not bool(v[[2, 3, 8, 9]].any())
+
+
+@pytest.mark.parametrize("n", [1, 4, 60])
+@pytest.mark.parametrize("aligned", [True, False])
+def test_sequences_without_new_tokens_have_no_pages(n, aligned):
+    """Their lengths may be anything and their entries of the table no pages: nobody reads them, and nothing is wrong."""
+    d, lengths = 64, [70, 200, 90, 33]
+    b = A.batch([0, n, 0, 0], [lengths[0], 200 + n, lengths[2], lengths[3]], 16, ragged=True)
+    q, kv = A.inputs(b, 4, 2, d, E.bf16)
+    (k, k_view, ld), (v, v_view, _) = A.cache(b, 2, d, E.bf16), A.cache(b, 2, d, E.bf16)
+    A.put(b, k_view, 1, kv[1][0])
+    A.put(b, v_view, 1, kv[1][1])
+    want, err, _ = A.wanted(b, q, kv, True, d ** -0.5, E.bf16)
+    for s in (0, 2, 3):
+        b.table[s] = -1 if s else A.FAR_PAGE
+    if not aligned:
+        wide = torch.empty(n, 4 * d + 4, dtype=q.dtype, device="cuda")
+        wide[:, :4 * d] = q.flatten(1)
+        q = wide[:, :4 * d]
+    plan = E.Attention(4, 2, d, page_size=16, ld_input=0 if aligned else 4 * d + 4, **ld)
+    out = A.poisoned(n, 4, d, dt=E.bf16)
+    torch.cuda.synchronize()
+    assert plan.enqueue(out, q, k, v, b.table, b.lengths_t, b.starts_t, rows=n, seqs=4) == 0, E.last_error()
+    assert plan.device_status() == 0
+    close(out, want, err, E.bf16)
