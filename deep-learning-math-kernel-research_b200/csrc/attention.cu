@@ -1,7 +1,7 @@
 // Attention for every shape, on CUDA cores.
 //
 // A warp takes one head of one new token (attend_row) and goes over the keys that the token sees.  Bound by the reductions of each score over the
-// lanes, some 40 instructions a key: 8192 tokens of 32 heads, causal, take 227 ms, where the tensor cores take 0.44.
+// lanes, some 40 instructions a key: 8192 tokens of 32 heads, causal, take 227 ms, where the tensor cores take 0.5.
 #include <cmath>
 
 #include "attention.cuh"

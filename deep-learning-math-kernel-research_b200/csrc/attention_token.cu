@@ -10,7 +10,7 @@
 // Products are mma.sync m16n8k16: 16 rows are the least a matrix instruction takes, and at HBM's rate (23 bytes per SM and cycle) one of them is wanted
 // every 22 cycles, far below what it can do; tcgen05 would pad 128 rows and bring each score through tensor memory.
 //
-// 64 x 1 tokens of 32 heads of 128 over 8 behind 500 to 16000: 333 us, 6.6 TB/s, a copy's rate.  Smaller calls wait: some 5 us until the first tiles are there (lengths, table,
+// 64 x 1 tokens of 32 heads of 128 over 8 behind 500 to 16000: 334 to 350 us, 6.2 to 6.6 TB/s, a copy's rate.  Smaller calls wait: some 5 us until the first tiles are there (lengths, table,
 // copies, one after the other), 3 to 6 for the join.
 #include <cmath>
 #include <type_traits>
